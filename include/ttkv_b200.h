@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define TTKV_ABI_VERSION 5
+#define TTKV_ABI_VERSION 6
 
 /* host-side refusals (return values) */
 #define TTKV_OK 0
@@ -50,6 +50,8 @@ extern "C" {
 #define TTKV_STATUS_QUERY 5        /* q_len > seq_len, or a query range outside the batch */
 #define TTKV_STATUS_TIMEOUT 6      /* a bounded wait on the tensor-core pipeline ran out */
 #define TTKV_STATUS_SEQ_BOUND 7    /* a seq_len above the call's max_seq_len (the read's bound) */
+#define TTKV_STATUS_POOL_EMPTY 8   /* the free list has too few blocks for a request of the step */
+#define TTKV_STATUS_POOL_FULL 9    /* more blocks released than the free list has room for */
 
 /* element types */
 #define TTKV_F32 0
@@ -355,6 +357,111 @@ int ttkv_fit_tail(const float* G1, const float* G2, const float* G3, int32_t n, 
                   int32_t r2, int32_t H, int32_t d, int32_t qbits, int32_t budget,
                   int8_t* coeff_q, float* coeff_scale, int8_t* dec_q, uint16_t* dec_scale,
                   float* decoder, void* scratch, size_t scratch_bytes, void* stream);
+
+/* ---------------------------------------------------------------- a paged cache held in 4 bits
+ * No counterpart in the reference: an addition of this library, for layers without a calibrated
+ * decoder (any keys, as the model gives them to its attention, stored after RoPE).
+ *
+ * A cache of one layer is [n_blocks][H][block_size / 16] panels; slot id = block * block_size +
+ * offset. A panel holds 16 tokens of one KV head in 16 (d + 8 d / group) contiguous bytes:
+ *   K codes   [16 tokens][4 a][d/32 w][8 lanes]          lane 32 w + 8 a + i, two codes per byte
+ *   V codes   [8 token pairs][8 b][d/32 j][2 tokens][4 lanes]     lane 32 j + 4 b + i
+ *   K meta    [16 tokens][d/group] (scale fp16, minimum fp16);    V meta the same
+ * (lower lane in the lower nibble): the order in which the tensor-core fragments of the read take
+ * them, so a fragment is one 16-byte load and a mask. A code c stands for minimum + scale * c.
+ *
+ * Quantisation of a group x (after clamping to +-57344): minimum m = fp16(min x), scale s =
+ * fp16((max x - min x) / 15), code = the integer nearest to (x - m) / s within 0..15 (ties to
+ * even; 0 where s = 0). The quotients are rounded once, from their exact values. A group that
+ * holds a NaN or an infinity reads back as NaN. */
+typedef struct ttkv_q4_cache {
+    uint8_t* base;         /* 16-byte aligned */
+    int64_t n_blocks;
+    int32_t H, d, group, block_size;   /* d 64 or 128; group 32, 64 or 128, at most d; block_size a
+                                          multiple of 16 */
+    int32_t flags;         /* TTKV_CACHE_SKIP_PAD or 0 */
+} ttkv_q4_cache_t;
+
+/* Bytes of one panel, 0 for a geometry that is not served. */
+size_t ttkv_q4_panel_bytes(int32_t d, int32_t group);
+
+/* Quantise k, v (token i at + i * stride elements, [H, d] contiguous) into slots[i], i < n. The
+ * slots of one call differ from each other (a slot given twice holds parts of both tokens). A slot
+ * outside the cache is refused on the device (TTKV_STATUS_SLOT_RANGE) and its token skipped; with
+ * TTKV_CACHE_SKIP_PAD a negative one is skipped silently. */
+int ttkv_q4_write(const ttkv_q4_cache_t* cache, const int64_t* slots, int32_t n,
+                  const void* k, int32_t k_dtype, int64_t k_stride,
+                  const void* v, int32_t v_dtype, int64_t v_stride, int32_t* status, void* stream);
+
+/* The stored values of slots[i] into k, v (laid out as for the write), rounded once to their types.
+ * Rows of skipped or refused slots are left as they were. */
+int ttkv_q4_read(const ttkv_q4_cache_t* cache, const int64_t* slots, int32_t n,
+                 void* k, int32_t k_dtype, int64_t k_stride,
+                 void* v, int32_t v_dtype, int64_t v_stride, int32_t* status, void* stream);
+
+/* Paging of a 4-bit read: request r's first seq_lens[r] tokens are stored in the blocks of row r. */
+typedef struct ttkv_q4_batch {
+    const int32_t* block_table;
+    int64_t bt_stride;
+    int32_t bt_cols;
+    const int32_t* seq_lens;
+    int32_t n_reqs;
+} ttkv_q4_batch_t;
+
+/* Decode: request r's one query (q + r * q_stride elements, [HQ, d], fp16 or bf16) over its stored
+ * tokens, into out + r * out_stride in q's type. A request with seq_len 0 gets zeros. A request
+ * longer than its block-table row is refused (TTKV_STATUS_ROW_SHORT), its rows left as they were;
+ * one with a block id outside the cache gets NaN (TTKV_STATUS_BLOCK_RANGE). The launch depends on
+ * nothing that varies with the batch but n_reqs, so a capture replays any lengths. */
+size_t ttkv_q4_decode_workspace_bytes(const ttkv_q4_cache_t* cache, int32_t n_reqs, int32_t HQ);
+int ttkv_q4_decode(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch,
+                   const void* q, int32_t q_dtype, int64_t q_stride, int32_t HQ, float scale,
+                   void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                   int32_t* status, void* stream);
+
+/* Chunks: request r's queries are rows q_start[r] .. + q_len[r] of q, query j at position
+ * seq_len - q_len + j, which sees the stored tokens up to and with its own position. max_q_len and
+ * max_seq_len bound the batch's q_len and seq_lens; a request above either is refused
+ * (TTKV_STATUS_QUERY, TTKV_STATUS_SEQ_BOUND), as is one with q_len > seq_len (TTKV_STATUS_QUERY) or
+ * with query rows outside [0, n_rows) (TTKV_STATUS_QUERY); its rows are left as they were. Rows of
+ * no request are left as they were. */
+size_t ttkv_q4_prefill_workspace_bytes(const ttkv_q4_cache_t* cache, int32_t n_reqs, int32_t HQ,
+                                       int32_t max_q_len, int32_t max_seq_len);
+int ttkv_q4_prefill(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch,
+                    const int32_t* q_start, const int32_t* q_len,
+                    const void* q, int32_t q_dtype, int64_t q_stride, int32_t n_rows, int32_t HQ,
+                    float scale, void* out, int64_t out_stride, int32_t max_q_len,
+                    int32_t max_seq_len, void* workspace, size_t workspace_bytes,
+                    int32_t* status, void* stream);
+
+/* ---------------------------------------------------------------- block tables on the device
+ * No counterpart in the reference, whose engine builds them on the host.
+ *
+ * ttkv_plan_step: request r has seq_lens[r] tokens after this step, of which query_start_loc[r+1] -
+ * query_start_loc[r] are new; it holds ceil((seq - new) / block_size) blocks in its row. The blocks
+ * it lacks are popped off the end of the free list (free_blocks[0 .. *free_count)), in request
+ * order, into its row; slots[t] and positions[t] (may be null) of every token t < n_tokens are
+ * written, -1 and 0 for tokens of no request. *free_count_out = blocks left (may be free_count).
+ * Requests are served in order until the list runs out: that one and every later one that needs a
+ * block get none (TTKV_STATUS_POOL_EMPTY). A refused request (that, a row too short:
+ * TTKV_STATUS_ROW_SHORT, new > seq or tokens outside n_tokens: TTKV_STATUS_QUERY) gets slots -1, and
+ * where its row has room the entry behind its held blocks becomes -1, so a read of it is refused too.
+ *
+ * ttkv_release_blocks: pushes the ceil(lens[r] / block_size) blocks of each request's row onto the
+ * free list, in request order (lens[r] <= 0: none). capacity = the entries free_blocks has room for;
+ * requests that do not fit are left out (TTKV_STATUS_POOL_FULL), every later one too.
+ *
+ * n_reqs is at most TTKV_PLAN_MAX_REQS. */
+#define TTKV_PLAN_MAX_REQS 16384
+int ttkv_plan_step(int32_t* block_table, int64_t bt_stride, int32_t bt_cols, const int32_t* seq_lens,
+                   const int32_t* query_start_loc, int32_t n_reqs, const int32_t* free_blocks,
+                   int32_t capacity, const int32_t* free_count, int32_t* free_count_out,
+                   int32_t block_size, int64_t* slots, int64_t* positions, int32_t n_tokens,
+                   int32_t* status, void* stream);
+int ttkv_release_blocks(const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
+                        const int32_t* lens, int32_t n_reqs, int32_t* free_blocks, int32_t capacity,
+                        const int32_t* free_count, int32_t* free_count_out, int32_t block_size,
+                        int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

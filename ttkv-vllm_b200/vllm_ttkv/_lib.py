@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import pathlib
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 LIB_PATH = pathlib.Path(__file__).resolve().parents[1] / "libttkv_sm100.so"
 
 # host-side refusal codes (ttkv_b200.h)
@@ -20,7 +20,9 @@ STATUS = {0: "ok", 1: "block index outside the cache", 2: "block-table row too s
           3: "decoder index outside the pool", 4: "slot id is PAD_SLOT_ID or outside the cache",
           5: "query range inconsistent with seq_len",
           6: "a bounded wait on the tensor-core pipeline ran out",
-          7: "a seq_len above the max_seq_len the read was given (its bound)"}
+          7: "a seq_len above the max_seq_len the read was given (its bound)",
+          8: "the free list has too few blocks for a request of the step",
+          9: "more blocks released than the free list has room for"}
 
 F32, F16, BF16 = 0, 1, 2
 CACHE_SKIP_PAD = 1                          # TTKV_CACHE_SKIP_PAD
@@ -60,9 +62,24 @@ class Peers(C.Structure):
                 ("signal", C.c_void_p * MAX_PEERS), ("epoch", C.c_void_p), ("ticket", C.c_void_p)]
 
 
+class Q4Cache(C.Structure):
+    """ttkv_q4_cache_t: a layer's 4-bit paged cache."""
+    _fields_ = [("base", C.c_void_p), ("n_blocks", C.c_int64), ("H", C.c_int32), ("d", C.c_int32),
+                ("group", C.c_int32), ("block_size", C.c_int32), ("flags", C.c_int32)]
+
+
+class Q4Batch(C.Structure):
+    """ttkv_q4_batch_t: the paging of a 4-bit read."""
+    _fields_ = [("block_table", C.c_void_p), ("bt_stride", C.c_int64), ("bt_cols", C.c_int32),
+                ("seq_lens", C.c_void_p), ("n_reqs", C.c_int32)]
+
+
+PLAN_MAX_REQS = 16384                       # TTKV_PLAN_MAX_REQS
+
 P, I32, I64, SZ, F = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_float
 LP, CP, BP, RP = C.POINTER(Layout), C.POINTER(Cache), C.POINTER(Batch), C.POINTER(Rope)
 PP = C.POINTER(Peers)
+QP, QB = C.POINTER(Q4Cache), C.POINTER(Q4Batch)
 
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
@@ -94,6 +111,16 @@ SIGNATURES = {
                                          I64, P, I64, I32, P, P, P, SZ, P, P]),
     "ttkv_select_pack_rows": (C.c_int, [CP, P, I32, P, I32, I32, I32, I32, I32, I32, I32, P, P]),
     "ttkv_fit_tail_scratch_bytes": (SZ, [I32, I32, I32, I32]),
+    "ttkv_q4_panel_bytes": (SZ, [I32, I32]),
+    "ttkv_q4_write": (C.c_int, [QP, P, I32, P, I32, I64, P, I32, I64, P, P]),
+    "ttkv_q4_read": (C.c_int, [QP, P, I32, P, I32, I64, P, I32, I64, P, P]),
+    "ttkv_q4_decode_workspace_bytes": (SZ, [QP, I32, I32]),
+    "ttkv_q4_decode": (C.c_int, [QP, QB, P, I32, I64, I32, F, P, I64, P, SZ, P, P]),
+    "ttkv_q4_prefill_workspace_bytes": (SZ, [QP, I32, I32, I32, I32]),
+    "ttkv_q4_prefill": (C.c_int, [QP, QB, P, P, P, I32, I64, I32, I32, F, P, I64, I32, I32, P, SZ,
+                                  P, P]),
+    "ttkv_plan_step": (C.c_int, [P, I64, I32, P, P, I32, P, I32, P, P, I32, P, P, I32, P, P]),
+    "ttkv_release_blocks": (C.c_int, [P, I64, I32, P, I32, P, I32, P, P, I32, P, P]),
     "ttkv_fit_tail": (C.c_int, [P, P, P, I32, I32, I32, I32, I32, I32, I32, P, P, P, P, P, P, SZ,
                                 P]),
 }

@@ -390,3 +390,224 @@ def fit_tail(G1, G2, G3, budget: int, qbits: int = 8):
         out["dec_scale"].data_ptr(), out["decoder"].data_ptr(), scratch.data_ptr(), scratch.numel(),
         _stream()))
     return out
+
+
+# ---------------------------------------------------------------- the 4-bit paged cache (vllm_ttkv.q4)
+def _same_device(dev: torch.device, *named) -> None:
+    for name, t in named:
+        if t is not None and t.device != dev:
+            _need_cuda(t)
+            raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+
+
+def _launch(dev: torch.device, fn, *args) -> None:
+    """Call a C entry on `dev`, which need not be the current device, and on its current stream."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+        return
+    with torch.cuda.device(dev):
+        _lib.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _heads_stride(t: torch.Tensor, heads: int, d: int, name: str) -> int:
+    """Stride between rows of a [n, heads, d] tensor whose [heads, d] rows are contiguous (a size-1
+    dimension may carry any stride)."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != d:
+        raise ValueError(f"{name} must be [n, {heads}, {d}], got {tuple(t.shape)}")
+    n, s = t.shape[0], t.stride()
+    if s[2] != 1 or (heads > 1 and s[1] != d):
+        raise ValueError(f"{name} must have contiguous [heads, d] rows (strides {s})")
+    if n > 1 and s[0] < heads * d:
+        raise ValueError(f"{name}'s rows overlap (strides {s})")
+    return s[0] if n > 1 else heads * d
+
+
+def _q4_cache(lay, cache: torch.Tensor, skip_pad: bool = False) -> _lib.Q4Cache:
+    _need_cuda(cache)
+    return _lib.Q4Cache(cache.data_ptr(), cache.shape[0], lay.H, lay.d, lay.group, lay.block_size(cache),
+                        _lib.CACHE_SKIP_PAD if skip_pad else 0)
+
+
+def _q4_store(fn, lay, cache, slots, k, v, status, skip_pad):
+    dev = cache.device
+    c_s = _q4_cache(lay, cache, skip_pad)
+    _same_device(dev, ("slot_mapping", slots), ("k", k), ("v", v), ("status", status))
+    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise TypeError("slot_mapping must be contiguous int64 [n]")
+    n = slots.shape[0]
+    ks, vs = _heads_stride(k, lay.H, lay.d, "k"), _heads_stride(v, lay.H, lay.d, "v")
+    if k.shape[0] < n or v.shape[0] < n:
+        raise ValueError(f"k and v hold {k.shape[0]} and {v.shape[0]} tokens for {n} slot ids")
+    st = status if status is not None else status_word(dev)
+    _launch(dev, fn, C.byref(c_s), slots.data_ptr(), n, k.data_ptr(), dtype_code(k), ks, v.data_ptr(),
+            dtype_code(v), vs, st.data_ptr())
+
+
+def q4_write_paged(lay, cache: torch.Tensor, slot_mapping: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                   status: torch.Tensor | None = None, skip_pad: bool = False) -> None:
+    """Quantise tokens k/v [n, H, d] (fp32, fp16 or bf16, rows of any stride) into their slots of a
+    4-bit cache (`lay`: a `q4.Q4Layout`). The slots of one call must differ. skip_pad: a negative slot
+    is skipped instead of refused (`check_status`)."""
+    _q4_store(_lib.lib().ttkv_q4_write, lay, cache, slot_mapping, k, v, status, skip_pad)
+
+
+def q4_read_paged(lay, cache: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                  status: torch.Tensor | None = None, skip_pad: bool = False) -> None:
+    """The values stored at `slots` into k/v [n, H, d] (fp32, fp16 or bf16): what the attention over
+    the cache sees. Rows of skipped or refused slots are left as they were."""
+    _q4_store(_lib.lib().ttkv_q4_read, lay, cache, slots, k, v, status, skip_pad)
+
+
+def _q4_batch(dev, block_table, seq_lens, n) -> _lib.Q4Batch:
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise TypeError(f"block_table and seq_lens must be int32, got {block_table.dtype} and {seq_lens.dtype}")
+    if block_table.dim() != 2 or (block_table.numel() > 0 and block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be [n_reqs, max_blocks] with unit column stride")
+    if block_table.shape[0] != n or seq_lens.dim() != 1 or seq_lens.shape[0] < n or \
+            (n > 1 and seq_lens.stride(0) != 1):
+        raise ValueError(f"{n} requests, {block_table.shape[0]} block-table rows, seq_lens {tuple(seq_lens.shape)}")
+    return _lib.Q4Batch(block_table.data_ptr(), block_table.stride(0) if n > 1 else block_table.shape[1],
+                        block_table.shape[1], seq_lens.data_ptr(), n)
+
+
+def _q4_queries(lay, q, out):
+    if q.dtype not in (torch.float16, torch.bfloat16) or out.dtype != q.dtype:
+        raise TypeError(f"queries and outputs are both float16 or both bfloat16, got {q.dtype} and {out.dtype}")
+    if q.dim() != 3 or q.shape[1] % lay.H or q.shape[1] == 0:
+        raise ValueError(f"q must be [n, HQ, {lay.d}] with HQ a multiple of H={lay.H}, got {tuple(q.shape)}")
+    HQ = q.shape[1]
+    return HQ, _heads_stride(q, HQ, lay.d, "q"), _heads_stride(out, HQ, lay.d, "out")
+
+
+def q4_decode_paged(lay, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    q: torch.Tensor, scale: float, out: torch.Tensor,
+                    status: torch.Tensor | None = None) -> torch.Tensor:
+    """Batched decode over a 4-bit cache: q [B, HQ, d] (fp16 or bf16; row r = request r) over the first
+    seq_lens[r] tokens of block_table row r, into out [B, HQ, d]. A request with seq_len 0 gets zeros.
+    Nothing is read back, and the launch depends only on the shapes: a captured call replays any
+    lengths. The scratch is allocated per call by torch, so calls on different streams, and captured
+    graphs, do not share it."""
+    dev = cache.device
+    c_s = _q4_cache(lay, cache)
+    _same_device(dev, ("block_table", block_table), ("seq_lens", seq_lens), ("q", q), ("out", out), ("status", status))
+    HQ, qs, os_ = _q4_queries(lay, q, out)
+    B = q.shape[0]
+    if out.shape[0] < B:
+        raise ValueError(f"{B} queries, {out.shape[0]} outputs")
+    b_s = _q4_batch(dev, block_table, seq_lens, B)
+    if B == 0:
+        return out
+    L = _lib.lib()
+    ws_n = L.ttkv_q4_decode_workspace_bytes(C.byref(c_s), B, HQ)
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+    st = status if status is not None else status_word(dev)
+    _launch(dev, L.ttkv_q4_decode, C.byref(c_s), C.byref(b_s), q.data_ptr(), dtype_code(q), qs, HQ, float(scale),
+            out.data_ptr(), os_, ws.data_ptr(), ws_n, st.data_ptr())
+    return out
+
+
+def q4_prefill_paged(lay, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                     q_start: torch.Tensor, q_len: torch.Tensor, q: torch.Tensor, scale: float,
+                     out: torch.Tensor, max_q_len: int, max_seq_len: int,
+                     status: torch.Tensor | None = None) -> torch.Tensor:
+    """Chunks over a 4-bit cache: request r's queries are rows q_start[r] .. +q_len[r] of q [N, HQ, d]
+    (fp16 or bf16), at positions seq_len - q_len + j, causal over the stored tokens (which include the
+    chunk's own). `max_q_len` and `max_seq_len` bound the batch (host numbers, no readback); a request
+    above them is refused on the device (`check_status`). Rows of no request are left as they were."""
+    dev = cache.device
+    c_s = _q4_cache(lay, cache)
+    _same_device(dev, ("block_table", block_table), ("seq_lens", seq_lens), ("q_start", q_start), ("q_len", q_len),
+                 ("q", q), ("out", out), ("status", status))
+    HQ, qs, os_ = _q4_queries(lay, q, out)
+    N, B = q.shape[0], block_table.shape[0]
+    if out.shape[0] < N:
+        raise ValueError(f"{N} queries, {out.shape[0]} outputs")
+    for name, t in (("q_start", q_start), ("q_len", q_len)):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < B or (B > 1 and t.stride(0) != 1):
+            raise TypeError(f"{name} must be contiguous int32 with one entry per request")
+    if max_q_len < 0 or max_seq_len < 0:
+        raise ValueError(f"max_q_len={max_q_len} and max_seq_len={max_seq_len} must not be negative")
+    b_s = _q4_batch(dev, block_table, seq_lens, B)
+    if B == 0 or N == 0:
+        return out
+    L = _lib.lib()
+    ws_n = L.ttkv_q4_prefill_workspace_bytes(C.byref(c_s), B, HQ, int(max_q_len), int(max_seq_len))
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+    st = status if status is not None else status_word(dev)
+    _launch(dev, L.ttkv_q4_prefill, C.byref(c_s), C.byref(b_s), q_start.data_ptr(), q_len.data_ptr(), q.data_ptr(),
+            dtype_code(q), qs, N, HQ, float(scale), out.data_ptr(), os_, int(max_q_len), int(max_seq_len),
+            ws.data_ptr(), ws_n, st.data_ptr())
+    return out
+
+
+# ---------------------------------------------------------------- block tables on the device
+def _plan_tables(block_table, lens, free_blocks, free_count, free_count_out, name):
+    _need_cuda(block_table)
+    dev = block_table.device
+    for what, t in (("block_table", block_table), (name, lens), ("free_blocks", free_blocks),
+                    ("free_count", free_count), ("free_count_out", free_count_out)):
+        if t.dtype != torch.int32:
+            raise TypeError(f"{what} must be int32, got {t.dtype}")
+        if t.device != dev:
+            raise ValueError(f"{what} is on {t.device}, the block table on {dev}")
+    if block_table.dim() != 2 or (block_table.numel() > 0 and block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be [n_reqs, max_blocks] with unit column stride")
+    n = block_table.shape[0]
+    if n > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_table's rows overlap")
+    if n > _lib.PLAN_MAX_REQS:
+        raise ValueError(f"{n} requests in one call: at most {_lib.PLAN_MAX_REQS}")
+    if lens.dim() != 1 or lens.shape[0] < n or (n > 1 and lens.stride(0) != 1):
+        raise ValueError(f"{name} must be contiguous with one entry per block-table row")
+    if free_blocks.dim() != 1 or not free_blocks.is_contiguous():
+        raise ValueError("free_blocks must be contiguous [capacity]")
+    if free_count.numel() != 1 or free_count_out.numel() != 1:
+        raise ValueError("free_count and free_count_out hold one number each")
+    return dev, n, (block_table.stride(0) if n > 1 else block_table.shape[1])
+
+
+def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor,
+              free_blocks: torch.Tensor, free_count: torch.Tensor, block_size: int, slot_mapping: torch.Tensor,
+              positions: torch.Tensor | None = None, free_count_out: torch.Tensor | None = None,
+              status: torch.Tensor | None = None) -> None:
+    """A step's block tables and slots from its lengths, on the device. Request r has seq_lens[r] tokens
+    after the step, query_start_loc[r+1] - query_start_loc[r] of them new; the blocks it lacks are taken
+    off the end of free_blocks[:free_count] in request order and written into its row of `block_table`
+    in place. slot_mapping (int64 [T]) and positions (int64 [T], optional) are written for every token,
+    -1 and 0 behind the last request's (the padding of a captured size, which `q4_write_paged` and
+    `write_paged` skip with skip_pad). The blocks left go to `free_count_out` (default: free_count).
+    A request that is refused (the list is empty, its row is short, its lengths disagree) has slots -1
+    and, behind the blocks it holds, a block id -1, which the reads refuse; see `check_status`."""
+    out = free_count if free_count_out is None else free_count_out
+    dev, n, stride = _plan_tables(block_table, seq_lens, free_blocks, free_count, out, "seq_lens")
+    _same_device(dev, ("query_start_loc", query_start_loc), ("slot_mapping", slot_mapping), ("positions", positions),
+                 ("status", status))
+    if query_start_loc.dtype != torch.int32 or query_start_loc.dim() != 1 or \
+            query_start_loc.shape[0] < n + 1 or not query_start_loc.is_contiguous():
+        raise TypeError("query_start_loc must be contiguous int32 with one entry more than there are requests")
+    for name, t in (("slot_mapping", slot_mapping), ("positions", positions)):
+        if t is not None and (t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous()):
+            raise TypeError(f"{name} must be contiguous int64 [tokens]")
+    T = slot_mapping.shape[0]
+    if positions is not None and positions.shape[0] < T:
+        raise ValueError(f"positions hold {positions.shape[0]} tokens, slot_mapping {T}")
+    st = status if status is not None else status_word(dev)
+    _launch(dev, _lib.lib().ttkv_plan_step, block_table.data_ptr(), stride, block_table.shape[1], seq_lens.data_ptr(),
+            query_start_loc.data_ptr(), n, free_blocks.data_ptr(), free_blocks.shape[0], free_count.data_ptr(),
+            out.data_ptr(), int(block_size), slot_mapping.data_ptr(),
+            None if positions is None else positions.data_ptr(), T, st.data_ptr())
+
+
+def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, free_blocks: torch.Tensor,
+                   free_count: torch.Tensor, block_size: int, free_count_out: torch.Tensor | None = None,
+                   status: torch.Tensor | None = None) -> None:
+    """Return the blocks of finished requests: the ceil(lens[r] / block_size) blocks of each row go onto
+    the end of free_blocks[:free_count], in request order (lens[r] = 0: none). The table's rows are left
+    as they are. Each block may be returned once."""
+    out = free_count if free_count_out is None else free_count_out
+    dev, n, stride = _plan_tables(block_table, lens, free_blocks, free_count, out, "lens")
+    _same_device(dev, ("status", status))
+    st = status if status is not None else status_word(dev)
+    _launch(dev, _lib.lib().ttkv_release_blocks, block_table.data_ptr(), stride, block_table.shape[1], lens.data_ptr(),
+            n, free_blocks.data_ptr(), free_blocks.shape[0], free_count.data_ptr(), out.data_ptr(), int(block_size),
+            st.data_ptr())
