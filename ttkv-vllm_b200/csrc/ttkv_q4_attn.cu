@@ -14,8 +14,8 @@
 // word (the next nibble's come out as c 2^-20: q is stored with the factor, o divided by it); eight
 // values cost five instructions. p_t s_t is rounded to fp16, an operand of the matrix product, after
 // scaling by a power of two that keeps the largest near 2^14. It multiplies c - 7.5 (the second sum
-// takes the rounded weight's share of 7.5, and is fp32), so the rounding error is that of weights on
-// centred values: 2^-12 of each term at most.
+// takes the rounded weight's share of 7.5: sum p' of a unit comes from one more product, with ones), so
+// the rounding error is that of weights on centred values: 2^-12 of each term at most.
 #include <algorithm>
 
 #include "ttkv_async.cuh"
@@ -27,7 +27,6 @@ namespace {
 using namespace q4;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWarps = 8;                   // warps of a streaming CTA, each on its own run of tokens
 constexpr int kUnit = 64;                   // tokens of a unit of work: one softmax step of a warp
 
 struct AttnParams {
@@ -48,9 +47,10 @@ struct AttnParams {
     void* out;
     int64_t out_stride;
     int32_t n_ctas;
-    int64_t* prefix;                        // [n_reqs + 1] units before each request (workspace)
+    int32_t* prefix;                        // [n_reqs + 1] units before each request (workspace)
     float* part_ml;                         // [n_ctas][2][rows][2]
     float* part_o;                          // [n_ctas][2][rows][D]
+    float* first;                           // [n_ctas][warps] parts of the warps' first segments
     int32_t* status;
 };
 
@@ -71,7 +71,7 @@ __device__ __forceinline__ Req request(const AttnParams& P, int r, bool tell) {
     if (P.q_len && a.ql > 0 &&
         (a.ql > a.seq || a.ql > P.max_q || a.q0 < 0 || int64_t(a.q0) + a.ql > P.n_rows)) code = TTKV_STATUS_QUERY;
     else if (P.max_seq > 0 && a.seq > P.max_seq && a.ql > 0) code = TTKV_STATUS_SEQ_BOUND;
-    else if ((int64_t(a.seq) + P.block_size - 1) / P.block_size > P.bt_cols && a.ql > 0) code = TTKV_STATUS_ROW_SHORT;
+    else if (a.seq > int64_t(P.bt_cols) * P.block_size && a.ql > 0) code = TTKV_STATUS_ROW_SHORT;
     if (code) {
         a.refused = true;
         if (tell) report(P.status, code);
@@ -80,12 +80,11 @@ __device__ __forceinline__ Req request(const AttnParams& P, int r, bool tell) {
     return a;
 }
 
-__device__ __forceinline__ int row_blocks(const Req& a, int G, int rows) { return int((int64_t(a.ql) * G + rows - 1) / rows); }
+__device__ __forceinline__ int row_blocks(const Req& a, int G, int rows) { return int((unsigned(a.ql) * unsigned(G) + rows - 1) / rows); }
 __device__ __forceinline__ int units_of(const Req& a) { return a.ql > 0 ? (a.seq + kUnit - 1) / kUnit : 0; }
 
-// The CTA that owns unit u of T shared out to n CTAs, CTA c owning [c T / n, (c + 1) T / n).
-__device__ __forceinline__ int64_t share_begin(int64_t c, int64_t T, int64_t n) { return c * T / n; }
-__device__ __forceinline__ int64_t owner_of(int64_t u, int64_t T, int64_t n) { return ((u + 1) * n - 1) / T; }
+// The list of T units shared out to n CTAs: CTA c owns [c S, (c + 1) S), S = ceil(T / n), cut at T.
+__device__ __forceinline__ int share_size(int T, int n) { return (T + n - 1) / n; }
 
 // ------------------------------------------------------------------ warp-level products
 // D += A (16 x 16, row) . B (16 x 8, column), fp16 operands and fp32 sums.
@@ -138,8 +137,8 @@ struct WarpRows {
     float q1[NT][2][NG], qm[NT][2];     // sums of q 2^e over each group; 2^-e scale log2(e)
     int lim[NT][2], min_lim;            // tokens each row sees; the fewest any row of the block does
     float m[NT][2], l[NT][2];           // running max (base 2) and this lane's share of the sum
-    float o[2 * NW][NT][4];             // (p s 2^vn) . c
-    float dsum[NT][2][NG];              // this lane's share of 2^vn p (m + 7.5 s) - 7.5 (p s 2^vn)
+    float o[2 * NW][NT][4];             // (p s 2^vn) . (c - 7.5)
+    float dsum[NT][2][NG];              // this lane's share of 2^vn p (m + 7.5 s)
     float vn;                           // 2^vn, the scaling of the weights
 
     __device__ __forceinline__ void start(const AttnParams& P, const Req& rq, int h, int rb, int lane) {
@@ -211,10 +210,17 @@ struct WarpRows {
         vn = 274877906944.f;                                     // 2^38: the least scale in [2^14, 2^15)
     }
 
-    // Tokens [t0, t0 + 64), panel p of them at pan[p] (null: none, or a block id outside the cache).
-    template <bool MASK>
-    __device__ __forceinline__ void step_masked(const uint8_t* const (&pan)[4], int t0, int seq, int lane) {
+    // Tokens [t0, t0 + 64) of the request, panel p of them at ring slot (slot + p) % RING. MASK: some row
+    // does not see all of them.
+    template <bool MASK, int RING>
+    __device__ __forceinline__ void step(const uint8_t* ring, int slot, int t0, int seq, int lane) {
         const int b = lane >> 2, a = lane & 3;
+        const uint8_t* pan[4];
+        #pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const int i = slot + p;
+            pan[p] = ring + (i >= RING ? i - RING : i) * panel_bytes(D, GRP);
+        }
         float s[4][NT][4];
         float tmax[NT][2], vmax = 0.f;
         #pragma unroll
@@ -331,6 +337,13 @@ struct WarpRows {
                     #pragma unroll
                     for (int k = 0; k < 4; ++k) o[i][nt][k] *= corr[nt][k & 1];
         }
+        float psum[NG][NT][4];                           // the unit's sum of p', the same in every row
+        #pragma unroll
+        for (int g = 0; g < NG; ++g)
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) psum[g][nt][i] = 0.f;
         #pragma unroll
         for (int p = 0; p < 4; ++p) {
             if (MASK && t0 + 16 * p >= seq) continue;
@@ -359,13 +372,16 @@ struct WarpRows {
                             if (t >= lim[nt][0]) w0 = d0 = 0.f;
                             if (t >= lim[nt][1]) w1 = d1 = 0.f;
                         }
-                        const __half2 wh = __floats2half2_rn(w0, w1);
-                        const float2 wf = __half22float2(wh);
-                        dsum[nt][0][g] += fmaf(-7.5f, wf.x, d0);
-                        dsum[nt][1][g] += fmaf(-7.5f, wf.y, d1);
-                        pf[g][nt][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&wh));
+                        dsum[nt][0][g] += d0;
+                        dsum[nt][1][g] += d1;
+                        pf[g][nt][i] = transpose8x8(half2_bits(w0, w1));
                     }
                 }
+            constexpr uint32_t ONES = 0x3c003c00u;
+            #pragma unroll
+            for (int g = 0; g < NG; ++g)
+                #pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816(psum[g][nt], ONES, ONES, ONES, ONES, pf[g][nt][0], pf[g][nt][1]);
             uint32_t lo[NW], hi[NW];                             // tokens 2 a, 2 a + 1 and those + 8
             load_words(pan[p] + 8 * D + a * D + b * (D / 8), lo);
             load_words(pan[p] + 8 * D + (a + 4) * D + b * (D / 8), hi);
@@ -382,6 +398,30 @@ struct WarpRows {
                 }
             }
         }
+        // centred at once, so that o stays as small as the values are: the products' sums are cut, not
+        // rounded, at 2^-23 of what they hold
+        #pragma unroll
+        for (int i = 0; i < 2 * NW; ++i)
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                #pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    o[i][nt][k] = fmaf(k < 2 ? -7.5f / 16777216.f : -7.5f / 1048576.f, psum[i / 2 / WPG][nt][k], o[i][nt][k]);
+    }
+
+    // f(row of the block, first of four output lanes, o, m, l) for what this lane holds of the rows.
+    template <typename F>
+    __device__ __forceinline__ void rows(F f, int lane) const {
+        const int b = lane >> 2, a = lane & 3;
+        #pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            #pragma unroll
+            for (int c = 0; c < 2; ++c)
+                #pragma unroll
+                for (int k = 0; k < NW; ++k)
+                    f(8 * nt + 2 * a + c, 32 * k + 4 * b,
+                      make_float4(o[2 * k][nt][c], o[2 * k][nt][2 + c], o[2 * k + 1][nt][c], o[2 * k + 1][nt][2 + c]),
+                      m[nt][c], l[nt][c]);
     }
 
     // Sums over the lanes that share columns; o becomes sum p V relative to m, l the whole sum.
@@ -412,6 +452,12 @@ struct WarpRows {
 // Weighted sum of partials (max m_i, sum l_i, rows o_i relative to m_i): relative to M = max m_i.
 __device__ __forceinline__ float part_weight(float m, float M) { return M == -INFINITY ? 1.f : ex2(m - M); }
 
+// Lanes ln .. + 4 of row i of a part of `rows` rows.
+__device__ __forceinline__ void put_part(float* part, int rows, int D, int i, int ln, float4 o, float m, float l) {
+    *reinterpret_cast<float4*>(part + i * D + ln) = o;
+    if (ln == 0) *reinterpret_cast<float2*>(part + rows * D + 2 * i) = make_float2(m, l);
+}
+
 // Four output values o / l from lane index `lane` (a multiple of 4) of row (query j, head g of h).
 __device__ __forceinline__ void store_out(const AttnParams& P, const Req& rq, int h, int row, int D, int lane, float4 o,
                                           float l) {
@@ -430,34 +476,81 @@ __device__ __forceinline__ void store_out(const AttnParams& P, const Req& rq, in
 
 // ------------------------------------------------------------------ the streaming kernel
 // The work is the list of (request, KV head, row block, 64-token unit), shared out evenly: CTA c of
-// n owns [c T / n, (c + 1) T / n), each of its warps an eighth of that. A warp's run crosses from one
-// (request, head, row block) to the next; what a run holds of one is a segment. A segment that is
+// n owns [c T / n, (c + 1) T / n), each of its warps an equal part of that. A warp's run crosses from
+// one (request, head, row block) to the next; what a run holds of one is a segment. A segment that is
 // whole writes its output; the others meet in shared memory at the end of the CTA, and what is still
 // a part then goes to the workspace for q4_merge_kernel (at most the CTA's first and its last).
+//
+// Every warp streams its own run through its own ring of panels in shared memory, filled by bulk
+// copies (a panel is one contiguous piece of memory) issued two units ahead, so no warp waits for
+// another and an SM keeps about 100 KB in flight, more than its share of bandwidth times latency
+// (44 GB/s x 1 us).
 template <int D, int GRP, int NT>
-__global__ void __launch_bounds__(32 * kWarps) q4_stream_kernel(const AttnParams P) {
+struct Stream {
+    static constexpr int PANEL = panel_bytes(D, GRP), RING = 8;                 // two units
+    // warps of an SM: 8 where a row block of 16 takes their registers, else 12, or 10 where the rings
+    // of 12 do not fit
+    static constexpr int WARPS = NT == 2 ? 8 : 12 * RING * PANEL <= 222 * 1024 ? 12 : 10;
+    static constexpr int THREADS = 32 * WARPS, ROWS = 8 * NT, SLOTS = 2 * WARPS;
+    static constexpr int PART = ROWS * (D + 2);                                 // floats of a part: o, then (m, l)
+    static constexpr int RING_BYTES = WARPS * RING * PANEL;
+    static constexpr int SMEM = std::max(WARPS * PART * 4, RING_BYTES) + WARPS * RING * 8;
+};
+
+// A place in the work list: unit ui of U of row block rb of KV head h of request r.
+struct Cursor {
+    int r, h, rb, ui, U, nrb, seq;
+};
+
+__device__ __forceinline__ void load_request(const AttnParams& P, Cursor& c, int rows) {
+    const Req a = request(P, c.r, false);
+    c.seq = a.seq;
+    c.U = units_of(a);
+    c.nrb = row_blocks(a, P.G, rows);
+}
+
+__device__ __forceinline__ void advance(const AttnParams& P, Cursor& c, int rows) {
+    if (++c.ui < c.U) return;
+    c.ui = 0;
+    if (++c.rb < c.nrb) return;
+    c.rb = 0;
+    if (++c.h < P.H) return;
+    c.h = 0;
+    do {                                                 // the next request with work: the run is not over
+        ++c.r;
+        load_request(P, c, rows);
+    } while (c.U == 0);
+}
+
+template <int D, int GRP, int NT>
+__global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kernel(const AttnParams P) {
     using Rows = WarpRows<D, GRP, NT>;
-    constexpr int ROWS = 8 * NT, SLOTS = 2 * kWarps;
-    extern __shared__ __align__(16) unsigned char smem[];
-    float* po = reinterpret_cast<float*>(smem);                                       // [SLOTS][ROWS][D]
-    float* pml = po + SLOTS * ROWS * D;                                               // [SLOTS][ROWS][2]
-    uint8_t* nan_panel = reinterpret_cast<uint8_t*>(pml + SLOTS * ROWS * 2);          // codes 0, scales NaN
-    __shared__ long long pre[32 * kWarps + 1], wsum[kWarps];
-    __shared__ long long pid[SLOTS];                     // first unit of the slot's (request, head, row block), -1: none
+    using S = Stream<D, GRP, NT>;
+    constexpr int ROWS = S::ROWS, SLOTS = S::SLOTS, WARPS = S::WARPS, THREADS = S::THREADS, RING = S::RING, PANEL = S::PANEL;
+    extern __shared__ __align__(128) unsigned char smem[];
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::SMEM - WARPS * RING * 8);
+    __shared__ int pre[THREADS + 1];
+    __shared__ long long wsum[WARPS];
+    __shared__ int pid[SLOTS];                           // first unit of the slot's (request, head, row block), -1: none
     __shared__ int pr[SLOTS], ph[SLOTS], prb[SLOTS];
+    __shared__ float pm[SLOTS][ROWS], pl[SLOTS][ROWS];   // max and sum of the parts' rows, then weight and sum
 
     const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
     const bool tell = blockIdx.x == 0;
+    uint8_t* ring = smem + w * RING * PANEL;
+    uint64_t* bar = bars + w * RING;
+    if (lane < RING) mbar_init(bar + lane, 1);
+    pdl_wait();
 
     // ---- units of the requests before each thread's share of them
-    const int per = (P.n_reqs + 32 * kWarps - 1) / (32 * kWarps);
+    const int per = (P.n_reqs + THREADS - 1) / THREADS;
     const int rlo = min(tid * per, P.n_reqs), rhi = min(rlo + per, P.n_reqs);
-    long long mine = 0;
+    long long sum = 0;
     for (int r = rlo; r < rhi; ++r) {
         const Req a = request(P, r, tell);
-        mine += (long long)P.H * row_blocks(a, P.G, ROWS) * units_of(a);
+        sum += (long long)P.H * row_blocks(a, P.G, ROWS) * units_of(a);
     }
-    long long inc = mine;
+    long long inc = sum;
     #pragma unroll
     for (int k = 1; k < 32; k <<= 1) {
         const long long y = __shfl_up_sync(0xffffffffu, inc, k);
@@ -465,137 +558,197 @@ __global__ void __launch_bounds__(32 * kWarps) q4_stream_kernel(const AttnParams
     }
     if (lane == 31) wsum[w] = inc;
     if (tid < SLOTS) pid[tid] = -1;
-    for (int i = tid; i < panel_bytes(D, GRP) / 4; i += 32 * kWarps)
-        reinterpret_cast<uint32_t*>(nan_panel)[i] = i < 16 * D / 4 ? 0u : 0x00007e00u;
     __syncthreads();
     for (int i = 0; i < w; ++i) inc += wsum[i];
-    pre[tid] = inc - mine;
-    if (tid == 32 * kWarps - 1) pre[tid + 1] = inc;
+    pre[tid] = int(inc - sum);
+    if (tid == THREADS - 1) {
+        // 2^31 units would read 2^37 tokens: reported, and nothing done
+        const bool vast = inc > 0x7fff0000;
+        pre[THREADS] = vast ? 0 : int(inc);
+        if (vast && tell) report(P.status, TTKV_STATUS_SEQ_BOUND);
+    }
     __syncthreads();
-    const long long T = pre[32 * kWarps];
+    const int T = pre[THREADS], share = share_size(T, P.n_ctas);
     if (tell) {
-        long long u = inc - mine;
+        int u = int(inc - sum);
         for (int r = rlo; r < rhi; ++r) {
             P.prefix[r] = u;
             const Req a = request(P, r, false);
-            u += (long long)P.H * row_blocks(a, P.G, ROWS) * units_of(a);
+            u += P.H * row_blocks(a, P.G, ROWS) * units_of(a);
         }
         if (tid == 0) P.prefix[P.n_reqs] = T;
     }
-    const long long ca = share_begin(blockIdx.x, T, P.n_ctas), cb = share_begin(blockIdx.x + 1, T, P.n_ctas);
+    pdl_trigger();
+    const int ca = min(int(blockIdx.x) * share, T), cb = min(ca + share, T);
     if (ca == cb) return;
 
     // ---- this warp's run
-    long long u = ca + w * (cb - ca) / kWarps;
-    const long long ue = ca + (w + 1) * (cb - ca) / kWarps;
+    Rows R;
+    bool held = false;
+    const int wshare = share_size(cb - ca, WARPS);
+    int u = min(ca + w * wshare, cb);
+    const int ue = min(u + wshare, cb);
     if (u < ue) {
-        int lo = 0, hi = 32 * kWarps - 1;                // the last chunk of requests that begins at or before u
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (pre[mid] <= u) lo = mid; else hi = mid - 1;
+        Cursor c;
+        {
+            int lo = 0, hi = THREADS - 1;                // the last chunk of requests that begins at or before u
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (pre[mid] <= u) lo = mid; else hi = mid - 1;
+            }
+            int off = u - pre[lo];
+            for (c.r = lo * per;; ++c.r) {
+                load_request(P, c, ROWS);
+                const int all = P.H * c.nrb * c.U;
+                if (off < all) break;
+                off -= all;
+            }
+            const int pair = off / c.U;
+            c.ui = off - pair * c.U;
+            c.h = pair / c.nrb;
+            c.rb = pair - c.h * c.nrb;
         }
-        int r = lo * per;
-        long long off = u - pre[lo];
-        bool first = true;
+        // fetching: lanes 0 to 3 each know the block of one panel of unit f, the next to be issued
+        Cursor f = c;
+        int uf = u;
+        int f_slot = 0, f_blk = 0;
+        auto look_up = [&]() {
+            const int t = f.ui * kUnit + 16 * lane;
+            if (uf < ue && lane < 4 && t < f.seq) f_blk = P.block_table[int64_t(f.r) * P.bt_stride + t / P.block_size];
+        };
+        auto issue = [&]() {
+            if (uf >= ue) return;
+            const int t = f.ui * kUnit + 16 * lane;
+            if (lane < 4 && t < f.seq) {
+                const int i = f_slot + lane >= RING ? f_slot + lane - RING : f_slot + lane;
+                if (f_blk >= 0 && f_blk < P.n_blocks) {
+                    const uint8_t* src = P.cache + ((int64_t(f_blk) * P.H + f.h) * (P.block_size / kPanelTokens) +
+                                                    (t % P.block_size) / kPanelTokens) * PANEL;
+                    mbar_expect_tx(bar + i, PANEL);
+                    bulk_g2s(ring + i * PANEL, src, PANEL, bar + i);
+                } else {                                 // NaN scales: the request's rows come out as NaN
+                    report(P.status, TTKV_STATUS_BLOCK_RANGE);
+                    uint32_t* d = reinterpret_cast<uint32_t*>(ring + i * PANEL);
+                    for (int k = 0; k < PANEL / 4; ++k) d[k] = k < 4 * D ? 0u : 0x00007e00u;
+                    fence_async_smem();
+                    mbar_expect_tx(bar + i, 0);
+                }
+            }
+            const int np = min(4, (f.seq - f.ui * kUnit + 15) / 16);
+            f_slot += np;
+            if (f_slot >= RING) f_slot -= RING;
+            if (++uf < ue) advance(P, f, ROWS);
+            look_up();
+        };
+        look_up();
+        issue();
+        int slot = 0;
+        uint32_t phases = 0;                             // bit i: the parity that slot i completes next
+        bool late = false;
         while (u < ue) {
-            const Req rq = request(P, r, false);
-            const int U = units_of(rq), nrb = row_blocks(rq, P.G, ROWS);
-            if (off >= (long long)P.H * nrb * U) { off -= (long long)P.H * nrb * U; ++r; continue; }
-            const int pair = int(off / U), ui = int(off - (long long)pair * U);
-            const int h = pair / nrb, rb = pair - h * nrb;
-            const int n_here = int(min((long long)(U - ui), ue - u));
-            Rows R;
-            R.start(P, rq, h, rb, lane);
-            const int32_t* brow = P.block_table + int64_t(r) * P.bt_stride;
+            const Req rq = request(P, c.r, false);
+            const int n_here = min(c.U - c.ui, ue - u), begin = c.ui;
+            R.start(P, rq, c.h, c.rb, lane);
             for (int i = 0; i < n_here; ++i) {
-                const int t0 = (ui + i) * kUnit;
-                const uint8_t* pan[4];
+                const int t0 = (begin + i) * kUnit, np = min(4, (rq.seq - t0 + 15) / 16);
+                issue();                                 // the next unit, into the slots of the one before this
+                bool ok = true;
                 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const int t = t0 + 16 * p;
-                    pan[p] = nullptr;
-                    if (t < rq.seq) {
-                        const int bi = t / P.block_size, blk = brow[bi];
-                        if (blk >= 0 && blk < P.n_blocks) {
-                            pan[p] = P.cache + ((int64_t(blk) * P.H + h) * (P.block_size / kPanelTokens) +
-                                                (t - bi * P.block_size) / kPanelTokens) * panel_bytes(D, GRP);
-                        } else {
-                            pan[p] = nan_panel;
-                            if (lane == 0) report(P.status, TTKV_STATUS_BLOCK_RANGE);
-                        }
+                    const int k = slot + p >= RING ? slot + p - RING : slot + p;
+                    if (p < np) {
+                        if (!late) ok = mbar_wait(bar + k, (phases >> k) & 1u) && ok;
+                        phases ^= 1u << k;
                     }
                 }
-                if (t0 + kUnit <= R.min_lim) R.template step_masked<false>(pan, t0, rq.seq, lane);
-                else R.template step_masked<true>(pan, t0, rq.seq, lane);
+                if (!__all_sync(0xffffffffu, ok)) {      // a copy never came: wait for the others, issue no more
+                    late = true;
+                    if (lane == 0) report(P.status, TTKV_STATUS_TIMEOUT);
+                    for (int k = (slot + np) % RING; k != f_slot; k = (k + 1) % RING) mbar_wait(bar + k, (phases >> k) & 1u);
+                    uf = ue;
+                }
+                if (t0 + kUnit <= R.min_lim) R.template step<false, RING>(ring, slot, t0, rq.seq, lane);
+                else R.template step<true, RING>(ring, slot, t0, rq.seq, lane);
+                slot += np;
+                if (slot >= RING) slot -= RING;
+                __syncwarp();                            // every lane has read the unit
             }
             R.finish();
-            const bool whole = ui == 0 && n_here == U;
-            const int slot = 2 * w + (first ? 0 : 1);
-            const int b = lane >> 2, a = lane & 3;
-            #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int i = 8 * nt + 2 * a + c, row = rb * ROWS + i;
-                    #pragma unroll
-                    for (int k = 0; k < D / 32; ++k) {
-                        const float4 o = make_float4(R.o[2 * k][nt][c], R.o[2 * k][nt][2 + c], R.o[2 * k + 1][nt][c],
-                                                     R.o[2 * k + 1][nt][2 + c]);
-                        if (!whole) *reinterpret_cast<float4*>(po + (slot * ROWS + i) * D + 32 * k + 4 * b) = o;
-                        else if (row < rq.ql * P.G) store_out(P, rq, h, row, D, 32 * k + 4 * b, o, R.l[nt][c]);
-                    }
-                    if (!whole && b == 0) {
-                        pml[(slot * ROWS + i) * 2] = R.m[nt][c];
-                        pml[(slot * ROWS + i) * 2 + 1] = R.l[nt][c];
-                    }
-                }
-            if (!whole && lane == 0) {
-                pid[slot] = u - ui;
-                pr[slot] = r;
-                ph[slot] = h;
-                prb[slot] = rb;
-            }
-            first = false;
             u += n_here;
-            off += n_here;
+            if (begin == 0 && n_here == c.U) {           // whole
+                R.rows([&](int i, int ln, float4 o, float m, float l) {
+                    if (c.rb * ROWS + i < rq.ql * P.G) store_out(P, rq, c.h, c.rb * ROWS + i, D, ln, o, l);
+                }, lane);
+            } else {
+                // a part: the run's last stays in registers until the rings are free, its first goes
+                // to the workspace
+                held = u == ue;
+                if (lane == 0) {
+                    const int e = 2 * w + (held ? 1 : 0);
+                    pid[e] = u - n_here - begin;
+                    pr[e] = c.r;
+                    ph[e] = c.h;
+                    prb[e] = c.rb;
+                }
+                if (!held) {
+                    float* part = P.first + (int64_t(blockIdx.x) * WARPS + w) * S::PART;
+                    R.rows([&](int i, int ln, float4 o, float m, float l) { put_part(part, ROWS, D, i, ln, o, m, l); }, lane);
+                }
+            }
+            c.ui += n_here - 1;
+            if (u < ue) advance(P, c, ROWS);
         }
+    }
+    __syncthreads();                                     // every copy has landed and been read
+    if (held) {
+        float* part = reinterpret_cast<float*>(smem) + w * S::PART;
+        R.rows([&](int i, int ln, float4 o, float m, float l) { put_part(part, ROWS, D, i, ln, o, m, l); }, lane);
     }
     __syncthreads();
 
     // ---- what the warps hold of the same (request, head, row block), joined
+    auto part_of = [&](int e) -> const float* {
+        return (e & 1) ? reinterpret_cast<const float*>(smem) + (e >> 1) * S::PART
+                       : P.first + (int64_t(blockIdx.x) * WARPS + (e >> 1)) * S::PART;
+    };
+    for (int k = tid; k < SLOTS * ROWS; k += THREADS) {
+        const int e = k / ROWS, i = k % ROWS;
+        if (pid[e] >= 0) {
+            const float2 ml = *reinterpret_cast<const float2*>(part_of(e) + ROWS * D + 2 * i);
+            pm[e][i] = ml.x;
+            pl[e][i] = ml.y;
+        }
+    }
+    __syncthreads();
     for (int s0 = 0; s0 < SLOTS;) {
-        const long long id = pid[s0];
+        const int id = pid[s0];
         int s1 = s0 + 1;
         if (id < 0) { s0 = s1; continue; }
-        int last = s0;
-        for (; s1 < SLOTS && (pid[s1] < 0 || pid[s1] == id); ++s1)
-            if (pid[s1] == id) last = s1;
+        while (s1 < SLOTS && (pid[s1] < 0 || pid[s1] == id)) ++s1;
         const Req rq = request(P, pr[s0], false);
-        const int h = ph[s0], rb = prb[s0];
+        const int h = ph[s0], rb = prb[s0], live = min(ROWS, rq.ql * P.G - rb * ROWS);
         const bool whole = id >= ca && id + units_of(rq) <= cb;
         const int64_t g0 = (int64_t(blockIdx.x) * 2 + (ca >= id ? 0 : 1)) * ROWS;
-        for (int e = tid; e < ROWS * (D / 4); e += 32 * kWarps) {
+        for (int e = tid; e < live * (D / 4); e += THREADS) {
             const int i = e / (D / 4), ln = 4 * (e - i * (D / 4));
             float M = -INFINITY;
-            for (int s = s0; s <= last; ++s)
-                if (pid[s] == id) M = fmaxf(M, pml[(s * ROWS + i) * 2]);
+            for (int k = s0; k < s1; ++k)
+                if (pid[k] >= 0) M = fmaxf(M, pm[k][i]);
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
             float l = 0.f;
-            for (int s = s0; s <= last; ++s) {
-                if (pid[s] != id) continue;
-                const float wt = part_weight(pml[(s * ROWS + i) * 2], M);
-                const float4 x = *reinterpret_cast<const float4*>(po + (s * ROWS + i) * D + ln);
-                l = fmaf(wt, pml[(s * ROWS + i) * 2 + 1], l);
+            #pragma unroll 4
+            for (int k = s0; k < s1; ++k) {
+                if (pid[k] < 0) continue;
+                const float wt = part_weight(pm[k][i], M);
+                const float4 x = *reinterpret_cast<const float4*>(part_of(k) + i * D + ln);
+                l = fmaf(wt, pl[k][i], l);
                 o.x = fmaf(wt, x.x, o.x); o.y = fmaf(wt, x.y, o.y); o.z = fmaf(wt, x.z, o.z); o.w = fmaf(wt, x.w, o.w);
             }
             if (whole) {
-                if (rb * ROWS + i < rq.ql * P.G) store_out(P, rq, h, rb * ROWS + i, D, ln, o, l);
+                store_out(P, rq, h, rb * ROWS + i, D, ln, o, l);
             } else {
                 *reinterpret_cast<float4*>(P.part_o + (g0 + i) * D + ln) = o;
-                if (ln == 0) {
-                    P.part_ml[(g0 + i) * 2] = M;
-                    P.part_ml[(g0 + i) * 2 + 1] = l;
-                }
+                if (ln == 0) *reinterpret_cast<float2*>(P.part_ml + (g0 + i) * 2) = make_float2(M, l);
             }
         }
         s0 = s1;
@@ -610,7 +763,7 @@ constexpr int kMergeThreads = 256;
 
 __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParams P, int D, int rows_block) {
     __shared__ float4 so[kMergeThreads];
-    __shared__ float sm[kMergeThreads / 16], sl[kMergeThreads / 16], smax[kMergeThreads / 32];
+    __shared__ float sl[kMergeThreads / 16], smax[kMergeThreads / 32];
     const int r = blockIdx.y, tid = threadIdx.x;
     const Req rq = request(P, r, false);
     const int per_head = P.max_q * P.G;
@@ -618,25 +771,20 @@ __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParam
     if (rq.ql <= 0 || row >= rq.ql * P.G) return;
     const int lanes = D / 4, grp = tid / lanes, ngrp = kMergeThreads / lanes, ln = 4 * (tid - grp * lanes);
     const int U = units_of(rq);
+    const int nrb = row_blocks(rq, P.G, rows_block), rb = row / rows_block, i = row - rb * rows_block;
+    pdl_wait();
     if (U == 0) {
         if (grp == 0) store_out(P, rq, h, row, D, ln, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
         return;
     }
-    const int nrb = row_blocks(rq, P.G, rows_block), rb = row / rows_block, i = row - rb * rows_block;
-    const int64_t T = P.prefix[P.n_reqs], n = P.n_ctas;
-    const int64_t u0 = P.prefix[r] + (int64_t(h) * nrb + rb) * U;
-    const int64_t c0 = owner_of(u0, T, n), c1 = owner_of(u0 + U - 1, T, n);
+    const int T = P.prefix[P.n_reqs], u0 = P.prefix[r] + (h * nrb + rb) * U, share = share_size(T, P.n_ctas);
+    if (T == 0) return;
+    const int c0 = u0 / share, c1 = (u0 + U - 1) / share;
     if (c0 == c1) return;                                        // that CTA has written the output
-    auto slot = [&](int64_t c) -> int64_t {
-        const int64_t a = share_begin(c, T, n);
-        if (a == share_begin(c + 1, T, n)) return -1;            // fewer units than CTAs: nothing there
-        return (c * 2 + (a >= u0 ? 0 : 1)) * rows_block + i;
-    };
+    // a part lies in its CTA's first place unless the CTA's share began before it
+    auto place = [&](int c) { return (int64_t(c) * 2 + (c * share >= u0 ? 0 : 1)) * rows_block + i; };
     float M = -INFINITY;
-    for (int64_t c = c0 + tid; c <= c1; c += kMergeThreads) {
-        const int64_t s = slot(c);
-        if (s >= 0) M = fmaxf(M, P.part_ml[2 * s]);
-    }
+    for (int c = c0 + tid; c <= c1; c += kMergeThreads) M = fmaxf(M, P.part_ml[2 * place(c)]);
     #pragma unroll
     for (int k = 1; k < 32; k <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
     if ((tid & 31) == 0) smax[tid >> 5] = M;
@@ -646,12 +794,12 @@ __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParam
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
     #pragma unroll 4
-    for (int64_t c = c0 + grp; c <= c1; c += ngrp) {
-        const int64_t s = slot(c);
-        if (s < 0) continue;
-        const float wt = part_weight(P.part_ml[2 * s], M);
+    for (int c = c0 + grp; c <= c1; c += ngrp) {
+        const int64_t s = place(c);
+        const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * s);
         const float4 x = *reinterpret_cast<const float4*>(P.part_o + s * D + ln);
-        l = fmaf(wt, P.part_ml[2 * s + 1], l);
+        const float wt = part_weight(ml.x, M);
+        l = fmaf(wt, ml.y, l);
         o.x = fmaf(wt, x.x, o.x); o.y = fmaf(wt, x.y, o.y); o.z = fmaf(wt, x.z, o.z); o.w = fmaf(wt, x.w, o.w);
     }
     so[tid] = o;
@@ -678,14 +826,24 @@ int sm_count(int* n) {
     return TTKV_OK;
 }
 
-constexpr int kMaxStreamCtas = 2 * 148;          // the workspace is sized for it (a B200 has 148 SMs)
+constexpr int kMaxStreamCtas = 148;              // one per SM of a B200; the workspace is sized for it
 
 // Rows a streaming warp takes at once: 8 (query, head) rows a fragment, two fragments above that.
 int stream_nt(int64_t rows) { return rows > 8 ? 2 : 1; }
 
-size_t stream_workspace(int d, int n_reqs, int nt) {
+// Workspace: units before each request, two parts a CTA for the merge, a part a warp.
+struct StreamWs {
+    size_t part_o, part_ml, first, bytes;
+};
+
+StreamWs stream_ws(int d, int n_reqs, int nt) {
+    StreamWs w;
     const size_t rows = size_t(kMaxStreamCtas) * 2 * 8 * nt;
-    return ((size_t(n_reqs) + 1) * 8 + 15) / 16 * 16 + rows * (d + 2) * sizeof(float);
+    w.part_o = ((size_t(n_reqs) + 1) * 4 + 15) / 16 * 16;
+    w.part_ml = w.part_o + rows * d * sizeof(float);
+    w.first = w.part_ml + rows * 2 * sizeof(float);
+    w.bytes = w.first + size_t(kMaxStreamCtas) * 12 * 8 * nt * (d + 2) * sizeof(float);
+    return w;
 }
 
 int check_attn(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch, const void* q, int32_t q_dtype,
@@ -705,30 +863,47 @@ int check_attn(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch, const
 }
 
 template <int D, int GRP, int NT>
-int launch_stream(AttnParams P, cudaStream_t st) {
+int launch_stream(const AttnParams& P, cudaStream_t st) {
+    using S = Stream<D, GRP, NT>;
     auto k = q4_stream_kernel<D, GRP, NT>;
     if (int e = raise_smem_limit(reinterpret_cast<const void*>(k), "q4_stream_kernel")) return e;
-    const size_t smem = size_t(2 * kWarps) * 8 * NT * (D + 2) * sizeof(float) + panel_bytes(D, GRP);
-    k<<<P.n_ctas, 32 * kWarps, smem, st>>>(P);
-    if (int e = check_launch("q4_stream_kernel")) return e;
-    q4_merge_kernel<<<dim3(unsigned(P.H * P.max_q * P.G), unsigned(P.n_reqs)), kMergeThreads, 0, st>>>(P, D, 8 * NT);
-    return check_launch("q4_merge_kernel");
+    // both may start while the kernel before them runs and wait for it themselves
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(P.n_ctas));
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cfg.attrs = pdl;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, k, P);
+    if (e != cudaSuccess) { cudaGetLastError(); return fail(TTKV_ERR_CUDA, "q4_stream_kernel: %s", cudaGetErrorString(e)); }
+    cfg.gridDim = dim3(unsigned(P.H * P.max_q * P.G), unsigned(P.n_reqs));
+    cfg.blockDim = dim3(kMergeThreads);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, q4_merge_kernel, P, D, 8 * NT);
+    if (e != cudaSuccess) { cudaGetLastError(); return fail(TTKV_ERR_CUDA, "q4_merge_kernel: %s", cudaGetErrorString(e)); }
+    return TTKV_OK;
 }
 
 int run_stream(const ttkv_q4_cache_t* c, AttnParams P, void* ws, size_t ws_bytes, cudaStream_t st) {
     const int nt = stream_nt(int64_t(P.max_q) * P.G);
-    if (!ws || ws_bytes < stream_workspace(c->d, P.n_reqs, nt))
-        return fail(TTKV_ERR_WORKSPACE, "4-bit read: workspace of %zu bytes, %zu needed", ws_bytes,
-                    stream_workspace(c->d, P.n_reqs, nt));
+    const StreamWs w = stream_ws(c->d, P.n_reqs, nt);
+    if (!ws || ws_bytes < w.bytes)
+        return fail(TTKV_ERR_WORKSPACE, "4-bit read: workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, w.bytes);
     if (reinterpret_cast<uintptr_t>(ws) & 15) return fail(TTKV_ERR_ALIGN, "4-bit read: workspace not 16-byte aligned");
     int sms = 0;
     if (int e = sm_count(&sms)) return e;
     P.n_ctas = std::min(sms, kMaxStreamCtas);
-    const size_t rows = size_t(P.n_ctas) * 2 * 8 * nt;
-    P.prefix = static_cast<int64_t*>(ws);
-    P.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + ((size_t(P.n_reqs) + 1) * 8 + 15) / 16 * 16);
-    P.part_ml = P.part_o + rows * c->d;
-#define TTKV_Q4_STREAM(D, GRP)                                                                         if (c->d == D && c->group == GRP) return nt == 2 ? launch_stream<D, GRP, 2>(P, st) : launch_stream<D, GRP, 1>(P, st);
+    char* base = static_cast<char*>(ws);
+    P.prefix = reinterpret_cast<int32_t*>(base);
+    P.part_o = reinterpret_cast<float*>(base + w.part_o);
+    P.part_ml = reinterpret_cast<float*>(base + w.part_ml);
+    P.first = reinterpret_cast<float*>(base + w.first);
+#define TTKV_Q4_STREAM(D, GRP)                                                                     \
+    if (c->d == D && c->group == GRP) return nt == 2 ? launch_stream<D, GRP, 2>(P, st) : launch_stream<D, GRP, 1>(P, st);
     TTKV_Q4_STREAM(64, 32) TTKV_Q4_STREAM(64, 64) TTKV_Q4_STREAM(128, 32) TTKV_Q4_STREAM(128, 64) TTKV_Q4_STREAM(128, 128)
 #undef TTKV_Q4_STREAM
     return fail(TTKV_ERR_UNSUPPORTED, "4-bit read: geometry");
@@ -753,7 +928,7 @@ using namespace ttkv;
 
 extern "C" size_t ttkv_q4_decode_workspace_bytes(const ttkv_q4_cache_t* cache, int32_t n_reqs, int32_t HQ) {
     if (!cache || cache->H < 1 || HQ < cache->H || n_reqs < 0) return 0;
-    return stream_workspace(cache->d, n_reqs, stream_nt(HQ / cache->H));
+    return stream_ws(cache->d, n_reqs, stream_nt(HQ / cache->H)).bytes;
 }
 
 extern "C" int ttkv_q4_decode(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch, const void* q,
@@ -771,7 +946,7 @@ extern "C" int ttkv_q4_decode(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_
 extern "C" size_t ttkv_q4_prefill_workspace_bytes(const ttkv_q4_cache_t* cache, int32_t n_reqs, int32_t HQ,
                                                   int32_t max_q_len, int32_t max_seq_len) {
     if (!cache || cache->H < 1 || HQ < cache->H || n_reqs < 0 || max_q_len < 0) return 0;
-    return stream_workspace(cache->d, n_reqs, stream_nt(int64_t(max_q_len) * (HQ / cache->H)));
+    return stream_ws(cache->d, n_reqs, stream_nt(int64_t(max_q_len) * (HQ / cache->H))).bytes;
 }
 
 extern "C" int ttkv_q4_prefill(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch, const int32_t* q_start,
