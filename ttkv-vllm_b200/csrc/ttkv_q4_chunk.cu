@@ -1,0 +1,665 @@
+// Chunks of queries over the 4-bit paged cache on the 5th-generation tensor cores.
+//
+//   S = Q K^T,  P = exp(scale S - m) masked,  O += P V,  out = O / sum P
+//
+// A chunk has many (query, head) rows per stored token, so products bound it, not memory: a CTA takes
+// 256 rows of one KV head (two tiles of 128, the M of an MMA, whose products and softmaxes run in
+// turn) over stored tiles of 128 tokens. Each stored tile is turned into fp16 operands once for both:
+// K^ = m + s c and V^, rounded once to fp16 (half a step, 2^-12 of an element; the codes as exact
+// operands with their scales applied to S and P would cost the softmax twice its instructions, and
+// with groups below d a product each). Scores, sums and O are fp32; P is fp16, at most 2^8: the
+// running maximum moves only when a row's exceeds it by 2^8 (then O in tensor memory is rescaled).
+//
+// Roles: two softmax warpgroups (a thread owns a row, i.e. a lane of tensor memory), a warpgroup that
+// dequantises K and one for V, two warps that issue the products, one per row tile. Operands are
+// double-buffered in shared memory in the 128-byte-swizzled K-major layout of the MMA; S is followed
+// by P in the same tensor-memory columns. The stored order of the codes needs no transposition: a K
+// word is a 16-byte chunk of its token's row (the dims of a chunk in the order 0 4 1 5 2 6 3 7, which
+// Q repeats), and four V words are chunks of eight tokens of four lanes.
+//
+// The work list is (request, KV head, row block, stored tile up to the block's causal limit), shared
+// out evenly to one CTA per SM as in the streaming kernel; the parts that a share's borders cut go
+// through the workspace to q4_chunk_merge_kernel.
+#include "ttkv_q4_attn.cuh"
+#include "ttkv_umma.cuh"
+
+namespace ttkv {
+namespace {
+
+using namespace q4;
+using namespace umma;
+
+constexpr int TN = 128;                      // stored tokens of a tile
+constexpr int TM = 128;                      // rows of a tile
+constexpr int CROWS = 2 * TM;                // rows of a block
+constexpr int kChunkThreads = 18 * 32;       // softmax 8 warps, K 4, V 4, products 2
+constexpr uint32_t kTmemCols = 512;          // S0, S1, O0, O1 at 128 columns each
+constexpr int kFlags = 8;                    // tiles whose NaN values are remembered
+
+// Row tiles' tensor memory: S (then P in its first 64 columns) and O.
+__device__ __forceinline__ uint32_t s_col(int x) { return 128u * x; }
+__device__ __forceinline__ uint32_t o_col(int x) { return 256u + 128u * x; }
+
+template <int D>
+struct ChunkSmem {
+    static constexpr int Q = TM * D * 2, K = TN * D * 2, V = D * TN * 2;
+    static constexpr int off_q = 0, off_k = 2 * Q, off_v = off_k + 2 * K, BYTES = off_v + 2 * V + 1024;
+    static constexpr int KATOM = TN * 128, VATOM = D * 128;   // 64 dims of 128 tokens; 64 tokens of D lanes
+};
+
+struct ChunkBars {
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2];        // operand stages
+    uint64_t qfull[2], sfull[2], pfull[2], pvdone[2];         // row tiles
+};
+
+// A CTA's (or a role's) place in the work list.
+struct Segments {
+    int u, ue;                               // the next unit and the end of the share
+    int r, h, rb, ui, U, nrb;                // request, KV head, row block, tile of U
+    Req rq;
+
+    // Tiles that row block b reads: up to the limit of its last query.
+    __device__ __forceinline__ static int tiles(const Req& a, int G, int b) {
+        const int last = min((b * CROWS + CROWS - 1) / G, a.ql - 1);
+        return (a.seq - a.ql + last + 1 + TN - 1) / TN;
+    }
+    __device__ __forceinline__ static int per_head(const Req& a, int G) {
+        const int n = row_blocks(a, G, CROWS);
+        int sum = 0;
+        for (int b = 0; b < n; ++b) sum += tiles(a, G, b);
+        return sum;
+    }
+    __device__ __forceinline__ void load(const AttnParams& P) {
+        rq = request(P, r, false);
+        nrb = row_blocks(rq, P.G, CROWS);
+    }
+    // To unit u, `off` units behind the first of request r (or of a later one).
+    __device__ __forceinline__ void seek(const AttnParams& P, int off) {
+        int ph;
+        for (;; ++r) {
+            load(P);
+            ph = per_head(rq, P.G);
+            if (off < ph * P.H) break;
+            off -= ph * P.H;
+        }
+        h = off / ph;
+        off -= h * ph;
+        for (rb = 0;; ++rb) {
+            U = tiles(rq, P.G, rb);
+            if (off < U) break;
+            off -= U;
+        }
+        ui = off;
+    }
+    __device__ __forceinline__ int here() const { return min(U - ui, ue - u); }   // tiles of this segment
+    __device__ __forceinline__ void skip(const AttnParams& P, int n) {           // past n tiles of it
+        u += n;
+        ui += n;
+        if (u >= ue || ui < U) return;
+        ui = 0;
+        if (++rb == nrb) {
+            rb = 0;
+            if (++h == P.H) {
+                h = 0;
+                do { ++r; load(P); } while (nrb == 0);
+            }
+        }
+        U = tiles(rq, P.G, rb);
+    }
+};
+
+__device__ __forceinline__ uint32_t h2u(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+__device__ __forceinline__ __half2 u2h(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+
+// Two codes of a word as exact fp16 integers: an fp16 1024 + c, less 1024. HI: the upper nibble of a
+// byte, 1024 + 16 c.
+template <bool HI>
+__device__ __forceinline__ __half2 codes2(uint32_t w) {
+    if (HI) return __hfma2(u2h((w & 0x00f000f0u) | 0x64006400u), u2h(0x2c002c00u), u2h(0xd400d400u));   // x / 16 - 64
+    return __hsub2(u2h((w & 0x000f000fu) | 0x64006400u), u2h(0x64006400u));
+}
+
+template <int D, int GRP>
+__global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnParams P) {
+    using S = ChunkSmem<D>;
+    constexpr int NG = D / GRP, NW = D / 32, WPG = GRP / 32, PANEL = panel_bytes(D, GRP);
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ ChunkBars B;
+    __shared__ uint32_t tmem_base;
+    __shared__ int pre[kChunkThreads + 1];
+    __shared__ long long wsum[kChunkThreads / 32];
+    __shared__ __align__(16) uint8_t vbad[kFlags][TN];                    // groups whose V is NaN, a bit each
+    __shared__ int any_bad[kFlags];
+
+    const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+    const bool tell = blockIdx.x == 0;
+    if (w == 16) tmem_alloc(&tmem_base, kTmemCols);
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&B.kfull[i], 128);
+            mbar_init(&B.kempty[i], 2);
+            mbar_init(&B.vfull[i], 128);
+            mbar_init(&B.vempty[i], 2);
+            mbar_init(&B.qfull[i], 128);
+            mbar_init(&B.sfull[i], 1);
+            mbar_init(&B.pfull[i], 128);
+            mbar_init(&B.pvdone[i], 1);
+        }
+    }
+    for (int i = tid; i < kFlags * TN; i += kChunkThreads) (&vbad[0][0])[i] = 0;
+    if (tid < kFlags) any_bad[tid] = 0;
+    pdl_wait();
+
+    // ---- units of the requests before each thread's share of them
+    const int per = (P.n_reqs + kChunkThreads - 1) / kChunkThreads;
+    const int rlo = min(tid * per, P.n_reqs), rhi = min(rlo + per, P.n_reqs);
+    long long sum = 0;
+    for (int r = rlo; r < rhi; ++r) {
+        const Req a = request(P, r, tell);
+        sum += (long long)P.H * Segments::per_head(a, P.G);
+    }
+    long long inc = sum;
+    #pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, inc, k);
+        if (lane >= k) inc += y;
+    }
+    if (lane == 31) wsum[w] = inc;
+    tc_before();
+    __syncthreads();
+    tc_after();
+    for (int i = 0; i < w; ++i) inc += wsum[i];
+    pre[tid] = int(inc - sum);
+    if (tid == kChunkThreads - 1) {
+        const bool vast = inc > 0x7fff0000;                   // 2^31 tiles: reported, and nothing done
+        pre[kChunkThreads] = vast ? 0 : int(inc);
+        if (vast && tell) report(P.status, TTKV_STATUS_SEQ_BOUND);
+    }
+    __syncthreads();
+    const int T = pre[kChunkThreads], share = share_size(T, P.n_ctas);
+    const int ca = min(int(blockIdx.x) * share, T), cb = min(ca + share, T);
+    pdl_trigger();
+    const uint32_t tmem = tmem_base;
+    bool dead = false;                                        // a bounded wait ran out: no further waits
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!dead && !mbar_wait(bar, parity & 1u)) {
+            dead = true;
+            report(P.status, TTKV_STATUS_TIMEOUT);
+        }
+    };
+    Segments sg;
+    sg.u = ca;
+    sg.ue = cb;
+    if (ca < cb) {
+        int lo = 0, hi = kChunkThreads - 1;                   // the last chunk of requests that begins at or before ca
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (pre[mid] <= ca) lo = mid; else hi = mid - 1;
+        }
+        sg.r = lo * per;
+        sg.seek(P, ca - pre[lo]);
+    }
+    if (tid == 0) {                                           // for the merge: no row block begun here and cut, so far
+        P.rec[8 * blockIdx.x] = -1;
+    }
+
+    if (ca == cb) {
+        // fewer tiles than CTAs: nothing to do
+    } else if (w < 8) {
+        // ============================================================== softmax: row tile x, row t
+        const int x = w >> 2, t = tid & 127;
+        const uint32_t lane_base = tmem + (uint32_t(32 * (w & 3)) << 16);
+        unsigned char* qb = smem + S::off_q + x * S::Q;
+        uint32_t n_s = 0, n_tile = 0;                         // S phases of this tile; stored tiles of the CTA
+        for (; sg.u < sg.ue;) {
+            const Req rq = sg.rq;
+            const int n = sg.here(), begin = sg.ui, U = sg.U, h = sg.h, rb = sg.rb, r = sg.r, u0 = sg.u - sg.ui;
+            const int n_rows = rq.ql * P.G, row = rb * CROWS + x * TM + t;
+            sg.skip(P, n);
+            if (rb * CROWS + x * TM >= n_rows) { n_tile += n; continue; }       // no rows in this tile
+            const bool live = row < n_rows;
+            const int j = live ? row / P.G : 0, g = live ? row - j * P.G : 0;
+            const int lim = live ? rq.seq - rq.ql + j + 1 : 0;                  // sees stored tokens below it
+            float qf;
+            {
+                const int64_t src = int64_t(rq.q0 + j) * P.q_stride + int64_t(h * P.G + g) * D;
+                uint4 raw[D / 8];
+                float big = 0.f;
+                #pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    raw[c] = make_uint4(0, 0, 0, 0);
+                    if (live) {
+                        if (P.q_vec) {
+                            raw[c] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) + src) + c);
+                        } else {
+                            const uint16_t* e = static_cast<const uint16_t*>(P.q) + src + 8 * c;
+                            raw[c] = make_uint4(e[0] | (uint32_t(e[1]) << 16), e[2] | (uint32_t(e[3]) << 16),
+                                                e[4] | (uint32_t(e[5]) << 16), e[6] | (uint32_t(e[7]) << 16));
+                        }
+                    }
+                }
+                auto pair = [&](uint32_t v) {
+                    if (P.dtype == TTKV_BF16)
+                        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+                    return __half22float2(u2h(v));
+                };
+                #pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    const uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 f = pair(v[k]);
+                        big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+                }
+                // e brings the row's largest |q| into [1, 2); a negative scale's sign goes to q
+                const int e = big > 0.f && big < INFINITY ? 127 - int(__float_as_uint(big) >> 23) : 0;
+                const float up = copysignf(__uint_as_float(uint32_t(min(127 + e, 254)) << 23), P.scale);
+                qf = fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e, 1)) << 23);
+                #pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    const float2 a = pair(raw[c].x), b = pair(raw[c].y), d = pair(raw[c].z), f = pair(raw[c].w);
+                    // dims 0 4 1 5 2 6 3 7, the order of a word's codes
+                    *reinterpret_cast<uint4*>(qb + (c >> 3) * S::KATOM + kmajor_off(t, c & 7)) =
+                        make_uint4(half2_bits(a.x * up, d.x * up), half2_bits(a.y * up, d.y * up),
+                                   half2_bits(b.x * up, f.x * up), half2_bits(b.y * up, f.y * up));
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(&B.qfull[x]);
+
+            float m = -INFINITY, l = 0.f;
+            uint32_t bad = 0;                                 // groups of V that are NaN in a token that this row sees
+            auto note_bad = [&](int i, int k) {               // tile i of the segment, k-th of the CTA: V consumed
+                const int f = k & (kFlags - 1);
+                if (*reinterpret_cast<volatile int*>(&any_bad[f]) == 0) return;
+                for (int c = 0; c < TN; ++c)
+                    if ((begin + i) * TN + c < lim) bad |= *reinterpret_cast<volatile uint8_t*>(&vbad[f][c]);
+            };
+            for (int i = 0; i < n; ++i) {
+                const int t0 = (begin + i) * TN;
+                wait(&B.sfull[x], n_s);
+                ++n_s;
+                tc_after();
+                if (i > 0) note_bad(i - 1, int(n_tile) - 1);
+                const int seen = lim - t0;                    // tokens of the tile that the row sees
+                const bool full = __all_sync(0xffffffffu, seen >= TN);
+                float mt = -INFINITY;
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float s[32];
+                    tmem_ld32(lane_base + s_col(x) + 32 * c, s);
+                    tmem_wait_ld();
+                    if (full) {
+                        #pragma unroll
+                        for (int k = 0; k < 32; ++k) mt = fmaxf(mt, s[k]);
+                    } else {
+                        #pragma unroll
+                        for (int k = 0; k < 32; ++k) mt = fmaxf(mt, 32 * c + k < seen ? s[k] : -INFINITY);
+                    }
+                }
+                mt *= qf;
+                float corr = 1.f;
+                if (mt > m + 8.f) {                           // (m is -inf at first)
+                    corr = m == -INFINITY ? 0.f : ex2(m - mt);
+                    m = mt;
+                    l *= corr;
+                }
+                if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                    #pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        float o[32];
+                        tmem_ld32(lane_base + o_col(x) + 32 * c, o);
+                        tmem_wait_ld();
+                        #pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] *= corr;
+                        tmem_st32(lane_base + o_col(x) + 32 * c, o);
+                    }
+                }
+                const float mm = m == -INFINITY ? 0.f : m;    // a row that sees nothing yet has weights of 0
+                float2 ls = make_float2(0.f, 0.f);
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float s[32];
+                    tmem_ld32(lane_base + s_col(x) + 32 * c, s);
+                    tmem_wait_ld();
+                    if (!full) {
+                        #pragma unroll
+                        for (int k = 0; k < 32; ++k) s[k] = 32 * c + k < seen ? s[k] : -INFINITY;
+                    }
+                    uint32_t p[16];
+                    #pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 a = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), make_float2(qf, qf), make_float2(-mm, -mm));
+                        float2 e = make_float2(ex2(a.x), ex2(a.y));
+                        if (!full) {                          // (-inf * 0 of an all-zero query is NaN)
+                            if (32 * c + 2 * k >= seen) e.x = 0.f;
+                            if (32 * c + 2 * k + 1 >= seen) e.y = 0.f;
+                        }
+                        ls = __fadd2_rn(ls, e);
+                        p[k] = half2_bits(e.x, e.y);
+                    }
+                    tmem_st16u(lane_base + s_col(x) + 16 * c, p);
+                }
+                l += ls.x + ls.y;
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_before();
+                mbar_arrive(&B.pfull[x]);
+                ++n_tile;
+            }
+            // ---- O / l, or the parts
+            wait(&B.pvdone[x], n_s - 1);
+            tc_after();
+            note_bad(n - 1, int(n_tile) - 1);
+            const bool whole = begin == 0 && n == U;
+            const int64_t pr = (int64_t(blockIdx.x) * 2 + (ca >= u0 ? 0 : 1)) * CROWS + x * TM + t;
+            const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+            const int64_t dst = int64_t(rq.q0 + j) * P.out_stride + int64_t(h * P.G + g) * D;
+            #pragma unroll
+            for (int c = 0; c < NW; ++c) {
+                float o[32];
+                tmem_ld32(lane_base + o_col(x) + 32 * c, o);  // column 32 c + 8 i + b holds lane 32 c + 4 b + i
+                tmem_wait_ld();
+                const float f = (bad >> (c / WPG)) & 1u ? __int_as_float(0x7fc00000) : inv;
+                if (live) {
+                    #pragma unroll
+                    for (int b = 0; b < 8; ++b) {
+                        const float4 v = make_float4(o[b] * f, o[8 + b] * f, o[16 + b] * f, o[24 + b] * f);
+                        if (!whole) *reinterpret_cast<float4*>(P.part_o + pr * D + 32 * c + 4 * b) = v;
+                        else store4(P, dst + 32 * c + 4 * b, v);
+                    }
+                }
+            }
+            if (live && !whole) *reinterpret_cast<float2*>(P.part_ml + 2 * pr) = make_float2(m, l);
+            if (x == 0 && t == 0 && begin == 0 && n < U) {    // begun here and cut: this CTA's entry of the merge
+                int32_t* rec = P.rec + 8 * blockIdx.x;
+                rec[0] = r;
+                rec[1] = h;
+                rec[2] = rb;
+                rec[3] = u0;
+                rec[4] = U;
+                rec[5] = share;
+            }
+        }
+    } else if (w < 12) {
+        // ============================================================== K of a tile as fp16 rows
+        const int wk = w - 8, lt = lane & 7, a = lane >> 3;   // token of 8 and chunk of its row
+        uint32_t kw[4][NW], km[4][NG];
+        auto load = [&]() {                                   // tile sg.ui: 8-token groups 4 i + wk
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t0 = sg.ui * TN + 32 * i + 16 * (wk >> 1), o = 8 * (wk & 1) + lt;
+                #pragma unroll
+                for (int k = 0; k < NW; ++k) kw[i][k] = 0u;
+                #pragma unroll
+                for (int k = 0; k < NG; ++k) km[i][k] = 0u;
+                if (t0 >= sg.rq.seq) continue;
+                const int bi = t0 / P.block_size;
+                const int blk = __ldg(P.block_table + int64_t(sg.r) * P.bt_stride + bi);
+                if (blk < 0 || blk >= P.n_blocks) {           // NaN keys: so are the rows that see them
+                    if (lane == 0) report(P.status, TTKV_STATUS_BLOCK_RANGE);
+                    if (t0 + o < sg.rq.seq) {
+                        #pragma unroll
+                        for (int k = 0; k < NG; ++k) km[i][k] = 0x7e00u;
+                    }
+                    continue;
+                }
+                const uint8_t* pan = P.cache + ((int64_t(blk) * P.H + sg.h) * (P.block_size / kPanelTokens) +
+                                                (t0 - bi * P.block_size) / kPanelTokens) * PANEL;
+                load_words(pan + o * (D / 2) + a * (D / 8), kw[i]);
+                if (t0 + o < sg.rq.seq) load_words(pan + k_meta_offset(D) + o * NG * 4, km[i]);
+            }
+        };
+        load();
+        uint32_t n_tile = 0;
+        while (sg.u < sg.ue) {
+            const int st = n_tile & 1;
+            wait(&B.kempty[st], (n_tile >> 1) + 1);
+            unsigned char* kb = smem + S::off_k + st * S::K;
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 32 * i + 8 * wk + lt;
+                #pragma unroll
+                for (int k = 0; k < NW; ++k) {
+                    const uint32_t meta = km[i][k / WPG], v = kw[i][k];
+                    const __half2 s2 = u2h(__byte_perm(meta, 0, 0x1010)), m2 = u2h(__byte_perm(meta, 0, 0x3232));
+                    const int c = 4 * k + a;
+                    *reinterpret_cast<uint4*>(kb + (c >> 3) * S::KATOM + kmajor_off(row, c & 7)) =
+                        make_uint4(h2u(__hfma2(codes2<false>(v), s2, m2)), h2u(__hfma2(codes2<true>(v), s2, m2)),
+                                   h2u(__hfma2(codes2<false>(v >> 8), s2, m2)), h2u(__hfma2(codes2<true>(v >> 8), s2, m2)));
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(&B.kfull[st]);
+            ++n_tile;
+            sg.skip(P, 1);
+            if (sg.u < sg.ue) load();
+        }
+    } else if (w < 16) {
+        // ============================================================== V of a tile, lanes by tokens
+        // a thread's words: group j of lanes, b of its quads, pairs of tokens 4 hh .. + 4 of a panel
+        constexpr int HP = D == 128 ? 1 : 2, TASKS = 4 / HP;  // half panels a warp takes at once
+        const int wv = w - 12, b = lane & 7, j = D == 128 ? lane >> 3 : (lane >> 3) & 1;
+        const int hsel = D == 128 ? 0 : lane >> 4;
+        uint32_t vw[TASKS][4], vm[TASKS][8];
+        auto load = [&]() {
+            #pragma unroll
+            for (int i = 0; i < TASKS; ++i) {
+                const int hp = 4 * (HP * i + hsel) + wv;      // half panel 0 .. 15 of the tile
+                const int t0 = sg.ui * TN + 16 * (hp >> 1), hh = hp & 1;
+                #pragma unroll
+                for (int k = 0; k < 4; ++k) vw[i][k] = 0u;
+                #pragma unroll
+                for (int k = 0; k < 8; ++k) vm[i][k] = 0u;
+                if (t0 >= sg.rq.seq) continue;
+                const int bi = t0 / P.block_size;
+                const int blk = __ldg(P.block_table + int64_t(sg.r) * P.bt_stride + bi);
+                if (blk < 0 || blk >= P.n_blocks) continue;   // (reported, and made NaN, with K)
+                const uint8_t* pan = P.cache + ((int64_t(blk) * P.H + sg.h) * (P.block_size / kPanelTokens) +
+                                                (t0 - bi * P.block_size) / kPanelTokens) * PANEL;
+                #pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    vw[i][k] = *reinterpret_cast<const uint32_t*>(pan + 8 * D + (4 * hh + k) * D + b * (D / 8) + 4 * j);
+                #pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (t0 + 8 * hh + k < sg.rq.seq)
+                        vm[i][k] = *reinterpret_cast<const uint32_t*>(pan + v_meta_offset(D, GRP) +
+                                                                      ((8 * hh + k) * NG + j / WPG) * 4);
+            }
+        };
+        load();
+        uint32_t n_tile = 0;
+        while (sg.u < sg.ue) {
+            const int st = n_tile & 1;
+            wait(&B.vempty[st], (n_tile >> 1) + 1);
+            // the flags of the tile four behind are read by every row that sees it (its successor's
+            // weights were written after that, and V of this tile follows them by two)
+            {
+                const int f = (n_tile + 4) & (kFlags - 1);
+                vbad[f][tid - 384] = 0;
+                if (tid == 384) any_bad[f] = 0;
+            }
+            unsigned char* vb = smem + S::off_v + st * S::V;
+            #pragma unroll
+            for (int i = 0; i < TASKS; ++i) {
+                const int hp = 4 * (HP * i + hsel) + wv;
+                uint32_t out[4][4];                           // [lane of the quad][pair of tokens]
+                #pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t ma = vm[i][2 * k], mb = vm[i][2 * k + 1];
+                    // a NaN scale counts as nothing here: a weight of 0 must not spread it. The rows that
+                    // see its token are told by flags
+                    if (((ma & 0x7fffu) > 0x7c00u) || ((mb & 0x7fffu) > 0x7c00u)) {
+                        const int f = n_tile & (kFlags - 1);
+                        #pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t& mx = e ? mb : ma;
+                            if ((mx & 0x7fffu) <= 0x7c00u) continue;
+                            mx = 0u;
+                            const int tok = 8 * hp + 2 * k + e;
+                            atomicOr(reinterpret_cast<unsigned*>(&vbad[f][tok & ~3]), (1u << (j / WPG)) << (8 * (tok & 3)));
+                            any_bad[f] = 1;
+                        }
+                    }
+                    const __half2 s2 = u2h(__byte_perm(ma, mb, 0x5410)), m2 = u2h(__byte_perm(ma, mb, 0x7632));
+                    const uint32_t v = vw[i][k];
+                    out[0][k] = h2u(__hfma2(codes2<false>(v), s2, m2));
+                    out[1][k] = h2u(__hfma2(codes2<true>(v), s2, m2));
+                    out[2][k] = h2u(__hfma2(codes2<false>(v >> 8), s2, m2));
+                    out[3][k] = h2u(__hfma2(codes2<true>(v >> 8), s2, m2));
+                }
+                #pragma unroll
+                for (int q = 0; q < 4; ++q)                   // lane 32 j + 4 b + q is row 32 j + 8 q + b, chunk hp
+                    *reinterpret_cast<uint4*>(vb + (hp >> 3) * S::VATOM + kmajor_off(32 * j + 8 * q + b, hp & 7)) =
+                        make_uint4(out[q][0], out[q][1], out[q][2], out[q][3]);
+            }
+            fence_async_smem();
+            mbar_arrive(&B.vfull[st]);
+            ++n_tile;
+            sg.skip(P, 1);
+            if (sg.u < sg.ue) load();
+        }
+    } else if (lane == 0) {
+        // ============================================================== the products of row tile x
+        const int x = w - 16;
+        constexpr uint32_t ID_S = idesc_f16(TM, TN, false, false), ID_PV = idesc_f16(TM, D, false, false);
+        const uint64_t dq = sw128_desc(smem_u32(smem + S::off_q + x * S::Q), 16, 1024);
+        uint32_t n_tile = 0, n_pv = 0, n_q = 0;
+        while (sg.u < sg.ue) {
+            const int n = sg.here();
+            const bool active = sg.rb * CROWS + x * TM < sg.rq.ql * P.G;
+            if (active) {
+                wait(&B.qfull[x], n_q);                       // (O of the segment before is read, P consumed)
+                ++n_q;
+            }
+            for (int i = 0; i < n; ++i, ++n_tile) {
+                const int st = n_tile & 1;
+                const uint32_t ph = n_tile >> 1;
+                wait(&B.kfull[st], ph);
+                if (!active) {
+                    mbar_arrive(&B.kempty[st]);
+                    wait(&B.vfull[st], ph);
+                    mbar_arrive(&B.vempty[st]);
+                    continue;
+                }
+                if (i > 0) wait(&B.pvdone[x], n_pv - 1);      // P of the tile before is read from S's columns
+                tc_after();
+                const uint64_t dk = sw128_desc(smem_u32(smem + S::off_k + st * S::K), 16, 1024);
+                #pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t step = uint64_t(((k >> 2) * S::KATOM + (k & 3) * 32) >> 4);
+                    mma_f16(tmem + s_col(x), dq + step, dk + step, ID_S, k > 0 ? 1u : 0u);
+                }
+                mma_commit(&B.sfull[x]);
+                mma_commit(&B.kempty[st]);
+                wait(&B.vfull[st], ph);
+                wait(&B.pfull[x], n_pv);
+                tc_after();
+                const uint64_t dv = sw128_desc(smem_u32(smem + S::off_v + st * S::V), 16, 1024);
+                #pragma unroll
+                for (int k = 0; k < TN / 16; ++k) {
+                    const uint64_t step = uint64_t(((k >> 2) * S::VATOM + (k & 3) * 32) >> 4);
+                    mma_f16_ts(tmem + o_col(x), tmem + s_col(x) + 8 * k, dv + step, ID_PV, (i > 0 || k > 0) ? 1u : 0u);
+                }
+                mma_commit(&B.pvdone[x]);
+                mma_commit(&B.vempty[st]);
+                ++n_pv;
+            }
+            sg.skip(P, n);
+        }
+        // every product has ended before the tensor memory is freed (their operands are read, too)
+        if (n_pv) mbar_wait(&B.pvdone[x], (n_pv - 1) & 1u);
+    }
+    __syncwarp();
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (w == 16) tmem_dealloc(tmem_base, kTmemCols);
+}
+
+// ------------------------------------------------------------------ the merge
+// Row block begun in CTA c and cut: its parts in c and in the CTAs behind it. A CTA of the merge takes
+// 8 rows of it.
+constexpr int kMergeRows = 8;
+
+template <int D>
+__global__ void __launch_bounds__(kMergeRows * (D / 4)) q4_chunk_merge_kernel(const AttnParams P) {
+    pdl_wait();
+    const int c0 = blockIdx.x;
+    const int4 a = *reinterpret_cast<const int4*>(P.rec + 8 * c0), b = *reinterpret_cast<const int4*>(P.rec + 8 * c0 + 4);
+    if (a.x < 0) return;
+    const int r = a.x, h = a.y, rb = a.z, u0 = a.w, U = b.x, share = b.y;
+    const Req rq = request(P, r, false);
+    const int i = blockIdx.y * kMergeRows + threadIdx.x / (D / 4), ln = 4 * (threadIdx.x % (D / 4));
+    const int row = rb * CROWS + i;
+    if (row >= rq.ql * P.G) return;
+    const int c1 = (u0 + U - 1) / share;
+    auto place = [&](int c) { return (int64_t(c) * 2 + (c * share >= u0 ? 0 : 1)) * CROWS + i; };
+    float M = -INFINITY;
+    for (int c = c0; c <= c1; ++c) M = fmaxf(M, P.part_ml[2 * place(c)]);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    #pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+        const int64_t s = place(c);
+        const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * s);
+        const float4 v = *reinterpret_cast<const float4*>(P.part_o + s * D + ln);
+        const float wt = part_weight(ml.x, M);
+        l = fmaf(wt, ml.y, l);
+        o.x = fmaf(wt, v.x, o.x); o.y = fmaf(wt, v.y, o.y); o.z = fmaf(wt, v.z, o.z); o.w = fmaf(wt, v.w, o.w);
+    }
+    store_out(P, rq, h, row, D, ln, o, l);
+}
+
+template <int D, int GRP>
+int launch_chunk(const AttnParams& P, cudaStream_t st) {
+    auto k = q4_chunk_kernel<D, GRP>;
+    if (int e = raise_smem_limit(reinterpret_cast<const void*>(k), "q4_chunk_kernel")) return e;
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(P.n_ctas));
+    cfg.blockDim = dim3(kChunkThreads);
+    cfg.dynamicSmemBytes = ChunkSmem<D>::BYTES;
+    cfg.stream = st;
+    cfg.attrs = pdl;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, k, P);
+    if (e != cudaSuccess) { cudaGetLastError(); return fail(TTKV_ERR_CUDA, "q4_chunk_kernel: %s", cudaGetErrorString(e)); }
+    cfg.gridDim = dim3(unsigned(P.n_ctas), CROWS / kMergeRows);
+    cfg.blockDim = dim3(kMergeRows * (D / 4));
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, q4_chunk_merge_kernel<D>, P);
+    if (e != cudaSuccess) { cudaGetLastError(); return fail(TTKV_ERR_CUDA, "q4_chunk_merge_kernel: %s", cudaGetErrorString(e)); }
+    return TTKV_OK;
+}
+
+}  // namespace
+
+namespace q4 {
+
+size_t chunk_workspace_bytes(int d) {
+    return size_t(kMaxCtas) * (8 * sizeof(int32_t) + 2 * CROWS * size_t(d + 2) * sizeof(float));
+}
+
+int run_chunk(const ttkv_q4_cache_t* c, AttnParams P, void* ws, size_t ws_bytes, cudaStream_t st) {
+    if (!ws || ws_bytes < chunk_workspace_bytes(c->d))
+        return fail(TTKV_ERR_WORKSPACE, "4-bit prefill: workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0,
+                    chunk_workspace_bytes(c->d));
+    if (reinterpret_cast<uintptr_t>(ws) & 15) return fail(TTKV_ERR_ALIGN, "4-bit read: workspace not 16-byte aligned");
+    int sms = 0;
+    if (int e = sm_count(&sms)) return e;
+    P.n_ctas = std::min(sms, kMaxCtas);
+    P.rec = static_cast<int32_t*>(ws);
+    P.part_ml = reinterpret_cast<float*>(P.rec + 8 * kMaxCtas);
+    P.part_o = P.part_ml + size_t(kMaxCtas) * 2 * CROWS * 2;
+#define TTKV_Q4_CHUNK(D, GRP) if (c->d == D && c->group == GRP) return launch_chunk<D, GRP>(P, st);
+    TTKV_Q4_CHUNK(64, 32) TTKV_Q4_CHUNK(64, 64) TTKV_Q4_CHUNK(128, 32) TTKV_Q4_CHUNK(128, 64) TTKV_Q4_CHUNK(128, 128)
+#undef TTKV_Q4_CHUNK
+    return fail(TTKV_ERR_UNSUPPORTED, "4-bit read: geometry");
+}
+
+}  // namespace q4
+}  // namespace ttkv

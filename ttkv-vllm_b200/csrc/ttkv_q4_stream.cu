@@ -18,73 +18,16 @@
 // the rounding error is that of weights on centred values: 2^-12 of each term at most.
 #include <algorithm>
 
-#include "ttkv_async.cuh"
-#include "ttkv_q4.cuh"
+#include "ttkv_q4_attn.cuh"
 
 namespace ttkv {
 namespace {
 
 using namespace q4;
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kUnit = 64;                   // tokens of a unit of work: one softmax step of a warp
 
-struct AttnParams {
-    const uint8_t* cache;
-    int64_t n_blocks;
-    int32_t H, G, block_size;
-    const int32_t* block_table;
-    int64_t bt_stride;
-    int32_t bt_cols;
-    const int32_t* seq_lens;
-    const int32_t* q_start;                 // null: one query per request
-    const int32_t* q_len;
-    int32_t n_reqs, n_rows, max_q, max_seq;
-    const void* q;
-    int32_t dtype, q_vec, out_vec;
-    int64_t q_stride;
-    float scale;
-    void* out;
-    int64_t out_stride;
-    int32_t n_ctas;
-    int32_t* prefix;                        // [n_reqs + 1] units before each request (workspace)
-    float* part_ml;                         // [n_ctas][2][rows][2]
-    float* part_o;                          // [n_ctas][2][rows][D]
-    float* first;                           // [n_ctas][warps] parts of the warps' first segments
-    int32_t* status;
-};
-
-// ------------------------------------------------------------------ the batch
-// A request's tokens, queries and rows (query, head of the group), or n = 0 where it is refused.
-struct Req {
-    int seq, ql, q0;
-    bool refused;
-};
-
-__device__ __forceinline__ Req request(const AttnParams& P, int r, bool tell) {
-    Req a;
-    a.seq = max(P.seq_lens[r], 0);
-    a.ql = P.q_len ? P.q_len[r] : 1;
-    a.q0 = P.q_start ? P.q_start[r] : r;
-    a.refused = false;
-    int code = 0;
-    if (P.q_len && a.ql > 0 &&
-        (a.ql > a.seq || a.ql > P.max_q || a.q0 < 0 || int64_t(a.q0) + a.ql > P.n_rows)) code = TTKV_STATUS_QUERY;
-    else if (P.max_seq > 0 && a.seq > P.max_seq && a.ql > 0) code = TTKV_STATUS_SEQ_BOUND;
-    else if (a.seq > int64_t(P.bt_cols) * P.block_size && a.ql > 0) code = TTKV_STATUS_ROW_SHORT;
-    if (code) {
-        a.refused = true;
-        if (tell) report(P.status, code);
-    }
-    if (a.refused || a.ql < 0) a.ql = 0;
-    return a;
-}
-
-__device__ __forceinline__ int row_blocks(const Req& a, int G, int rows) { return int((unsigned(a.ql) * unsigned(G) + rows - 1) / rows); }
 __device__ __forceinline__ int units_of(const Req& a) { return a.ql > 0 ? (a.seq + kUnit - 1) / kUnit : 0; }
-
-// The list of T units shared out to n CTAs: CTA c owns [c S, (c + 1) S), S = ceil(T / n), cut at T.
-__device__ __forceinline__ int share_size(int T, int n) { return (T + n - 1) / n; }
 
 // ------------------------------------------------------------------ warp-level products
 // D += A (16 x 16, row) . B (16 x 8, column), fp16 operands and fp32 sums.
@@ -100,30 +43,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
-    if constexpr (N == 4) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else if constexpr (N == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[0] = u.x; w[1] = u.y;
-    } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
 }
 
 // ------------------------------------------------------------------ one warp's rows
@@ -447,32 +366,6 @@ struct WarpRows {
                     o[i][nt][k] = fmaf(o[i][nt][k], k < 2 ? 16777216.f : 1048576.f, dsum[nt][k & 1][i / 2 / WPG]) * back;
     }
 };
-
-// ------------------------------------------------------------------ partial results
-// Weighted sum of partials (max m_i, sum l_i, rows o_i relative to m_i): relative to M = max m_i.
-__device__ __forceinline__ float part_weight(float m, float M) { return M == -INFINITY ? 1.f : ex2(m - M); }
-
-// Lanes ln .. + 4 of row i of a part of `rows` rows.
-__device__ __forceinline__ void put_part(float* part, int rows, int D, int i, int ln, float4 o, float m, float l) {
-    *reinterpret_cast<float4*>(part + i * D + ln) = o;
-    if (ln == 0) *reinterpret_cast<float2*>(part + rows * D + 2 * i) = make_float2(m, l);
-}
-
-// Four output values o / l from lane index `lane` (a multiple of 4) of row (query j, head g of h).
-__device__ __forceinline__ void store_out(const AttnParams& P, const Req& rq, int h, int row, int D, int lane, float4 o,
-                                          float l) {
-    const int j = row / P.G, g = row - j * P.G;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int64_t i = int64_t(rq.q0 + j) * P.out_stride + int64_t(h * P.G + g) * D + lane;
-    const float x[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-    if (P.out_vec) {
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + i) =
-            make_uint2(pack2(x[0], x[1], P.dtype), pack2(x[2], x[3], P.dtype));
-    } else {
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) store_elt(P.out, P.dtype, i + k, x[k]);
-    }
-}
 
 // ------------------------------------------------------------------ the streaming kernel
 // The work is the list of (request, KV head, row block, 64-token unit), shared out evenly: CTA c of
@@ -816,17 +709,6 @@ __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParam
 }
 
 // ------------------------------------------------------------------ host
-int sm_count(int* n) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-        cudaGetLastError();
-        return fail(TTKV_ERR_CUDA, "no CUDA device");
-    }
-    return TTKV_OK;
-}
-
-constexpr int kMaxStreamCtas = 148;              // one per SM of a B200; the workspace is sized for it
 
 // Rows a streaming warp takes at once: 8 (query, head) rows a fragment, two fragments above that.
 int stream_nt(int64_t rows) { return rows > 8 ? 2 : 1; }
@@ -838,11 +720,11 @@ struct StreamWs {
 
 StreamWs stream_ws(int d, int n_reqs, int nt) {
     StreamWs w;
-    const size_t rows = size_t(kMaxStreamCtas) * 2 * 8 * nt;
+    const size_t rows = size_t(kMaxCtas) * 2 * 8 * nt;
     w.part_o = ((size_t(n_reqs) + 1) * 4 + 15) / 16 * 16;
     w.part_ml = w.part_o + rows * d * sizeof(float);
     w.first = w.part_ml + rows * 2 * sizeof(float);
-    w.bytes = w.first + size_t(kMaxStreamCtas) * 12 * 8 * nt * (d + 2) * sizeof(float);
+    w.bytes = w.first + size_t(kMaxCtas) * 12 * 8 * nt * (d + 2) * sizeof(float);
     return w;
 }
 
@@ -896,7 +778,7 @@ int run_stream(const ttkv_q4_cache_t* c, AttnParams P, void* ws, size_t ws_bytes
     if (reinterpret_cast<uintptr_t>(ws) & 15) return fail(TTKV_ERR_ALIGN, "4-bit read: workspace not 16-byte aligned");
     int sms = 0;
     if (int e = sm_count(&sms)) return e;
-    P.n_ctas = std::min(sms, kMaxStreamCtas);
+    P.n_ctas = std::min(sms, kMaxCtas);
     char* base = static_cast<char*>(ws);
     P.prefix = reinterpret_cast<int32_t*>(base);
     P.part_o = reinterpret_cast<float*>(base + w.part_o);
@@ -943,10 +825,15 @@ extern "C" int ttkv_q4_decode(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_
     return run_stream(cache, P, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
+// Chunks of at most this many (query, head) rows a KV head are streamed, the cache read once per 16 of
+// them; above it the chunk kernel's tiles are fuller.
+constexpr int kStreamRows = 32;
+
 extern "C" size_t ttkv_q4_prefill_workspace_bytes(const ttkv_q4_cache_t* cache, int32_t n_reqs, int32_t HQ,
                                                   int32_t max_q_len, int32_t max_seq_len) {
     if (!cache || cache->H < 1 || HQ < cache->H || n_reqs < 0 || max_q_len < 0) return 0;
-    return stream_ws(cache->d, n_reqs, stream_nt(int64_t(max_q_len) * (HQ / cache->H))).bytes;
+    const int64_t rows = int64_t(max_q_len) * (HQ / cache->H);
+    return rows > kStreamRows ? chunk_workspace_bytes(cache->d) : stream_ws(cache->d, n_reqs, stream_nt(rows)).bytes;
 }
 
 extern "C" int ttkv_q4_prefill(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch, const int32_t* q_start,
@@ -961,5 +848,7 @@ extern "C" int ttkv_q4_prefill(const ttkv_q4_cache_t* cache, const ttkv_q4_batch
     if (int64_t(max_q_len) * HQ > 0x7fffffff) return fail(TTKV_ERR_UNSUPPORTED, "4-bit prefill: %d queries of %d heads", max_q_len, HQ);
     AttnParams P = attn_params(cache, batch, q, q_dtype, q_stride, HQ, scale, out, out_stride, status);
     P.q_start = q_start; P.q_len = q_len; P.n_rows = n_rows; P.max_q = max_q_len; P.max_seq = std::max(max_seq_len, 1);
-    return run_stream(cache, P, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return int64_t(max_q_len) * P.G > kStreamRows ? run_chunk(cache, P, workspace, workspace_bytes, st)
+                                                  : run_stream(cache, P, workspace, workspace_bytes, st);
 }
