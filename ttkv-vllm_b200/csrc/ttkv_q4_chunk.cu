@@ -119,6 +119,20 @@ __device__ __forceinline__ __half2 codes2(uint32_t w) {
     return __hsub2(u2h((w & 0x000f000fu) | 0x64006400u), u2h(0x64006400u));
 }
 
+// The panels of a stored tile, one each in lanes 0 to 7: index in the cache, or that there is none or
+// that its block id is outside the cache.
+constexpr int kNoPanel = -1, kBadPanel = -2;
+
+__device__ __forceinline__ int panels_of(const AttnParams& P, int r, int h, int tile, int seq, int lane) {
+    const int t = tile * TN + 16 * lane;
+    if (lane >= 8 || t >= seq) return kNoPanel;
+    const int bi = t / P.block_size;
+    const int blk = __ldg(P.block_table + int64_t(r) * P.bt_stride + bi);
+    if (blk < 0 || blk >= P.n_blocks) return kBadPanel;
+    // (an index of panels: the memory of a GPU holds fewer than 2^31)
+    return int((int64_t(blk) * P.H + h) * (P.block_size / kPanelTokens)) + (t - bi * P.block_size) / kPanelTokens;
+}
+
 template <int D, int GRP>
 __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnParams P) {
     using S = ChunkSmem<D>;
@@ -285,18 +299,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 if (i > 0) note_bad(i - 1, int(n_tile) - 1);
                 const int seen = lim - t0;                    // tokens of the tile that the row sees
                 const bool full = __all_sync(0xffffffffu, seen >= TN);
+                // (the loops over columns stay rolled: four roles share the instruction cache)
                 float mt = -INFINITY;
-                #pragma unroll
+                #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     float s[32];
                     tmem_ld32(lane_base + s_col(x) + 32 * c, s);
                     tmem_wait_ld();
+                    const int vis = full ? 32 : seen - 32 * c;
                     if (full) {
                         #pragma unroll
                         for (int k = 0; k < 32; ++k) mt = fmaxf(mt, s[k]);
                     } else {
                         #pragma unroll
-                        for (int k = 0; k < 32; ++k) mt = fmaxf(mt, 32 * c + k < seen ? s[k] : -INFINITY);
+                        for (int k = 0; k < 32; ++k) mt = fmaxf(mt, k < vis ? s[k] : -INFINITY);
                     }
                 }
                 mt *= qf;
@@ -307,7 +323,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     l *= corr;
                 }
                 if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-                    #pragma unroll
+                    #pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
                         float o[32];
                         tmem_ld32(lane_base + o_col(x) + 32 * c, o);
@@ -319,24 +335,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 }
                 const float mm = m == -INFINITY ? 0.f : m;    // a row that sees nothing yet has weights of 0
                 float2 ls = make_float2(0.f, 0.f);
-                #pragma unroll
+                #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     float s[32];
                     tmem_ld32(lane_base + s_col(x) + 32 * c, s);
                     tmem_wait_ld();
+                    #pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 a = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), make_float2(qf, qf), make_float2(-mm, -mm));
+                        s[2 * k] = a.x;
+                        s[2 * k + 1] = a.y;
+                    }
                     if (!full) {
+                        const int vis = seen - 32 * c;
                         #pragma unroll
-                        for (int k = 0; k < 32; ++k) s[k] = 32 * c + k < seen ? s[k] : -INFINITY;
+                        for (int k = 0; k < 32; ++k) s[k] = k < vis ? s[k] : -INFINITY;
                     }
                     uint32_t p[16];
                     #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float2 a = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), make_float2(qf, qf), make_float2(-mm, -mm));
-                        float2 e = make_float2(ex2(a.x), ex2(a.y));
-                        if (!full) {                          // (-inf * 0 of an all-zero query is NaN)
-                            if (32 * c + 2 * k >= seen) e.x = 0.f;
-                            if (32 * c + 2 * k + 1 >= seen) e.y = 0.f;
-                        }
+                        const float2 e = make_float2(ex2(s[2 * k]), ex2(s[2 * k + 1]));
                         ls = __fadd2_rn(ls, e);
                         p[k] = half2_bits(e.x, e.y);
                     }
@@ -385,56 +403,68 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
     } else if (w < 12) {
         // ============================================================== K of a tile as fp16 rows
         const int wk = w - 8, lt = lane & 7, a = lane >> 3;   // token of 8 and chunk of its row
-        uint32_t kw[4][NW], km[4][NG];
-        auto load = [&]() {                                   // tile sg.ui: 8-token groups 4 i + wk
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t0 = sg.ui * TN + 32 * i + 16 * (wk >> 1), o = 8 * (wk & 1) + lt;
-                #pragma unroll
-                for (int k = 0; k < NW; ++k) kw[i][k] = 0u;
-                #pragma unroll
-                for (int k = 0; k < NG; ++k) km[i][k] = 0u;
-                if (t0 >= sg.rq.seq) continue;
-                const int bi = t0 / P.block_size;
-                const int blk = __ldg(P.block_table + int64_t(sg.r) * P.bt_stride + bi);
-                if (blk < 0 || blk >= P.n_blocks) {           // NaN keys: so are the rows that see them
-                    if (lane == 0) report(P.status, TTKV_STATUS_BLOCK_RANGE);
-                    if (t0 + o < sg.rq.seq) {
-                        #pragma unroll
-                        for (int k = 0; k < NG; ++k) km[i][k] = 0x7e00u;
-                    }
-                    continue;
-                }
-                const uint8_t* pan = P.cache + ((int64_t(blk) * P.H + sg.h) * (P.block_size / kPanelTokens) +
-                                                (t0 - bi * P.block_size) / kPanelTokens) * PANEL;
-                load_words(pan + o * (D / 2) + a * (D / 8), kw[i]);
-                if (t0 + o < sg.rq.seq) load_words(pan + k_meta_offset(D) + o * NG * 4, km[i]);
-            }
-        };
-        load();
+        const int o = 8 * (wk & 1) + lt;                      // 8-token groups 4 i + wk: this token of panel 2 i + wk / 2
         uint32_t n_tile = 0;
         while (sg.u < sg.ue) {
-            const int st = n_tile & 1;
-            wait(&B.kempty[st], (n_tile >> 1) + 1);
-            unsigned char* kb = smem + S::off_k + st * S::K;
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 32 * i + 8 * wk + lt;
+            const int n = sg.here(), first = sg.ui, seq = sg.rq.seq, h = sg.h, r = sg.r;
+            sg.skip(P, n);
+            uint32_t kw[4][NW], km[4][NG], nw[4][NW], nm[4][NG];
+            int ids = panels_of(P, r, h, first, seq, lane);
+            auto load = [&](int tile) {
                 #pragma unroll
-                for (int k = 0; k < NW; ++k) {
-                    const uint32_t meta = km[i][k / WPG], v = kw[i][k];
-                    const __half2 s2 = u2h(__byte_perm(meta, 0, 0x1010)), m2 = u2h(__byte_perm(meta, 0, 0x3232));
-                    const int c = 4 * k + a;
-                    *reinterpret_cast<uint4*>(kb + (c >> 3) * S::KATOM + kmajor_off(row, c & 7)) =
-                        make_uint4(h2u(__hfma2(codes2<false>(v), s2, m2)), h2u(__hfma2(codes2<true>(v), s2, m2)),
-                                   h2u(__hfma2(codes2<false>(v >> 8), s2, m2)), h2u(__hfma2(codes2<true>(v >> 8), s2, m2)));
+                for (int i = 0; i < 4; ++i) {
+                    const int p = 2 * i + (wk >> 1), t = tile * TN + 16 * p + o;
+                    const int id = __shfl_sync(0xffffffffu, ids, p);
+                    const uint8_t* pan = P.cache + int64_t(max(id, 0)) * PANEL;
+                    #pragma unroll
+                    for (int k = 0; k < NW; ++k) nw[i][k] = 0u;
+                    #pragma unroll
+                    for (int k = 0; k < NG; ++k) nm[i][k] = id == kBadPanel ? 0x7e00u : 0u;   // NaN keys: so are the rows that see them
+                    if (id >= 0) {
+                        load_words(pan + o * (D / 2) + a * (D / 8), nw[i]);
+                        load_words(pan + k_meta_offset(D) + o * NG * 4, nm[i]);
+                    } else if (id == kBadPanel && lane == 0) {
+                        report(P.status, TTKV_STATUS_BLOCK_RANGE);
+                    }
+                    if (t >= seq) {
+                        #pragma unroll
+                        for (int k = 0; k < NG; ++k) nm[i][k] = 0u;
+                    }
                 }
+            };
+            load(first);
+            ids = panels_of(P, r, h, first + 1, seq, lane);
+            for (int it = 0; it < n; ++it, ++n_tile) {
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    #pragma unroll
+                    for (int k = 0; k < NW; ++k) kw[i][k] = nw[i][k];
+                    #pragma unroll
+                    for (int k = 0; k < NG; ++k) km[i][k] = nm[i][k];
+                }
+                if (it + 1 < n) {
+                    load(first + it + 1);
+                    ids = panels_of(P, r, h, first + it + 2, seq, lane);
+                }
+                const int st = n_tile & 1;
+                wait(&B.kempty[st], (n_tile >> 1) + 1);
+                unsigned char* kb = smem + S::off_k + st * S::K;
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = 32 * i + 8 * wk + lt;
+                    #pragma unroll
+                    for (int k = 0; k < NW; ++k) {
+                        const uint32_t meta = km[i][k / WPG], v = kw[i][k];
+                        const __half2 s2 = u2h(__byte_perm(meta, 0, 0x1010)), m2 = u2h(__byte_perm(meta, 0, 0x3232));
+                        const int c = 4 * k + a;
+                        *reinterpret_cast<uint4*>(kb + (c >> 3) * S::KATOM + kmajor_off(row, c & 7)) =
+                            make_uint4(h2u(__hfma2(codes2<false>(v), s2, m2)), h2u(__hfma2(codes2<true>(v), s2, m2)),
+                                       h2u(__hfma2(codes2<false>(v >> 8), s2, m2)), h2u(__hfma2(codes2<true>(v >> 8), s2, m2)));
+                    }
+                }
+                fence_async_smem();
+                mbar_arrive(&B.kfull[st]);
             }
-            fence_async_smem();
-            mbar_arrive(&B.kfull[st]);
-            ++n_tile;
-            sg.skip(P, 1);
-            if (sg.u < sg.ue) load();
         }
     } else if (w < 16) {
         // ============================================================== V of a tile, lanes by tokens
@@ -442,83 +472,93 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         constexpr int HP = D == 128 ? 1 : 2, TASKS = 4 / HP;  // half panels a warp takes at once
         const int wv = w - 12, b = lane & 7, j = D == 128 ? lane >> 3 : (lane >> 3) & 1;
         const int hsel = D == 128 ? 0 : lane >> 4;
-        uint32_t vw[TASKS][4], vm[TASKS][8];
-        auto load = [&]() {
-            #pragma unroll
-            for (int i = 0; i < TASKS; ++i) {
-                const int hp = 4 * (HP * i + hsel) + wv;      // half panel 0 .. 15 of the tile
-                const int t0 = sg.ui * TN + 16 * (hp >> 1), hh = hp & 1;
-                #pragma unroll
-                for (int k = 0; k < 4; ++k) vw[i][k] = 0u;
-                #pragma unroll
-                for (int k = 0; k < 8; ++k) vm[i][k] = 0u;
-                if (t0 >= sg.rq.seq) continue;
-                const int bi = t0 / P.block_size;
-                const int blk = __ldg(P.block_table + int64_t(sg.r) * P.bt_stride + bi);
-                if (blk < 0 || blk >= P.n_blocks) continue;   // (reported, and made NaN, with K)
-                const uint8_t* pan = P.cache + ((int64_t(blk) * P.H + sg.h) * (P.block_size / kPanelTokens) +
-                                                (t0 - bi * P.block_size) / kPanelTokens) * PANEL;
-                #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    vw[i][k] = *reinterpret_cast<const uint32_t*>(pan + 8 * D + (4 * hh + k) * D + b * (D / 8) + 4 * j);
-                #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (t0 + 8 * hh + k < sg.rq.seq)
-                        vm[i][k] = *reinterpret_cast<const uint32_t*>(pan + v_meta_offset(D, GRP) +
-                                                                      ((8 * hh + k) * NG + j / WPG) * 4);
-            }
-        };
-        load();
         uint32_t n_tile = 0;
         while (sg.u < sg.ue) {
-            const int st = n_tile & 1;
-            wait(&B.vempty[st], (n_tile >> 1) + 1);
-            // the flags of the tile four behind are read by every row that sees it (its successor's
-            // weights were written after that, and V of this tile follows them by two)
-            {
-                const int f = (n_tile + 4) & (kFlags - 1);
-                vbad[f][tid - 384] = 0;
-                if (tid == 384) any_bad[f] = 0;
-            }
-            unsigned char* vb = smem + S::off_v + st * S::V;
-            #pragma unroll
-            for (int i = 0; i < TASKS; ++i) {
-                const int hp = 4 * (HP * i + hsel) + wv;
-                uint32_t out[4][4];                           // [lane of the quad][pair of tokens]
+            const int n = sg.here(), first = sg.ui, seq = sg.rq.seq, h = sg.h, r = sg.r;
+            sg.skip(P, n);
+            // the scale and minimum of token 8 hp + b for group j, each lane one; the others by shuffles
+            uint32_t vw[TASKS][4], vm[TASKS], nw[TASKS][4], nm[TASKS];
+            int ids = panels_of(P, r, h, first, seq, lane);
+            auto load = [&](int tile) {
                 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint32_t ma = vm[i][2 * k], mb = vm[i][2 * k + 1];
-                    // a NaN scale counts as nothing here: a weight of 0 must not spread it. The rows that
-                    // see its token are told by flags
-                    if (((ma & 0x7fffu) > 0x7c00u) || ((mb & 0x7fffu) > 0x7c00u)) {
-                        const int f = n_tile & (kFlags - 1);
+                for (int i = 0; i < TASKS; ++i) {
+                    const int hp = 4 * (HP * i + hsel) + wv, hh = hp & 1;      // half panel 0 .. 15 of the tile
+                    const int id = __shfl_sync(0xffffffffu, ids, hp >> 1);
+                    const uint8_t* pan = P.cache + int64_t(max(id, 0)) * PANEL;
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) nw[i][k] = 0u;
+                    nm[i] = 0u;
+                    if (id >= 0) {                            // (a bad block is reported, and made NaN, with K)
                         #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            uint32_t& mx = e ? mb : ma;
-                            if ((mx & 0x7fffu) <= 0x7c00u) continue;
-                            mx = 0u;
-                            const int tok = 8 * hp + 2 * k + e;
+                        for (int k = 0; k < 4; ++k)
+                            nw[i][k] = *reinterpret_cast<const uint32_t*>(pan + 8 * D + (4 * hh + k) * D + b * (D / 8) + 4 * j);
+                        if (tile * TN + 8 * hp + b < seq)
+                            nm[i] = *reinterpret_cast<const uint32_t*>(pan + v_meta_offset(D, GRP) + ((8 * hh + b) * NG + j / WPG) * 4);
+                    }
+                }
+            };
+            load(first);
+            ids = panels_of(P, r, h, first + 1, seq, lane);
+            for (int it = 0; it < n; ++it, ++n_tile) {
+                bool nan = false;
+                #pragma unroll
+                for (int i = 0; i < TASKS; ++i) {
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) vw[i][k] = nw[i][k];
+                    vm[i] = nm[i];
+                    nan |= (vm[i] & 0x7fffu) > 0x7c00u;
+                }
+                if (it + 1 < n) {
+                    load(first + it + 1);
+                    ids = panels_of(P, r, h, first + it + 2, seq, lane);
+                }
+                const int st = n_tile & 1;
+                wait(&B.vempty[st], (n_tile >> 1) + 1);
+                // the flags of the tile four behind are read by every row that sees it (its successor's
+                // weights were written after that, and V of this tile follows them by two)
+                {
+                    const int f = (n_tile + 4) & (kFlags - 1);
+                    vbad[f][tid - 384] = 0;
+                    if (tid == 384) any_bad[f] = 0;
+                }
+                // a NaN scale counts as nothing here: a weight of 0 must not spread it. The rows that see
+                // its token are told by flags
+                if (__any_sync(0xffffffffu, nan)) {
+                    const int f = n_tile & (kFlags - 1);
+                    #pragma unroll
+                    for (int i = 0; i < TASKS; ++i) {
+                        if ((vm[i] & 0x7fffu) > 0x7c00u) {
+                            const int tok = 8 * (4 * (HP * i + hsel) + wv) + b;
+                            vm[i] = 0u;
                             atomicOr(reinterpret_cast<unsigned*>(&vbad[f][tok & ~3]), (1u << (j / WPG)) << (8 * (tok & 3)));
                             any_bad[f] = 1;
                         }
                     }
-                    const __half2 s2 = u2h(__byte_perm(ma, mb, 0x5410)), m2 = u2h(__byte_perm(ma, mb, 0x7632));
-                    const uint32_t v = vw[i][k];
-                    out[0][k] = h2u(__hfma2(codes2<false>(v), s2, m2));
-                    out[1][k] = h2u(__hfma2(codes2<true>(v), s2, m2));
-                    out[2][k] = h2u(__hfma2(codes2<false>(v >> 8), s2, m2));
-                    out[3][k] = h2u(__hfma2(codes2<true>(v >> 8), s2, m2));
                 }
+                unsigned char* vb = smem + S::off_v + st * S::V;
                 #pragma unroll
-                for (int q = 0; q < 4; ++q)                   // lane 32 j + 4 b + q is row 32 j + 8 q + b, chunk hp
-                    *reinterpret_cast<uint4*>(vb + (hp >> 3) * S::VATOM + kmajor_off(32 * j + 8 * q + b, hp & 7)) =
-                        make_uint4(out[q][0], out[q][1], out[q][2], out[q][3]);
+                for (int i = 0; i < TASKS; ++i) {
+                    const int hp = 4 * (HP * i + hsel) + wv;
+                    uint32_t out[4][4];                       // [lane of the quad][pair of tokens]
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t ma = __shfl_sync(0xffffffffu, vm[i], (lane & 24) + 2 * k);
+                        const uint32_t mb = __shfl_sync(0xffffffffu, vm[i], (lane & 24) + 2 * k + 1);
+                        const __half2 s2 = u2h(__byte_perm(ma, mb, 0x5410)), m2 = u2h(__byte_perm(ma, mb, 0x7632));
+                        const uint32_t v = vw[i][k];
+                        out[0][k] = h2u(__hfma2(codes2<false>(v), s2, m2));
+                        out[1][k] = h2u(__hfma2(codes2<true>(v), s2, m2));
+                        out[2][k] = h2u(__hfma2(codes2<false>(v >> 8), s2, m2));
+                        out[3][k] = h2u(__hfma2(codes2<true>(v >> 8), s2, m2));
+                    }
+                    #pragma unroll
+                    for (int q = 0; q < 4; ++q)               // lane 32 j + 4 b + q is row 32 j + 8 q + b, chunk hp
+                        *reinterpret_cast<uint4*>(vb + (hp >> 3) * S::VATOM + kmajor_off(32 * j + 8 * q + b, hp & 7)) =
+                            make_uint4(out[q][0], out[q][1], out[q][2], out[q][3]);
+                }
+                fence_async_smem();
+                mbar_arrive(&B.vfull[st]);
             }
-            fence_async_smem();
-            mbar_arrive(&B.vfull[st]);
-            ++n_tile;
-            sg.skip(P, 1);
-            if (sg.u < sg.ue) load();
         }
     } else if (lane == 0) {
         // ============================================================== the products of row tile x
