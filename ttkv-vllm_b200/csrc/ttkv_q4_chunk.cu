@@ -12,10 +12,11 @@
 //
 // Roles: two softmax warpgroups (a thread owns a row, i.e. a lane of tensor memory), a warpgroup that
 // dequantises K and one for V, two warps that issue the products, one per row tile. Operands are
-// double-buffered in shared memory in the 128-byte-swizzled K-major layout of the MMA; S is followed
-// by P in the same tensor-memory columns. The stored order of the codes needs no transposition: a K
-// word is a 16-byte chunk of its token's row (the dims of a chunk in the order 0 4 1 5 2 6 3 7, which
-// Q repeats), and four V words are chunks of eight tokens of four lanes.
+// double-buffered in shared memory in the 128-byte-swizzled K-major layout of the MMA. Scores are made
+// 64 tokens at a time into two buffers in turn, so the next half's product runs under this half's
+// softmax, whose P replaces the scores in place. The stored order of the codes needs no transposition:
+// a K word is a 16-byte chunk of its token's row (the dims of a chunk in the order 0 4 1 5 2 6 3 7,
+// which Q repeats), and four V words are chunks of eight tokens of four lanes.
 //
 // The work list is (request, KV head, row block, stored tile up to the block's causal limit), shared
 // out evenly to one CTA per SM as in the streaming kernel; the parts that a share's borders cut go
@@ -32,12 +33,17 @@ using namespace umma;
 constexpr int TN = 128;                      // stored tokens of a tile
 constexpr int TM = 128;                      // rows of a tile
 constexpr int CROWS = 2 * TM;                // rows of a block
-constexpr int kChunkThreads = 18 * 32;       // softmax 8 warps, K 4, V 4, products 2
-constexpr uint32_t kTmemCols = 512;          // S0, S1, O0, O1 at 128 columns each
+constexpr int TH = TN / 2;                   // tokens of a half, the step of the softmax
+constexpr int kChunkThreads = 20 * 32;       // softmax 8 warps, K 4, V 4, products 2 (of 4)
+// Registers a thread: at launch, and of each role after its own setting. A warpgroup waits in its
+// setting until the others have given theirs up, so the shares must not exceed the launch's total.
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 128, kRegsOperands = 80, kRegsProducts = 64;
+static_assert(2 * kRegsSoftmax + 2 * kRegsOperands + kRegsProducts <= 5 * kRegsLaunch, "register shares");
+constexpr uint32_t kTmemCols = 512;          // S of row tile 0 and 1, O of each, at 128 columns
 constexpr int kFlags = 8;                    // tiles whose NaN values are remembered
 
-// Row tiles' tensor memory: S (then P in its first 64 columns) and O.
-__device__ __forceinline__ uint32_t s_col(int x) { return 128u * x; }
+// Row tiles' tensor memory: S of a half in buffer y (then P in its first 32 columns) and O.
+__device__ __forceinline__ uint32_t s_col(int x, uint32_t y) { return 128u * x + 64u * y; }
 __device__ __forceinline__ uint32_t o_col(int x) { return 256u + 128u * x; }
 
 template <int D>
@@ -49,7 +55,9 @@ struct ChunkSmem {
 
 struct ChunkBars {
     uint64_t kfull[2], kempty[2], vfull[2], vempty[2];        // operand stages
-    uint64_t qfull[2], sfull[2], pfull[2], pvdone[2];         // row tiles
+    // row tiles; of halves one for each buffer: a half is waited for before the one after the next is made,
+    // so no phase is missed
+    uint64_t qfull[2], sfull[2][2], pfull[2][2], pvdone[2][2];
 };
 
 // A CTA's (or a role's) place in the work list.
@@ -156,9 +164,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             mbar_init(&B.vfull[i], 128);
             mbar_init(&B.vempty[i], 2);
             mbar_init(&B.qfull[i], 128);
-            mbar_init(&B.sfull[i], 1);
-            mbar_init(&B.pfull[i], 128);
-            mbar_init(&B.pvdone[i], 1);
+            for (int y = 0; y < 2; ++y) {
+                mbar_init(&B.sfull[i][y], 1);
+                mbar_init(&B.pfull[i][y], 128);
+                mbar_init(&B.pvdone[i][y], 1);
+            }
         }
     }
     for (int i = tid; i < kFlags * TN; i += kChunkThreads) (&vbad[0][0])[i] = 0;
@@ -218,14 +228,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         P.rec[8 * blockIdx.x] = -1;
     }
 
-    if (ca == cb) {
-        // fewer tiles than CTAs: nothing to do
-    } else if (w < 8) {
+    if (w < 8) {                                              // (fewer tiles than CTAs: nothing to do in any role)
         // ============================================================== softmax: row tile x, row t
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegsSoftmax));
         const int x = w >> 2, t = tid & 127;
         const uint32_t lane_base = tmem + (uint32_t(32 * (w & 3)) << 16);
         unsigned char* qb = smem + S::off_q + x * S::Q;
-        uint32_t n_s = 0, n_tile = 0;                         // S phases of this tile; stored tiles of the CTA
+        uint32_t n_s = 0, n_tile = 0;                         // halves of this row tile; stored tiles of the CTA
         for (; sg.u < sg.ue;) {
             const Req rq = sg.rq;
             const int n = sg.here(), begin = sg.ui, U = sg.U, h = sg.h, rb = sg.rb, r = sg.r, u0 = sg.u - sg.ui;
@@ -270,7 +279,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 // e brings the row's largest |q| into [1, 2); a negative scale's sign goes to q
                 const int e = big > 0.f && big < INFINITY ? 127 - int(__float_as_uint(big) >> 23) : 0;
                 const float up = copysignf(__uint_as_float(uint32_t(min(127 + e, 254)) << 23), P.scale);
-                qf = fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e, 1)) << 23);
+                // (not 0, which would make NaN of a masked score of -inf)
+                qf = fmaxf(fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e, 1)) << 23), 1e-38f);
                 #pragma unroll
                 for (int c = 0; c < D / 8; ++c) {
                     const float2 a = pair(raw[c].x), b = pair(raw[c].y), d = pair(raw[c].z), f = pair(raw[c].w);
@@ -285,37 +295,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
 
             float m = -INFINITY, l = 0.f;
             uint32_t bad = 0;                                 // groups of V that are NaN in a token that this row sees
-            auto note_bad = [&](int i, int k) {               // tile i of the segment, k-th of the CTA: V consumed
-                const int f = k & (kFlags - 1);
+            auto note_bad = [&](int i, uint32_t k) {          // tile i of the segment, k-th of the CTA: V consumed
+                const uint32_t f = k & (kFlags - 1);
                 if (*reinterpret_cast<volatile int*>(&any_bad[f]) == 0) return;
                 for (int c = 0; c < TN; ++c)
                     if ((begin + i) * TN + c < lim) bad |= *reinterpret_cast<volatile uint8_t*>(&vbad[f][c]);
             };
-            for (int i = 0; i < n; ++i) {
-                const int t0 = (begin + i) * TN;
-                wait(&B.sfull[x], n_s);
-                ++n_s;
+            for (int i = 0; i < 2 * n; ++i, ++n_s) {          // halves
+                const uint32_t sc = lane_base + s_col(x, n_s & 1);
+                wait(&B.sfull[x][n_s & 1], n_s >> 1);                       // (and P . V of the half before the last has ended)
                 tc_after();
-                if (i > 0) note_bad(i - 1, int(n_tile) - 1);
-                const int seen = lim - t0;                    // tokens of the tile that the row sees
-                const bool full = __all_sync(0xffffffffu, seen >= TN);
-                // (the loops over columns stay rolled: four roles share the instruction cache)
-                float mt = -INFINITY;
-                #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float s[32];
-                    tmem_ld32(lane_base + s_col(x) + 32 * c, s);
-                    tmem_wait_ld();
-                    const int vis = full ? 32 : seen - 32 * c;
-                    if (full) {
+                if (i > 0 && (i & 1) == 0) note_bad((i >> 1) - 1, n_tile + (i >> 1) - 1);
+                const int seen = lim - (begin * TN + i * TH); // tokens of the half that the row sees
+                const bool full = __all_sync(0xffffffffu, seen >= TH);
+                float s[2][32];
+                tmem_ld32(sc, s[0]);
+                tmem_ld32(sc + 32, s[1]);
+                tmem_wait_ld();
+                if (!full) {
+                    #pragma unroll
+                    for (int c = 0; c < 2; ++c)
                         #pragma unroll
-                        for (int k = 0; k < 32; ++k) mt = fmaxf(mt, s[k]);
-                    } else {
-                        #pragma unroll
-                        for (int k = 0; k < 32; ++k) mt = fmaxf(mt, k < vis ? s[k] : -INFINITY);
-                    }
+                        for (int k = 0; k < 32; ++k) s[c][k] = 32 * c + k < seen ? s[c][k] : -INFINITY;
                 }
-                mt *= qf;
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                #pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    #pragma unroll
+                    for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], s[c][k]);
+                const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * qf;
                 float corr = 1.f;
                 if (mt > m + 8.f) {                           // (m is -inf at first)
                     corr = m == -INFINITY ? 0.f : ex2(m - mt);
@@ -323,53 +331,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     l *= corr;
                 }
                 if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                    wait(&B.pvdone[x][(n_s - 1) & 1], (n_s - 1) >> 1);    // O holds every half before this one
+                    tc_after();
                     #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        float o[32];
-                        tmem_ld32(lane_base + o_col(x) + 32 * c, o);
+                    for (int c = 0; c < D / 16; ++c) {
+                        float o[16];
+                        tmem_ld16(lane_base + o_col(x) + 16 * c, o);
                         tmem_wait_ld();
+                        uint32_t v[16];
                         #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] *= corr;
-                        tmem_st32(lane_base + o_col(x) + 32 * c, o);
+                        for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(o[k] * corr);
+                        tmem_st16u(lane_base + o_col(x) + 16 * c, v);
                     }
                 }
                 const float mm = m == -INFINITY ? 0.f : m;    // a row that sees nothing yet has weights of 0
                 float2 ls = make_float2(0.f, 0.f);
-                #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float s[32];
-                    tmem_ld32(lane_base + s_col(x) + 32 * c, s);
-                    tmem_wait_ld();
-                    #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 a = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), make_float2(qf, qf), make_float2(-mm, -mm));
-                        s[2 * k] = a.x;
-                        s[2 * k + 1] = a.y;
-                    }
-                    if (!full) {
-                        const int vis = seen - 32 * c;
-                        #pragma unroll
-                        for (int k = 0; k < 32; ++k) s[k] = k < vis ? s[k] : -INFINITY;
-                    }
+                #pragma unroll
+                for (int c = 0; c < 2; ++c) {
                     uint32_t p[16];
                     #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float2 e = make_float2(ex2(s[2 * k]), ex2(s[2 * k + 1]));
+                        const float2 a = __ffma2_rn(make_float2(s[c][2 * k], s[c][2 * k + 1]), make_float2(qf, qf), make_float2(-mm, -mm));
+                        const float2 e = make_float2(ex2(a.x), ex2(a.y));
                         ls = __fadd2_rn(ls, e);
                         p[k] = half2_bits(e.x, e.y);
                     }
-                    tmem_st16u(lane_base + s_col(x) + 16 * c, p);
+                    tmem_st16u(sc + 16 * c, p);
                 }
                 l += ls.x + ls.y;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_before();
-                mbar_arrive(&B.pfull[x]);
-                ++n_tile;
+                mbar_arrive(&B.pfull[x][n_s & 1]);
             }
+            n_tile += n;
             // ---- O / l, or the parts
-            wait(&B.pvdone[x], n_s - 1);
+            wait(&B.pvdone[x][(n_s - 1) & 1], (n_s - 1) >> 1);
             tc_after();
-            note_bad(n - 1, int(n_tile) - 1);
+            note_bad(n - 1, n_tile - 1);
             const bool whole = begin == 0 && n == U;
             const int64_t pr = (int64_t(blockIdx.x) * 2 + (ca >= u0 ? 0 : 1)) * CROWS + x * TM + t;
             const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
@@ -377,7 +375,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             #pragma unroll
             for (int c = 0; c < NW; ++c) {
                 float o[32];
-                tmem_ld32(lane_base + o_col(x) + 32 * c, o);  // column 32 c + 8 i + b holds lane 32 c + 4 b + i
+                tmem_ld32(lane_base + o_col(x) + 32u * c, o); // column 32 c + 8 i + b holds lane 32 c + 4 b + i
                 tmem_wait_ld();
                 const float f = (bad >> (c / WPG)) & 1u ? __int_as_float(0x7fc00000) : inv;
                 if (live) {
@@ -402,59 +400,46 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         }
     } else if (w < 12) {
         // ============================================================== K of a tile as fp16 rows
-        const int wk = w - 8, lt = lane & 7, a = lane >> 3;   // token of 8 and chunk of its row
-        const int o = 8 * (wk & 1) + lt;                      // 8-token groups 4 i + wk: this token of panel 2 i + wk / 2
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOperands));
+        // 8-token groups 4 i + wk: lane (b token of it, a chunk of its row), i.e. token o of panel 2 i + wk / 2
+        const int wk = w - 8, b = lane & 7, a = lane >> 3, o = 8 * (wk & 1) + b;
         uint32_t n_tile = 0;
         while (sg.u < sg.ue) {
             const int n = sg.here(), first = sg.ui, seq = sg.rq.seq, h = sg.h, r = sg.r;
             sg.skip(P, n);
-            uint32_t kw[4][NW], km[4][NG], nw[4][NW], nm[4][NG];
+            uint32_t kw[4][NW], km[4][NG];
             int ids = panels_of(P, r, h, first, seq, lane);
             auto load = [&](int tile) {
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int p = 2 * i + (wk >> 1), t = tile * TN + 16 * p + o;
+                    const int p = 2 * i + (wk >> 1);
                     const int id = __shfl_sync(0xffffffffu, ids, p);
                     const uint8_t* pan = P.cache + int64_t(max(id, 0)) * PANEL;
-                    #pragma unroll
-                    for (int k = 0; k < NW; ++k) nw[i][k] = 0u;
-                    #pragma unroll
-                    for (int k = 0; k < NG; ++k) nm[i][k] = id == kBadPanel ? 0x7e00u : 0u;   // NaN keys: so are the rows that see them
                     if (id >= 0) {
-                        load_words(pan + o * (D / 2) + a * (D / 8), nw[i]);
-                        load_words(pan + k_meta_offset(D) + o * NG * 4, nm[i]);
-                    } else if (id == kBadPanel && lane == 0) {
-                        report(P.status, TTKV_STATUS_BLOCK_RANGE);
-                    }
-                    if (t >= seq) {
+                        load_words(pan + o * (D / 2) + a * (D / 8), kw[i]);
+                        load_words(pan + k_meta_offset(D) + o * NG * 4, km[i]);
+                    } else {
                         #pragma unroll
-                        for (int k = 0; k < NG; ++k) nm[i][k] = 0u;
+                        for (int k = 0; k < NW; ++k) kw[i][k] = 0u;
+                        #pragma unroll
+                        for (int k = 0; k < NG; ++k) km[i][k] = id == kBadPanel ? 0x7e00u : 0u;   // NaN keys: so are the rows that see them
+                        if (id == kBadPanel && lane == 0) report(P.status, TTKV_STATUS_BLOCK_RANGE);
                     }
                 }
             };
             load(first);
             ids = panels_of(P, r, h, first + 1, seq, lane);
             for (int it = 0; it < n; ++it, ++n_tile) {
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    #pragma unroll
-                    for (int k = 0; k < NW; ++k) kw[i][k] = nw[i][k];
-                    #pragma unroll
-                    for (int k = 0; k < NG; ++k) km[i][k] = nm[i][k];
-                }
-                if (it + 1 < n) {
-                    load(first + it + 1);
-                    ids = panels_of(P, r, h, first + it + 2, seq, lane);
-                }
                 const int st = n_tile & 1;
                 wait(&B.kempty[st], (n_tile >> 1) + 1);
                 unsigned char* kb = smem + S::off_k + st * S::K;
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int row = 32 * i + 8 * wk + lt;
+                    const int row = 32 * i + 8 * wk + b;
+                    const bool none = (first + it) * TN + row >= seq;          // behind the last token: zeros
                     #pragma unroll
                     for (int k = 0; k < NW; ++k) {
-                        const uint32_t meta = km[i][k / WPG], v = kw[i][k];
+                        const uint32_t meta = none ? 0u : km[i][k / WPG], v = kw[i][k];
                         const __half2 s2 = u2h(__byte_perm(meta, 0, 0x1010)), m2 = u2h(__byte_perm(meta, 0, 0x3232));
                         const int c = 4 * k + a;
                         *reinterpret_cast<uint4*>(kb + (c >> 3) * S::KATOM + kmajor_off(row, c & 7)) =
@@ -464,11 +449,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 }
                 fence_async_smem();
                 mbar_arrive(&B.kfull[st]);
+                if (it + 1 < n) {                             // the next tile's, and the blocks of the one behind it
+                    load(first + it + 1);
+                    ids = panels_of(P, r, h, first + it + 2, seq, lane);
+                }
             }
         }
     } else if (w < 16) {
         // ============================================================== V of a tile, lanes by tokens
-        // a thread's words: group j of lanes, b of its quads, pairs of tokens 4 hh .. + 4 of a panel
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOperands));
+        // half panels 4 i + wv: lane (j group of lanes, b of its quads), pairs of tokens 4 hh .. + 4 of the panel
         constexpr int HP = D == 128 ? 1 : 2, TASKS = 4 / HP;  // half panels a warp takes at once
         const int wv = w - 12, b = lane & 7, j = D == 128 ? lane >> 3 : (lane >> 3) & 1;
         const int hsel = D == 128 ? 0 : lane >> 4;
@@ -476,8 +466,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         while (sg.u < sg.ue) {
             const int n = sg.here(), first = sg.ui, seq = sg.rq.seq, h = sg.h, r = sg.r;
             sg.skip(P, n);
-            // the scale and minimum of token 8 hp + b for group j, each lane one; the others by shuffles
-            uint32_t vw[TASKS][4], vm[TASKS], nw[TASKS][4], nm[TASKS];
+            // the scale and minimum of token 8 hp + b for group j, one a lane; the others by shuffles
+            uint32_t vw[TASKS][4], vm[TASKS];
             int ids = panels_of(P, r, h, first, seq, lane);
             auto load = [&](int tile) {
                 #pragma unroll
@@ -485,37 +475,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     const int hp = 4 * (HP * i + hsel) + wv, hh = hp & 1;      // half panel 0 .. 15 of the tile
                     const int id = __shfl_sync(0xffffffffu, ids, hp >> 1);
                     const uint8_t* pan = P.cache + int64_t(max(id, 0)) * PANEL;
+                    vm[i] = 0u;
                     #pragma unroll
-                    for (int k = 0; k < 4; ++k) nw[i][k] = 0u;
-                    nm[i] = 0u;
+                    for (int k = 0; k < 4; ++k) vw[i][k] = 0u;
                     if (id >= 0) {                            // (a bad block is reported, and made NaN, with K)
                         #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            nw[i][k] = *reinterpret_cast<const uint32_t*>(pan + 8 * D + (4 * hh + k) * D + b * (D / 8) + 4 * j);
+                            vw[i][k] = *reinterpret_cast<const uint32_t*>(pan + 8 * D + (4 * hh + k) * D + b * (D / 8) + 4 * j);
                         if (tile * TN + 8 * hp + b < seq)
-                            nm[i] = *reinterpret_cast<const uint32_t*>(pan + v_meta_offset(D, GRP) + ((8 * hh + b) * NG + j / WPG) * 4);
+                            vm[i] = *reinterpret_cast<const uint32_t*>(pan + v_meta_offset(D, GRP) + ((8 * hh + b) * NG + j / WPG) * 4);
                     }
                 }
             };
             load(first);
             ids = panels_of(P, r, h, first + 1, seq, lane);
             for (int it = 0; it < n; ++it, ++n_tile) {
-                bool nan = false;
-                #pragma unroll
-                for (int i = 0; i < TASKS; ++i) {
-                    #pragma unroll
-                    for (int k = 0; k < 4; ++k) vw[i][k] = nw[i][k];
-                    vm[i] = nm[i];
-                    nan |= (vm[i] & 0x7fffu) > 0x7c00u;
-                }
-                if (it + 1 < n) {
-                    load(first + it + 1);
-                    ids = panels_of(P, r, h, first + it + 2, seq, lane);
-                }
                 const int st = n_tile & 1;
                 wait(&B.vempty[st], (n_tile >> 1) + 1);
-                // the flags of the tile four behind are read by every row that sees it (its successor's
-                // weights were written after that, and V of this tile follows them by two)
+                // the flags of the tile four behind are read by every row that sees it (the first half of its
+                // successor does, and V of this tile follows that by more)
                 {
                     const int f = (n_tile + 4) & (kFlags - 1);
                     vbad[f][tid - 384] = 0;
@@ -523,6 +501,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 }
                 // a NaN scale counts as nothing here: a weight of 0 must not spread it. The rows that see
                 // its token are told by flags
+                bool nan = false;
+                #pragma unroll
+                for (int i = 0; i < TASKS; ++i) nan |= (vm[i] & 0x7fffu) > 0x7c00u;
                 if (__any_sync(0xffffffffu, nan)) {
                     const int f = n_tile & (kFlags - 1);
                     #pragma unroll
@@ -558,58 +539,77 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 }
                 fence_async_smem();
                 mbar_arrive(&B.vfull[st]);
+                if (it + 1 < n) {
+                    load(first + it + 1);
+                    ids = panels_of(P, r, h, first + it + 2, seq, lane);
+                }
             }
         }
-    } else if (lane == 0) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsProducts));
+        if (w < 18 && lane == 0) {
         // ============================================================== the products of row tile x
         const int x = w - 16;
-        constexpr uint32_t ID_S = idesc_f16(TM, TN, false, false), ID_PV = idesc_f16(TM, D, false, false);
+        constexpr uint32_t ID_S = idesc_f16(TM, TH, false, false), ID_PV = idesc_f16(TM, D, false, false);
         const uint64_t dq = sw128_desc(smem_u32(smem + S::off_q + x * S::Q), 16, 1024);
-        uint32_t n_tile = 0, n_pv = 0, n_q = 0;
+        const uint64_t dk0 = sw128_desc(smem_u32(smem + S::off_k), 16, 1024), dv0 = sw128_desc(smem_u32(smem + S::off_v), 16, 1024);
+        uint32_t n_tile = 0, n_s = 0, n_pv = 0, n_q = 0;      // stored tiles; halves scored; halves summed
+        // S of half `half` of the k-th tile of the CTA, into the buffer of its turn
+        auto score = [&](uint32_t k, int half) {
+            const int st = k & 1;
+            if (half == 0) wait(&B.kfull[st], k >> 1);
+            tc_after();
+            const uint64_t dk = dk0 + uint64_t((st * S::K + half * TH * 128) >> 4);
+            #pragma unroll
+            for (int e = 0; e < D / 16; ++e) {
+                const uint64_t step = uint64_t(((e >> 2) * S::KATOM + (e & 3) * 32) >> 4);
+                mma_f16(tmem + s_col(x, n_s & 1), dq + step, dk + step, ID_S, e > 0 ? 1u : 0u);
+            }
+            mma_commit(&B.sfull[x][n_s & 1]);
+            if (half) mma_commit(&B.kempty[st]);
+            ++n_s;
+        };
         while (sg.u < sg.ue) {
             const int n = sg.here();
-            const bool active = sg.rb * CROWS + x * TM < sg.rq.ql * P.G;
-            if (active) {
-                wait(&B.qfull[x], n_q);                       // (O of the segment before is read, P consumed)
-                ++n_q;
-            }
-            for (int i = 0; i < n; ++i, ++n_tile) {
-                const int st = n_tile & 1;
-                const uint32_t ph = n_tile >> 1;
-                wait(&B.kfull[st], ph);
-                if (!active) {
+            if (sg.rb * CROWS + x * TM >= sg.rq.ql * P.G) {   // no rows: the operands are passed on
+                for (int i = 0; i < n; ++i, ++n_tile) {
+                    const int st = n_tile & 1;
+                    wait(&B.kfull[st], n_tile >> 1);
                     mbar_arrive(&B.kempty[st]);
-                    wait(&B.vfull[st], ph);
+                    wait(&B.vfull[st], n_tile >> 1);
                     mbar_arrive(&B.vempty[st]);
-                    continue;
                 }
-                if (i > 0) wait(&B.pvdone[x], n_pv - 1);      // P of the tile before is read from S's columns
+                sg.skip(P, n);
+                continue;
+            }
+            wait(&B.qfull[x], n_q);                           // (O of the segment before is read, P consumed)
+            ++n_q;
+            score(n_tile, 0);
+            for (int i = 0; i < 2 * n; ++i) {
+                const uint32_t k = n_tile + (i >> 1);
+                const int st = k & 1, half = i & 1;
+                if (i + 1 < 2 * n) {                          // the next half's scores, once P of the half before this
+                    if (i > 0) wait(&B.pvdone[x][(n_pv - 1) & 1], (n_pv - 1) >> 1);   // one has been read from their buffer
+                    score(n_tile + ((i + 1) >> 1), (i + 1) & 1);
+                }
+                if (half == 0) wait(&B.vfull[st], k >> 1);
+                wait(&B.pfull[x][n_pv & 1], n_pv >> 1);
                 tc_after();
-                const uint64_t dk = sw128_desc(smem_u32(smem + S::off_k + st * S::K), 16, 1024);
+                const uint64_t dv = dv0 + uint64_t((st * S::V + half * S::VATOM) >> 4);
                 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint64_t step = uint64_t(((k >> 2) * S::KATOM + (k & 3) * 32) >> 4);
-                    mma_f16(tmem + s_col(x), dq + step, dk + step, ID_S, k > 0 ? 1u : 0u);
-                }
-                mma_commit(&B.sfull[x]);
-                mma_commit(&B.kempty[st]);
-                wait(&B.vfull[st], ph);
-                wait(&B.pfull[x], n_pv);
-                tc_after();
-                const uint64_t dv = sw128_desc(smem_u32(smem + S::off_v + st * S::V), 16, 1024);
-                #pragma unroll
-                for (int k = 0; k < TN / 16; ++k) {
-                    const uint64_t step = uint64_t(((k >> 2) * S::VATOM + (k & 3) * 32) >> 4);
-                    mma_f16_ts(tmem + o_col(x), tmem + s_col(x) + 8 * k, dv + step, ID_PV, (i > 0 || k > 0) ? 1u : 0u);
-                }
-                mma_commit(&B.pvdone[x]);
-                mma_commit(&B.vempty[st]);
+                for (int e = 0; e < TH / 16; ++e)
+                    mma_f16_ts(tmem + o_col(x), tmem + s_col(x, n_pv & 1) + 8 * e, dv + uint64_t((e * 32) >> 4), ID_PV,
+                               (i > 0 || e > 0) ? 1u : 0u);
+                mma_commit(&B.pvdone[x][n_pv & 1]);
+                if (half) mma_commit(&B.vempty[st]);
                 ++n_pv;
             }
+            n_tile += n;
             sg.skip(P, n);
         }
         // every product has ended before the tensor memory is freed (their operands are read, too)
-        if (n_pv) mbar_wait(&B.pvdone[x], (n_pv - 1) & 1u);
+        if (n_pv) mbar_wait(&B.pvdone[x][(n_pv - 1) & 1], ((n_pv - 1) >> 1) & 1u);
+        }
     }
     __syncwarp();
     tc_before();
@@ -656,6 +656,11 @@ template <int D, int GRP>
 int launch_chunk(const AttnParams& P, cudaStream_t st) {
     auto k = q4_chunk_kernel<D, GRP>;
     if (int e = raise_smem_limit(reinterpret_cast<const void*>(k), "q4_chunk_kernel")) return e;
+    cudaFuncAttributes fa{};
+    if (cudaFuncGetAttributes(&fa, k) != cudaSuccess || fa.numRegs != kRegsLaunch) {
+        cudaGetLastError();
+        return fail(TTKV_ERR_CUDA, "q4_chunk_kernel: built with %d registers a thread, its roles share %d", fa.numRegs, kRegsLaunch);
+    }
     cudaLaunchAttribute pdl[1];
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
