@@ -7,16 +7,19 @@
 // turn) over stored tiles of 128 tokens. Each stored tile is turned into fp16 operands once for both:
 // K^ = m + s c and V^, rounded once to fp16 (half a step, 2^-12 of an element; the codes as exact
 // operands with their scales applied to S and P would cost the softmax twice its instructions, and
-// with groups below d a product each). Scores, sums and O are fp32; P is fp16, at most 2^8: the
-// running maximum moves only when a row's exceeds it by 2^8 (then O in tensor memory is rescaled).
+// with groups below d a product each). Scores, sums and O are fp32; P is fp16, at most 2^15: the
+// running maximum moves only when weights outgrow that (then O in tensor memory is rescaled).
 //
 // Roles: two softmax warpgroups (a thread owns a row, i.e. a lane of tensor memory), a warpgroup that
-// dequantises K and one for V, two warps that issue the products, one per row tile. Operands are
+// dequantises K and one for V, two warps that issue the products, one per row tile, and a warp that
+// fetches the stored panels, by bulk copies into a ring a tile and a half deep. Operands are
 // double-buffered in shared memory in the 128-byte-swizzled K-major layout of the MMA. Scores are made
 // 64 tokens at a time into two buffers in turn, so the next half's product runs under this half's
 // softmax, whose P replaces the scores in place. The stored order of the codes needs no transposition:
 // a K word is a 16-byte chunk of its token's row (the dims of a chunk in the order 0 4 1 5 2 6 3 7,
-// which Q repeats), and four V words are chunks of eight tokens of four lanes.
+// which Q repeats), and four V words are chunks of eight tokens of four lanes. The roles' loops are
+// kept short (rolled where the data lies in shared memory): together they have to stay in the SM's
+// instruction cache, and unrolled they streamed 19 KB of code per tile through it.
 //
 // The work list is (request, KV head, row block, stored tile up to the block's causal limit), shared
 // out evenly to one CTA per SM as in the streaming kernel; the parts that a share's borders cut go
@@ -34,27 +37,31 @@ constexpr int TN = 128;                      // stored tokens of a tile
 constexpr int TM = 128;                      // rows of a tile
 constexpr int CROWS = 2 * TM;                // rows of a block
 constexpr int TH = TN / 2;                   // tokens of a half, the step of the softmax
-constexpr int kChunkThreads = 20 * 32;       // softmax 8 warps, K 4, V 4, products 2 (of 4)
+constexpr int kChunkThreads = 20 * 32;       // softmax 8 warps, K 4, V 4, products 2, fetching 1 (and 1 idle)
 // Registers a thread: at launch, and of each role after its own setting. A warpgroup waits in its
 // setting until the others have given theirs up, so the shares must not exceed the launch's total.
 constexpr int kRegsLaunch = 96, kRegsSoftmax = 128, kRegsOperands = 80, kRegsProducts = 64;
 static_assert(2 * kRegsSoftmax + 2 * kRegsOperands + kRegsProducts <= 5 * kRegsLaunch, "register shares");
 constexpr uint32_t kTmemCols = 512;          // S of row tile 0 and 1, O of each, at 128 columns
+constexpr float kWeightMost = 32768.f;       // of a half's weights in all: each is a finite fp16
 constexpr int kFlags = 8;                    // tiles whose NaN values are remembered
 
 // Row tiles' tensor memory: S of a half in buffer y (then P in its first 32 columns) and O.
 __device__ __forceinline__ uint32_t s_col(int x, uint32_t y) { return 128u * x + 64u * y; }
 __device__ __forceinline__ uint32_t o_col(int x) { return 256u + 128u * x; }
 
-template <int D>
+template <int D, int GRP>
 struct ChunkSmem {
     static constexpr int Q = TM * D * 2, K = TN * D * 2, V = D * TN * 2;
-    static constexpr int off_q = 0, off_k = 2 * Q, off_v = off_k + 2 * K, BYTES = off_v + 2 * V + 1024;
+    static constexpr int PANEL = panel_bytes(D, GRP), RING = std::min(16, 28160 / PANEL);
+    static constexpr int off_q = 0, off_k = 2 * Q, off_v = off_k + 2 * K, off_ring = off_v + 2 * V;
+    static constexpr int BYTES = off_ring + RING * PANEL + 1024;
     static constexpr int KATOM = TN * 128, VATOM = D * 128;   // 64 dims of 128 tokens; 64 tokens of D lanes
 };
 
 struct ChunkBars {
     uint64_t kfull[2], kempty[2], vfull[2], vempty[2];        // operand stages
+    uint64_t rfull[16], rempty[16];                           // panels of the ring
     // row tiles; of halves one for each buffer: a half is waited for before the one after the next is made,
     // so no phase is missed
     uint64_t qfull[2], sfull[2][2], pfull[2][2], pvdone[2][2];
@@ -141,10 +148,26 @@ __device__ __forceinline__ int panels_of(const AttnParams& P, int r, int h, int 
     return int((int64_t(blk) * P.H + h) * (P.block_size / kPanelTokens)) + (t - bi * P.block_size) / kPanelTokens;
 }
 
+// Bounded wait for a barrier's phase (about 2 s). The clock is read once in many tries, and a warp with
+// time to spare sleeps in between: polling takes issue slots from the warps that it waits for.
+template <bool IDLE>
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
+    if (mbar_try(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (;;) {
+        #pragma unroll 1
+        for (int i = 0; i < 64; ++i) {
+            if (IDLE) __nanosleep(64);
+            if (mbar_try(bar, parity)) return true;
+        }
+        if (clock64() - t0 > kWaitCycles) return false;
+    }
+}
+
 template <int D, int GRP>
 __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnParams P) {
-    using S = ChunkSmem<D>;
-    constexpr int NG = D / GRP, NW = D / 32, WPG = GRP / 32, PANEL = panel_bytes(D, GRP);
+    using S = ChunkSmem<D, GRP>;
+    constexpr int NG = D / GRP, NW = D / 32, WPG = GRP / 32, PANEL = S::PANEL, RING = S::RING;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ ChunkBars B;
@@ -170,6 +193,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 mbar_init(&B.pvdone[i][y], 1);
             }
         }
+    }
+    if (tid < RING) {
+        mbar_init(&B.rfull[tid], 1);
+        mbar_init(&B.rempty[tid], 2);
     }
     for (int i = tid; i < kFlags * TN; i += kChunkThreads) (&vbad[0][0])[i] = 0;
     if (tid < kFlags) any_bad[tid] = 0;
@@ -207,7 +234,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
     const uint32_t tmem = tmem_base;
     bool dead = false;                                        // a bounded wait ran out: no further waits
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!dead && !mbar_wait(bar, parity & 1u)) {
+        if (!dead && !wait_phase<false>(bar, parity & 1u)) {
+            dead = true;
+            report(P.status, TTKV_STATUS_TIMEOUT);
+        }
+    };
+    auto wait_idle = [&](uint64_t* bar, uint32_t parity) {    // by warps that are ahead of the others
+        if (!dead && !wait_phase<true>(bar, parity & 1u)) {
             dead = true;
             report(P.status, TTKV_STATUS_TIMEOUT);
         }
@@ -247,47 +280,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             float qf;
             {
                 const int64_t src = int64_t(rq.q0 + j) * P.q_stride + int64_t(h * P.G + g) * D;
-                uint4 raw[D / 8];
-                float big = 0.f;
-                #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    raw[c] = make_uint4(0, 0, 0, 0);
-                    if (live) {
-                        if (P.q_vec) {
-                            raw[c] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) + src) + c);
-                        } else {
-                            const uint16_t* e = static_cast<const uint16_t*>(P.q) + src + 8 * c;
-                            raw[c] = make_uint4(e[0] | (uint32_t(e[1]) << 16), e[2] | (uint32_t(e[3]) << 16),
-                                                e[4] | (uint32_t(e[5]) << 16), e[6] | (uint32_t(e[7]) << 16));
-                        }
-                    }
-                }
-                auto pair = [&](uint32_t v) {
-                    if (P.dtype == TTKV_BF16)
-                        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-                    return __half22float2(u2h(v));
-                };
-                #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    const uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+                // a chunk of eight dims, twice: for the row's largest |q|, then as an operand
+                auto chunk = [&](int c, float (&v)[8]) {
                     #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float2 f = pair(v[k]);
-                        big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-                    }
+                    for (int k = 0; k < 8; ++k) v[k] = 0.f;
+                    if (live) load8(P.q, P.dtype, src + 8 * c, P.q_vec, v);
+                };
+                float big = 0.f;
+                #pragma unroll 1
+                for (int c = 0; c < D / 8; c += 4) {
+                    float v[4][8];
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) chunk(c + k, v[k]);
+                    #pragma unroll
+                    for (int k = 0; k < 32; ++k) big = fmaxf(big, fabsf(v[k >> 3][k & 7]));
                 }
-                // e brings the row's largest |q| into [1, 2); a negative scale's sign goes to q
+                // e brings it into [1, 2); a negative scale's sign goes to q
                 const int e = big > 0.f && big < INFINITY ? 127 - int(__float_as_uint(big) >> 23) : 0;
                 const float up = copysignf(__uint_as_float(uint32_t(min(127 + e, 254)) << 23), P.scale);
                 // (not 0, which would make NaN of a masked score of -inf)
                 qf = fmaxf(fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e, 1)) << 23), 1e-38f);
-                #pragma unroll
+                #pragma unroll 1
                 for (int c = 0; c < D / 8; ++c) {
-                    const float2 a = pair(raw[c].x), b = pair(raw[c].y), d = pair(raw[c].z), f = pair(raw[c].w);
+                    float v[8];
+                    chunk(c, v);
+                    #pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] *= up;
                     // dims 0 4 1 5 2 6 3 7, the order of a word's codes
                     *reinterpret_cast<uint4*>(qb + (c >> 3) * S::KATOM + kmajor_off(t, c & 7)) =
-                        make_uint4(half2_bits(a.x * up, d.x * up), half2_bits(a.y * up, d.y * up),
-                                   half2_bits(b.x * up, f.x * up), half2_bits(b.y * up, f.y * up));
+                        make_uint4(half2_bits(v[0], v[4]), half2_bits(v[1], v[5]), half2_bits(v[2], v[6]), half2_bits(v[3], v[7]));
                 }
             }
             fence_async_smem();
@@ -308,57 +329,66 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 if (i > 0 && (i & 1) == 0) note_bad((i >> 1) - 1, n_tile + (i >> 1) - 1);
                 const int seen = lim - (begin * TN + i * TH); // tokens of the half that the row sees
                 const bool full = __all_sync(0xffffffffu, seen >= TH);
-                float s[2][32];
-                tmem_ld32(sc, s[0]);
-                tmem_ld32(sc + 32, s[1]);
-                tmem_wait_ld();
-                if (!full) {
+                // weights against the maximum so far, which may be exceeded as long as no fp16 weight overflows:
+                // the half's sum tells. The maximum is looked for in the first half and, rarely, when it does
+                uint32_t p[2][16];
+                float sum;
+                for (bool raise = i == 0;; raise = true) {
+                    float s[2][32];
+                    tmem_ld32(sc, s[0]);
+                    tmem_ld32(sc + 32, s[1]);
+                    tmem_wait_ld();
+                    if (!full) {
+                        #pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            #pragma unroll
+                            for (int k = 0; k < 32; ++k) s[c][k] = 32 * c + k < seen ? s[c][k] : -INFINITY;
+                    }
+                    if (raise) {
+                        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        #pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            #pragma unroll
+                            for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], s[c][k]);
+                        const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * qf;
+                        float corr = 1.f;
+                        if (mt > m) {                         // (m is -inf at first)
+                            corr = m == -INFINITY ? 0.f : ex2(m - mt);
+                            m = mt;
+                            l *= corr;
+                        }
+                        if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                            wait(&B.pvdone[x][(n_s - 1) & 1], (n_s - 1) >> 1);    // O holds every half before this one
+                            tc_after();
+                            #pragma unroll 1
+                            for (int c = 0; c < D / 16; ++c) {
+                                float o[16];
+                                tmem_ld16(lane_base + o_col(x) + 16 * c, o);
+                                tmem_wait_ld();
+                                uint32_t v[16];
+                                #pragma unroll
+                                for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(o[k] * corr);
+                                tmem_st16u(lane_base + o_col(x) + 16 * c, v);
+                            }
+                        }
+                    }
+                    const float mm = m == -INFINITY ? 0.f : m;    // a row that sees nothing yet has weights of 0
+                    float2 ls = make_float2(0.f, 0.f);
                     #pragma unroll
                     for (int c = 0; c < 2; ++c)
                         #pragma unroll
-                        for (int k = 0; k < 32; ++k) s[c][k] = 32 * c + k < seen ? s[c][k] : -INFINITY;
+                        for (int k = 0; k < 16; ++k) {
+                            const float2 a = __ffma2_rn(make_float2(s[c][2 * k], s[c][2 * k + 1]), make_float2(qf, qf), make_float2(-mm, -mm));
+                            const float2 e = make_float2(ex2(a.x), ex2(a.y));
+                            ls = __fadd2_rn(ls, e);
+                            p[c][k] = half2_bits(e.x, e.y);
+                        }
+                    sum = ls.x + ls.y;
+                    if (raise || !__any_sync(0xffffffffu, sum > kWeightMost)) break;
                 }
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                #pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    #pragma unroll
-                    for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], s[c][k]);
-                const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * qf;
-                float corr = 1.f;
-                if (mt > m + 8.f) {                           // (m is -inf at first)
-                    corr = m == -INFINITY ? 0.f : ex2(m - mt);
-                    m = mt;
-                    l *= corr;
-                }
-                if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-                    wait(&B.pvdone[x][(n_s - 1) & 1], (n_s - 1) >> 1);    // O holds every half before this one
-                    tc_after();
-                    #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
-                        float o[16];
-                        tmem_ld16(lane_base + o_col(x) + 16 * c, o);
-                        tmem_wait_ld();
-                        uint32_t v[16];
-                        #pragma unroll
-                        for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(o[k] * corr);
-                        tmem_st16u(lane_base + o_col(x) + 16 * c, v);
-                    }
-                }
-                const float mm = m == -INFINITY ? 0.f : m;    // a row that sees nothing yet has weights of 0
-                float2 ls = make_float2(0.f, 0.f);
-                #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t p[16];
-                    #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 a = __ffma2_rn(make_float2(s[c][2 * k], s[c][2 * k + 1]), make_float2(qf, qf), make_float2(-mm, -mm));
-                        const float2 e = make_float2(ex2(a.x), ex2(a.y));
-                        ls = __fadd2_rn(ls, e);
-                        p[k] = half2_bits(e.x, e.y);
-                    }
-                    tmem_st16u(sc + 16 * c, p);
-                }
-                l += ls.x + ls.y;
+                l += sum;
+                tmem_st16u(sc, p[0]);
+                tmem_st16u(sc + 16, p[1]);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_before();
                 mbar_arrive(&B.pfull[x][n_s & 1]);
@@ -372,18 +402,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             const int64_t pr = (int64_t(blockIdx.x) * 2 + (ca >= u0 ? 0 : 1)) * CROWS + x * TM + t;
             const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
             const int64_t dst = int64_t(rq.q0 + j) * P.out_stride + int64_t(h * P.G + g) * D;
-            #pragma unroll
+            #pragma unroll 1
             for (int c = 0; c < NW; ++c) {
                 float o[32];
                 tmem_ld32(lane_base + o_col(x) + 32u * c, o); // column 32 c + 8 i + b holds lane 32 c + 4 b + i
                 tmem_wait_ld();
                 const float f = (bad >> (c / WPG)) & 1u ? __int_as_float(0x7fc00000) : inv;
-                if (live) {
+                if (!live) continue;
+                if (!whole) {
                     #pragma unroll
-                    for (int b = 0; b < 8; ++b) {
-                        const float4 v = make_float4(o[b] * f, o[8 + b] * f, o[16 + b] * f, o[24 + b] * f);
-                        if (!whole) *reinterpret_cast<float4*>(P.part_o + pr * D + 32 * c + 4 * b) = v;
-                        else store4(P, dst + 32 * c + 4 * b, v);
+                    for (int b = 0; b < 8; ++b)
+                        *reinterpret_cast<float4*>(P.part_o + pr * D + 32 * c + 4 * b) =
+                            make_float4(o[b] * f, o[8 + b] * f, o[16 + b] * f, o[24 + b] * f);
+                } else {
+                    #pragma unroll
+                    for (int b = 0; b < 8; b += 2) {
+                        const float v[8] = {o[b] * f, o[8 + b] * f, o[16 + b] * f, o[24 + b] * f,
+                                            o[b + 1] * f, o[9 + b] * f, o[17 + b] * f, o[25 + b] * f};
+                        store8(P.out, P.dtype, dst + 32 * c + 4 * b, P.out_vec == 2, v);
                     }
                 }
             }
@@ -401,97 +437,58 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
     } else if (w < 12) {
         // ============================================================== K of a tile as fp16 rows
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOperands));
-        // 8-token groups 4 i + wk: lane (b token of it, a chunk of its row), i.e. token o of panel 2 i + wk / 2
-        const int wk = w - 8, b = lane & 7, a = lane >> 3, o = 8 * (wk & 1) + b;
+        // panels wk and wk + 4, eight tokens at a time: lane (b token of them, a chunk of its row)
+        const int wk = w - 8, b = lane & 7, a = lane >> 3;
         uint32_t n_tile = 0;
         while (sg.u < sg.ue) {
-            const int n = sg.here(), first = sg.ui, seq = sg.rq.seq, h = sg.h, r = sg.r;
+            const int n = sg.here(), first = sg.ui, seq = sg.rq.seq;
             sg.skip(P, n);
-            uint32_t kw[4][NW], km[4][NG];
-            int ids = panels_of(P, r, h, first, seq, lane);
-            auto load = [&](int tile) {
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int p = 2 * i + (wk >> 1);
-                    const int id = __shfl_sync(0xffffffffu, ids, p);
-                    const uint8_t* pan = P.cache + int64_t(max(id, 0)) * PANEL;
-                    if (id >= 0) {
-                        load_words(pan + o * (D / 2) + a * (D / 8), kw[i]);
-                        load_words(pan + k_meta_offset(D) + o * NG * 4, km[i]);
-                    } else {
-                        #pragma unroll
-                        for (int k = 0; k < NW; ++k) kw[i][k] = 0u;
-                        #pragma unroll
-                        for (int k = 0; k < NG; ++k) km[i][k] = id == kBadPanel ? 0x7e00u : 0u;   // NaN keys: so are the rows that see them
-                        if (id == kBadPanel && lane == 0) report(P.status, TTKV_STATUS_BLOCK_RANGE);
-                    }
-                }
-            };
-            load(first);
-            ids = panels_of(P, r, h, first + 1, seq, lane);
             for (int it = 0; it < n; ++it, ++n_tile) {
                 const int st = n_tile & 1;
-                wait(&B.kempty[st], (n_tile >> 1) + 1);
+                wait_idle(&B.kempty[st], (n_tile >> 1) + 1);
                 unsigned char* kb = smem + S::off_k + st * S::K;
-                #pragma unroll
+                #pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
-                    const int row = 32 * i + 8 * wk + b;
+                    const int p = wk + 4 * (i >> 1), o = 8 * (i & 1) + b, row = 16 * p + o;
+                    const uint32_t g = 8 * n_tile + p, slot = g % RING;
+                    const unsigned char* pan = smem + S::off_ring + slot * PANEL;
+                    if ((i & 1) == 0) wait(&B.rfull[slot], g / RING);
+                    uint32_t kw[NW], km[NG];
+                    load_words(pan + o * (D / 2) + a * (D / 8), kw);
+                    load_words(pan + k_meta_offset(D) + o * NG * 4, km);
                     const bool none = (first + it) * TN + row >= seq;          // behind the last token: zeros
                     #pragma unroll
                     for (int k = 0; k < NW; ++k) {
-                        const uint32_t meta = none ? 0u : km[i][k / WPG], v = kw[i][k];
+                        const uint32_t meta = none ? 0u : km[k / WPG], v = kw[k];
                         const __half2 s2 = u2h(__byte_perm(meta, 0, 0x1010)), m2 = u2h(__byte_perm(meta, 0, 0x3232));
                         const int c = 4 * k + a;
                         *reinterpret_cast<uint4*>(kb + (c >> 3) * S::KATOM + kmajor_off(row, c & 7)) =
                             make_uint4(h2u(__hfma2(codes2<false>(v), s2, m2)), h2u(__hfma2(codes2<true>(v), s2, m2)),
                                        h2u(__hfma2(codes2<false>(v >> 8), s2, m2)), h2u(__hfma2(codes2<true>(v >> 8), s2, m2)));
                     }
+                    if (i & 1) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&B.rempty[slot]);
+                    }
                 }
                 fence_async_smem();
                 mbar_arrive(&B.kfull[st]);
-                if (it + 1 < n) {                             // the next tile's, and the blocks of the one behind it
-                    load(first + it + 1);
-                    ids = panels_of(P, r, h, first + it + 2, seq, lane);
-                }
             }
         }
     } else if (w < 16) {
         // ============================================================== V of a tile, lanes by tokens
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOperands));
-        // half panels 4 i + wv: lane (j group of lanes, b of its quads), pairs of tokens 4 hh .. + 4 of the panel
-        constexpr int HP = D == 128 ? 1 : 2, TASKS = 4 / HP;  // half panels a warp takes at once
+        // panels wv and wv + 4, half a panel (eight tokens, pairs 4 hh .. + 4) at a time: lane (j group of
+        // lanes, b of its quads); with heads of 64 both halves at once
+        constexpr int STEPS = D == 128 ? 4 : 2;
         const int wv = w - 12, b = lane & 7, j = D == 128 ? lane >> 3 : (lane >> 3) & 1;
-        const int hsel = D == 128 ? 0 : lane >> 4;
         uint32_t n_tile = 0;
         while (sg.u < sg.ue) {
-            const int n = sg.here(), first = sg.ui, seq = sg.rq.seq, h = sg.h, r = sg.r;
+            const int n = sg.here(), first = sg.ui, seq = sg.rq.seq;
             sg.skip(P, n);
-            // the scale and minimum of token 8 hp + b for group j, one a lane; the others by shuffles
-            uint32_t vw[TASKS][4], vm[TASKS];
-            int ids = panels_of(P, r, h, first, seq, lane);
-            auto load = [&](int tile) {
-                #pragma unroll
-                for (int i = 0; i < TASKS; ++i) {
-                    const int hp = 4 * (HP * i + hsel) + wv, hh = hp & 1;      // half panel 0 .. 15 of the tile
-                    const int id = __shfl_sync(0xffffffffu, ids, hp >> 1);
-                    const uint8_t* pan = P.cache + int64_t(max(id, 0)) * PANEL;
-                    vm[i] = 0u;
-                    #pragma unroll
-                    for (int k = 0; k < 4; ++k) vw[i][k] = 0u;
-                    if (id >= 0) {                            // (a bad block is reported, and made NaN, with K)
-                        #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            vw[i][k] = *reinterpret_cast<const uint32_t*>(pan + 8 * D + (4 * hh + k) * D + b * (D / 8) + 4 * j);
-                        if (tile * TN + 8 * hp + b < seq)
-                            vm[i] = *reinterpret_cast<const uint32_t*>(pan + v_meta_offset(D, GRP) + ((8 * hh + b) * NG + j / WPG) * 4);
-                    }
-                }
-            };
-            load(first);
-            ids = panels_of(P, r, h, first + 1, seq, lane);
             for (int it = 0; it < n; ++it, ++n_tile) {
                 const int st = n_tile & 1;
-                wait(&B.vempty[st], (n_tile >> 1) + 1);
+                wait_idle(&B.vempty[st], (n_tile >> 1) + 1);
                 // the flags of the tile four behind are read by every row that sees it (the first half of its
                 // successor does, and V of this tile follows that by more)
                 {
@@ -499,34 +496,54 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     vbad[f][tid - 384] = 0;
                     if (tid == 384) any_bad[f] = 0;
                 }
-                // a NaN scale counts as nothing here: a weight of 0 must not spread it. The rows that see
-                // its token are told by flags
-                bool nan = false;
-                #pragma unroll
-                for (int i = 0; i < TASKS; ++i) nan |= (vm[i] & 0x7fffu) > 0x7c00u;
-                if (__any_sync(0xffffffffu, nan)) {
-                    const int f = n_tile & (kFlags - 1);
+                unsigned char* vb = smem + S::off_v + st * S::V;
+                const bool tail = (first + it + 1) * TN > seq;
+                #pragma unroll 1
+                for (int i = 0; i < STEPS; ++i) {
+                    const int p = wv + 4 * (D == 128 ? i >> 1 : i), hh = D == 128 ? i & 1 : lane >> 4;
+                    const uint32_t g = 8 * n_tile + p, slot = g % RING;
+                    const unsigned char* pan = smem + S::off_ring + slot * PANEL;
+                    if (D == 64 || (i & 1) == 0) wait(&B.rfull[slot], g / RING);
+                    uint32_t vw[4], vm[8];
                     #pragma unroll
-                    for (int i = 0; i < TASKS; ++i) {
-                        if ((vm[i] & 0x7fffu) > 0x7c00u) {
-                            const int tok = 8 * (4 * (HP * i + hsel) + wv) + b;
-                            vm[i] = 0u;
+                    for (int k = 0; k < 4; ++k)
+                        vw[k] = *reinterpret_cast<const uint32_t*>(pan + 8 * D + (4 * hh + k) * D + b * (D / 8) + 4 * j);
+                    if constexpr (NG == 1) {
+                        uint32_t (&lo)[4] = *reinterpret_cast<uint32_t (*)[4]>(vm), (&hi)[4] = *reinterpret_cast<uint32_t (*)[4]>(vm + 4);
+                        load_words(pan + v_meta_offset(D, GRP) + 32 * hh, lo);
+                        load_words(pan + v_meta_offset(D, GRP) + 32 * hh + 16, hi);
+                    } else {
+                        #pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            vm[k] = *reinterpret_cast<const uint32_t*>(pan + v_meta_offset(D, GRP) + ((8 * hh + k) * NG + j / WPG) * 4);
+                    }
+                    const int hp = 2 * p + hh;                // chunk of eight tokens of the tile
+                    if (tail) {                               // behind the last token: zeros
+                        #pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if ((first + it) * TN + 8 * hp + k >= seq) vm[k] = 0u;
+                    }
+                    // a NaN scale counts as nothing here: a weight of 0 must not spread it. The rows that see
+                    // its token are told by flags
+                    bool nan = false;
+                    #pragma unroll
+                    for (int k = 0; k < 8; ++k) nan |= (vm[k] & 0x7fffu) > 0x7c00u;
+                    if (__any_sync(0xffffffffu, nan)) {
+                        const int f = n_tile & (kFlags - 1);
+                        #pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            if ((vm[k] & 0x7fffu) <= 0x7c00u) continue;
+                            const int tok = 8 * hp + k;
+                            vm[k] = 0u;
                             atomicOr(reinterpret_cast<unsigned*>(&vbad[f][tok & ~3]), (1u << (j / WPG)) << (8 * (tok & 3)));
                             any_bad[f] = 1;
                         }
                     }
-                }
-                unsigned char* vb = smem + S::off_v + st * S::V;
-                #pragma unroll
-                for (int i = 0; i < TASKS; ++i) {
-                    const int hp = 4 * (HP * i + hsel) + wv;
                     uint32_t out[4][4];                       // [lane of the quad][pair of tokens]
                     #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const uint32_t ma = __shfl_sync(0xffffffffu, vm[i], (lane & 24) + 2 * k);
-                        const uint32_t mb = __shfl_sync(0xffffffffu, vm[i], (lane & 24) + 2 * k + 1);
+                        const uint32_t ma = vm[2 * k], mb = vm[2 * k + 1], v = vw[k];
                         const __half2 s2 = u2h(__byte_perm(ma, mb, 0x5410)), m2 = u2h(__byte_perm(ma, mb, 0x7632));
-                        const uint32_t v = vw[i][k];
                         out[0][k] = h2u(__hfma2(codes2<false>(v), s2, m2));
                         out[1][k] = h2u(__hfma2(codes2<true>(v), s2, m2));
                         out[2][k] = h2u(__hfma2(codes2<false>(v >> 8), s2, m2));
@@ -536,13 +553,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     for (int q = 0; q < 4; ++q)               // lane 32 j + 4 b + q is row 32 j + 8 q + b, chunk hp
                         *reinterpret_cast<uint4*>(vb + (hp >> 3) * S::VATOM + kmajor_off(32 * j + 8 * q + b, hp & 7)) =
                             make_uint4(out[q][0], out[q][1], out[q][2], out[q][3]);
+                    if (D == 64 || (i & 1)) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&B.rempty[slot]);
+                    }
                 }
                 fence_async_smem();
                 mbar_arrive(&B.vfull[st]);
-                if (it + 1 < n) {
-                    load(first + it + 1);
-                    ids = panels_of(P, r, h, first + it + 2, seq, lane);
-                }
             }
         }
     } else {
@@ -584,14 +601,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             }
             wait(&B.qfull[x], n_q);                           // (O of the segment before is read, P consumed)
             ++n_q;
-            score(n_tile, 0);
-            for (int i = 0; i < 2 * n; ++i) {
-                const uint32_t k = n_tile + (i >> 1);
-                const int st = k & 1, half = i & 1;
+            for (int i = -1; i < 2 * n; ++i) {
                 if (i + 1 < 2 * n) {                          // the next half's scores, once P of the half before this
                     if (i > 0) wait(&B.pvdone[x][(n_pv - 1) & 1], (n_pv - 1) >> 1);   // one has been read from their buffer
                     score(n_tile + ((i + 1) >> 1), (i + 1) & 1);
                 }
+                if (i < 0) continue;
+                const uint32_t k = n_tile + (i >> 1);
+                const int st = k & 1, half = i & 1;
                 if (half == 0) wait(&B.vfull[st], k >> 1);
                 wait(&B.pfull[x][n_pv & 1], n_pv >> 1);
                 tc_after();
@@ -609,6 +626,37 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         }
         // every product has ended before the tensor memory is freed (their operands are read, too)
         if (n_pv) mbar_wait(&B.pvdone[x][(n_pv - 1) & 1], ((n_pv - 1) >> 1) & 1u);
+        } else if (w == 18) {
+            // ========================================================== the stored panels, one each of lanes 0 to 7
+            uint32_t g = lane;                                // panels of the CTA
+            while (sg.u < sg.ue) {
+                const int n = sg.here(), first = sg.ui, seq = sg.rq.seq, h = sg.h, r = sg.r;
+                sg.skip(P, n);
+                int id = panels_of(P, r, h, first, seq, lane);
+                for (int it = 0; it < n; ++it, g += 8) {
+                    const int next = it + 1 < n ? panels_of(P, r, h, first + it + 1, seq, lane) : kNoPanel;
+                    if (lane < 8) {
+                        const uint32_t slot = g % RING;
+                        wait_idle(&B.rempty[slot], g / RING + 1);
+                        unsigned char* pan = smem + S::off_ring + slot * PANEL;
+                        if (id >= 0) {
+                            mbar_expect_tx(&B.rfull[slot], PANEL);
+                            bulk_g2s(pan, P.cache + int64_t(id) * PANEL, PANEL, &B.rfull[slot]);
+                        } else {
+                            if (id == kBadPanel) {            // NaN keys: so are the rows that see them
+                                report(P.status, TTKV_STATUS_BLOCK_RANGE);
+                                for (int k = 0; k < 2 * 16 * NG; ++k)
+                                    reinterpret_cast<uint32_t*>(pan + k_meta_offset(D))[k] = k < 16 * NG ? 0x7e00u : 0u;
+                                fence_async_smem();
+                            }
+                            mbar_arrive(&B.rfull[slot]);      // (behind the last token nothing is read but codes)
+                        }
+                    }
+                    id = next;
+                }
+            }
+            // every copy has landed: the operands' warps have waited for it, or the wait is made up for
+            if (lane < 8 && g >= 8 + uint32_t(lane)) mbar_wait(&B.rfull[(g - 8) % RING], ((g - 8) / RING) & 1u);
         }
     }
     __syncwarp();
@@ -667,7 +715,7 @@ int launch_chunk(const AttnParams& P, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(P.n_ctas));
     cfg.blockDim = dim3(kChunkThreads);
-    cfg.dynamicSmemBytes = ChunkSmem<D>::BYTES;
+    cfg.dynamicSmemBytes = ChunkSmem<D, GRP>::BYTES;
     cfg.stream = st;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;

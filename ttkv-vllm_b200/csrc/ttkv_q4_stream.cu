@@ -799,7 +799,7 @@ AttnParams attn_params(const ttkv_q4_cache_t* c, const ttkv_q4_batch_t* b, const
     P.n_reqs = b->n_reqs; P.q = q; P.dtype = dtype; P.q_stride = q_stride; P.scale = scale;
     P.out = out; P.out_stride = out_stride; P.status = status;
     P.q_vec = rows_aligned(q, dtype, q_stride);
-    P.out_vec = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && (out_stride & 3) == 0;
+    P.out_vec = rows_aligned(out, dtype, out_stride) ? 2 : (reinterpret_cast<uintptr_t>(out) & 7) == 0 && (out_stride & 3) == 0;
     return P;
 }
 
