@@ -164,6 +164,15 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
     }
 }
 
+// Eight 16-bit elements to memory that is not 16-byte aligned.
+__device__ __forceinline__ void store_chunk_unaligned(uint16_t* p, uint4 v) {
+    #pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t u = i < 4 ? (i < 2 ? v.x : v.y) : (i < 6 ? v.z : v.w);
+        p[i] = uint16_t(u >> (16 * (i & 1)));
+    }
+}
+
 template <int D, int GRP>
 __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnParams P) {
     using S = ChunkSmem<D, GRP>;
@@ -277,38 +286,61 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             const bool live = row < n_rows;
             const int j = live ? row / P.G : 0, g = live ? row - j * P.G : 0;
             const int lim = live ? rq.seq - rq.ql + j + 1 : 0;                  // sees stored tokens below it
-            float qf;
+            float qf = 0.f;
             {
-                const int64_t src = int64_t(rq.q0 + j) * P.q_stride + int64_t(h * P.G + g) * D;
-                // a chunk of eight dims, twice: for the row's largest |q|, then as an operand
-                auto chunk = [&](int c, float (&v)[8]) {
-                    #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = 0.f;
-                    if (live) load8(P.q, P.dtype, src + 8 * c, P.q_vec, v);
+                // the warp's 32 rows, D / 8 lanes to a row, a chunk of eight dims each
+                constexpr int LPR = D / 8, RPI = 32 / LPR;    // lanes a row, rows at once
+                const int c = lane % LPR;
+                const int64_t src = live ? int64_t(rq.q0 + j) * P.q_stride + int64_t(h * P.G + g) * D : -1;
+                auto place = [&](int i) -> uint4* {           // the chunk of row i RPI + lane / LPR of the warp
+                    return reinterpret_cast<uint4*>(qb + (c >> 3) * S::KATOM + kmajor_off(t - lane + i * RPI + lane / LPR, c & 7));
                 };
-                float big = 0.f;
-                #pragma unroll 1
-                for (int c = 0; c < D / 8; c += 4) {
-                    float v[4][8];
+                // as it is, all loads in flight at once; then each chunk in place
+                if (P.q_vec) {
+                    uint4 raw[LPR];
                     #pragma unroll
-                    for (int k = 0; k < 4; ++k) chunk(c + k, v[k]);
+                    for (int i = 0; i < LPR; ++i) {
+                        const int64_t from = __shfl_sync(0xffffffffu, src, i * RPI + lane / LPR);
+                        raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) + max(from, int64_t(0)) + 8 * c));
+                    }
                     #pragma unroll
-                    for (int k = 0; k < 32; ++k) big = fmaxf(big, fabsf(v[k >> 3][k & 7]));
+                    for (int i = 0; i < LPR; ++i) *place(i) = raw[i];
+                } else {
+                    #pragma unroll 1
+                    for (int i = 0; i < LPR; ++i) {
+                        const int64_t from = __shfl_sync(0xffffffffu, src, i * RPI + lane / LPR);
+                        const uint16_t* p = static_cast<const uint16_t*>(P.q) + max(from, int64_t(0)) + 8 * c;
+                        *place(i) = make_uint4(p[0] | (uint32_t(p[1]) << 16), p[2] | (uint32_t(p[3]) << 16),
+                                               p[4] | (uint32_t(p[5]) << 16), p[6] | (uint32_t(p[7]) << 16));
+                    }
                 }
-                // e brings it into [1, 2); a negative scale's sign goes to q
-                const int e = big > 0.f && big < INFINITY ? 127 - int(__float_as_uint(big) >> 23) : 0;
-                const float up = copysignf(__uint_as_float(uint32_t(min(127 + e, 254)) << 23), P.scale);
-                // (not 0, which would make NaN of a masked score of -inf)
-                qf = fmaxf(fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e, 1)) << 23), 1e-38f);
                 #pragma unroll 1
-                for (int c = 0; c < D / 8; ++c) {
-                    float v[8];
-                    chunk(c, v);
+                for (int i = 0; i < LPR; ++i) {
+                    const uint4 raw = *place(i);
+                    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+                    const bool none = __shfl_sync(0xffffffffu, src, i * RPI + lane / LPR) < 0;
+                    float v[8], big = 0.f;
                     #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] *= up;
+                    for (int z = 0; z < 4; ++z) {
+                        float2 f = P.dtype == TTKV_BF16
+                            ? make_float2(__uint_as_float(u[z] << 16), __uint_as_float(u[z] & 0xffff0000u)) : __half22float2(u2h(u[z]));
+                        if (none) f = make_float2(0.f, 0.f);
+                        v[2 * z] = f.x;
+                        v[2 * z + 1] = f.y;
+                        big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+                    #pragma unroll
+                    for (int z = 1; z < LPR; z <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, z));
+                    // e brings the row's largest |q| into [1, 2); a negative scale's sign goes to q
+                    const int e = big > 0.f && big < INFINITY ? 127 - int(__float_as_uint(big) >> 23) : 0;
+                    const float up = copysignf(__uint_as_float(uint32_t(min(127 + e, 254)) << 23), P.scale);
                     // dims 0 4 1 5 2 6 3 7, the order of a word's codes
-                    *reinterpret_cast<uint4*>(qb + (c >> 3) * S::KATOM + kmajor_off(t, c & 7)) =
-                        make_uint4(half2_bits(v[0], v[4]), half2_bits(v[1], v[5]), half2_bits(v[2], v[6]), half2_bits(v[3], v[7]));
+                    *place(i) = make_uint4(half2_bits(v[0] * up, v[4] * up), half2_bits(v[1] * up, v[5] * up),
+                                           half2_bits(v[2] * up, v[6] * up), half2_bits(v[3] * up, v[7] * up));
+                    const int e_row = __shfl_sync(0xffffffffu, e, (lane % RPI) * LPR);
+                    if (lane / RPI == i)                      // this lane's own row
+                        // (not 0, which would make NaN of a masked score of -inf)
+                        qf = fmaxf(fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e_row, 1)) << 23), 1e-38f);
                 }
             }
             fence_async_smem();
@@ -399,27 +431,49 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             tc_after();
             note_bad(n - 1, n_tile - 1);
             const bool whole = begin == 0 && n == U;
+            // 32 output lanes at a time, through the warp's rows of Q (read by the last product) so that
+            // neighbouring lanes of the warp write neighbouring bytes
             const int64_t pr = (int64_t(blockIdx.x) * 2 + (ca >= u0 ? 0 : 1)) * CROWS + x * TM + t;
             const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-            const int64_t dst = int64_t(rq.q0 + j) * P.out_stride + int64_t(h * P.G + g) * D;
+            const int64_t dst = !live ? -1 : whole ? int64_t(rq.q0 + j) * P.out_stride + int64_t(h * P.G + g) * D : pr * D;
+            uint4* stage = reinterpret_cast<uint4*>(qb + (w & 3) * 4096);
             #pragma unroll 1
             for (int c = 0; c < NW; ++c) {
                 float o[32];
                 tmem_ld32(lane_base + o_col(x) + 32u * c, o); // column 32 c + 8 i + b holds lane 32 c + 4 b + i
                 tmem_wait_ld();
                 const float f = (bad >> (c / WPG)) & 1u ? __int_as_float(0x7fc00000) : inv;
-                if (!live) continue;
-                if (!whole) {
+                #pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] *= f;
+                __syncwarp();
+                if (!whole) {                                 // 128 bytes a row: 8 lanes, 4 rows at once
                     #pragma unroll
                     for (int b = 0; b < 8; ++b)
-                        *reinterpret_cast<float4*>(P.part_o + pr * D + 32 * c + 4 * b) =
-                            make_float4(o[b] * f, o[8 + b] * f, o[16 + b] * f, o[24 + b] * f);
-                } else {
+                        stage[8 * lane + (b ^ (lane & 7))] = make_uint4(__float_as_uint(o[b]), __float_as_uint(o[8 + b]),
+                                                                        __float_as_uint(o[16 + b]), __float_as_uint(o[24 + b]));
+                    __syncwarp();
+                    #pragma unroll 2
+                    for (int k = 0; k < 8; ++k) {
+                        const int rl = 4 * k + (lane >> 3), b = lane & 7;
+                        const int64_t to = __shfl_sync(0xffffffffu, dst, rl);
+                        if (to >= 0) *reinterpret_cast<uint4*>(P.part_o + to + 32 * c + 4 * b) = stage[8 * rl + (b ^ (rl & 7))];
+                    }
+                } else {                                      // 64 bytes a row: 4 lanes, 8 rows at once
                     #pragma unroll
-                    for (int b = 0; b < 8; b += 2) {
-                        const float v[8] = {o[b] * f, o[8 + b] * f, o[16 + b] * f, o[24 + b] * f,
-                                            o[b + 1] * f, o[9 + b] * f, o[17 + b] * f, o[25 + b] * f};
-                        store8(P.out, P.dtype, dst + 32 * c + 4 * b, P.out_vec == 2, v);
+                    for (int b = 0; b < 8; b += 2)
+                        stage[4 * lane + ((b >> 1) ^ ((lane >> 1) & 3))] =
+                            make_uint4(pack2(o[b], o[8 + b], P.dtype), pack2(o[16 + b], o[24 + b], P.dtype),
+                                       pack2(o[b + 1], o[9 + b], P.dtype), pack2(o[17 + b], o[25 + b], P.dtype));
+                    __syncwarp();
+                    #pragma unroll 1
+                    for (int k = 0; k < 4; ++k) {
+                        const int rl = 8 * k + (lane >> 2), b = lane & 3;
+                        const int64_t to = __shfl_sync(0xffffffffu, dst, rl);
+                        if (to < 0) continue;
+                        uint16_t* p = static_cast<uint16_t*>(P.out) + to + 32 * c + 8 * b;
+                        const uint4 v = stage[4 * rl + (b ^ ((rl >> 1) & 3))];
+                        if (P.out_vec == 2) *reinterpret_cast<uint4*>(p) = v;
+                        else store_chunk_unaligned(p, v);
                     }
                 }
             }
@@ -437,8 +491,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
     } else if (w < 12) {
         // ============================================================== K of a tile as fp16 rows
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOperands));
-        // panels wk and wk + 4, eight tokens at a time: lane (b token of them, a chunk of its row)
-        const int wk = w - 8, b = lane & 7, a = lane >> 3;
+        // panels wk and wk + 4, eight tokens at a time: lane (b token of them, a chunk of its row), so that
+        // eight lanes read 128 bytes of codes and write eight different chunks of the swizzled rows
+        const int wk = w - 8, b = (lane >> 3) ^ ((lane & 4) ? 5 : 0), a = lane & 3;
         uint32_t n_tile = 0;
         while (sg.u < sg.ue) {
             const int n = sg.here(), first = sg.ui, seq = sg.rq.seq;
@@ -667,37 +722,56 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
 }
 
 // ------------------------------------------------------------------ the merge
-// Row block begun in CTA c and cut: its parts in c and in the CTAs behind it. A CTA of the merge takes
-// 8 rows of it.
-constexpr int kMergeRows = 8;
+// Row block begun in CTA c and cut: its parts in c and in the CTAs behind it (one or two as a rule). A
+// CTA of the merge takes 32 rows of it, a thread four lanes of four rows, whose loads are in flight
+// together.
+constexpr int kMergeRows = 32, kMergeEach = 4;
 
 template <int D>
-__global__ void __launch_bounds__(kMergeRows * (D / 4)) q4_chunk_merge_kernel(const AttnParams P) {
+__global__ void __launch_bounds__(kMergeRows / kMergeEach * (D / 4)) q4_chunk_merge_kernel(const AttnParams P) {
+    constexpr int STEP = kMergeRows / kMergeEach;
     pdl_wait();
     const int c0 = blockIdx.x;
     const int4 a = *reinterpret_cast<const int4*>(P.rec + 8 * c0), b = *reinterpret_cast<const int4*>(P.rec + 8 * c0 + 4);
     if (a.x < 0) return;
     const int r = a.x, h = a.y, rb = a.z, u0 = a.w, U = b.x, share = b.y;
-    const Req rq = request(P, r, false);
-    const int i = blockIdx.y * kMergeRows + threadIdx.x / (D / 4), ln = 4 * (threadIdx.x % (D / 4));
-    const int row = rb * CROWS + i;
-    if (row >= rq.ql * P.G) return;
+    const int i0 = blockIdx.y * kMergeRows + threadIdx.x / (D / 4), ln = 4 * (threadIdx.x % (D / 4));
     const int c1 = (u0 + U - 1) / share;
-    auto place = [&](int c) { return (int64_t(c) * 2 + (c * share >= u0 ? 0 : 1)) * CROWS + i; };
-    float M = -INFINITY;
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, P.part_ml[2 * place(c)]);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-    #pragma unroll 4
+    auto place = [&](int c) { return (int64_t(c) * 2 + (c * share >= u0 ? 0 : 1)) * CROWS + i0; };
+    float m[kMergeEach], l[kMergeEach];
+    float4 o[kMergeEach];
+    #pragma unroll
+    for (int k = 0; k < kMergeEach; ++k) {
+        m[k] = -INFINITY;
+        l[k] = 0.f;
+        o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const Req rq = request(P, r, false);
+    const int n_rows = rq.ql * P.G - rb * CROWS;              // rows of the block (the parts of others are not written)
     for (int c = c0; c <= c1; ++c) {
         const int64_t s = place(c);
-        const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * s);
-        const float4 v = *reinterpret_cast<const float4*>(P.part_o + s * D + ln);
-        const float wt = part_weight(ml.x, M);
-        l = fmaf(wt, ml.y, l);
-        o.x = fmaf(wt, v.x, o.x); o.y = fmaf(wt, v.y, o.y); o.z = fmaf(wt, v.z, o.z); o.w = fmaf(wt, v.w, o.w);
+        float2 ml[kMergeEach];
+        float4 v[kMergeEach];
+        #pragma unroll
+        for (int k = 0; k < kMergeEach; ++k) {
+            const bool in = i0 + k * STEP < n_rows;
+            ml[k] = in ? *reinterpret_cast<const float2*>(P.part_ml + 2 * (s + k * STEP)) : make_float2(-INFINITY, 0.f);
+            v[k] = in ? *reinterpret_cast<const float4*>(P.part_o + (s + k * STEP) * D + ln) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        #pragma unroll
+        for (int k = 0; k < kMergeEach; ++k) {
+            const float M = fmaxf(m[k], ml[k].x), wo = part_weight(m[k], M), wn = part_weight(ml[k].x, M);
+            m[k] = M;
+            l[k] = l[k] * wo + ml[k].y * wn;
+            o[k].x = o[k].x * wo + v[k].x * wn;
+            o[k].y = o[k].y * wo + v[k].y * wn;
+            o[k].z = o[k].z * wo + v[k].z * wn;
+            o[k].w = o[k].w * wo + v[k].w * wn;
+        }
     }
-    store_out(P, rq, h, row, D, ln, o, l);
+    #pragma unroll
+    for (int k = 0; k < kMergeEach; ++k)
+        if (i0 + k * STEP < n_rows) store_out(P, rq, h, rb * CROWS + i0 + k * STEP, D, ln, o[k], l[k]);
 }
 
 template <int D, int GRP>
@@ -722,7 +796,7 @@ int launch_chunk(const AttnParams& P, cudaStream_t st) {
     cudaError_t e = cudaLaunchKernelEx(&cfg, k, P);
     if (e != cudaSuccess) { cudaGetLastError(); return fail(TTKV_ERR_CUDA, "q4_chunk_kernel: %s", cudaGetErrorString(e)); }
     cfg.gridDim = dim3(unsigned(P.n_ctas), CROWS / kMergeRows);
-    cfg.blockDim = dim3(kMergeRows * (D / 4));
+    cfg.blockDim = dim3(kMergeRows / kMergeEach * (D / 4));
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, q4_chunk_merge_kernel<D>, P);
     if (e != cudaSuccess) { cudaGetLastError(); return fail(TTKV_ERR_CUDA, "q4_chunk_merge_kernel: %s", cudaGetErrorString(e)); }
