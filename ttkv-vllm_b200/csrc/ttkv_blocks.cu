@@ -6,12 +6,17 @@
 // lies in slot table[r][p / bs] * bs + p % bs. All integers.
 //
 // Bound: launch and load latency (a step moves a few KB to a few hundred KB). So one launch, one
-// cluster of 8 CTAs: every CTA repeats the prefix sum over all requests (a few hundred loads) rather
-// than waiting for another CTA's, keeps each request's start in shared memory, and fills its share
-// of the tokens and of the table rows. The cluster's barrier orders every CTA's read of the count
-// before the write of the new one, which may be the same word.
+// cluster of CTAs (one CTA for a small step): every CTA repeats the prefix sum over all requests (a few
+// hundred loads) rather than waiting for another CTA's, keeps each request's lengths and its end in the
+// free list in shared memory, and then takes its share of the blocks that change hands and of the
+// tokens, each found by a binary search, so that a step has two rounds of loads whatever its mix of
+// lengths. The cluster's barrier orders every CTA's read of the count before the write of the new one,
+// which may be the same word.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
+#include "ttkv_async.cuh"
 #include "ttkv_common.cuh"
 
 namespace ttkv {
@@ -20,6 +25,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kPlanCtas = 8;        // the largest portable cluster
+constexpr int kPlanSmall = 2048;    // tokens and requests that one CTA takes alone
 constexpr int kPlanThreads = 512;
 
 struct PlanParams {
@@ -66,10 +72,18 @@ __device__ __forceinline__ long long scan_inclusive(long long v, long long* wsum
     return v + before;
 }
 
-// base[r]: request r's first entry of its range of the free list, counted from the list's end (plan)
-// or from its old end (release); -1: refused. Returns the blocks taken or returned in all.
+// A request in shared memory: its tokens, its start (plan) and the end of its range of the free list,
+// counted from the list's end (plan) or from its old end (release). A refused request's range is empty
+// and its length is kept as ~seq.
+struct PlanSmem {
+    int32_t* len;
+    int32_t* end;
+    int32_t* start;                                  // [n_reqs + 1]
+};
+
+// Fills len and end; returns the blocks taken or returned in all.
 template <bool RELEASE>
-__device__ int assign_ranges(const PlanParams& P, int avail, int32_t* base, long long* wsum, int32_t* taken) {
+__device__ int assign_ranges(const PlanParams& P, int avail, const PlanSmem& M, long long* wsum, int32_t* taken) {
     const int tid = threadIdx.x;
     const bool first = blockIdx.x == 0;
     long long carry = 0;
@@ -77,14 +91,16 @@ __device__ int assign_ranges(const PlanParams& P, int avail, int32_t* base, long
     __syncthreads();
     for (int r0 = 0; r0 < P.n_reqs; r0 += kPlanThreads) {
         const int r = r0 + tid;
-        int need = 0;
+        int need = 0, seq = 0;
         bool ok = r < P.n_reqs;
         if (ok) {
-            const int seq = P.lens[r];
+            seq = P.lens[r];
             if (RELEASE) {
                 need = blocks_of(seq, P.bs);
             } else {
                 const int a = P.qsl[r], b = P.qsl[r + 1];
+                M.start[r] = a;
+                if (r == P.n_reqs - 1) M.start[P.n_reqs] = b;
                 if (a < 0 || b < a || b > P.n_tokens || seq < b - a) {
                     ok = false;
                     if (first) report(P.status, TTKV_STATUS_QUERY);
@@ -100,89 +116,100 @@ __device__ int assign_ranges(const PlanParams& P, int avail, int32_t* base, long
         }
         long long total;
         const long long end = carry + scan_inclusive(need, wsum, total);
-        if (ok && need > 0 && end > avail) {                 // and so for every later request with a need
+        if (ok && need > 0 && end > avail) {         // and so for every later request with a need
             ok = false;
             if (first) report(P.status, RELEASE ? TTKV_STATUS_POOL_FULL : TTKV_STATUS_POOL_EMPTY);
         }
-        if (r < P.n_reqs) base[r] = ok ? int32_t(min(end - need, (long long)avail)) : -1;
         if (ok && need > 0) atomicMax(taken, int32_t(end));
+        if (r < P.n_reqs) {
+            M.len[r] = ok ? seq : ~max(seq, 0);
+            M.end[r] = ok || end <= avail ? int32_t(min(end, (long long)avail)) : -1;
+        }
         carry += total;
     }
     __syncthreads();
-    return *taken;
+    // from the first refusal for want of room on, every end is the last one granted
+    const int used = *taken;
+    for (int r = tid; r < P.n_reqs; r += kPlanThreads)
+        if (M.end[r] < 0 || M.end[r] > used) M.end[r] = used;
+    if (!RELEASE && P.n_reqs == 0 && tid == 0) M.start[0] = 0;
+    __syncthreads();
+    return used;
 }
 
-__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanParams P) {
+// The first request whose value in `ends` is above e (n_reqs: none).
+__device__ __forceinline__ int find(const int32_t* ends, int n_reqs, int e) {
+    int lo = 0, hi = n_reqs;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (ends[mid] <= e) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanParams P) {
     extern __shared__ int32_t plan_smem[];
     __shared__ long long wsum[32];
     __shared__ int32_t taken;
-    int32_t* base = plan_smem;                       // [n_reqs]
-    int32_t* start = plan_smem + P.n_reqs;           // [n_reqs + 1] query_start_loc
-    const int tid = threadIdx.x, rank = blockIdx.x;
+    const PlanSmem M{plan_smem, plan_smem + P.n_reqs, plan_smem + 2 * P.n_reqs};
+    const int at = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
+    pdl_wait();
+    pdl_trigger();
     const int count = min(max(*P.count, 0), P.capacity);
-    for (int r = tid; r <= P.n_reqs; r += kPlanThreads) start[r] = P.qsl[r];
-    const int used = assign_ranges<false>(P, count, base, wsum, &taken);
+    const int used = assign_ranges<false>(P, count, M, wsum, &taken);
 
-    // the table rows: a warp per request
-    const int lane = tid & 31;
-    for (int r = rank * (kPlanThreads / 32) + (tid >> 5); r < P.n_reqs; r += kPlanCtas * (kPlanThreads / 32)) {
-        const int seq = P.lens[r], ql = start[r + 1] - start[r];
-        int32_t* row = P.table + int64_t(r) * P.bt_stride;
-        const int held = blocks_of(seq - max(ql, 0), P.bs);
-        if (base[r] < 0) {
-            if (lane == 0 && held < P.bt_cols) row[held] = -1;
-            continue;
-        }
-        const int want = blocks_of(seq, P.bs);
-        for (int i = held + lane; i < want; i += 32) row[i] = P.free_blocks[count - 1 - (base[r] + i - held)];
+    // a refused request's row: no block behind those that it holds
+    for (int r = at; r < P.n_reqs; r += step) {
+        if (M.len[r] >= 0) continue;
+        const int held = blocks_of(~M.len[r] - max(M.start[r + 1] - M.start[r], 0), P.bs);
+        if (held < P.bt_cols) P.table[int64_t(r) * P.bt_stride + held] = -1;
     }
-
-    // the tokens: request by a binary search of the starts
-    for (int t = rank * kPlanThreads + tid; t < P.n_tokens; t += kPlanCtas * kPlanThreads) {
-        int lo = 0, hi = P.n_reqs;                   // the last r with start[r] <= t
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (start[mid + 1] <= t) lo = mid + 1; else hi = mid;
-        }
+    // the blocks taken, into their rows
+    for (int e = at; e < used; e += step) {
+        const int r = find(M.end, P.n_reqs, e), first = r ? M.end[r - 1] : 0;
+        const int held = blocks_of(M.len[r] - (M.start[r + 1] - M.start[r]), P.bs);
+        P.table[int64_t(r) * P.bt_stride + held + (e - first)] = P.free_blocks[count - 1 - e];
+    }
+    // the tokens
+    for (int t = at; t < P.n_tokens; t += step) {
+        const int r = find(M.start + 1, P.n_reqs, t);
         int64_t slot = -1;
         int pos = 0;
-        if (lo < P.n_reqs && t >= start[lo] && base[lo] >= 0) {
-            const int seq = P.lens[lo], ql = start[lo + 1] - start[lo];
-            pos = seq - ql + (t - start[lo]);
-            const int held = blocks_of(seq - ql, P.bs), bi = int(unsigned(pos) / unsigned(P.bs));
-            const int blk = bi < held ? P.table[int64_t(lo) * P.bt_stride + bi]
-                                      : P.free_blocks[count - 1 - (base[lo] + bi - held)];
+        if (r < P.n_reqs && t >= M.start[r] && M.len[r] >= 0) {
+            const int ql = M.start[r + 1] - M.start[r], first = r ? M.end[r - 1] : 0;
+            pos = M.len[r] - ql + (t - M.start[r]);
+            const int held = blocks_of(M.len[r] - ql, P.bs), bi = int(unsigned(pos) / unsigned(P.bs));
+            const int blk = bi < held ? P.table[int64_t(r) * P.bt_stride + bi] : P.free_blocks[count - 1 - (first + bi - held)];
             if (blk >= 0) slot = int64_t(blk) * P.bs + (pos - bi * P.bs);
         }
         P.slots[t] = slot;
         if (P.positions) P.positions[t] = pos;
     }
     cg::this_cluster().sync();                       // every CTA has read the count
-    if (rank == 0 && tid == 0) *P.count_out = count - used;
+    if (at == 0) *P.count_out = count - used;
 }
 
-__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) release_blocks_kernel(const PlanParams P) {
+__global__ void __launch_bounds__(kPlanThreads) release_blocks_kernel(const PlanParams P) {
     extern __shared__ int32_t plan_smem[];
     __shared__ long long wsum[32];
     __shared__ int32_t taken;
-    int32_t* base = plan_smem;
-    const int tid = threadIdx.x, rank = blockIdx.x, lane = tid & 31;
+    const PlanSmem M{plan_smem, plan_smem + P.n_reqs, nullptr};
+    const int at = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
+    pdl_wait();
+    pdl_trigger();
     const int count = min(max(*P.count, 0), P.capacity);
-    const int used = assign_ranges<true>(P, P.capacity - count, base, wsum, &taken);
-    for (int r = rank * (kPlanThreads / 32) + (tid >> 5); r < P.n_reqs; r += kPlanCtas * (kPlanThreads / 32)) {
-        if (base[r] < 0) continue;
-        const int n = blocks_of(P.lens[r], P.bs);
-        const int32_t* row = P.table + int64_t(r) * P.bt_stride;
-        bool bad = false;
-        for (int i = lane; i < n; i += 32) {
-            const int32_t id = row[i];
-            bad |= id < 0;
-            P.free_blocks[count + base[r] + i] = id;
-        }
-        if (bad) report(P.status, TTKV_STATUS_BLOCK_RANGE);
+    const int used = assign_ranges<true>(P, P.capacity - count, M, wsum, &taken);
+    bool bad = false;
+    #pragma unroll 4
+    for (int e = at; e < used; e += step) {
+        const int r = find(M.end, P.n_reqs, e);
+        const int32_t id = __ldg(P.table + int64_t(r) * P.bt_stride + (e - (r ? M.end[r - 1] : 0)));
+        bad |= id < 0;
+        P.free_blocks[count + e] = id;
     }
+    if (bad) report(P.status, TTKV_STATUS_BLOCK_RANGE);
     cg::this_cluster().sync();
-    if (rank == 0 && tid == 0) *P.count_out = count + used;
+    if (at == 0) *P.count_out = count + used;
 }
 
 int check_plan(const PlanParams& P) {
@@ -199,10 +226,28 @@ int check_plan(const PlanParams& P) {
 }
 
 template <typename K>
-int launch_plan(K kernel, const PlanParams& P, size_t smem, const char* what, void* stream) {
+int launch_plan(K kernel, const PlanParams& P, int work, size_t smem, const char* what, void* stream) {
     if (int e = raise_smem_limit(reinterpret_cast<const void*>(kernel), what)) return e;
-    kernel<<<kPlanCtas, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(P);
-    return check_launch(what);
+    const unsigned ctas = work <= kPlanSmall ? 1 : kPlanCtas;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(TTKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    }
+    return TTKV_OK;
 }
 
 }  // namespace
@@ -220,7 +265,8 @@ extern "C" int ttkv_plan_step(int32_t* block_table, int64_t bt_stride, int32_t b
                  slots, positions, n_tokens, status};
     if (int e = check_plan(P)) return e;
     if (!query_start_loc || (n_tokens > 0 && !slots)) return fail(TTKV_ERR_ARG, "plan: null pointer");
-    return launch_plan(plan_step_kernel, P, (2 * size_t(n_reqs) + 1) * sizeof(int32_t), "plan_step_kernel", stream);
+    return launch_plan(plan_step_kernel, P, std::max(n_tokens, n_reqs), (3 * size_t(n_reqs) + 1) * sizeof(int32_t),
+                       "plan_step_kernel", stream);
 }
 
 extern "C" int ttkv_release_blocks(const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
@@ -230,5 +276,7 @@ extern "C" int ttkv_release_blocks(const int32_t* block_table, int64_t bt_stride
     PlanParams P{const_cast<int32_t*>(block_table), bt_stride, bt_cols, lens, nullptr, n_reqs, free_blocks,
                  capacity, free_count, free_count_out, block_size, nullptr, nullptr, 0, status};
     if (int e = check_plan(P)) return e;
-    return launch_plan(release_blocks_kernel, P, (size_t(n_reqs) + 1) * sizeof(int32_t), "release_blocks_kernel", stream);
+    // (how many blocks come back is known on the device only: a row holds up to bt_cols)
+    return launch_plan(release_blocks_kernel, P, int(std::min(int64_t(n_reqs) * bt_cols, int64_t(kPlanSmall) + 1)),
+                       (2 * size_t(n_reqs) + 1) * sizeof(int32_t), "release_blocks_kernel", stream);
 }
