@@ -385,83 +385,104 @@ typedef struct ttkv_q4_cache {
 /* Bytes of one panel, 0 for a geometry that is not served. */
 size_t ttkv_q4_panel_bytes(int32_t d, int32_t group);
 
+/* The calls below take one struct, so that a binding passes one pointer. */
+
 /* Quantise k, v (token i at + i * stride elements, [H, d] contiguous) into slots[i], i < n. The
  * slots of one call differ from each other (a slot given twice holds parts of both tokens). A slot
  * outside the cache is refused on the device (TTKV_STATUS_SLOT_RANGE) and its token skipped; with
- * TTKV_CACHE_SKIP_PAD a negative one is skipped silently. */
-int ttkv_q4_write(const ttkv_q4_cache_t* cache, const int64_t* slots, int32_t n,
-                  const void* k, int32_t k_dtype, int64_t k_stride,
-                  const void* v, int32_t v_dtype, int64_t v_stride, int32_t* status, void* stream);
+ * TTKV_CACHE_SKIP_PAD a negative one is skipped silently. ttkv_q4_read: the stored values of slots[i]
+ * into k, v, rounded once to their types; rows of skipped or refused slots are left as they were. */
+typedef struct ttkv_q4_store_args {
+    ttkv_q4_cache_t cache;
+    const int64_t* slots;
+    void* k;
+    void* v;
+    int64_t k_stride, v_stride;
+    int32_t n, k_dtype, v_dtype;
+    int32_t* status;
+    void* stream;
+} ttkv_q4_store_args_t;
 
-/* The stored values of slots[i] into k, v (laid out as for the write), rounded once to their types.
- * Rows of skipped or refused slots are left as they were. */
-int ttkv_q4_read(const ttkv_q4_cache_t* cache, const int64_t* slots, int32_t n,
-                 void* k, int32_t k_dtype, int64_t k_stride,
-                 void* v, int32_t v_dtype, int64_t v_stride, int32_t* status, void* stream);
+int ttkv_q4_write(const ttkv_q4_store_args_t* args);
+int ttkv_q4_read(const ttkv_q4_store_args_t* args);
 
-/* Paging of a 4-bit read: request r's first seq_lens[r] tokens are stored in the blocks of row r. */
-typedef struct ttkv_q4_batch {
-    const int32_t* block_table;
-    int64_t bt_stride;
-    int32_t bt_cols;
-    const int32_t* seq_lens;
-    int32_t n_reqs;
-} ttkv_q4_batch_t;
-
-/* Decode: request r's one query (q + r * q_stride elements, [HQ, d], fp16 or bf16) over its stored
- * tokens, into out + r * out_stride in q's type. A request with seq_len 0 gets zeros. A request
- * longer than its block-table row is refused (TTKV_STATUS_ROW_SHORT), its rows left as they were;
- * one with a block id outside the cache gets NaN (TTKV_STATUS_BLOCK_RANGE). The launch depends on
- * nothing that varies with the batch but n_reqs, so a capture replays any lengths. */
-size_t ttkv_q4_decode_workspace_bytes(const ttkv_q4_cache_t* cache, int32_t n_reqs, int32_t HQ);
-int ttkv_q4_decode(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch,
-                   const void* q, int32_t q_dtype, int64_t q_stride, int32_t HQ, float scale,
-                   void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
-                   int32_t* status, void* stream);
-
-/* Chunks: request r's queries are rows q_start[r] .. + q_len[r] of q, query j at position
+/* Attention over a 4-bit cache. Request r's first seq_lens[r] tokens are stored in the blocks of row r
+ * of the table; queries and outputs are fp16 or bf16 (`dtype`), [HQ, d] contiguous, rows q_stride and
+ * out_stride elements apart.
+ *
+ * Decode: request r's one query is row r (q_start, q_len, n_rows, max_q_len and max_seq_len are not
+ * read). A request with seq_len 0 gets zeros. The launch depends on nothing that varies with the batch
+ * but n_reqs, so a capture replays any lengths.
+ *
+ * Prefill: request r's queries are rows q_start[r] .. + q_len[r] of n_rows, query j at position
  * seq_len - q_len + j, which sees the stored tokens up to and with its own position. max_q_len and
  * max_seq_len bound the batch's q_len and seq_lens; a request above either is refused
- * (TTKV_STATUS_QUERY, TTKV_STATUS_SEQ_BOUND), as is one with q_len > seq_len (TTKV_STATUS_QUERY) or
- * with query rows outside [0, n_rows) (TTKV_STATUS_QUERY); its rows are left as they were. Rows of
- * no request are left as they were. */
-size_t ttkv_q4_prefill_workspace_bytes(const ttkv_q4_cache_t* cache, int32_t n_reqs, int32_t HQ,
-                                       int32_t max_q_len, int32_t max_seq_len);
-int ttkv_q4_prefill(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch,
-                    const int32_t* q_start, const int32_t* q_len,
-                    const void* q, int32_t q_dtype, int64_t q_stride, int32_t n_rows, int32_t HQ,
-                    float scale, void* out, int64_t out_stride, int32_t max_q_len,
-                    int32_t max_seq_len, void* workspace, size_t workspace_bytes,
-                    int32_t* status, void* stream);
+ * (TTKV_STATUS_QUERY, TTKV_STATUS_SEQ_BOUND), as is one with q_len > seq_len or with query rows outside
+ * [0, n_rows) (TTKV_STATUS_QUERY). Rows of no request are left as they were.
+ *
+ * Both: a request longer than its block-table row is refused (TTKV_STATUS_ROW_SHORT); a refused
+ * request's rows are left as they were. Queries that see a block id outside the cache get NaN
+ * (TTKV_STATUS_BLOCK_RANGE). `workspace` is 16-byte aligned and used by one call at a time. */
+typedef struct ttkv_q4_attn_args {
+    ttkv_q4_cache_t cache;
+    const int32_t* block_table;
+    const int32_t* seq_lens;
+    const int32_t* q_start;
+    const int32_t* q_len;
+    const void* q;
+    void* out;
+    int64_t bt_stride, q_stride, out_stride;
+    int32_t bt_cols, n_reqs, n_rows, HQ, dtype, max_q_len, max_seq_len;
+    float scale;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t* status;
+    void* stream;
+} ttkv_q4_attn_args_t;
+
+size_t ttkv_q4_decode_workspace_bytes(int32_t d, int32_t n_reqs, int32_t group_heads);
+int ttkv_q4_decode(const ttkv_q4_attn_args_t* args);
+/* group_heads = HQ / H in both */
+size_t ttkv_q4_prefill_workspace_bytes(int32_t d, int32_t n_reqs, int32_t group_heads, int32_t max_q_len);
+int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args);
 
 /* ---------------------------------------------------------------- block tables on the device
  * No counterpart in the reference, whose engine builds them on the host.
  *
- * ttkv_plan_step: request r has seq_lens[r] tokens after this step, of which query_start_loc[r+1] -
- * query_start_loc[r] are new; it holds ceil((seq - new) / block_size) blocks in its row. The blocks
+ * ttkv_plan_step: request r has lens[r] tokens after this step, of which query_start_loc[r+1] -
+ * query_start_loc[r] are new; it holds ceil((len - new) / block_size) blocks in its row. The blocks
  * it lacks are popped off the end of the free list (free_blocks[0 .. *free_count)), in request
  * order, into its row; slots[t] and positions[t] (may be null) of every token t < n_tokens are
  * written, -1 and 0 for tokens of no request. *free_count_out = blocks left (may be free_count).
  * Requests are served in order until the list runs out: that one and every later one that needs a
  * block get none (TTKV_STATUS_POOL_EMPTY). A refused request (that, a row too short:
- * TTKV_STATUS_ROW_SHORT, new > seq or tokens outside n_tokens: TTKV_STATUS_QUERY) gets slots -1, and
+ * TTKV_STATUS_ROW_SHORT, new > len or tokens outside n_tokens: TTKV_STATUS_QUERY) gets slots -1, and
  * where its row has room the entry behind its held blocks becomes -1, so a read of it is refused too.
  *
  * ttkv_release_blocks: pushes the ceil(lens[r] / block_size) blocks of each request's row onto the
  * free list, in request order (lens[r] <= 0: none). capacity = the entries free_blocks has room for;
- * requests that do not fit are left out (TTKV_STATUS_POOL_FULL), every later one too.
+ * requests that do not fit are left out (TTKV_STATUS_POOL_FULL), every later one too. (query_start_loc,
+ * slots, positions and n_tokens are not read.)
  *
  * n_reqs is at most TTKV_PLAN_MAX_REQS. */
 #define TTKV_PLAN_MAX_REQS 16384
-int ttkv_plan_step(int32_t* block_table, int64_t bt_stride, int32_t bt_cols, const int32_t* seq_lens,
-                   const int32_t* query_start_loc, int32_t n_reqs, const int32_t* free_blocks,
-                   int32_t capacity, const int32_t* free_count, int32_t* free_count_out,
-                   int32_t block_size, int64_t* slots, int64_t* positions, int32_t n_tokens,
-                   int32_t* status, void* stream);
-int ttkv_release_blocks(const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
-                        const int32_t* lens, int32_t n_reqs, int32_t* free_blocks, int32_t capacity,
-                        const int32_t* free_count, int32_t* free_count_out, int32_t block_size,
-                        int32_t* status, void* stream);
+typedef struct ttkv_plan_args {
+    int32_t* block_table;
+    const int32_t* lens;
+    const int32_t* query_start_loc;
+    int32_t* free_blocks;
+    const int32_t* free_count;
+    int32_t* free_count_out;
+    int64_t* slots;
+    int64_t* positions;
+    int64_t bt_stride;
+    int32_t bt_cols, n_reqs, capacity, block_size, n_tokens;
+    int32_t* status;
+    void* stream;
+} ttkv_plan_args_t;
+
+int ttkv_plan_step(const ttkv_plan_args_t* args);
+int ttkv_release_blocks(const ttkv_plan_args_t* args);
 
 #ifdef __cplusplus
 }

@@ -60,85 +60,117 @@ def test_ops_run_only_on_the_gpu():
 A = 1 << 20
 
 
-def _cache(**kw):
-    f = dict(base=A, n_blocks=4, H=2, d=128, group=64, block_size=16, flags=0) | kw
-    return _lib.Q4Cache(*(f[n] for n, _ in _lib.Q4Cache._fields_))
+CACHE = dict(base=A, n_blocks=4, H=2, d=128, group=64, block_size=16, flags=0)
+STORE = CACHE | dict(slots=A, k=A, v=A, k_stride=256, v_stride=256, n=4, k_dtype=2, v_dtype=2, status=A, stream=0)
+ATTN = CACHE | dict(block_table=A, seq_lens=A, q_start=A, q_len=A, q=A, out=A, bt_stride=4, q_stride=512, out_stride=512,
+                    bt_cols=4, n_reqs=3, n_rows=9, HQ=4, dtype=2, max_q_len=3, max_seq_len=9, scale=1.0, workspace=A,
+                    workspace_bytes=1 << 30, status=A, stream=0)
+PLAN = dict(block_table=A, lens=A, query_start_loc=A, free_blocks=A, free_count=A, free_count_out=A, slots=A, positions=A,
+            bt_stride=8, bt_cols=8, n_reqs=3, capacity=50, block_size=16, n_tokens=9, status=A, stream=0)
+PACKINGS = {"store": (_lib.Q4StoreArgs, _lib.Q4_STORE, STORE), "attn": (_lib.Q4AttnArgs, _lib.Q4_ATTN, ATTN),
+            "plan": (_lib.PlanArgs, _lib.PLAN, PLAN)}
 
 
-def _batch(**kw):
-    f = dict(block_table=A, bt_stride=4, bt_cols=4, seq_lens=A, n_reqs=3) | kw
-    return _lib.Q4Batch(*(f[n] for n, _ in _lib.Q4Batch._fields_))
+def _call(fn, fields, packing, **kw):
+    return fn(packing.pack(*(fields | kw).values()))
+
+
+def _store(fn, **kw):
+    return _call(fn, STORE, _lib.Q4_STORE, **kw)
+
+
+def _attn(fn, **kw):
+    return _call(fn, ATTN, _lib.Q4_ATTN, **kw)
+
+
+def _plan(fn, **kw):
+    return _call(fn, PLAN, _lib.PLAN, **kw)
+
+
+@pytest.mark.parametrize("name", PACKINGS)
+def test_packings_match_the_structs(name):
+    """A packed call lays its fields out as the C struct does: distinct values come back by name."""
+    cls, packing, fields = PACKINGS[name]
+    flat = {}
+    for f, t in cls._fields_:
+        if issubclass(t, C.Structure):
+            flat |= dict(t._fields_)
+        else:
+            flat[f] = t
+    assert list(flat) == list(fields)
+    values = {f: float(i) if t is C.c_float else i + 1 for i, (f, t) in enumerate(flat.items())}
+    raw = packing.pack(*values.values())
+    assert len(raw) == C.sizeof(cls)
+    got = cls.from_buffer_copy(raw)
+    for f, v in values.items():
+        assert getattr(got if hasattr(got, f) else got.cache, f) == v, f
 
 
 BAD_CACHES = [(dict(d=96), _lib.ERR_UNSUPPORTED), (dict(group=16), _lib.ERR_UNSUPPORTED),
               (dict(d=64, group=128), _lib.ERR_UNSUPPORTED), (dict(block_size=8), _lib.ERR_UNSUPPORTED),
-              (dict(block_size=40), _lib.ERR_UNSUPPORTED), (dict(H=0), _lib.ERR_ARG), (dict(base=None), _lib.ERR_ARG),
+              (dict(block_size=40), _lib.ERR_UNSUPPORTED), (dict(H=0), _lib.ERR_ARG), (dict(base=0), _lib.ERR_ARG),
               (dict(n_blocks=-1), _lib.ERR_ARG), (dict(base=A + 8), _lib.ERR_ALIGN), (dict(H=70000), _lib.ERR_UNSUPPORTED)]
 
 
 @pytest.mark.parametrize("kw,code", BAD_CACHES)
 def test_bad_caches(kw, code):
-    L, c, b = _lib.lib(), C.byref(_cache(**kw)), C.byref(_batch())
-    assert L.ttkv_q4_write(c, A, 1, A, 2, 256, A, 2, 256, A, None) == code
-    assert L.ttkv_q4_read(c, A, 1, A, 2, 256, A, 2, 256, A, None) == code
-    assert L.ttkv_q4_decode(c, b, A, 2, 512, 4, 1.0, A, 512, A, 1 << 30, A, None) == code
-    assert L.ttkv_q4_prefill(c, b, A, A, A, 2, 512, 9, 4, 1.0, A, 512, 3, 9, A, 1 << 30, A, None) == code
+    L = _lib.lib()
+    assert _store(L.ttkv_q4_write, **kw) == code
+    assert _store(L.ttkv_q4_read, **kw) == code
+    assert _attn(L.ttkv_q4_decode, **kw) == code
+    assert _attn(L.ttkv_q4_prefill, **kw) == code
     assert L.ttkv_last_error()
 
 
 def test_store_refusals():
-    L, c = _lib.lib(), C.byref(_cache())
-    ok = [A, 4, A, 2, 256, A, 2, 256]
-    for i, v, code in ((0, None, _lib.ERR_ARG), (1, -1, _lib.ERR_ARG), (2, None, _lib.ERR_ARG), (3, 3, _lib.ERR_ARG),
-                       (4, 255, _lib.ERR_ARG), (6, -1, _lib.ERR_ARG), (7, 0, _lib.ERR_ARG), (2, A + 1, _lib.ERR_ALIGN)):
-        args = list(ok)
-        args[i] = v
+    L = _lib.lib()
+    for kw, code in ((dict(slots=0), _lib.ERR_ARG), (dict(n=-1), _lib.ERR_ARG), (dict(k=0), _lib.ERR_ARG),
+                     (dict(k_dtype=3), _lib.ERR_ARG), (dict(k_stride=255), _lib.ERR_ARG), (dict(v_dtype=-1), _lib.ERR_ARG),
+                     (dict(v_stride=0), _lib.ERR_ARG), (dict(k=A + 1), _lib.ERR_ALIGN),
+                     (dict(v=A + 2, v_dtype=0), _lib.ERR_ALIGN)):
         for fn in (L.ttkv_q4_write, L.ttkv_q4_read):
-            assert fn(c, *args, A, None) == code, (i, v)
-    assert L.ttkv_q4_write(None, *ok, A, None) == _lib.ERR_ARG
-    assert L.ttkv_q4_write(c, A, 4, A + 2, 0, 256, A, 2, 256, A, None) == _lib.ERR_ALIGN
-    assert L.ttkv_q4_write(c, None, 0, None, 2, 256, None, 2, 256, A, None) == _lib.OK       # nothing to do
+            assert _store(fn, **kw) == code, kw
+            assert fn(None) == _lib.ERR_ARG
+    assert _store(L.ttkv_q4_write, n=0, slots=0, k=0, v=0) == _lib.OK          # nothing to do
 
 
 def test_attention_refusals():
-    L, c = _lib.lib(), C.byref(_cache())
-    ws = L.ttkv_q4_decode_workspace_bytes(c, 3, 4)
-    assert ws > 0
-    ok = [A, 2, 512, 4, 1.0, A, 512, A, ws]
-    for i, v, code in ((0, None, _lib.ERR_ARG), (1, 0, _lib.ERR_UNSUPPORTED), (2, -1, _lib.ERR_ARG), (3, 3, _lib.ERR_ARG),
-                       (3, 1, _lib.ERR_ARG), (5, None, _lib.ERR_ARG), (6, -8, _lib.ERR_ARG), (7, None, _lib.ERR_WORKSPACE),
-                       (8, ws - 1, _lib.ERR_WORKSPACE), (7, A + 4, _lib.ERR_ALIGN), (0, A + 1, _lib.ERR_ALIGN)):
-        args = list(ok)
-        args[i] = v
-        assert L.ttkv_q4_decode(c, C.byref(_batch()), *args, A, None) == code, (i, v)
-    for kw, code in ((dict(block_table=None), _lib.ERR_ARG), (dict(seq_lens=None), _lib.ERR_ARG), (dict(n_reqs=-1), _lib.ERR_ARG),
-                     (dict(bt_cols=-1), _lib.ERR_ARG), (dict(n_reqs=70000), _lib.ERR_UNSUPPORTED)):
-        assert L.ttkv_q4_decode(c, C.byref(_batch(**kw)), *ok, A, None) == code, kw
-    assert L.ttkv_q4_decode(c, None, *ok, A, None) == _lib.ERR_ARG
-    assert L.ttkv_q4_decode(c, C.byref(_batch(n_reqs=0)), *ok, A, None) == _lib.OK
-    b = C.byref(_batch())
-    ws = L.ttkv_q4_prefill_workspace_bytes(c, 3, 4, 64, 100)
-    for args in ((None, A, 64, 100), (A, None, 64, 100), (A, A, -1, 100), (A, A, 64, -1)):
-        assert L.ttkv_q4_prefill(c, b, args[0], args[1], A, 2, 512, 99, 4, 1.0, A, 512, args[2], args[3], A, ws, A, None) == _lib.ERR_ARG
-    assert L.ttkv_q4_prefill(c, b, A, A, A, 2, 512, 0, 4, 1.0, A, 512, 64, 100, A, ws, A, None) == _lib.OK
+    L = _lib.lib()
+    ws = L.ttkv_q4_decode_workspace_bytes(128, 3, 2)
+    wp = [L.ttkv_q4_prefill_workspace_bytes(128, 3, 2, n) for n in (3, 64)]
+    assert ws > 0 and min(wp) > 0
+    both = ((dict(q=0), _lib.ERR_ARG), (dict(out=0), _lib.ERR_ARG), (dict(dtype=0), _lib.ERR_UNSUPPORTED),
+            (dict(q_stride=-1), _lib.ERR_ARG), (dict(out_stride=-8), _lib.ERR_ARG), (dict(HQ=3), _lib.ERR_ARG),
+            (dict(HQ=1), _lib.ERR_ARG), (dict(workspace=0), _lib.ERR_WORKSPACE), (dict(workspace=A + 4), _lib.ERR_ALIGN),
+            (dict(q=A + 1), _lib.ERR_ALIGN), (dict(block_table=0), _lib.ERR_ARG), (dict(seq_lens=0), _lib.ERR_ARG),
+            (dict(n_reqs=-1), _lib.ERR_ARG), (dict(bt_cols=-1), _lib.ERR_ARG), (dict(n_reqs=70000), _lib.ERR_UNSUPPORTED))
+    for fn, extra in ((L.ttkv_q4_decode, {}), (L.ttkv_q4_prefill, {}), (L.ttkv_q4_prefill, dict(max_q_len=64))):
+        for kw, code in both:
+            assert _attn(fn, **(extra | kw)) == code, kw
+        assert _attn(fn, n_reqs=0, **extra) == _lib.OK
+        assert fn(None) == _lib.ERR_ARG
+    assert _attn(L.ttkv_q4_decode, workspace_bytes=ws - 1) == _lib.ERR_WORKSPACE
+    for n, need in zip((3, 64), wp):
+        assert _attn(L.ttkv_q4_prefill, max_q_len=n, workspace_bytes=need - 1) == _lib.ERR_WORKSPACE
+    for kw in (dict(q_start=0), dict(q_len=0), dict(max_q_len=-1), dict(max_seq_len=-1), dict(n_rows=-1)):
+        assert _attn(L.ttkv_q4_prefill, **kw) == _lib.ERR_ARG, kw
+    assert _attn(L.ttkv_q4_prefill, max_q_len=2 ** 30) == _lib.ERR_UNSUPPORTED
+    assert _attn(L.ttkv_q4_prefill, n_rows=0) == _lib.OK
 
 
 def test_plan_refusals():
     L = _lib.lib()
-    ok = [A, 8, 8, A, A, 3, A, 50, A, A, 16, A, A, 9]
-    for i, v, code in ((0, None, _lib.ERR_ARG), (1, 7, _lib.ERR_ARG), (2, -1, _lib.ERR_ARG), (3, None, _lib.ERR_ARG),
-                       (4, None, _lib.ERR_ARG), (5, -1, _lib.ERR_ARG), (6, None, _lib.ERR_ARG), (7, -1, _lib.ERR_ARG),
-                       (8, None, _lib.ERR_ARG), (9, None, _lib.ERR_ARG), (10, 0, _lib.ERR_ARG), (11, None, _lib.ERR_ARG),
-                       (13, -1, _lib.ERR_ARG), (5, _lib.PLAN_MAX_REQS + 1, _lib.ERR_UNSUPPORTED)):
-        args = list(ok)
-        args[i] = v
-        assert L.ttkv_plan_step(*args, A, None) == code, (i, v)
-    ok = [A, 8, 8, A, 3, A, 50, A, A, 16]
-    for i, v, code in ((0, None, _lib.ERR_ARG), (3, None, _lib.ERR_ARG), (5, None, _lib.ERR_ARG), (7, None, _lib.ERR_ARG),
-                       (8, None, _lib.ERR_ARG), (9, -16, _lib.ERR_ARG), (4, _lib.PLAN_MAX_REQS + 1, _lib.ERR_UNSUPPORTED)):
-        args = list(ok)
-        args[i] = v
-        assert L.ttkv_release_blocks(*args, A, None) == code, (i, v)
+    both = ((dict(block_table=0), _lib.ERR_ARG), (dict(bt_stride=7), _lib.ERR_ARG), (dict(bt_cols=-1), _lib.ERR_ARG),
+            (dict(lens=0), _lib.ERR_ARG), (dict(n_reqs=-1), _lib.ERR_ARG), (dict(free_blocks=0), _lib.ERR_ARG),
+            (dict(capacity=-1), _lib.ERR_ARG), (dict(free_count=0), _lib.ERR_ARG), (dict(free_count_out=0), _lib.ERR_ARG),
+            (dict(block_size=0), _lib.ERR_ARG), (dict(block_size=-16), _lib.ERR_ARG),
+            (dict(n_reqs=_lib.PLAN_MAX_REQS + 1), _lib.ERR_UNSUPPORTED))
+    for fn in (L.ttkv_plan_step, L.ttkv_release_blocks):
+        for kw, code in both:
+            assert _plan(fn, **kw) == code, kw
+        assert fn(None) == _lib.ERR_ARG
+    for kw in (dict(query_start_loc=0), dict(slots=0), dict(n_tokens=-1)):
+        assert _plan(L.ttkv_plan_step, **kw) == _lib.ERR_ARG, kw
 
 
 def test_structs_match_the_header(tmp_path):
@@ -146,7 +178,8 @@ def test_structs_match_the_header(tmp_path):
     if cc is None:
         pytest.skip("no C compiler")
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "ttkv_b200.h"', "int main(void) {"]
-    structs = {"ttkv_q4_cache_t": _lib.Q4Cache, "ttkv_q4_batch_t": _lib.Q4Batch}
+    structs = {"ttkv_q4_cache_t": _lib.Q4Cache, "ttkv_q4_store_args_t": _lib.Q4StoreArgs,
+               "ttkv_q4_attn_args_t": _lib.Q4AttnArgs, "ttkv_plan_args_t": _lib.PlanArgs}
     for name, py in structs.items():
         lines.append(f'printf("%zu\\n", sizeof({name}));')
         lines += [f'printf("%zu\\n", offsetof({name}, {f}));' for f, _ in py._fields_]

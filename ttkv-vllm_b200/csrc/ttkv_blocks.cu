@@ -28,23 +28,7 @@ constexpr int kPlanCtas = 8;        // the largest portable cluster
 constexpr int kPlanSmall = 2048;    // tokens and requests that one CTA takes alone
 constexpr int kPlanThreads = 512;
 
-struct PlanParams {
-    int32_t* table;
-    int64_t bt_stride;
-    int32_t bt_cols;
-    const int32_t* lens;            // seq_lens of a plan, lens of a release
-    const int32_t* qsl;
-    int32_t n_reqs;
-    int32_t* free_blocks;
-    int32_t capacity;
-    const int32_t* count;
-    int32_t* count_out;
-    int32_t bs;
-    int64_t* slots;
-    int64_t* positions;
-    int32_t n_tokens;
-    int32_t* status;
-};
+using PlanParams = ttkv_plan_args_t;
 
 __device__ __forceinline__ int blocks_of(int tokens, int bs) {
     return tokens > 0 ? int((unsigned(tokens) + unsigned(bs) - 1u) / unsigned(bs)) : 0;
@@ -96,19 +80,19 @@ __device__ int assign_ranges(const PlanParams& P, int avail, const PlanSmem& M, 
         if (ok) {
             seq = P.lens[r];
             if (RELEASE) {
-                need = blocks_of(seq, P.bs);
+                need = blocks_of(seq, P.block_size);
             } else {
-                const int a = P.qsl[r], b = P.qsl[r + 1];
+                const int a = P.query_start_loc[r], b = P.query_start_loc[r + 1];
                 M.start[r] = a;
                 if (r == P.n_reqs - 1) M.start[P.n_reqs] = b;
                 if (a < 0 || b < a || b > P.n_tokens || seq < b - a) {
                     ok = false;
                     if (first) report(P.status, TTKV_STATUS_QUERY);
                 } else {
-                    need = blocks_of(seq, P.bs) - blocks_of(seq - (b - a), P.bs);
+                    need = blocks_of(seq, P.block_size) - blocks_of(seq - (b - a), P.block_size);
                 }
             }
-            if (ok && blocks_of(seq, P.bs) > P.bt_cols) {
+            if (ok && blocks_of(seq, P.block_size) > P.bt_cols) {
                 ok = false;
                 need = 0;
                 if (first) report(P.status, TTKV_STATUS_ROW_SHORT);
@@ -155,20 +139,20 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanParam
     const int at = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
     pdl_wait();
     pdl_trigger();
-    const int count = min(max(*P.count, 0), P.capacity);
+    const int count = min(max(*P.free_count, 0), P.capacity);
     const int used = assign_ranges<false>(P, count, M, wsum, &taken);
 
     // a refused request's row: no block behind those that it holds
     for (int r = at; r < P.n_reqs; r += step) {
         if (M.len[r] >= 0) continue;
-        const int held = blocks_of(~M.len[r] - max(M.start[r + 1] - M.start[r], 0), P.bs);
-        if (held < P.bt_cols) P.table[int64_t(r) * P.bt_stride + held] = -1;
+        const int held = blocks_of(~M.len[r] - max(M.start[r + 1] - M.start[r], 0), P.block_size);
+        if (held < P.bt_cols) P.block_table[int64_t(r) * P.bt_stride + held] = -1;
     }
     // the blocks taken, into their rows
     for (int e = at; e < used; e += step) {
         const int r = find(M.end, P.n_reqs, e), first = r ? M.end[r - 1] : 0;
-        const int held = blocks_of(M.len[r] - (M.start[r + 1] - M.start[r]), P.bs);
-        P.table[int64_t(r) * P.bt_stride + held + (e - first)] = P.free_blocks[count - 1 - e];
+        const int held = blocks_of(M.len[r] - (M.start[r + 1] - M.start[r]), P.block_size);
+        P.block_table[int64_t(r) * P.bt_stride + held + (e - first)] = P.free_blocks[count - 1 - e];
     }
     // the tokens
     for (int t = at; t < P.n_tokens; t += step) {
@@ -178,15 +162,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanParam
         if (r < P.n_reqs && t >= M.start[r] && M.len[r] >= 0) {
             const int ql = M.start[r + 1] - M.start[r], first = r ? M.end[r - 1] : 0;
             pos = M.len[r] - ql + (t - M.start[r]);
-            const int held = blocks_of(M.len[r] - ql, P.bs), bi = int(unsigned(pos) / unsigned(P.bs));
-            const int blk = bi < held ? P.table[int64_t(r) * P.bt_stride + bi] : P.free_blocks[count - 1 - (first + bi - held)];
-            if (blk >= 0) slot = int64_t(blk) * P.bs + (pos - bi * P.bs);
+            const int held = blocks_of(M.len[r] - ql, P.block_size), bi = int(unsigned(pos) / unsigned(P.block_size));
+            const int blk = bi < held ? P.block_table[int64_t(r) * P.bt_stride + bi] : P.free_blocks[count - 1 - (first + bi - held)];
+            if (blk >= 0) slot = int64_t(blk) * P.block_size + (pos - bi * P.block_size);
         }
         P.slots[t] = slot;
         if (P.positions) P.positions[t] = pos;
     }
     cg::this_cluster().sync();                       // every CTA has read the count
-    if (at == 0) *P.count_out = count - used;
+    if (at == 0) *P.free_count_out = count - used;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) release_blocks_kernel(const PlanParams P) {
@@ -197,28 +181,29 @@ __global__ void __launch_bounds__(kPlanThreads) release_blocks_kernel(const Plan
     const int at = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
     pdl_wait();
     pdl_trigger();
-    const int count = min(max(*P.count, 0), P.capacity);
+    const int count = min(max(*P.free_count, 0), P.capacity);
     const int used = assign_ranges<true>(P, P.capacity - count, M, wsum, &taken);
     bool bad = false;
     #pragma unroll 4
     for (int e = at; e < used; e += step) {
         const int r = find(M.end, P.n_reqs, e);
-        const int32_t id = __ldg(P.table + int64_t(r) * P.bt_stride + (e - (r ? M.end[r - 1] : 0)));
+        const int32_t id = __ldg(P.block_table + int64_t(r) * P.bt_stride + (e - (r ? M.end[r - 1] : 0)));
         bad |= id < 0;
         P.free_blocks[count + e] = id;
     }
     if (bad) report(P.status, TTKV_STATUS_BLOCK_RANGE);
     cg::this_cluster().sync();
-    if (at == 0) *P.count_out = count + used;
+    if (at == 0) *P.free_count_out = count + used;
 }
 
-int check_plan(const PlanParams& P) {
-    if (!P.count || !P.count_out || (P.n_reqs > 0 && !P.lens) || (P.n_reqs > 0 && P.bt_cols > 0 && !P.table) ||
-        (P.capacity > 0 && !P.free_blocks))
+int check_plan(const ttkv_plan_args_t* p) {
+    if (!p) return fail(TTKV_ERR_ARG, "plan: null arguments");
+    const ttkv_plan_args_t& P = *p;
+    if (!P.free_count || !P.free_count_out || (P.n_reqs > 0 && !P.lens) ||
+        (P.n_reqs > 0 && P.bt_cols > 0 && !P.block_table) || (P.capacity > 0 && !P.free_blocks))
         return fail(TTKV_ERR_ARG, "plan: null pointer");
-    if (P.n_reqs < 0 || P.bt_cols < 0 || P.capacity < 0 || P.n_tokens < 0)
-        return fail(TTKV_ERR_ARG, "plan: a negative size");
-    if (P.bs < 1) return fail(TTKV_ERR_ARG, "plan: block size %d", P.bs);
+    if (P.n_reqs < 0 || P.bt_cols < 0 || P.capacity < 0 || P.n_tokens < 0) return fail(TTKV_ERR_ARG, "plan: a negative size");
+    if (P.block_size < 1) return fail(TTKV_ERR_ARG, "plan: block size %d", P.block_size);
     if (P.n_reqs > 1 && P.bt_stride < P.bt_cols) return fail(TTKV_ERR_ARG, "plan: block-table rows overlap");
     if (P.n_reqs > TTKV_PLAN_MAX_REQS)
         return fail(TTKV_ERR_UNSUPPORTED, "plan: %d requests > %d", P.n_reqs, TTKV_PLAN_MAX_REQS);
@@ -226,7 +211,7 @@ int check_plan(const PlanParams& P) {
 }
 
 template <typename K>
-int launch_plan(K kernel, const PlanParams& P, int work, size_t smem, const char* what, void* stream) {
+int launch_plan(K kernel, const PlanParams& P, int work, size_t smem, const char* what) {
     if (int e = raise_smem_limit(reinterpret_cast<const void*>(kernel), what)) return e;
     const unsigned ctas = work <= kPlanSmall ? 1 : kPlanCtas;
     cudaLaunchAttribute attr[2];
@@ -239,7 +224,7 @@ int launch_plan(K kernel, const PlanParams& P, int work, size_t smem, const char
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kPlanThreads);
     cfg.dynamicSmemBytes = smem;
-    cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.stream = static_cast<cudaStream_t>(P.stream);
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P);
@@ -255,28 +240,17 @@ int launch_plan(K kernel, const PlanParams& P, int work, size_t smem, const char
 
 using namespace ttkv;
 
-extern "C" int ttkv_plan_step(int32_t* block_table, int64_t bt_stride, int32_t bt_cols, const int32_t* seq_lens,
-                              const int32_t* query_start_loc, int32_t n_reqs, const int32_t* free_blocks,
-                              int32_t capacity, const int32_t* free_count, int32_t* free_count_out,
-                              int32_t block_size, int64_t* slots, int64_t* positions, int32_t n_tokens,
-                              int32_t* status, void* stream) {
-    PlanParams P{block_table, bt_stride, bt_cols, seq_lens, query_start_loc, n_reqs,
-                 const_cast<int32_t*>(free_blocks), capacity, free_count, free_count_out, block_size,
-                 slots, positions, n_tokens, status};
-    if (int e = check_plan(P)) return e;
-    if (!query_start_loc || (n_tokens > 0 && !slots)) return fail(TTKV_ERR_ARG, "plan: null pointer");
-    return launch_plan(plan_step_kernel, P, std::max(n_tokens, n_reqs), (3 * size_t(n_reqs) + 1) * sizeof(int32_t),
-                       "plan_step_kernel", stream);
+extern "C" int ttkv_plan_step(const ttkv_plan_args_t* args) {
+    if (int e = check_plan(args)) return e;
+    if (!args->query_start_loc || (args->n_tokens > 0 && !args->slots)) return fail(TTKV_ERR_ARG, "plan: null pointer");
+    return launch_plan(plan_step_kernel, *args, std::max(args->n_tokens, args->n_reqs),
+                       (3 * size_t(args->n_reqs) + 1) * sizeof(int32_t), "plan_step_kernel");
 }
 
-extern "C" int ttkv_release_blocks(const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
-                                   const int32_t* lens, int32_t n_reqs, int32_t* free_blocks, int32_t capacity,
-                                   const int32_t* free_count, int32_t* free_count_out, int32_t block_size,
-                                   int32_t* status, void* stream) {
-    PlanParams P{const_cast<int32_t*>(block_table), bt_stride, bt_cols, lens, nullptr, n_reqs, free_blocks,
-                 capacity, free_count, free_count_out, block_size, nullptr, nullptr, 0, status};
-    if (int e = check_plan(P)) return e;
+extern "C" int ttkv_release_blocks(const ttkv_plan_args_t* args) {
+    if (int e = check_plan(args)) return e;
     // (how many blocks come back is known on the device only: a row holds up to bt_cols)
-    return launch_plan(release_blocks_kernel, P, int(std::min(int64_t(n_reqs) * bt_cols, int64_t(kPlanSmall) + 1)),
-                       (2 * size_t(n_reqs) + 1) * sizeof(int32_t), "release_blocks_kernel", stream);
+    return launch_plan(release_blocks_kernel, *args,
+                       int(std::min(int64_t(args->n_reqs) * args->bt_cols, int64_t(kPlanSmall) + 1)),
+                       (2 * size_t(args->n_reqs) + 1) * sizeof(int32_t), "release_blocks_kernel");
 }

@@ -188,31 +188,33 @@ __global__ void __launch_bounds__(kStoreThreads) q4_read_kernel(const StoreParam
     store8(P.v, P.v_dtype, tok * P.v_stride + h * D + 8 * i, P.v_vec, x);
 }
 
-int check_store(const ttkv_q4_cache_t* c, const int64_t* slots, int32_t n, const void* k, int32_t k_dtype,
-                int64_t k_stride, const void* v, int32_t v_dtype, int64_t v_stride) {
-    if (int e = check_cache(c)) return e;
-    if (n < 0 || (n > 0 && (!slots || !k || !v))) return fail(TTKV_ERR_ARG, "4-bit store: null pointer or a negative count");
-    if (k_dtype < TTKV_F32 || k_dtype > TTKV_BF16 || v_dtype < TTKV_F32 || v_dtype > TTKV_BF16)
+int check_store(const ttkv_q4_store_args_t* a) {
+    if (!a) return fail(TTKV_ERR_ARG, "4-bit store: null arguments");
+    if (int e = check_cache(&a->cache)) return e;
+    if (a->n < 0 || (a->n > 0 && (!a->slots || !a->k || !a->v)))
+        return fail(TTKV_ERR_ARG, "4-bit store: null pointer or a negative count");
+    if (a->k_dtype < TTKV_F32 || a->k_dtype > TTKV_BF16 || a->v_dtype < TTKV_F32 || a->v_dtype > TTKV_BF16)
         return fail(TTKV_ERR_ARG, "4-bit store: K or V type");
-    const int64_t row = int64_t(c->H) * c->d;
-    if (n > 1 && (k_stride < row || v_stride < row)) return fail(TTKV_ERR_ARG, "4-bit store: token strides below H * d");
-    if ((reinterpret_cast<uintptr_t>(k) & (k_dtype == TTKV_F32 ? 3 : 1)) ||
-        (reinterpret_cast<uintptr_t>(v) & (v_dtype == TTKV_F32 ? 3 : 1)))
+    const int64_t row = int64_t(a->cache.H) * a->cache.d;
+    if (a->n > 1 && (a->k_stride < row || a->v_stride < row)) return fail(TTKV_ERR_ARG, "4-bit store: token strides below H * d");
+    if ((reinterpret_cast<uintptr_t>(a->k) & (a->k_dtype == TTKV_F32 ? 3 : 1)) ||
+        (reinterpret_cast<uintptr_t>(a->v) & (a->v_dtype == TTKV_F32 ? 3 : 1)))
         return fail(TTKV_ERR_ALIGN, "4-bit store: K or V not aligned to its type");
     return TTKV_OK;
 }
 
 template <bool WRITE>
-int launch_store(const ttkv_q4_cache_t* c, const int64_t* slots, int32_t n, void* k, int32_t k_dtype,
-                 int64_t k_stride, void* v, int32_t v_dtype, int64_t v_stride, int32_t* status, void* stream) {
-    if (int e = check_store(c, slots, n, k, k_dtype, k_stride, v, v_dtype, v_stride)) return e;
-    if (n == 0) return TTKV_OK;
+int launch_store(const ttkv_q4_store_args_t* a) {
+    if (int e = check_store(a)) return e;
+    if (a->n == 0) return TTKV_OK;
+    const ttkv_q4_cache_t* c = &a->cache;
+    const int32_t n = a->n;
     int shift = -1;
     for (int b = 0; b < 31; ++b)
         if (c->block_size == (1 << b)) shift = b;
-    StoreParams P{c->base, c->n_blocks * c->block_size, c->H, c->block_size, shift, slots, n, c->flags & TTKV_CACHE_SKIP_PAD,
-                  k, v, k_dtype, v_dtype, rows_aligned(k, k_dtype, k_stride), rows_aligned(v, v_dtype, v_stride),
-                  k_stride, v_stride, status};
+    StoreParams P{c->base, c->n_blocks * c->block_size, c->H, c->block_size, shift, a->slots, n, c->flags & TTKV_CACHE_SKIP_PAD,
+                  a->k, a->v, a->k_dtype, a->v_dtype, rows_aligned(a->k, a->k_dtype, a->k_stride),
+                  rows_aligned(a->v, a->v_dtype, a->v_stride), a->k_stride, a->v_stride, a->status};
     const int per = kStoreThreads / (c->d / 8), ctas = (n + per - 1) / per;
     // may start while the kernel before it runs, and waits for it before its first access
     cudaLaunchAttribute pdl[1];
@@ -221,7 +223,7 @@ int launch_store(const ttkv_q4_cache_t* c, const int64_t* slots, int32_t n, void
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(ctas), unsigned(c->H));
     cfg.blockDim = dim3(kStoreThreads);
-    cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.stream = static_cast<cudaStream_t>(a->stream);
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
     cudaError_t e = cudaErrorInvalidValue;
@@ -247,14 +249,6 @@ extern "C" size_t ttkv_q4_panel_bytes(int32_t d, int32_t group) {
     return q4::geometry_ok(d, group) ? size_t(q4::panel_bytes(d, group)) : 0;
 }
 
-extern "C" int ttkv_q4_write(const ttkv_q4_cache_t* cache, const int64_t* slots, int32_t n, const void* k,
-                             int32_t k_dtype, int64_t k_stride, const void* v, int32_t v_dtype, int64_t v_stride,
-                             int32_t* status, void* stream) {
-    return launch_store<true>(cache, slots, n, const_cast<void*>(k), k_dtype, k_stride, const_cast<void*>(v), v_dtype,
-                              v_stride, status, stream);
-}
+extern "C" int ttkv_q4_write(const ttkv_q4_store_args_t* args) { return launch_store<true>(args); }
 
-extern "C" int ttkv_q4_read(const ttkv_q4_cache_t* cache, const int64_t* slots, int32_t n, void* k, int32_t k_dtype,
-                            int64_t k_stride, void* v, int32_t v_dtype, int64_t v_stride, int32_t* status, void* stream) {
-    return launch_store<false>(cache, slots, n, k, k_dtype, k_stride, v, v_dtype, v_stride, status, stream);
-}
+extern "C" int ttkv_q4_read(const ttkv_q4_store_args_t* args) { return launch_store<false>(args); }

@@ -728,18 +728,18 @@ StreamWs stream_ws(int d, int n_reqs, int nt) {
     return w;
 }
 
-int check_attn(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch, const void* q, int32_t q_dtype,
-               int64_t q_stride, int32_t HQ, const void* out, int64_t out_stride) {
-    if (int e = check_cache(cache)) return e;
-    if (!batch || batch->n_reqs < 0 || batch->bt_cols < 0) return fail(TTKV_ERR_ARG, "4-bit read: batch");
-    if (batch->n_reqs > 65535) return fail(TTKV_ERR_UNSUPPORTED, "4-bit read: %d requests in one call", batch->n_reqs);
-    if (batch->n_reqs > 0 && (!batch->seq_lens || !q || !out || (batch->bt_cols > 0 && !batch->block_table)))
+int check_attn(const ttkv_q4_attn_args_t* a) {
+    if (!a) return fail(TTKV_ERR_ARG, "4-bit read: null arguments");
+    if (int e = check_cache(&a->cache)) return e;
+    if (a->n_reqs < 0 || a->bt_cols < 0) return fail(TTKV_ERR_ARG, "4-bit read: batch");
+    if (a->n_reqs > 65535) return fail(TTKV_ERR_UNSUPPORTED, "4-bit read: %d requests in one call", a->n_reqs);
+    if (a->n_reqs > 0 && (!a->seq_lens || !a->q || !a->out || (a->bt_cols > 0 && !a->block_table)))
         return fail(TTKV_ERR_ARG, "4-bit read: null pointer");
-    if (HQ < cache->H || HQ % cache->H) return fail(TTKV_ERR_ARG, "HQ=%d is not a multiple of H=%d", HQ, cache->H);
-    if (q_dtype != TTKV_F16 && q_dtype != TTKV_BF16)
+    if (a->HQ < a->cache.H || a->HQ % a->cache.H) return fail(TTKV_ERR_ARG, "HQ=%d is not a multiple of H=%d", a->HQ, a->cache.H);
+    if (a->dtype != TTKV_F16 && a->dtype != TTKV_BF16)
         return fail(TTKV_ERR_UNSUPPORTED, "4-bit read: queries and outputs are fp16 or bf16");
-    if (q_stride < 0 || out_stride < 0) return fail(TTKV_ERR_ARG, "4-bit read: a negative stride");
-    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 1)
+    if (a->q_stride < 0 || a->out_stride < 0) return fail(TTKV_ERR_ARG, "4-bit read: a negative stride");
+    if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 1)
         return fail(TTKV_ERR_ALIGN, "4-bit read: q or out at an odd address");
     return TTKV_OK;
 }
@@ -791,64 +791,59 @@ int run_stream(const ttkv_q4_cache_t* c, AttnParams P, void* ws, size_t ws_bytes
     return fail(TTKV_ERR_UNSUPPORTED, "4-bit read: geometry");
 }
 
-AttnParams attn_params(const ttkv_q4_cache_t* c, const ttkv_q4_batch_t* b, const void* q, int32_t dtype,
-                       int64_t q_stride, int32_t HQ, float scale, void* out, int64_t out_stride, int32_t* status) {
+AttnParams attn_params(const ttkv_q4_attn_args_t* a) {
+    const ttkv_q4_cache_t* c = &a->cache;
     AttnParams P{};
-    P.cache = c->base; P.n_blocks = c->n_blocks; P.H = c->H; P.G = HQ / c->H; P.block_size = c->block_size;
-    P.block_table = b->block_table; P.bt_stride = b->bt_stride; P.bt_cols = b->bt_cols; P.seq_lens = b->seq_lens;
-    P.n_reqs = b->n_reqs; P.q = q; P.dtype = dtype; P.q_stride = q_stride; P.scale = scale;
-    P.out = out; P.out_stride = out_stride; P.status = status;
-    P.q_vec = rows_aligned(q, dtype, q_stride);
-    P.out_vec = rows_aligned(out, dtype, out_stride) ? 2 : (reinterpret_cast<uintptr_t>(out) & 7) == 0 && (out_stride & 3) == 0;
+    P.cache = c->base; P.n_blocks = c->n_blocks; P.H = c->H; P.G = a->HQ / c->H; P.block_size = c->block_size;
+    P.block_table = a->block_table; P.bt_stride = a->bt_stride; P.bt_cols = a->bt_cols; P.seq_lens = a->seq_lens;
+    P.n_reqs = a->n_reqs; P.q = a->q; P.dtype = a->dtype; P.q_stride = a->q_stride; P.scale = a->scale;
+    P.out = a->out; P.out_stride = a->out_stride; P.status = a->status;
+    P.q_vec = rows_aligned(a->q, a->dtype, a->q_stride);
+    P.out_vec = rows_aligned(a->out, a->dtype, a->out_stride) ? 2
+              : (reinterpret_cast<uintptr_t>(a->out) & 7) == 0 && (a->out_stride & 3) == 0;
     return P;
-}
-
-}  // namespace
-}  // namespace ttkv
-
-using namespace ttkv;
-
-extern "C" size_t ttkv_q4_decode_workspace_bytes(const ttkv_q4_cache_t* cache, int32_t n_reqs, int32_t HQ) {
-    if (!cache || cache->H < 1 || HQ < cache->H || n_reqs < 0) return 0;
-    return stream_ws(cache->d, n_reqs, stream_nt(HQ / cache->H)).bytes;
-}
-
-extern "C" int ttkv_q4_decode(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch, const void* q,
-                              int32_t q_dtype, int64_t q_stride, int32_t HQ, float scale, void* out,
-                              int64_t out_stride, void* workspace, size_t workspace_bytes, int32_t* status,
-                              void* stream) {
-    if (int e = check_attn(cache, batch, q, q_dtype, q_stride, HQ, out, out_stride)) return e;
-    if (batch->n_reqs == 0) return TTKV_OK;
-    AttnParams P = attn_params(cache, batch, q, q_dtype, q_stride, HQ, scale, out, out_stride, status);
-    P.n_rows = batch->n_reqs;
-    P.max_q = 1;
-    return run_stream(cache, P, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 // Chunks of at most this many (query, head) rows a KV head are streamed, the cache read once per 16 of
 // them; above it the chunk kernel's tiles are fuller.
 constexpr int kStreamRows = 32;
 
-extern "C" size_t ttkv_q4_prefill_workspace_bytes(const ttkv_q4_cache_t* cache, int32_t n_reqs, int32_t HQ,
-                                                  int32_t max_q_len, int32_t max_seq_len) {
-    if (!cache || cache->H < 1 || HQ < cache->H || n_reqs < 0 || max_q_len < 0) return 0;
-    const int64_t rows = int64_t(max_q_len) * (HQ / cache->H);
-    return rows > kStreamRows ? chunk_workspace_bytes(cache->d) : stream_ws(cache->d, n_reqs, stream_nt(rows)).bytes;
+}  // namespace
+}  // namespace ttkv
+
+using namespace ttkv;
+
+extern "C" size_t ttkv_q4_decode_workspace_bytes(int32_t d, int32_t n_reqs, int32_t group_heads) {
+    return n_reqs < 0 ? 0 : stream_ws(d, n_reqs, stream_nt(group_heads)).bytes;
 }
 
-extern "C" int ttkv_q4_prefill(const ttkv_q4_cache_t* cache, const ttkv_q4_batch_t* batch, const int32_t* q_start,
-                               const int32_t* q_len, const void* q, int32_t q_dtype, int64_t q_stride, int32_t n_rows,
-                               int32_t HQ, float scale, void* out, int64_t out_stride, int32_t max_q_len,
-                               int32_t max_seq_len, void* workspace, size_t workspace_bytes, int32_t* status,
-                               void* stream) {
-    if (int e = check_attn(cache, batch, q, q_dtype, q_stride, HQ, out, out_stride)) return e;
-    if (max_q_len < 0 || max_seq_len < 0 || n_rows < 0) return fail(TTKV_ERR_ARG, "4-bit prefill: a negative size");
-    if (batch->n_reqs > 0 && (!q_start || !q_len)) return fail(TTKV_ERR_ARG, "4-bit prefill: q_start or q_len missing");
-    if (batch->n_reqs == 0 || n_rows == 0 || max_q_len == 0) return TTKV_OK;
-    if (int64_t(max_q_len) * HQ > 0x7fffffff) return fail(TTKV_ERR_UNSUPPORTED, "4-bit prefill: %d queries of %d heads", max_q_len, HQ);
-    AttnParams P = attn_params(cache, batch, q, q_dtype, q_stride, HQ, scale, out, out_stride, status);
-    P.q_start = q_start; P.q_len = q_len; P.n_rows = n_rows; P.max_q = max_q_len; P.max_seq = std::max(max_seq_len, 1);
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return int64_t(max_q_len) * P.G > kStreamRows ? run_chunk(cache, P, workspace, workspace_bytes, st)
-                                                  : run_stream(cache, P, workspace, workspace_bytes, st);
+extern "C" int ttkv_q4_decode(const ttkv_q4_attn_args_t* args) {
+    if (int e = check_attn(args)) return e;
+    if (args->n_reqs == 0) return TTKV_OK;
+    AttnParams P = attn_params(args);
+    P.n_rows = args->n_reqs;
+    P.max_q = 1;
+    return run_stream(&args->cache, P, args->workspace, args->workspace_bytes, static_cast<cudaStream_t>(args->stream));
+}
+
+extern "C" size_t ttkv_q4_prefill_workspace_bytes(int32_t d, int32_t n_reqs, int32_t group_heads, int32_t max_q_len) {
+    if (n_reqs < 0 || max_q_len < 0) return 0;
+    const int64_t rows = int64_t(max_q_len) * group_heads;
+    return rows > kStreamRows ? chunk_workspace_bytes(d) : stream_ws(d, n_reqs, stream_nt(rows)).bytes;
+}
+
+extern "C" int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args) {
+    if (int e = check_attn(args)) return e;
+    if (args->max_q_len < 0 || args->max_seq_len < 0 || args->n_rows < 0) return fail(TTKV_ERR_ARG, "4-bit prefill: a negative size");
+    if (args->n_reqs > 0 && (!args->q_start || !args->q_len)) return fail(TTKV_ERR_ARG, "4-bit prefill: q_start or q_len missing");
+    if (args->n_reqs == 0 || args->n_rows == 0 || args->max_q_len == 0) return TTKV_OK;
+    if (int64_t(args->max_q_len) * args->HQ > 0x7fffffff)
+        return fail(TTKV_ERR_UNSUPPORTED, "4-bit prefill: %d queries of %d heads", args->max_q_len, args->HQ);
+    AttnParams P = attn_params(args);
+    P.q_start = args->q_start; P.q_len = args->q_len; P.n_rows = args->n_rows; P.max_q = args->max_q_len;
+    P.max_seq = std::max(args->max_seq_len, 1);
+    const cudaStream_t st = static_cast<cudaStream_t>(args->stream);
+    return int64_t(args->max_q_len) * P.G > kStreamRows
+        ? run_chunk(&args->cache, P, args->workspace, args->workspace_bytes, st)
+        : run_stream(&args->cache, P, args->workspace, args->workspace_bytes, st);
 }

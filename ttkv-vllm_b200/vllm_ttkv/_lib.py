@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import pathlib
+import struct
 
 ABI_VERSION = 6
 LIB_PATH = pathlib.Path(__file__).resolve().parents[1] / "libttkv_sm100.so"
@@ -68,18 +69,46 @@ class Q4Cache(C.Structure):
                 ("group", C.c_int32), ("block_size", C.c_int32), ("flags", C.c_int32)]
 
 
-class Q4Batch(C.Structure):
-    """ttkv_q4_batch_t: the paging of a 4-bit read."""
-    _fields_ = [("block_table", C.c_void_p), ("bt_stride", C.c_int64), ("bt_cols", C.c_int32),
-                ("seq_lens", C.c_void_p), ("n_reqs", C.c_int32)]
+class Q4StoreArgs(C.Structure):
+    """ttkv_q4_store_args_t: a write into, or a read-back from, a 4-bit cache."""
+    _fields_ = [("cache", Q4Cache), ("slots", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("n", C.c_int32), ("k_dtype", C.c_int32),
+                ("v_dtype", C.c_int32), ("status", C.c_void_p), ("stream", C.c_void_p)]
 
+
+class Q4AttnArgs(C.Structure):
+    """ttkv_q4_attn_args_t: attention over a 4-bit cache."""
+    _fields_ = [("cache", Q4Cache), ("block_table", C.c_void_p), ("seq_lens", C.c_void_p),
+                ("q_start", C.c_void_p), ("q_len", C.c_void_p), ("q", C.c_void_p), ("out", C.c_void_p),
+                ("bt_stride", C.c_int64), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("bt_cols", C.c_int32), ("n_reqs", C.c_int32), ("n_rows", C.c_int32), ("HQ", C.c_int32),
+                ("dtype", C.c_int32), ("max_q_len", C.c_int32), ("max_seq_len", C.c_int32), ("scale", C.c_float),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
+class PlanArgs(C.Structure):
+    """ttkv_plan_args_t: a step's block tables, or the release of finished requests'."""
+    _fields_ = [("block_table", C.c_void_p), ("lens", C.c_void_p), ("query_start_loc", C.c_void_p),
+                ("free_blocks", C.c_void_p), ("free_count", C.c_void_p), ("free_count_out", C.c_void_p),
+                ("slots", C.c_void_p), ("positions", C.c_void_p), ("bt_stride", C.c_int64),
+                ("bt_cols", C.c_int32), ("n_reqs", C.c_int32), ("capacity", C.c_int32),
+                ("block_size", C.c_int32), ("n_tokens", C.c_int32), ("status", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
+# The same three as one `struct` packing each, in the fields' order (the C layout's padding is the
+# native alignment's): a call packs its arguments and passes the bytes, which costs about 1 us where a
+# ctypes call of as many arguments costs 7.
+Q4_STORE = struct.Struct("@PqiiiiiPPPqqiiiPP")
+Q4_ATTN = struct.Struct("@PqiiiiiPPPPPPqqqiiiiiiifPNPP")
+PLAN = struct.Struct("@PPPPPPPPqiiiiiPP")
 
 PLAN_MAX_REQS = 16384                       # TTKV_PLAN_MAX_REQS
 
 P, I32, I64, SZ, F = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_float
 LP, CP, BP, RP = C.POINTER(Layout), C.POINTER(Cache), C.POINTER(Batch), C.POINTER(Rope)
 PP = C.POINTER(Peers)
-QP, QB = C.POINTER(Q4Cache), C.POINTER(Q4Batch)
 
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
@@ -112,15 +141,14 @@ SIGNATURES = {
     "ttkv_select_pack_rows": (C.c_int, [CP, P, I32, P, I32, I32, I32, I32, I32, I32, I32, P, P]),
     "ttkv_fit_tail_scratch_bytes": (SZ, [I32, I32, I32, I32]),
     "ttkv_q4_panel_bytes": (SZ, [I32, I32]),
-    "ttkv_q4_write": (C.c_int, [QP, P, I32, P, I32, I64, P, I32, I64, P, P]),
-    "ttkv_q4_read": (C.c_int, [QP, P, I32, P, I32, I64, P, I32, I64, P, P]),
-    "ttkv_q4_decode_workspace_bytes": (SZ, [QP, I32, I32]),
-    "ttkv_q4_decode": (C.c_int, [QP, QB, P, I32, I64, I32, F, P, I64, P, SZ, P, P]),
-    "ttkv_q4_prefill_workspace_bytes": (SZ, [QP, I32, I32, I32, I32]),
-    "ttkv_q4_prefill": (C.c_int, [QP, QB, P, P, P, I32, I64, I32, I32, F, P, I64, I32, I32, P, SZ,
-                                  P, P]),
-    "ttkv_plan_step": (C.c_int, [P, I64, I32, P, P, I32, P, I32, P, P, I32, P, P, I32, P, P]),
-    "ttkv_release_blocks": (C.c_int, [P, I64, I32, P, I32, P, I32, P, P, I32, P, P]),
+    "ttkv_q4_write": (C.c_int, [P]),
+    "ttkv_q4_read": (C.c_int, [P]),
+    "ttkv_q4_decode_workspace_bytes": (SZ, [I32, I32, I32]),
+    "ttkv_q4_decode": (C.c_int, [P]),
+    "ttkv_q4_prefill_workspace_bytes": (SZ, [I32, I32, I32, I32]),
+    "ttkv_q4_prefill": (C.c_int, [P]),
+    "ttkv_plan_step": (C.c_int, [P]),
+    "ttkv_release_blocks": (C.c_int, [P]),
     "ttkv_fit_tail": (C.c_int, [P, P, P, I32, I32, I32, I32, I32, I32, I32, P, P, P, P, P, P, SZ,
                                 P]),
 }

@@ -35,10 +35,8 @@ class Q4Layout:
             raise ValueError(f"head dim {self.d}: the 4-bit cache serves 64 and 128")
         if self.group not in (32, 64, 128) or self.group > self.d:
             raise ValueError(f"groups of {self.group} lanes: 32, 64 or 128, at most d={self.d}")
-
-    @property
-    def panel_bytes(self) -> int:
-        return PANEL_TOKENS * (self.d + 8 * (self.d // self.group))
+        # bytes of a panel: 16 tokens of one head
+        object.__setattr__(self, "panel_bytes", PANEL_TOKENS * (self.d + 8 * (self.d // self.group)))
 
     def bytes_per_token(self) -> int:
         """Cache bytes of one token over the layer's heads."""
@@ -58,10 +56,11 @@ class Q4Layout:
 
     def block_size(self, cache: torch.Tensor) -> int:
         """The block size of a cache tensor of this layout; raises if it is not one."""
-        if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous():
+        shape = cache.shape
+        if cache.dtype != torch.uint8 or len(shape) != 4 or not cache.is_contiguous():
             raise ValueError(f"expected a contiguous uint8 [blocks, H, block_size/16, bytes] cache, got "
-                             f"{tuple(cache.shape)} {cache.dtype}")
-        if cache.shape[1] != self.H or cache.shape[3] != self.panel_bytes or cache.shape[2] < 1:
-            raise ValueError(f"a cache of shape {tuple(cache.shape)} does not hold H={self.H} heads in panels of "
+                             f"{tuple(shape)} {cache.dtype}")
+        if shape[1] != self.H or shape[3] != self.panel_bytes or shape[2] < 1:
+            raise ValueError(f"a cache of shape {tuple(shape)} does not hold H={self.H} heads in panels of "
                              f"{self.panel_bytes} bytes")
-        return cache.shape[2] * PANEL_TOKENS
+        return shape[2] * PANEL_TOKENS
