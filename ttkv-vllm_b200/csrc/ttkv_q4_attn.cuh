@@ -16,7 +16,7 @@ constexpr int kMaxCtas = 148;               // one CTA per SM of a B200; workspa
 struct AttnParams {
     const uint8_t* cache;
     int64_t n_blocks;
-    int32_t H, G, block_size;
+    int32_t H, G, block_size, bs_shift;     // log2 of the block size, -1 where it is no power of two
     const int32_t* block_table;
     int64_t bt_stride;
     int32_t bt_cols;
@@ -31,7 +31,6 @@ struct AttnParams {
     void* out;
     int64_t out_stride;
     int32_t n_ctas;
-    int32_t* prefix;                        // [n_reqs + 1] units before each request (workspace)
     float* part_ml;                         // [n_ctas][2][rows of a block][2]
     float* part_o;                          // [n_ctas][2][rows of a block][D]
     float* first;                           // [n_ctas][warps] parts of the warps' first segments (streaming kernel)
@@ -97,12 +96,6 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
 // ------------------------------------------------------------------ partial results
 // Weighted sum of partials (max m_i, sum l_i, rows o_i relative to m_i): relative to M = max m_i.
 __device__ __forceinline__ float part_weight(float m, float M) { return M == -INFINITY ? 1.f : ex2(m - M); }
-
-// Lanes ln .. + 4 of row i of a part of `rows` rows.
-__device__ __forceinline__ void put_part(float* part, int rows, int D, int i, int ln, float4 o, float m, float l) {
-    *reinterpret_cast<float4*>(part + i * D + ln) = o;
-    if (ln == 0) *reinterpret_cast<float2*>(part + rows * D + 2 * i) = make_float2(m, l);
-}
 
 // Four output values from element i of the output.
 __device__ __forceinline__ void store4(const AttnParams& P, int64_t i, float4 x) {

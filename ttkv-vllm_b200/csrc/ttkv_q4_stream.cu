@@ -49,16 +49,24 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // Fragment places of lane (b = lane / 4, a = lane % 4): stored tokens b and b + 8 of a panel as rows
 // of S^T, rows 2 a and 2 a + 1 of each block of 8 (query, head) rows as its columns; output lanes
 // 32 j + 4 b + (0..3) as rows of O^T.
+//
+// Weights are taken against a maximum that is looked for only when it has to move: in a segment's first
+// unit, and when a lane's sum of a unit's weights passes 2^9. V scales are brought into [2^5, 2^6) by a
+// power of two, so the products that become fp16 stay below 2^15 and keep their precision down to
+// weights of 2^-19 of the largest; the power falls when a larger scale comes.
+constexpr float kWeightsMost = 512.f;
+
 template <int D, int GRP, int NT>
 struct WarpRows {
-    static constexpr int NW = D / 32, NG = D / GRP, WPG = GRP / 32, ROWS = 8 * NT;
+    static constexpr int NW = D / 32, NG = D / GRP, WPG = GRP / 32, ROWS = 8 * NT, PANEL = panel_bytes(D, GRP);
     uint32_t qf[NT][2 * NW][2];         // q 2^e as B fragments, lanes 8 a + (0..7) of each 32
     float q1[NT][2][NG], qm[NT][2];     // sums of q 2^e over each group; 2^-e scale log2(e)
     int lim[NT][2], min_lim;            // tokens each row sees; the fewest any row of the block does
-    float m[NT][2], l[NT][2];           // running max (base 2) and this lane's share of the sum
+    float m[NT][2], l[NT][2];           // maximum so far (base 2) and this lane's share of the sum
     float o[2 * NW][NT][4];             // (p s 2^vn) . (c - 7.5)
     float dsum[NT][2][NG];              // this lane's share of 2^vn p (m + 7.5 s)
-    float vn;                           // 2^vn, the scaling of the weights
+    uint32_t vexp;                      // fp16 exponent field of the largest V scale so far; vn = 20 - vexp
+    bool fresh;                         // no unit yet
 
     __device__ __forceinline__ void start(const AttnParams& P, const Req& rq, int h, int rb, int lane) {
         const int b = lane >> 2, a = lane & 3;
@@ -70,15 +78,32 @@ struct WarpRows {
             const int row = rb * ROWS + 8 * nt + b;
             const bool live = row < n_rows;
             const int j = live ? row / P.G : 0, g = live ? row - j * P.G : 0;
-            const int64_t src = int64_t(rq.q0 + j) * P.q_stride + int64_t(h * P.G + g) * D + 8 * a;
+            const uint16_t* src = static_cast<const uint16_t*>(P.q) + int64_t(rq.q0 + j) * P.q_stride + int64_t(h * P.G + g) * D + 8 * a;
+            uint4 raw[NW];
+            if (P.q_vec) {
+                #pragma unroll
+                for (int w = 0; w < NW; ++w) raw[w] = __ldg(reinterpret_cast<const uint4*>(src + 32 * w));
+            } else {
+                #pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const uint16_t* e = src + 32 * w;
+                    raw[w] = make_uint4(e[0] | (uint32_t(e[1]) << 16), e[2] | (uint32_t(e[3]) << 16),
+                                        e[4] | (uint32_t(e[5]) << 16), e[6] | (uint32_t(e[7]) << 16));
+                }
+            }
             float x[NW][8], big = 0.f;
             #pragma unroll
             for (int w = 0; w < NW; ++w) {
+                const uint32_t u[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
                 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[w][i] = 0.f;
-                if (live) load8(P.q, P.dtype, src + 32 * w, P.q_vec, x[w]);
-                #pragma unroll
-                for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[w][i]));
+                for (int i = 0; i < 4; ++i) {
+                    float2 f = P.dtype == TTKV_BF16 ? make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u))
+                                                    : __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+                    if (!live) f = make_float2(0.f, 0.f);
+                    x[w][2 * i] = f.x;
+                    x[w][2 * i + 1] = f.y;
+                    big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
             }
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
@@ -124,131 +149,151 @@ struct WarpRows {
                 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.f;
         }
-        #pragma unroll
-        for (int k = 4; k < 32; k <<= 1) min_lim = min(min_lim, __shfl_xor_sync(0xffffffffu, min_lim, k));
-        vn = 274877906944.f;                                     // 2^38: the least scale in [2^14, 2^15)
+        min_lim = __reduce_min_sync(0xffffffffu, min_lim);
+        vexp = 0;
+        fresh = true;
     }
 
-    // Tokens [t0, t0 + 64) of the request, panel p of them at ring slot (slot + p) % RING. MASK: some row
-    // does not see all of them.
-    template <bool MASK, int RING>
-    __device__ __forceinline__ void step(const uint8_t* ring, int slot, int t0, int seq, int lane) {
+    // Tokens [t0, t0 + 64) of the request, four panels one behind the other. Panels behind the last token
+    // hold whatever was there: codes are finite whatever their bits, and scales of tokens that a row does
+    // not see are not used.
+    __device__ __forceinline__ void step(const uint8_t* unit, int t0, int seq, int lane) {
         const int b = lane >> 2, a = lane & 3;
-        const uint8_t* pan[4];
+        const bool tail = t0 + kUnit > min_lim;                   // some row does not see all of them
+        const uint8_t* kp = unit + b * (D / 2) + a * (D / 8);
+        const uint8_t* vp = unit + 8 * D + a * D + b * (D / 8);
+        const uint8_t* mp = unit + k_meta_offset(D) + b * NG * 4;
+        constexpr int VM = v_meta_offset(D, GRP) - k_meta_offset(D);
+
+        bool moved = false;
+        float s[4][NT][4], ls[NT][2], corr[NT][2];
         #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const int i = slot + p;
-            pan[p] = ring + (i >= RING ? i - RING : i) * panel_bytes(D, GRP);
-        }
-        float s[4][NT][4];
-        float tmax[NT][2], vmax = 0.f;
-        #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) tmax[nt][0] = tmax[nt][1] = -INFINITY;
-        #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const int ta = t0 + 16 * p + b;                       // this lane's tokens: ta and ta + 8
-            if (MASK && t0 + 16 * p >= seq) {                     // no token of this panel (warp-uniform)
+        for (int nt = 0; nt < NT; ++nt) corr[nt][0] = corr[nt][1] = 1.f;
+        for (bool raise = fresh;; raise = true) {
+            #pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                uint32_t lo[NW], hi[NW], sm[2][NG];
+                load_words(kp + p * PANEL, lo);
+                load_words(kp + p * PANEL + 8 * (D / 2), hi);
+                load_words(mp + p * PANEL, sm[0]);
+                load_words(mp + p * PANEL + 8 * NG * 4, sm[1]);
+                float acc[NG][NT][4];
+                #pragma unroll
+                for (int g = 0; g < NG; ++g)
+                    #pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[g][nt][i] = 0.f;
+                #pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const uint32_t l8 = lo[w] >> 8, h8 = hi[w] >> 8;
+                    #pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(acc[w / WPG][nt], lo[w] & 0x000f000fu, hi[w] & 0x000f000fu, lo[w] & 0x00f000f0u,
+                                 hi[w] & 0x00f000f0u, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+                        mma16816(acc[w / WPG][nt], l8 & 0x000f000fu, h8 & 0x000f000fu, l8 & 0x00f000f0u, h8 & 0x00f000f0u,
+                                 qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+                    }
+                }
+                float2 f[2][NG];
+                #pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    #pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        f[i][g] = __half22float2(*reinterpret_cast<const __half2*>(&sm[i][g]));
+                        f[i][g].x *= 16777216.f;                  // 2^24 of the codes
+                    }
                 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[p][nt][i] = -INFINITY;
-                continue;
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = i & 1;
+                        float x = f[i >> 1][0].y * q1[nt][c][0];
+                        x = fmaf(f[i >> 1][0].x, acc[0][nt][i], x);
+                        #pragma unroll
+                        for (int g = 1; g < NG; ++g) {
+                            x = fmaf(f[i >> 1][g].y, q1[nt][c][g], x);
+                            x = fmaf(f[i >> 1][g].x, acc[g][nt][i], x);
+                        }
+                        s[p][nt][i] = x * qm[nt][c];
+                    }
+                if (tail) {
+                    #pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (t0 + 16 * p + b + 8 * (i >> 1) >= lim[nt][i & 1]) s[p][nt][i] = -INFINITY;
+                }
             }
-            uint32_t lo[NW], hi[NW], sm[2][NG];
-            load_words(pan[p] + b * (D / 2) + a * (D / 8), lo);
-            load_words(pan[p] + (b + 8) * (D / 2) + a * (D / 8), hi);
-            load_words(pan[p] + k_meta_offset(D) + b * NG * 4, sm[0]);
-            load_words(pan[p] + k_meta_offset(D) + (b + 8) * NG * 4, sm[1]);
-            float acc[NG][NT][4];
-            #pragma unroll
-            for (int g = 0; g < NG; ++g)
+            if (raise) {
+                moved = true;
                 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[g][nt][i] = 0.f;
-            #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const uint32_t l8 = lo[w] >> 8, h8 = hi[w] >> 8;
-                #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma16816(acc[w / WPG][nt], lo[w] & 0x000f000fu, hi[w] & 0x000f000fu, lo[w] & 0x00f000f0u,
-                             hi[w] & 0x00f000f0u, qf[nt][2 * w][0], qf[nt][2 * w][1]);
-                    mma16816(acc[w / WPG][nt], l8 & 0x000f000fu, h8 & 0x000f000fu, l8 & 0x00f000f0u, h8 & 0x00f000f0u,
-                             qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
-                }
+                    for (int c = 0; c < 2; ++c) {
+                        float mx = -INFINITY;
+                        #pragma unroll
+                        for (int p = 0; p < 4; ++p) mx = fmaxf(mx, fmaxf(s[p][nt][c], s[p][nt][2 + c]));
+                        #pragma unroll
+                        for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+                        mx = fmaxf(mx, m[nt][c]);
+                        corr[nt][c] = m[nt][c] == -INFINITY ? 1.f : ex2(m[nt][c] - mx);
+                        m[nt][c] = mx;
+                    }
             }
-            float2 f[2][NG];
-            #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    f[i][g] = __half22float2(*reinterpret_cast<const __half2*>(&sm[i][g]));
-                    f[i][g].x *= 16777216.f;                      // 2^24 of the codes
-                }
+            bool over = false;
             #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = i & 1;
-                    float x = 0.f;
+                for (int c = 0; c < 2; ++c) {
+                    const float mm = m[nt][c] == -INFINITY ? 0.f : m[nt][c];  // a row that sees nothing has weights of 0
+                    float t = 0.f;
                     #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const float u = fmaf(f[i >> 1][g].x, acc[g][nt][i], f[i >> 1][g].y * q1[nt][c][g]);
-                        x = g ? x + u : u;
+                    for (int p = 0; p < 4; ++p) {
+                        s[p][nt][c] = ex2(s[p][nt][c] - mm);
+                        s[p][nt][2 + c] = ex2(s[p][nt][2 + c] - mm);
+                        t += s[p][nt][c] + s[p][nt][2 + c];
                     }
-                    x *= qm[nt][c];
-                    if (MASK && ta + 8 * (i >> 1) >= lim[nt][c]) x = -INFINITY;
-                    s[p][nt][i] = x;
-                    tmax[nt][c] = fmaxf(tmax[nt][c], x);
+                    ls[nt][c] = t;
+                    over |= t > kWeightsMost;
                 }
+            if (raise || !__any_sync(0xffffffffu, over)) break;
         }
-        // the V scales of this lane's tokens (each token's lanes hold the same): their largest keeps
-        // the fp16 weights in range
-        uint32_t vm[4][2][NG];
-        #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const bool live = !MASK || t0 + 16 * p + b + 8 * i < seq;
-                if (live) load_words(pan[p] + v_meta_offset(D, GRP) + (b + 8 * i) * NG * 4, vm[p][i]);
-                #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    if (!live) vm[p][i][g] = 0u;
-                    vmax = fmaxf(vmax, __half2float(__ushort_as_half(uint16_t(vm[p][i][g] & 0xffffu))));
-                }
-            }
-        }
-        #pragma unroll
-        for (int k = 4; k < 32; k <<= 1) {
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, k));
-            #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                tmax[nt][0] = fmaxf(tmax[nt][0], __shfl_xor_sync(0xffffffffu, tmax[nt][0], k));
-                tmax[nt][1] = fmaxf(tmax[nt][1], __shfl_xor_sync(0xffffffffu, tmax[nt][1], k));
-            }
-        }
-        // 2^vn with vmax 2^vn in [2^14, 2^15); it only falls, and what is summed falls with it
-        float vfall = 1.f;
-        {
-            const float want = vmax > 0.f ? __uint_as_float(uint32_t(268 - int(__float_as_uint(vmax) >> 23)) << 23) : vn;
-            if (want < vn) { vfall = want / vn; vn = want; }
-        }
-        bool moved = vfall != 1.f;
-        float corr[NT][2];
+        fresh = false;
         #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float mn = fmaxf(m[nt][c], tmax[nt][c]);
-                corr[nt][c] = m[nt][c] == -INFINITY ? 1.f : ex2(m[nt][c] - mn);
-                moved |= corr[nt][c] != 1.f;
-                m[nt][c] = mn;
-                l[nt][c] *= corr[nt][c];
-                corr[nt][c] *= vfall;
+            for (int c = 0; c < 2; ++c) l[nt][c] = fmaf(l[nt][c], corr[nt][c], ls[nt][c]);
+        // the V scales of this lane's tokens (each token's lanes hold the same); the largest's exponent
+        uint32_t vm[4][2][NG], vmax = 0;
+        #pragma unroll
+        for (int p = 0; p < 4; ++p)
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                load_words(mp + p * PANEL + VM + i * 8 * NG * 4, vm[p][i]);
+                if (tail && t0 + 16 * p + b + 8 * i >= seq) {
+                    #pragma unroll
+                    for (int g = 0; g < NG; ++g) vm[p][i][g] = 0u;
+                }
                 #pragma unroll
-                for (int g = 0; g < NG; ++g) dsum[nt][c][g] *= corr[nt][c];
+                for (int g = 0; g < NG; ++g) vmax = __vmaxu2(vmax, vm[p][i][g]);
             }
-        if (__any_sync(0xffffffffu, moved)) {
+        vmax = __reduce_max_sync(0xffffffffu, (vmax >> 10) & 31u);
+        const uint32_t ve = max(vexp, vmax);
+        const float vfall = __uint_as_float((127u + vexp - ve) << 23);        // 2^(old - new)
+        moved |= ve != vexp;
+        vexp = ve;
+        const float vn = __uint_as_float((127u + 20u - ve) << 23);
+
+        if (moved) {                                              // (the same in every lane)
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                #pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    corr[nt][c] *= vfall;
+                    #pragma unroll
+                    for (int g = 0; g < NG; ++g) dsum[nt][c][g] *= corr[nt][c];
+                }
             #pragma unroll
             for (int i = 0; i < 2 * NW; ++i)
                 #pragma unroll
@@ -256,7 +301,7 @@ struct WarpRows {
                     #pragma unroll
                     for (int k = 0; k < 4; ++k) o[i][nt][k] *= corr[nt][k & 1];
         }
-        float psum[NG][NT][4];                           // the unit's sum of p', the same in every row
+        float psum[NG][NT][4];                                    // the unit's sum of p', the same in every row
         #pragma unroll
         for (int g = 0; g < NG; ++g)
             #pragma unroll
@@ -265,16 +310,6 @@ struct WarpRows {
                 for (int i = 0; i < 4; ++i) psum[g][nt][i] = 0.f;
         #pragma unroll
         for (int p = 0; p < 4; ++p) {
-            if (MASK && t0 + 16 * p >= seq) continue;
-            float pr[NT][4];
-            #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float mm = MASK && m[nt][i & 1] == -INFINITY ? 0.f : m[nt][i & 1];
-                    pr[nt][i] = ex2(s[p][nt][i] - mm);
-                    l[nt][i & 1] += pr[nt][i];
-                }
             uint32_t pf[NG][NT][2];
             #pragma unroll
             for (int g = 0; g < NG; ++g)
@@ -284,9 +319,9 @@ struct WarpRows {
                     const float sv = sm.x * vn, mid = fmaf(7.5f, sv, sm.y * vn);
                     #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        const float p0 = pr[nt][2 * i], p1 = pr[nt][2 * i + 1];
+                        const float p0 = s[p][nt][2 * i], p1 = s[p][nt][2 * i + 1];
                         float w0 = p0 * sv, w1 = p1 * sv, d0 = p0 * mid, d1 = p1 * mid;
-                        if (MASK) {                              // a weight of 0 on a NaN counts as none
+                        if (tail) {                               // a weight of 0 on a NaN counts as none
                             const int t = t0 + 16 * p + b + 8 * i;
                             if (t >= lim[nt][0]) w0 = d0 = 0.f;
                             if (t >= lim[nt][1]) w1 = d1 = 0.f;
@@ -301,9 +336,9 @@ struct WarpRows {
             for (int g = 0; g < NG; ++g)
                 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma16816(psum[g][nt], ONES, ONES, ONES, ONES, pf[g][nt][0], pf[g][nt][1]);
-            uint32_t lo[NW], hi[NW];                             // tokens 2 a, 2 a + 1 and those + 8
-            load_words(pan[p] + 8 * D + a * D + b * (D / 8), lo);
-            load_words(pan[p] + 8 * D + (a + 4) * D + b * (D / 8), hi);
+            uint32_t lo[NW], hi[NW];                              // tokens 2 a, 2 a + 1 and those + 8
+            load_words(vp + p * PANEL, lo);
+            load_words(vp + p * PANEL + 4 * D, hi);
             #pragma unroll
             for (int w = 0; w < NW; ++w) {
                 const uint32_t l8 = lo[w] >> 8, h8 = hi[w] >> 8;
@@ -328,24 +363,9 @@ struct WarpRows {
                     o[i][nt][k] = fmaf(k < 2 ? -7.5f / 16777216.f : -7.5f / 1048576.f, psum[i / 2 / WPG][nt][k], o[i][nt][k]);
     }
 
-    // f(row of the block, first of four output lanes, o, m, l) for what this lane holds of the rows.
-    template <typename F>
-    __device__ __forceinline__ void rows(F f, int lane) const {
-        const int b = lane >> 2, a = lane & 3;
-        #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-            #pragma unroll
-            for (int c = 0; c < 2; ++c)
-                #pragma unroll
-                for (int k = 0; k < NW; ++k)
-                    f(8 * nt + 2 * a + c, 32 * k + 4 * b,
-                      make_float4(o[2 * k][nt][c], o[2 * k][nt][2 + c], o[2 * k + 1][nt][c], o[2 * k + 1][nt][2 + c]),
-                      m[nt][c], l[nt][c]);
-    }
-
     // Sums over the lanes that share columns; o becomes sum p V relative to m, l the whole sum.
     __device__ __forceinline__ void finish() {
-        const float back = 1.f / vn;
+        const float back = __uint_as_float((127u + vexp - 20u) << 23);
         #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             #pragma unroll
@@ -365,32 +385,72 @@ struct WarpRows {
                 for (int k = 0; k < 4; ++k)                       // rows + 8 of a fragment came in as c 2^-20
                     o[i][nt][k] = fmaf(o[i][nt][k], k < 2 ? 16777216.f : 1048576.f, dsum[nt][k & 1][i / 2 / WPG]) * back;
     }
+
+    __device__ __forceinline__ float4 four(int nt, int c, int k) const {      // output lanes 32 k + 4 b + (0..3)
+        return make_float4(o[2 * k][nt][c], o[2 * k][nt][2 + c], o[2 * k + 1][nt][c], o[2 * k + 1][nt][2 + c]);
+    }
+
+    // As a part: [ROWS][D] of o, then (m, l) of each row.
+    __device__ __forceinline__ void put_part(float* part, int lane) const {
+        const int b = lane >> 2, a = lane & 3;
+        #pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            #pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int i = 8 * nt + 2 * a + c;
+                #pragma unroll
+                for (int k = 0; k < NW; ++k) *reinterpret_cast<float4*>(part + i * D + 32 * k + 4 * b) = four(nt, c, k);
+                if (b == 0) *reinterpret_cast<float2*>(part + ROWS * D + 2 * i) = make_float2(m[nt][c], l[nt][c]);
+            }
+    }
+
+    // As outputs.
+    __device__ __forceinline__ void put_out(const AttnParams& P, const Req& rq, int h, int rb, int lane) const {
+        const int b = lane >> 2, a = lane & 3;
+        #pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            #pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int row = rb * ROWS + 8 * nt + 2 * a + c;
+                if (row >= rq.ql * P.G) continue;
+                const int j = row / P.G, g = row - j * P.G;
+                const int64_t at = int64_t(rq.q0 + j) * P.out_stride + int64_t(h * P.G + g) * D + 4 * b;
+                const float inv = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];
+                #pragma unroll
+                for (int k = 0; k < NW; ++k) {
+                    const float4 v = four(nt, c, k);
+                    store4(P, at + 32 * k, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                }
+            }
+    }
 };
 
 // ------------------------------------------------------------------ the streaming kernel
 // The work is the list of (request, KV head, row block, 64-token unit), shared out evenly: CTA c of
 // n owns [c T / n, (c + 1) T / n), each of its warps an equal part of that. A warp's run crosses from
-// one (request, head, row block) to the next; what a run holds of one is a segment. A segment that is
-// whole writes its output; the others meet in shared memory at the end of the CTA, and what is still
-// a part then goes to the workspace for q4_merge_kernel (at most the CTA's first and its last).
+// one (request, head, row block) to the next; what a run holds of one is a segment. Starting and ending
+// a segment costs about as much as a unit (its queries, its sums), so each one counts as a unit more.
+// A segment that is whole writes its output; the others meet in shared memory at the end of the CTA,
+// and what is still a part then goes to the workspace for q4_merge_kernel (at most the CTA's first and
+// its last).
 //
-// Every warp streams its own run through its own ring of panels in shared memory, filled by bulk
-// copies (a panel is one contiguous piece of memory) issued two units ahead, so no warp waits for
-// another and an SM keeps about 100 KB in flight, more than its share of bandwidth times latency
-// (44 GB/s x 1 us).
+// Every warp streams its own run through its own ring of three units in shared memory, filled by bulk
+// copies (a panel is one contiguous piece of memory), two units ahead of the one that is worked on, so
+// no warp waits for another and an SM keeps about 140 KB in flight, more than its share of bandwidth
+// times latency (44 GB/s x 1 us). 8 warps of an SM: with 10 or 12 their registers spill, and a batch of 64
+// requests of up to 14402 tokens took 142 and 136 us against 133.
 template <int D, int GRP, int NT>
 struct Stream {
-    static constexpr int PANEL = panel_bytes(D, GRP), RING = 8;                 // two units
-    // warps of an SM: 8 where a row block of 16 takes their registers, else 12, or 10 where the rings
-    // of 12 do not fit
-    static constexpr int WARPS = NT == 2 ? 8 : 12 * RING * PANEL <= 222 * 1024 ? 12 : 10;
+    static constexpr int PANEL = panel_bytes(D, GRP), UNIT = 4 * PANEL, RING = 12 * PANEL * 8 <= 216 * 1024 ? 3 : 2;
+    static constexpr int WARPS = 8;
     static constexpr int THREADS = 32 * WARPS, ROWS = 8 * NT, SLOTS = 2 * WARPS;
     static constexpr int PART = ROWS * (D + 2);                                 // floats of a part: o, then (m, l)
-    static constexpr int RING_BYTES = WARPS * RING * PANEL;
+    static constexpr int RING_BYTES = WARPS * RING * UNIT;
     static constexpr int SMEM = std::max(WARPS * PART * 4, RING_BYTES) + WARPS * RING * 8;
 };
 
-// A place in the work list: unit ui of U of row block rb of KV head h of request r.
+// A place in the work list: unit ui of the U (and one more that counts for the segment) of row block rb
+// of KV head h of request r.
 struct Cursor {
     int r, h, rb, ui, U, nrb, seq;
 };
@@ -402,14 +462,19 @@ __device__ __forceinline__ void load_request(const AttnParams& P, Cursor& c, int
     c.nrb = row_blocks(a, P.G, rows);
 }
 
-__device__ __forceinline__ void advance(const AttnParams& P, Cursor& c, int rows) {
-    if (++c.ui < c.U) return;
+__device__ __forceinline__ int list_units(const Req& a, int G, int rows) {      // of one KV head
+    const int U = units_of(a);
+    return U ? row_blocks(a, G, rows) * (U + 1) : 0;
+}
+
+// To the next row block; the run is not over, so there is one.
+__device__ __forceinline__ void next_block(const AttnParams& P, Cursor& c, int rows) {
     c.ui = 0;
     if (++c.rb < c.nrb) return;
     c.rb = 0;
     if (++c.h < P.H) return;
     c.h = 0;
-    do {                                                 // the next request with work: the run is not over
+    do {
         ++c.r;
         load_request(P, c, rows);
     } while (c.U == 0);
@@ -419,18 +484,18 @@ template <int D, int GRP, int NT>
 __global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kernel(const AttnParams P) {
     using Rows = WarpRows<D, GRP, NT>;
     using S = Stream<D, GRP, NT>;
-    constexpr int ROWS = S::ROWS, SLOTS = S::SLOTS, WARPS = S::WARPS, THREADS = S::THREADS, RING = S::RING, PANEL = S::PANEL;
+    constexpr int ROWS = S::ROWS, SLOTS = S::SLOTS, WARPS = S::WARPS, THREADS = S::THREADS, PANEL = S::PANEL, RING = S::RING;
     extern __shared__ __align__(128) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::SMEM - WARPS * RING * 8);
     __shared__ int pre[THREADS + 1];
     __shared__ long long wsum[WARPS];
     __shared__ int pid[SLOTS];                           // first unit of the slot's (request, head, row block), -1: none
     __shared__ int pr[SLOTS], ph[SLOTS], prb[SLOTS];
-    __shared__ float pm[SLOTS][ROWS], pl[SLOTS][ROWS];   // max and sum of the parts' rows, then weight and sum
+    __shared__ float pm[SLOTS][ROWS], pl[SLOTS][ROWS];   // max and sum of the parts' rows
 
     const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
     const bool tell = blockIdx.x == 0;
-    uint8_t* ring = smem + w * RING * PANEL;
+    uint8_t* ring = smem + w * RING * S::UNIT;
     uint64_t* bar = bars + w * RING;
     if (lane < RING) mbar_init(bar + lane, 1);
     pdl_wait();
@@ -439,10 +504,7 @@ __global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kern
     const int per = (P.n_reqs + THREADS - 1) / THREADS;
     const int rlo = min(tid * per, P.n_reqs), rhi = min(rlo + per, P.n_reqs);
     long long sum = 0;
-    for (int r = rlo; r < rhi; ++r) {
-        const Req a = request(P, r, tell);
-        sum += (long long)P.H * row_blocks(a, P.G, ROWS) * units_of(a);
-    }
+    for (int r = rlo; r < rhi; ++r) sum += (long long)P.H * list_units(request(P, r, tell), P.G, ROWS);
     long long inc = sum;
     #pragma unroll
     for (int k = 1; k < 32; k <<= 1) {
@@ -462,15 +524,6 @@ __global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kern
     }
     __syncthreads();
     const int T = pre[THREADS], share = share_size(T, P.n_ctas);
-    if (tell) {
-        int u = int(inc - sum);
-        for (int r = rlo; r < rhi; ++r) {
-            P.prefix[r] = u;
-            const Req a = request(P, r, false);
-            u += P.H * row_blocks(a, P.G, ROWS) * units_of(a);
-        }
-        if (tid == 0) P.prefix[P.n_reqs] = T;
-    }
     pdl_trigger();
     const int ca = min(int(blockIdx.x) * share, T), cb = min(ca + share, T);
     if (ca == cb) return;
@@ -478,9 +531,8 @@ __global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kern
     // ---- this warp's run
     Rows R;
     bool held = false;
-    const int wshare = share_size(cb - ca, WARPS);
-    int u = min(ca + w * wshare, cb);
-    const int ue = min(u + wshare, cb);
+    int u = ca + w * (cb - ca) / WARPS;
+    const int ue = ca + (w + 1) * (cb - ca) / WARPS;
     if (u < ue) {
         Cursor c;
         {
@@ -492,111 +544,101 @@ __global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kern
             int off = u - pre[lo];
             for (c.r = lo * per;; ++c.r) {
                 load_request(P, c, ROWS);
-                const int all = P.H * c.nrb * c.U;
+                const int all = c.U ? P.H * c.nrb * (c.U + 1) : 0;
                 if (off < all) break;
                 off -= all;
             }
-            const int pair = off / c.U;
-            c.ui = off - pair * c.U;
+            const int pair = off / (c.U + 1);
+            c.ui = off - pair * (c.U + 1);
             c.h = pair / c.nrb;
             c.rb = pair - c.h * c.nrb;
         }
         // fetching: lanes 0 to 3 each know the block of one panel of unit f, the next to be issued
         Cursor f = c;
-        int uf = u;
-        int f_slot = 0, f_blk = 0;
-        auto look_up = [&]() {
+        int uf = u, f_blk = 0;
+        uint32_t n_f = 0, i_f = 0;                       // units issued, and the next one's place
+        const int ppb = P.block_size / kPanelTokens;     // panels of a block
+        auto block_of = [&](int t) { return P.bs_shift >= 0 ? t >> P.bs_shift : t / P.block_size; };
+        auto look_up = [&]() {                           // f to a unit, and its blocks
+            while (uf < ue && f.ui >= f.U) {
+                if (++uf < ue) next_block(P, f, ROWS);
+            }
             const int t = f.ui * kUnit + 16 * lane;
-            if (uf < ue && lane < 4 && t < f.seq) f_blk = P.block_table[int64_t(f.r) * P.bt_stride + t / P.block_size];
+            if (uf < ue && lane < 4 && t < f.seq) f_blk = P.block_table[int64_t(f.r) * P.bt_stride + block_of(t)];
         };
         auto issue = [&]() {
             if (uf >= ue) return;
             const int t = f.ui * kUnit + 16 * lane;
-            if (lane < 4 && t < f.seq) {
-                const int i = f_slot + lane >= RING ? f_slot + lane - RING : f_slot + lane;
-                if (f_blk >= 0 && f_blk < P.n_blocks) {
-                    const uint8_t* src = P.cache + ((int64_t(f_blk) * P.H + f.h) * (P.block_size / kPanelTokens) +
-                                                    (t % P.block_size) / kPanelTokens) * PANEL;
-                    mbar_expect_tx(bar + i, PANEL);
-                    bulk_g2s(ring + i * PANEL, src, PANEL, bar + i);
-                } else {                                 // NaN scales: the request's rows come out as NaN
+            const bool mine = lane < 4 && t < f.seq, good = mine && f_blk >= 0 && f_blk < P.n_blocks;
+            const uint32_t goods = __ballot_sync(0xffffffffu, good);
+            uint8_t* dst = ring + i_f * S::UNIT + lane * PANEL;
+            if (__any_sync(0xffffffffu, mine && !good)) {
+                if (mine && !good) {                     // NaN scales: the request's rows come out as NaN
                     report(P.status, TTKV_STATUS_BLOCK_RANGE);
-                    uint32_t* d = reinterpret_cast<uint32_t*>(ring + i * PANEL);
-                    for (int k = 0; k < PANEL / 4; ++k) d[k] = k < 4 * D ? 0u : 0x00007e00u;
+                    uint32_t* d = reinterpret_cast<uint32_t*>(dst);
+                    for (int k = 4 * D; k < PANEL / 4; ++k) d[k] = 0x00007e00u;
                     fence_async_smem();
-                    mbar_expect_tx(bar + i, 0);
                 }
+                __syncwarp();
             }
-            const int np = min(4, (f.seq - f.ui * kUnit + 15) / 16);
-            f_slot += np;
-            if (f_slot >= RING) f_slot -= RING;
-            if (++uf < ue) advance(P, f, ROWS);
+            if (lane == 0) mbar_expect_tx(bar + i_f, __popc(goods) * PANEL);
+            if (good) {
+                const int64_t pan = (int64_t(f_blk) * P.H + f.h) * ppb + ((t - block_of(t) * P.block_size) >> 4);
+                bulk_g2s(dst, P.cache + pan * PANEL, PANEL, bar + i_f);
+            }
+            ++n_f;
+            i_f = i_f + 1 == RING ? 0 : i_f + 1;
+            ++f.ui;
+            ++uf;
             look_up();
         };
         look_up();
-        issue();
-        int slot = 0;
-        uint32_t phases = 0;                             // bit i: the parity that slot i completes next
+        #pragma unroll 1
+        for (int i = 1; i < RING; ++i) issue();
+        uint32_t n_c = 0, i_c = 0, ph_c = 0;             // units consumed, the place of the next and its phase
         bool late = false;
         while (u < ue) {
-            const Req rq = request(P, c.r, false);
-            const int n_here = min(c.U - c.ui, ue - u), begin = c.ui;
-            R.start(P, rq, c.h, c.rb, lane);
-            for (int i = 0; i < n_here; ++i) {
-                const int t0 = (begin + i) * kUnit, np = min(4, (rq.seq - t0 + 15) / 16);
-                issue();                                 // the next unit, into the slots of the one before this
-                bool ok = true;
-                #pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const int k = slot + p >= RING ? slot + p - RING : slot + p;
-                    if (p < np) {
-                        if (!late) ok = mbar_wait(bar + k, (phases >> k) & 1u) && ok;
-                        phases ^= 1u << k;
+            const int n_list = min(c.U + 1 - c.ui, ue - u), n_here = min(c.U - c.ui, n_list), begin = c.ui;
+            u += n_list;
+            if (n_here > 0) {
+                const Req rq = request(P, c.r, false);
+                R.start(P, rq, c.h, c.rb, lane);
+                for (int i = 0; i < n_here; ++i) {
+                    issue();                             // a unit, into the place of the one before this
+                    const bool ok = late || mbar_wait(bar + i_c, ph_c);
+                    if (!__all_sync(0xffffffffu, ok)) {  // a copy never came: wait for the others, issue no more
+                        late = true;
+                        if (lane == 0) report(P.status, TTKV_STATUS_TIMEOUT);
+                        for (uint32_t k = n_c + 1; k < n_f; ++k) mbar_wait(bar + k % RING, (k / RING) & 1u);
+                        uf = ue;
                     }
+                    R.step(ring + i_c * S::UNIT, (begin + i) * kUnit, rq.seq, lane);
+                    __syncwarp();                        // every lane has read the unit
+                    ++n_c;
+                    if (++i_c == RING) { i_c = 0; ph_c ^= 1u; }
                 }
-                if (!__all_sync(0xffffffffu, ok)) {      // a copy never came: wait for the others, issue no more
-                    late = true;
-                    if (lane == 0) report(P.status, TTKV_STATUS_TIMEOUT);
-                    for (int k = (slot + np) % RING; k != f_slot; k = (k + 1) % RING) mbar_wait(bar + k, (phases >> k) & 1u);
-                    uf = ue;
-                }
-                if (t0 + kUnit <= R.min_lim) R.template step<false, RING>(ring, slot, t0, rq.seq, lane);
-                else R.template step<true, RING>(ring, slot, t0, rq.seq, lane);
-                slot += np;
-                if (slot >= RING) slot -= RING;
-                __syncwarp();                            // every lane has read the unit
-            }
-            R.finish();
-            u += n_here;
-            if (begin == 0 && n_here == c.U) {           // whole
-                R.rows([&](int i, int ln, float4 o, float m, float l) {
-                    if (c.rb * ROWS + i < rq.ql * P.G) store_out(P, rq, c.h, c.rb * ROWS + i, D, ln, o, l);
-                }, lane);
-            } else {
-                // a part: the run's last stays in registers until the rings are free, its first goes
-                // to the workspace
-                held = u == ue;
-                if (lane == 0) {
-                    const int e = 2 * w + (held ? 1 : 0);
-                    pid[e] = u - n_here - begin;
-                    pr[e] = c.r;
-                    ph[e] = c.h;
-                    prb[e] = c.rb;
-                }
-                if (!held) {
-                    float* part = P.first + (int64_t(blockIdx.x) * WARPS + w) * S::PART;
-                    R.rows([&](int i, int ln, float4 o, float m, float l) { put_part(part, ROWS, D, i, ln, o, m, l); }, lane);
+                R.finish();
+                if (begin == 0 && n_here == c.U) {       // whole
+                    R.put_out(P, rq, c.h, c.rb, lane);
+                } else {
+                    // a part: the run's last stays in registers until the rings are free, its first goes
+                    // to the workspace
+                    held = u == ue;
+                    if (lane == 0) {
+                        const int e = 2 * w + (held ? 1 : 0);
+                        pid[e] = u - n_list - begin;
+                        pr[e] = c.r;
+                        ph[e] = c.h;
+                        prb[e] = c.rb;
+                    }
+                    if (!held) R.put_part(P.first + (int64_t(blockIdx.x) * WARPS + w) * S::PART, lane);
                 }
             }
-            c.ui += n_here - 1;
-            if (u < ue) advance(P, c, ROWS);
+            if (u < ue) next_block(P, c, ROWS);
         }
     }
     __syncthreads();                                     // every copy has landed and been read
-    if (held) {
-        float* part = reinterpret_cast<float*>(smem) + w * S::PART;
-        R.rows([&](int i, int ln, float4 o, float m, float l) { put_part(part, ROWS, D, i, ln, o, m, l); }, lane);
-    }
+    if (held) R.put_part(reinterpret_cast<float*>(smem) + w * S::PART, lane);
     __syncthreads();
 
     // ---- what the warps hold of the same (request, head, row block), joined
@@ -651,13 +693,15 @@ __global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kern
 // ------------------------------------------------------------------ the merge
 // One CTA per (request, KV head, row): the parts that the CTAs left of its (request, head, row block),
 // found from the shares; also the zeros of an empty request. D / 4 threads take four lanes each of
-// one part, the CTA's thread groups different parts.
+// one part, the CTA's thread groups different parts. It is launched early and finds its place in the
+// list, a sum over the requests as in the streaming kernel, while that one still runs.
 constexpr int kMergeThreads = 256;
 
 __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParams P, int D, int rows_block) {
     __shared__ float4 so[kMergeThreads];
-    __shared__ float sl[kMergeThreads / 16], smax[kMergeThreads / 32];
-    const int r = blockIdx.y, tid = threadIdx.x;
+    __shared__ float2 sml[kMergeThreads / 16];
+    __shared__ long long sbefore[kMergeThreads / 32], sall[kMergeThreads / 32];
+    const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const Req rq = request(P, r, false);
     const int per_head = P.max_q * P.G;
     const int h = blockIdx.x / per_head, row = blockIdx.x - h * per_head;
@@ -665,45 +709,63 @@ __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParam
     const int lanes = D / 4, grp = tid / lanes, ngrp = kMergeThreads / lanes, ln = 4 * (tid - grp * lanes);
     const int U = units_of(rq);
     const int nrb = row_blocks(rq, P.G, rows_block), rb = row / rows_block, i = row - rb * rows_block;
+    long long before = 0, all = 0;
+    for (int k = tid; k < P.n_reqs; k += kMergeThreads) {
+        const long long n = (long long)P.H * list_units(request(P, k, false), P.G, rows_block);
+        all += n;
+        before += k < r ? n : 0;
+    }
+    #pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, k);
+        before += __shfl_xor_sync(0xffffffffu, before, k);
+    }
+    if (lane == 0) {
+        sbefore[tid >> 5] = before;
+        sall[tid >> 5] = all;
+    }
+    __syncthreads();
+    before = all = 0;
+    #pragma unroll
+    for (int k = 0; k < kMergeThreads / 32; ++k) {
+        before += sbefore[k];
+        all += sall[k];
+    }
     pdl_wait();
     if (U == 0) {
         if (grp == 0) store_out(P, rq, h, row, D, ln, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
         return;
     }
-    const int T = P.prefix[P.n_reqs], u0 = P.prefix[r] + (h * nrb + rb) * U, share = share_size(T, P.n_ctas);
-    if (T == 0) return;
+    if (all > 0x7fff0000) return;                                // (refused, as the streaming kernel has reported)
+    const int share = share_size(int(all), P.n_ctas), u0 = int(before) + (h * nrb + rb) * (U + 1);
     const int c0 = u0 / share, c1 = (u0 + U - 1) / share;
     if (c0 == c1) return;                                        // that CTA has written the output
     // a part lies in its CTA's first place unless the CTA's share began before it
     auto place = [&](int c) { return (int64_t(c) * 2 + (c * share >= u0 ? 0 : 1)) * rows_block + i; };
-    float M = -INFINITY;
-    for (int c = c0 + tid; c <= c1; c += kMergeThreads) M = fmaxf(M, P.part_ml[2 * place(c)]);
-    #pragma unroll
-    for (int k = 1; k < 32; k <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-    if ((tid & 31) == 0) smax[tid >> 5] = M;
-    __syncthreads();
-    #pragma unroll
-    for (int k = 0; k < kMergeThreads / 32; ++k) M = fmaxf(M, smax[k]);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
+    float m = -INFINITY, l = 0.f;
     #pragma unroll 4
     for (int c = c0 + grp; c <= c1; c += ngrp) {
         const int64_t s = place(c);
         const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * s);
         const float4 x = *reinterpret_cast<const float4*>(P.part_o + s * D + ln);
-        const float wt = part_weight(ml.x, M);
-        l = fmaf(wt, ml.y, l);
-        o.x = fmaf(wt, x.x, o.x); o.y = fmaf(wt, x.y, o.y); o.z = fmaf(wt, x.z, o.z); o.w = fmaf(wt, x.w, o.w);
+        const float M = fmaxf(m, ml.x), wo = part_weight(m, M), wn = part_weight(ml.x, M);
+        m = M;
+        l = l * wo + ml.y * wn;
+        o.x = o.x * wo + x.x * wn; o.y = o.y * wo + x.y * wn; o.z = o.z * wo + x.z * wn; o.w = o.w * wo + x.w * wn;
     }
     so[tid] = o;
-    if (ln == 0) sl[grp] = l;
+    if (ln == 0) sml[grp] = make_float2(m, l);
     __syncthreads();
     if (grp) return;
+    for (int k = 0; k < ngrp; ++k) m = fmaxf(m, sml[k].x);
     l = 0.f;
-    for (int k = 0; k < ngrp; ++k) l += sl[k];
-    for (int k = 1; k < ngrp; ++k) {
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < ngrp; ++k) {
+        const float wt = part_weight(sml[k].x, m);
         const float4 x = so[k * lanes + tid];
-        o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        l = fmaf(wt, sml[k].y, l);
+        o.x = fmaf(wt, x.x, o.x); o.y = fmaf(wt, x.y, o.y); o.z = fmaf(wt, x.z, o.z); o.w = fmaf(wt, x.w, o.w);
     }
     store_out(P, rq, h, row, D, ln, o, l);
 }
@@ -713,18 +775,17 @@ __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParam
 // Rows a streaming warp takes at once: 8 (query, head) rows a fragment, two fragments above that.
 int stream_nt(int64_t rows) { return rows > 8 ? 2 : 1; }
 
-// Workspace: units before each request, two parts a CTA for the merge, a part a warp.
+// Workspace: two parts a CTA for the merge, a part a warp.
 struct StreamWs {
-    size_t part_o, part_ml, first, bytes;
+    size_t part_ml, first, bytes;
 };
 
-StreamWs stream_ws(int d, int n_reqs, int nt) {
+StreamWs stream_ws(int d, int nt) {
     StreamWs w;
     const size_t rows = size_t(kMaxCtas) * 2 * 8 * nt;
-    w.part_o = ((size_t(n_reqs) + 1) * 4 + 15) / 16 * 16;
-    w.part_ml = w.part_o + rows * d * sizeof(float);
+    w.part_ml = rows * d * sizeof(float);
     w.first = w.part_ml + rows * 2 * sizeof(float);
-    w.bytes = w.first + size_t(kMaxCtas) * 12 * 8 * nt * (d + 2) * sizeof(float);
+    w.bytes = w.first + size_t(kMaxCtas) * Stream<128, 128, 1>::WARPS * 8 * nt * (d + 2) * sizeof(float);
     return w;
 }
 
@@ -772,7 +833,7 @@ int launch_stream(const AttnParams& P, cudaStream_t st) {
 
 int run_stream(const ttkv_q4_cache_t* c, AttnParams P, void* ws, size_t ws_bytes, cudaStream_t st) {
     const int nt = stream_nt(int64_t(P.max_q) * P.G);
-    const StreamWs w = stream_ws(c->d, P.n_reqs, nt);
+    const StreamWs w = stream_ws(c->d, nt);
     if (!ws || ws_bytes < w.bytes)
         return fail(TTKV_ERR_WORKSPACE, "4-bit read: workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, w.bytes);
     if (reinterpret_cast<uintptr_t>(ws) & 15) return fail(TTKV_ERR_ALIGN, "4-bit read: workspace not 16-byte aligned");
@@ -780,8 +841,7 @@ int run_stream(const ttkv_q4_cache_t* c, AttnParams P, void* ws, size_t ws_bytes
     if (int e = sm_count(&sms)) return e;
     P.n_ctas = std::min(sms, kMaxCtas);
     char* base = static_cast<char*>(ws);
-    P.prefix = reinterpret_cast<int32_t*>(base);
-    P.part_o = reinterpret_cast<float*>(base + w.part_o);
+    P.part_o = reinterpret_cast<float*>(base);
     P.part_ml = reinterpret_cast<float*>(base + w.part_ml);
     P.first = reinterpret_cast<float*>(base + w.first);
 #define TTKV_Q4_STREAM(D, GRP)                                                                     \
@@ -795,6 +855,9 @@ AttnParams attn_params(const ttkv_q4_attn_args_t* a) {
     const ttkv_q4_cache_t* c = &a->cache;
     AttnParams P{};
     P.cache = c->base; P.n_blocks = c->n_blocks; P.H = c->H; P.G = a->HQ / c->H; P.block_size = c->block_size;
+    P.bs_shift = -1;
+    for (int b = 0; b < 31; ++b)
+        if (c->block_size == (1 << b)) P.bs_shift = b;
     P.block_table = a->block_table; P.bt_stride = a->bt_stride; P.bt_cols = a->bt_cols; P.seq_lens = a->seq_lens;
     P.n_reqs = a->n_reqs; P.q = a->q; P.dtype = a->dtype; P.q_stride = a->q_stride; P.scale = a->scale;
     P.out = a->out; P.out_stride = a->out_stride; P.status = a->status;
@@ -814,7 +877,7 @@ constexpr int kStreamRows = 32;
 using namespace ttkv;
 
 extern "C" size_t ttkv_q4_decode_workspace_bytes(int32_t d, int32_t n_reqs, int32_t group_heads) {
-    return n_reqs < 0 ? 0 : stream_ws(d, n_reqs, stream_nt(group_heads)).bytes;
+    return n_reqs < 0 ? 0 : stream_ws(d, stream_nt(group_heads)).bytes;
 }
 
 extern "C" int ttkv_q4_decode(const ttkv_q4_attn_args_t* args) {
@@ -829,7 +892,7 @@ extern "C" int ttkv_q4_decode(const ttkv_q4_attn_args_t* args) {
 extern "C" size_t ttkv_q4_prefill_workspace_bytes(int32_t d, int32_t n_reqs, int32_t group_heads, int32_t max_q_len) {
     if (n_reqs < 0 || max_q_len < 0) return 0;
     const int64_t rows = int64_t(max_q_len) * group_heads;
-    return rows > kStreamRows ? chunk_workspace_bytes(d) : stream_ws(d, n_reqs, stream_nt(rows)).bytes;
+    return rows > kStreamRows ? chunk_workspace_bytes(d) : stream_ws(d, stream_nt(rows)).bytes;
 }
 
 extern "C" int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args) {
