@@ -67,43 +67,26 @@ ATTN = CACHE | dict(block_table=A, seq_lens=A, q_start=A, q_len=A, q=A, out=A, b
                     workspace_bytes=1 << 30, status=A, stream=0)
 PLAN = dict(block_table=A, lens=A, query_start_loc=A, free_blocks=A, free_count=A, free_count_out=A, slots=A, positions=A,
             bt_stride=8, bt_cols=8, n_reqs=3, capacity=50, block_size=16, n_tokens=9, status=A, stream=0)
-PACKINGS = {"store": (_lib.Q4StoreArgs, _lib.Q4_STORE, STORE), "attn": (_lib.Q4AttnArgs, _lib.Q4_ATTN, ATTN),
-            "plan": (_lib.PlanArgs, _lib.PLAN, PLAN)}
 
 
-def _call(fn, fields, packing, **kw):
-    return fn(packing.pack(*(fields | kw).values()))
+def _call(fn, cls, fields):
+    """A C entry on a struct filled by name."""
+    a = cls()
+    for f, v in fields.items():
+        setattr(a if hasattr(a, f) else a.cache, f, v)
+    return fn(C.byref(a))
 
 
 def _store(fn, **kw):
-    return _call(fn, STORE, _lib.Q4_STORE, **kw)
+    return _call(fn, _lib.Q4StoreArgs, STORE | kw)
 
 
 def _attn(fn, **kw):
-    return _call(fn, ATTN, _lib.Q4_ATTN, **kw)
+    return _call(fn, _lib.Q4AttnArgs, ATTN | kw)
 
 
 def _plan(fn, **kw):
-    return _call(fn, PLAN, _lib.PLAN, **kw)
-
-
-@pytest.mark.parametrize("name", PACKINGS)
-def test_packings_match_the_structs(name):
-    """A packed call lays its fields out as the C struct does: distinct values come back by name."""
-    cls, packing, fields = PACKINGS[name]
-    flat = {}
-    for f, t in cls._fields_:
-        if issubclass(t, C.Structure):
-            flat |= dict(t._fields_)
-        else:
-            flat[f] = t
-    assert list(flat) == list(fields)
-    values = {f: float(i) if t is C.c_float else i + 1 for i, (f, t) in enumerate(flat.items())}
-    raw = packing.pack(*values.values())
-    assert len(raw) == C.sizeof(cls)
-    got = cls.from_buffer_copy(raw)
-    for f, v in values.items():
-        assert getattr(got if hasattr(got, f) else got.cache, f) == v, f
+    return _call(fn, _lib.PlanArgs, PLAN | kw)
 
 
 BAD_CACHES = [(dict(d=96), _lib.ERR_UNSUPPORTED), (dict(group=16), _lib.ERR_UNSUPPORTED),

@@ -63,7 +63,8 @@ struct WarpRows {
     float q1[NT][2][NG], qm[NT][2];     // sums of q 2^e over each group; 2^-e scale log2(e)
     int lim[NT][2], min_lim;            // tokens each row sees; the fewest any row of the block does
     float m[NT][2], l[NT][2];           // maximum so far (base 2) and this lane's share of the sum
-    float o[2 * NW][NT][4];             // (p s 2^vn) . (c - 7.5)
+    float o[2 * NW][NT][4];             // (p s 2^vn) . (c - 7.5), less 3.75 `pre` (2^-24 or 2^-20 of it)
+    float pre[NT][2][NG];               // sum of p s 2^vn over the unit before
     float dsum[NT][2][NG];              // this lane's share of 2^vn p (m + 7.5 s)
     uint32_t vexp;                      // fp16 exponent field of the largest V scale so far; vn = 20 - vexp
     bool fresh;                         // no unit yet
@@ -137,7 +138,7 @@ struct WarpRows {
                 #pragma unroll
                 for (int k = 0; k < NG; ++k) {
                     q1[nt][c][k] = __shfl_sync(0xffffffffu, sum[k], from);
-                    dsum[nt][c][k] = 0.f;
+                    dsum[nt][c][k] = pre[nt][c][k] = 0.f;
                 }
                 qm[nt][c] = __shfl_sync(0xffffffffu, fac, from);
                 lim[nt][c] = __shfl_sync(0xffffffffu, seen, from);
@@ -292,7 +293,10 @@ struct WarpRows {
                 for (int c = 0; c < 2; ++c) {
                     corr[nt][c] *= vfall;
                     #pragma unroll
-                    for (int g = 0; g < NG; ++g) dsum[nt][c][g] *= corr[nt][c];
+                    for (int g = 0; g < NG; ++g) {
+                        dsum[nt][c][g] *= corr[nt][c];
+                        pre[nt][c][g] *= corr[nt][c];
+                    }
                 }
             #pragma unroll
             for (int i = 0; i < 2 * NW; ++i)
@@ -353,14 +357,25 @@ struct WarpRows {
             }
         }
         // centred at once, so that o stays as small as the values are: the products' sums are cut, not
-        // rounded, at 2^-23 of what they hold
+        // rounded, at 2^-23 of what they hold. And ahead by half of what the next unit is likely to add, so
+        // that o runs from below zero to above it and the cuts fall on both sides
+        float shift[NG][NT][2];
+        #pragma unroll
+        for (int g = 0; g < NG; ++g)
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                #pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    shift[g][nt][c] = fmaf(3.75f, pre[nt][c][g], -11.25f * psum[g][nt][c]);
+                    pre[nt][c][g] = psum[g][nt][c];
+                }
         #pragma unroll
         for (int i = 0; i < 2 * NW; ++i)
             #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    o[i][nt][k] = fmaf(k < 2 ? -7.5f / 16777216.f : -7.5f / 1048576.f, psum[i / 2 / WPG][nt][k], o[i][nt][k]);
+                    o[i][nt][k] = fmaf(k < 2 ? 1.f / 16777216.f : 1.f / 1048576.f, shift[i / 2 / WPG][nt][k & 1], o[i][nt][k]);
     }
 
     // Sums over the lanes that share columns; o becomes sum p V relative to m, l the whole sum.
@@ -376,6 +391,8 @@ struct WarpRows {
                     #pragma unroll
                     for (int g = 0; g < NG; ++g) dsum[nt][c][g] += __shfl_xor_sync(0xffffffffu, dsum[nt][c][g], k);
                 }
+                #pragma unroll
+                for (int g = 0; g < NG; ++g) dsum[nt][c][g] = fmaf(3.75f, pre[nt][c][g], dsum[nt][c][g]);
             }
         #pragma unroll
         for (int i = 0; i < 2 * NW; ++i)

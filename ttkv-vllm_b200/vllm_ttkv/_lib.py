@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes as C
 import pathlib
-import struct
 
 ABI_VERSION = 6
 LIB_PATH = pathlib.Path(__file__).resolve().parents[1] / "libttkv_sm100.so"
@@ -97,13 +96,6 @@ class PlanArgs(C.Structure):
                 ("stream", C.c_void_p)]
 
 
-# The same three as one `struct` packing each, in the fields' order (the C layout's padding is the
-# native alignment's): a call packs its arguments and passes the bytes, which costs about 1 us where a
-# ctypes call of as many arguments costs 7.
-Q4_STORE = struct.Struct("@PqiiiiiPPPqqiiiPP")
-Q4_ATTN = struct.Struct("@PqiiiiiPPPPPPqqqiiiiiiifPNPP")
-PLAN = struct.Struct("@PPPPPPPPqiiiiiPP")
-
 PLAN_MAX_REQS = 16384                       # TTKV_PLAN_MAX_REQS
 
 P, I32, I64, SZ, F = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_float
@@ -154,6 +146,8 @@ SIGNATURES = {
 }
 
 _LIB = None
+_BINDING = None
+BINDING_PATH = LIB_PATH.with_name("_ttkv_torch.so")
 
 
 class TTKVError(RuntimeError):
@@ -185,6 +179,22 @@ def lib():
     if _LIB is None:
         _LIB = load()
     return _LIB
+
+
+def torch_binding():
+    """The module `_ttkv_torch` (csrc/ttkv_torch.cpp): the 4-bit cache's and the block tables' calls on
+    torch tensors. As for the library, there is nothing in its place when it has not been built."""
+    global _BINDING
+    if _BINDING is None:
+        lib()                                        # its ABI version is checked; the binding links to it
+        if not BINDING_PATH.exists():
+            raise ImportError(f"{BINDING_PATH} is missing: run `vllm_ttkv._build.build()`")
+        from importlib import machinery, util
+        loader = machinery.ExtensionFileLoader("_ttkv_torch", str(BINDING_PATH))
+        module = util.module_from_spec(util.spec_from_loader("_ttkv_torch", loader))
+        loader.exec_module(module)
+        _BINDING = module
+    return _BINDING
 
 
 def check(code: int):

@@ -8,7 +8,6 @@ status word; `check_status()` reads it once (one readback) and raises.
 from __future__ import annotations
 
 import ctypes as C
-import functools
 
 import torch
 
@@ -394,97 +393,20 @@ def fit_tail(G1, G2, G3, budget: int, qbits: int = 8):
 
 
 # ---------------------------------------------------------------- the 4-bit paged cache (vllm_ttkv.q4)
-# These calls are short on the GPU, so their host side is kept lean: attributes of a tensor are read
-# once, and a call's arguments go to the library as one packed struct.
-def _device_of(t: torch.Tensor) -> int:
-    i = t.get_device()
-    if i < 0:
-        _need_cuda(t)
-    return i
-
-
-def _elsewhere(dev: int, *named):
-    """Raise for the first of the (name, tensor) pairs that is not on device `dev`."""
-    for name, t in named:
-        if t is not None and t.get_device() != dev:
-            _need_cuda(t)
-            raise ValueError(f"{name} is on {t.device}, the cache or block table on cuda:{dev}")
-
-
-def _status_ptr(dev: int, status: torch.Tensor | None) -> int:
-    if status is None:
-        status = _STATUS_OF.get(dev)
-        if status is None:
-            status = _STATUS_OF[dev] = status_word(torch.device("cuda", dev))
-    elif status.dtype != torch.int32 or status.get_device() != dev:
-        raise ValueError(f"status must be an int32 word on cuda:{dev}")
-    return status.data_ptr()
-
-
+# These calls are a few microseconds long on the GPU, so their arguments are checked and passed on by
+# the compiled binding: TypeError for a wrong type, ValueError for a wrong shape, stride or device.
 _STATUS_OF: dict = {}                    # device index -> its status word (`status_word`)
 
 
-def _launch(dev: int, fn, packing, *args) -> None:
-    """Call a C entry with its packed arguments and device `dev`'s current stream, which need not be
-    the current device's."""
-    if dev == torch.cuda.current_device():
-        code = fn(packing.pack(*args, torch.cuda.current_stream(dev).cuda_stream))
-    else:
-        with torch.cuda.device(dev):
-            code = fn(packing.pack(*args, torch.cuda.current_stream(dev).cuda_stream))
-    if code:
-        _lib.check(code)
-
-
-def _rows_of(t: torch.Tensor, heads: int, d: int, name: str):
-    """(rows, stride between rows) of a [n, heads, d] tensor whose [heads, d] rows are contiguous (a
-    size-1 dimension may carry any stride)."""
-    shape, st = t.shape, t.stride()
-    if len(shape) != 3 or shape[1] != heads or shape[2] != d:
-        raise ValueError(f"{name} must be [n, {heads}, {d}], got {tuple(shape)}")
-    n = shape[0]
-    if st[2] != 1 or (st[1] != d and heads > 1):
-        raise ValueError(f"{name} must have contiguous [heads, d] rows (strides {st})")
-    if n < 2:
-        return n, heads * d
-    if st[0] < heads * d:
-        raise ValueError(f"{name}'s rows overlap (strides {st})")
-    return n, st[0]
-
-
-def _vector(t: torch.Tensor, dtype, least: int, name: str) -> int:
-    """The address of a contiguous 1-D tensor of at least `least` entries."""
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 1 or t.numel() < least or not (t.is_contiguous() or least < 2):
-        raise ValueError(f"{name} must be contiguous with {least} entries at least, got {tuple(t.shape)} strided {t.stride()}")
-    return t.data_ptr()
-
-
-def _table_of(t: torch.Tensor):
-    """(requests, blocks a row, stride between rows) of a block table."""
-    if t.dtype != torch.int32 or t.dim() != 2:
-        raise TypeError(f"block_table must be int32 [n_reqs, max_blocks], got {tuple(t.shape)} {t.dtype}")
-    n, cols = t.shape
-    st = t.stride()
-    if n * cols and cols > 1 and st[1] != 1:
-        raise ValueError("block_table must have unit column stride")
-    return n, cols, st[0] if n > 1 else cols
-
-
-def _q4_store(fn, lay, cache, slots, k, v, status, skip_pad):
-    dev = _device_of(cache)
-    _elsewhere(dev, ("slot_mapping", slots), ("k", k), ("v", v))
-    block_size = lay.block_size(cache)
-    n = slots.numel()
-    sp = _vector(slots, torch.int64, n, "slot_mapping")
-    nk, ks = _rows_of(k, lay.H, lay.d, "k")
-    nv, vs = _rows_of(v, lay.H, lay.d, "v")
-    if nk < n or nv < n:
-        raise ValueError(f"k and v hold {nk} and {nv} tokens for {n} slot ids")
-    _launch(dev, fn, _lib.Q4_STORE, cache.data_ptr(), cache.shape[0], lay.H, lay.d, lay.group, block_size,
-            _lib.CACHE_SKIP_PAD if skip_pad else 0, sp, k.data_ptr(), v.data_ptr(), ks, vs, n, dtype_code(k),
-            dtype_code(v), _status_ptr(dev, status))
+def _status_of(t: torch.Tensor, status: torch.Tensor | None) -> torch.Tensor:
+    if status is not None:
+        return status
+    dev = t.get_device()
+    st = _STATUS_OF.get(dev)
+    if st is None:
+        _need_cuda(t)
+        st = _STATUS_OF[dev] = status_word(torch.device("cuda", dev))
+    return st
 
 
 def q4_write_paged(lay, cache: torch.Tensor, slot_mapping: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -492,39 +414,18 @@ def q4_write_paged(lay, cache: torch.Tensor, slot_mapping: torch.Tensor, k: torc
     """Quantise tokens k/v [n, H, d] (fp32, fp16 or bf16, rows of any stride) into their slots of a
     4-bit cache (`lay`: a `q4.Q4Layout`). The slots of one call must differ. skip_pad: a negative slot
     is skipped instead of refused (`check_status`)."""
-    _q4_store(_lib.lib().ttkv_q4_write, lay, cache, slot_mapping, k, v, status, skip_pad)
+    code = _lib.torch_binding().store(True, lay.key, cache, slot_mapping, k, v, _status_of(cache, status), bool(skip_pad))
+    if code:
+        _lib.check(code)
 
 
 def q4_read_paged(lay, cache: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                   status: torch.Tensor | None = None, skip_pad: bool = False) -> None:
     """The values stored at `slots` into k/v [n, H, d] (fp32, fp16 or bf16): what the attention over
     the cache sees. Rows of skipped or refused slots are left as they were."""
-    _q4_store(_lib.lib().ttkv_q4_read, lay, cache, slots, k, v, status, skip_pad)
-
-
-@functools.lru_cache(maxsize=4096)
-def _q4_decode_scratch(d: int, n_reqs: int, group_heads: int) -> int:
-    return _lib.lib().ttkv_q4_decode_workspace_bytes(d, n_reqs, group_heads)
-
-
-@functools.lru_cache(maxsize=4096)
-def _q4_prefill_scratch(d: int, n_reqs: int, group_heads: int, max_q_len: int) -> int:
-    return _lib.lib().ttkv_q4_prefill_workspace_bytes(d, n_reqs, group_heads, max_q_len)
-
-
-def _q4_queries(lay, q, out):
-    """(rows, HQ, q's stride, out's stride, type code)."""
-    dt = q.dtype
-    if (dt != torch.float16 and dt != torch.bfloat16) or out.dtype != dt:
-        raise TypeError(f"queries and outputs are both float16 or both bfloat16, got {dt} and {out.dtype}")
-    if q.dim() != 3 or q.shape[1] % lay.H or q.shape[1] == 0:
-        raise ValueError(f"q must be [n, HQ, {lay.d}] with HQ a multiple of H={lay.H}, got {tuple(q.shape)}")
-    HQ = q.shape[1]
-    n, qs = _rows_of(q, HQ, lay.d, "q")
-    n_out, os_ = _rows_of(out, HQ, lay.d, "out")
-    if n_out < n:
-        raise ValueError(f"{n} queries, {n_out} outputs")
-    return n, HQ, qs, os_, _DTYPE[dt]
+    code = _lib.torch_binding().store(False, lay.key, cache, slots, k, v, _status_of(cache, status), bool(skip_pad))
+    if code:
+        _lib.check(code)
 
 
 def q4_decode_paged(lay, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -535,21 +436,9 @@ def q4_decode_paged(lay, cache: torch.Tensor, block_table: torch.Tensor, seq_len
     Nothing is read back, and the launch depends only on the shapes: a captured call replays any
     lengths. The scratch is allocated per call by torch, so calls on different streams, and captured
     graphs, do not share it."""
-    dev = _device_of(cache)
-    _elsewhere(dev, ("block_table", block_table), ("seq_lens", seq_lens), ("q", q), ("out", out))
-    block_size = lay.block_size(cache)
-    n, HQ, qs, os_, dt = _q4_queries(lay, q, out)
-    B, cols, bts = _table_of(block_table)
-    if B != n:
-        raise ValueError(f"{n} queries, {B} block-table rows")
-    slp = _vector(seq_lens, torch.int32, n, "seq_lens")
-    if n == 0:
-        return out
-    ws_n = _q4_decode_scratch(lay.d, n, HQ // lay.H)
-    ws = torch.empty(ws_n, dtype=torch.uint8, device=cache.device)
-    _launch(dev, _lib.lib().ttkv_q4_decode, _lib.Q4_ATTN, cache.data_ptr(), cache.shape[0], lay.H, lay.d, lay.group,
-            block_size, 0, block_table.data_ptr(), slp, 0, 0, q.data_ptr(), out.data_ptr(), bts, qs, os_, cols, n, n, HQ,
-            dt, 1, 0, scale, ws.data_ptr(), ws_n, _status_ptr(dev, status))
+    code = _lib.torch_binding().attend(lay.key, cache, block_table, seq_lens, q, scale, out, _status_of(cache, status))
+    if code:
+        _lib.check(code)
     return out
 
 
@@ -561,48 +450,14 @@ def q4_prefill_paged(lay, cache: torch.Tensor, block_table: torch.Tensor, seq_le
     (fp16 or bf16), at positions seq_len - q_len + j, causal over the stored tokens (which include the
     chunk's own). `max_q_len` and `max_seq_len` bound the batch (host numbers, no readback); a request
     above them is refused on the device (`check_status`). Rows of no request are left as they were."""
-    dev = _device_of(cache)
-    _elsewhere(dev, ("block_table", block_table), ("seq_lens", seq_lens), ("q_start", q_start), ("q_len", q_len),
-               ("q", q), ("out", out))
-    block_size = lay.block_size(cache)
-    n, HQ, qs, os_, dt = _q4_queries(lay, q, out)
-    B, cols, bts = _table_of(block_table)
-    slp, qsp, qlp = (_vector(t, torch.int32, B, name) for name, t in
-                     (("seq_lens", seq_lens), ("q_start", q_start), ("q_len", q_len)))
-    max_q_len, max_seq_len = int(max_q_len), int(max_seq_len)
-    if max_q_len < 0 or max_seq_len < 0:
-        raise ValueError(f"max_q_len={max_q_len} and max_seq_len={max_seq_len} must not be negative")
-    if B == 0 or n == 0:
-        return out
-    ws_n = _q4_prefill_scratch(lay.d, B, HQ // lay.H, max_q_len)
-    ws = torch.empty(ws_n, dtype=torch.uint8, device=cache.device)
-    _launch(dev, _lib.lib().ttkv_q4_prefill, _lib.Q4_ATTN, cache.data_ptr(), cache.shape[0], lay.H, lay.d, lay.group,
-            block_size, 0, block_table.data_ptr(), slp, qsp, qlp, q.data_ptr(), out.data_ptr(), bts, qs, os_, cols, B, n,
-            HQ, dt, max_q_len, max_seq_len, scale, ws.data_ptr(), ws_n, _status_ptr(dev, status))
+    code = _lib.torch_binding().attend(lay.key, cache, block_table, seq_lens, q, scale, out, _status_of(cache, status),
+                                       q_start, q_len, max_q_len, max_seq_len)
+    if code:
+        _lib.check(code)
     return out
 
 
 # ---------------------------------------------------------------- block tables on the device
-def _plan_args(block_table, lens, name, free_blocks, free_count, free_count_out):
-    """(device, the table's geometry, the addresses) that a plan and a release share."""
-    dev = _device_of(block_table)
-    _elsewhere(dev, (name, lens), ("free_blocks", free_blocks), ("free_count", free_count),
-               ("free_count_out", free_count_out))
-    n, cols, stride = _table_of(block_table)
-    if n > 1 and stride < cols:
-        raise ValueError("block_table's rows overlap")
-    if n > _lib.PLAN_MAX_REQS:
-        raise ValueError(f"{n} requests in one call: at most {_lib.PLAN_MAX_REQS}")
-    capacity = free_blocks.numel()
-    out = free_count if free_count_out is None else free_count_out
-    if free_count.numel() != 1 or out.numel() != 1:
-        raise ValueError("free_count and free_count_out hold one number each")
-    if free_count.dtype != torch.int32 or out.dtype != torch.int32:
-        raise TypeError(f"free_count and free_count_out must be int32, got {free_count.dtype} and {out.dtype}")
-    return (dev, n, cols, stride, _vector(lens, torch.int32, n, name), capacity,
-            _vector(free_blocks, torch.int32, capacity, "free_blocks"), free_count.data_ptr(), out.data_ptr())
-
-
 def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor,
               free_blocks: torch.Tensor, free_count: torch.Tensor, block_size: int, slot_mapping: torch.Tensor,
               positions: torch.Tensor | None = None, free_count_out: torch.Tensor | None = None,
@@ -615,15 +470,11 @@ def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc
     `write_paged` skip with skip_pad). The blocks left go to `free_count_out` (default: free_count).
     A request that is refused (the list is empty, its row is short, its lengths disagree) has slots -1
     and, behind the blocks it holds, a block id -1, which the reads refuse; see `check_status`."""
-    dev, n, cols, stride, lp, capacity, fp, cp, op = _plan_args(block_table, seq_lens, "seq_lens", free_blocks,
-                                                                free_count, free_count_out)
-    _elsewhere(dev, ("query_start_loc", query_start_loc), ("slot_mapping", slot_mapping), ("positions", positions))
-    qp = _vector(query_start_loc, torch.int32, n + 1, "query_start_loc")
-    T = slot_mapping.numel()
-    sp = _vector(slot_mapping, torch.int64, T, "slot_mapping")
-    pp = 0 if positions is None else _vector(positions, torch.int64, T, "positions")
-    _launch(dev, _lib.lib().ttkv_plan_step, _lib.PLAN, block_table.data_ptr(), lp, qp, fp, cp, op, sp, pp, stride, cols, n,
-            capacity, int(block_size), T, _status_ptr(dev, status))
+    code = _lib.torch_binding().plan(block_table, seq_lens, free_blocks, free_count,
+                                     free_count if free_count_out is None else free_count_out, block_size,
+                                     _status_of(block_table, status), query_start_loc, slot_mapping, positions)
+    if code:
+        _lib.check(code)
 
 
 def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, free_blocks: torch.Tensor,
@@ -632,7 +483,8 @@ def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, free_blocks: t
     """Return the blocks of finished requests: the ceil(lens[r] / block_size) blocks of each row go onto
     the end of free_blocks[:free_count], in request order (lens[r] = 0: none). The table's rows are left
     as they are. Each block may be returned once."""
-    dev, n, cols, stride, lp, capacity, fp, cp, op = _plan_args(block_table, lens, "lens", free_blocks, free_count,
-                                                                free_count_out)
-    _launch(dev, _lib.lib().ttkv_release_blocks, _lib.PLAN, block_table.data_ptr(), lp, 0, fp, cp, op, 0, 0, stride, cols,
-            n, capacity, int(block_size), 0, _status_ptr(dev, status))
+    code = _lib.torch_binding().plan(block_table, lens, free_blocks, free_count,
+                                     free_count if free_count_out is None else free_count_out, block_size,
+                                     _status_of(block_table, status))
+    if code:
+        _lib.check(code)

@@ -37,6 +37,8 @@ class Q4Layout:
             raise ValueError(f"groups of {self.group} lanes: 32, 64 or 128, at most d={self.d}")
         # bytes of a panel: 16 tokens of one head
         object.__setattr__(self, "panel_bytes", PANEL_TOKENS * (self.d + 8 * (self.d // self.group)))
+        # what the calls need of it
+        object.__setattr__(self, "key", (self.H, self.d, self.group, self.panel_bytes))
 
     def bytes_per_token(self) -> int:
         """Cache bytes of one token over the layer's heads."""
