@@ -54,6 +54,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // unit, and when a lane's sum of a unit's weights passes 2^9. V scales are brought into [2^5, 2^6) by a
 // power of two, so the products that become fp16 stay below 2^15 and keep their precision down to
 // weights of 2^-19 of the largest; the power falls when a larger scale comes.
+//
+// The tensor cores do not round a product of a subnormal, they cut it toward zero near 2^-18 of the
+// step's largest, and over a long row cuts of products that are all positive show: 4e-4 of the output
+// at 131071 tokens. So odd panels go in as -p' (15 - c), whose cuts are to the other side, and what is
+// left to centre is 7.5 times the difference of even and odd weights.
 constexpr float kWeightsMost = 512.f;
 
 template <int D, int GRP, int NT>
@@ -63,8 +68,7 @@ struct WarpRows {
     float q1[NT][2][NG], qm[NT][2];     // sums of q 2^e over each group; 2^-e scale log2(e)
     int lim[NT][2], min_lim;            // tokens each row sees; the fewest any row of the block does
     float m[NT][2], l[NT][2];           // maximum so far (base 2) and this lane's share of the sum
-    float o[2 * NW][NT][4];             // (p s 2^vn) . (c - 7.5), less 3.75 `pre` (2^-24 or 2^-20 of it)
-    float pre[NT][2][NG];               // sum of p s 2^vn over the unit before
+    float o[2 * NW][NT][4];             // (p s 2^vn) . (c - 7.5), 2^-24 of it or (rows + 8 of a fragment) 2^-20
     float dsum[NT][2][NG];              // this lane's share of 2^vn p (m + 7.5 s)
     uint32_t vexp;                      // fp16 exponent field of the largest V scale so far; vn = 20 - vexp
     bool fresh;                         // no unit yet
@@ -138,7 +142,7 @@ struct WarpRows {
                 #pragma unroll
                 for (int k = 0; k < NG; ++k) {
                     q1[nt][c][k] = __shfl_sync(0xffffffffu, sum[k], from);
-                    dsum[nt][c][k] = pre[nt][c][k] = 0.f;
+                    dsum[nt][c][k] = 0.f;
                 }
                 qm[nt][c] = __shfl_sync(0xffffffffu, fac, from);
                 lim[nt][c] = __shfl_sync(0xffffffffu, seen, from);
@@ -293,10 +297,7 @@ struct WarpRows {
                 for (int c = 0; c < 2; ++c) {
                     corr[nt][c] *= vfall;
                     #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        dsum[nt][c][g] *= corr[nt][c];
-                        pre[nt][c][g] *= corr[nt][c];
-                    }
+                    for (int g = 0; g < NG; ++g) dsum[nt][c][g] *= corr[nt][c];
                 }
             #pragma unroll
             for (int i = 0; i < 2 * NW; ++i)
@@ -305,13 +306,14 @@ struct WarpRows {
                     #pragma unroll
                     for (int k = 0; k < 4; ++k) o[i][nt][k] *= corr[nt][k & 1];
         }
-        float psum[NG][NT][4];                                    // the unit's sum of p', the same in every row
+        float psum[NG][NT][4];                                    // 15 times the unit's signed sum of p'
         #pragma unroll
         for (int g = 0; g < NG; ++g)
             #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) psum[g][nt][i] = 0.f;
+        constexpr uint32_t L = 0x000f000fu, H = 0x00f000f0u;
         #pragma unroll
         for (int p = 0; p < 4; ++p) {
             uint32_t pf[NG][NT][2];
@@ -320,7 +322,7 @@ struct WarpRows {
                 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&vm[p][i][g]));
-                    const float sv = sm.x * vn, mid = fmaf(7.5f, sv, sm.y * vn);
+                    const float sv = sm.x * (p & 1 ? -vn : vn), mid = fmaf(p & 1 ? -7.5f : 7.5f, sv, sm.y * vn);
                     #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const float p0 = s[p][nt][2 * i], p1 = s[p][nt][2 * i + 1];
@@ -335,47 +337,32 @@ struct WarpRows {
                         pf[g][nt][i] = transpose8x8(half2_bits(w0, w1));
                     }
                 }
-            constexpr uint32_t ONES = 0x3c003c00u;
             #pragma unroll
             for (int g = 0; g < NG; ++g)
                 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16816(psum[g][nt], ONES, ONES, ONES, ONES, pf[g][nt][0], pf[g][nt][1]);
+                for (int nt = 0; nt < NT; ++nt)
+                    mma16816(psum[g][nt], L, H, L, H, pf[g][nt][0], pf[g][nt][1]);
             uint32_t lo[NW], hi[NW];                              // tokens 2 a, 2 a + 1 and those + 8
             load_words(vp + p * PANEL, lo);
             load_words(vp + p * PANEL + 4 * D, hi);
             #pragma unroll
             for (int w = 0; w < NW; ++w) {
+                if (p & 1) { lo[w] = ~lo[w]; hi[w] = ~hi[w]; }
                 const uint32_t l8 = lo[w] >> 8, h8 = hi[w] >> 8;
                 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const uint32_t b0 = pf[w / WPG][nt][0], b1 = pf[w / WPG][nt][1];
-                    mma16816(o[2 * w][nt], lo[w] & 0x000f000fu, lo[w] & 0x00f000f0u, hi[w] & 0x000f000fu,
-                             hi[w] & 0x00f000f0u, b0, b1);
-                    mma16816(o[2 * w + 1][nt], l8 & 0x000f000fu, l8 & 0x00f000f0u, h8 & 0x000f000fu, h8 & 0x00f000f0u,
-                             b0, b1);
+                    mma16816(o[2 * w][nt], lo[w] & L, lo[w] & H, hi[w] & L, hi[w] & H, b0, b1);
+                    mma16816(o[2 * w + 1][nt], l8 & L, l8 & H, h8 & L, h8 & H, b0, b1);
                 }
             }
         }
-        // centred at once, so that o stays as small as the values are: the products' sums are cut, not
-        // rounded, at 2^-23 of what they hold. And ahead by half of what the next unit is likely to add, so
-        // that o runs from below zero to above it and the cuts fall on both sides
-        float shift[NG][NT][2];
-        #pragma unroll
-        for (int g = 0; g < NG; ++g)
-            #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    shift[g][nt][c] = fmaf(3.75f, pre[nt][c][g], -11.25f * psum[g][nt][c]);
-                    pre[nt][c][g] = psum[g][nt][c];
-                }
         #pragma unroll
         for (int i = 0; i < 2 * NW; ++i)
             #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    o[i][nt][k] = fmaf(k < 2 ? 1.f / 16777216.f : 1.f / 1048576.f, shift[i / 2 / WPG][nt][k & 1], o[i][nt][k]);
+                for (int k = 0; k < 4; ++k) o[i][nt][k] = fmaf(-0.5f, psum[i / 2 / WPG][nt][k], o[i][nt][k]);
     }
 
     // Sums over the lanes that share columns; o becomes sum p V relative to m, l the whole sum.
@@ -391,8 +378,6 @@ struct WarpRows {
                     #pragma unroll
                     for (int g = 0; g < NG; ++g) dsum[nt][c][g] += __shfl_xor_sync(0xffffffffu, dsum[nt][c][g], k);
                 }
-                #pragma unroll
-                for (int g = 0; g < NG; ++g) dsum[nt][c][g] = fmaf(3.75f, pre[nt][c][g], dsum[nt][c][g]);
             }
         #pragma unroll
         for (int i = 0; i < 2 * NW; ++i)
