@@ -43,7 +43,7 @@ def _batch(rng, n, q_hi, hi, bs, cols, spare):
 
 
 @pytest.mark.parametrize("n,q_hi,hi,bs", [(1, 1, 1, 16), (1, 500, 900, 16), (7, 1, 200, 1), (64, 1, 3000, 16), (513, 40, 300, 32),
-                                          (1500, 3, 50, 17)])
+                                          (1500, 3, 50, 17), (2048, 2, 40, 16), (2049, 2, 40, 16), (16384, 1, 20, 16)])
 @pytest.mark.parametrize("pad", [0, 13])
 def test_plan(n, q_hi, hi, bs, pad):
     rng = np.random.default_rng(n + bs)

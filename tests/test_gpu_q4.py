@@ -68,7 +68,7 @@ def _check_rows(out, q, K, V, scale, G, dtype, chunk):
         R = np.abs(V[:, h // G]).max()
         tol = e * np.abs(want[:, h]) + 2 * 2.0 ** -12 * R
         if chunk:
-            A = max(1.0, scale * (np.abs(q[:, h]) @ np.abs(K[:, h // G]).T).max())
+            A = max(1.0, abs(scale) * (np.abs(q[:, h]) @ np.abs(K[:, h // G]).T).max())
             tol = tol + 2 * 2.0 ** -11 * A * R
         err = np.abs(out[:, h] - want[:, h])
         assert np.all(err <= tol), (h, float((err / tol).max()), float(err.max()))
@@ -491,7 +491,192 @@ def test_serving_run():
         assert int(count) == n_blocks - held
 
 
+# ------------------------------------------------------------------ what the documentation allows besides
+@pytest.mark.parametrize("bs", [48, 80, 2048])
+@pytest.mark.parametrize("ql", [1, 3, 150])
+def test_block_sizes(bs, ql):
+    """Units of 64 tokens and tiles of 128 that begin and end inside blocks."""
+    lay, seqs = _lay(2, 64, 32), [ql, 47 + ql, 1000 + ql]
+    cache, table, K, V = _filled(lay, seqs, bs, seed=bs)
+    q = torch.randn(3 * ql, 4, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    starts = _prefill(lay, cache, table, seqs, [ql] * 3, q, 0.125, out)
+    for r, a in enumerate(starts):
+        _check_rows(_np(out[a:a + ql]), _np(q[a:a + ql]), K[r], V[r], 0.125, 2, torch.float16, True)
+
+
+@pytest.mark.parametrize("ql", [1, 100])
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_scales_of_any_sign(ql, scale):
+    lay, n = _lay(1, 128, 64), 400
+    cache, table, K, V = _filled(lay, [n], 16, seed=1)
+    q = torch.randn(ql, 3, 128, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    _prefill(lay, cache, table, [n], [ql], q, scale, out)
+    _check_rows(_np(out), _np(q), K[0], V[0], scale, 3, torch.float16, True)
+
+
+@pytest.mark.parametrize("ql", [2, 140])
+def test_a_query_of_no_number_spoils_its_own_row_alone(ql):
+    lay, n = _lay(1, 64, 32), 500
+    cache, table, K, V = _filled(lay, [n], 16, seed=1)
+    q = torch.randn(ql, 4, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+    q[1, 2, 5], q[ql - 1, 0, 9] = float("nan"), float("inf")
+    out = torch.empty_like(q)
+    _prefill(lay, cache, table, [n], [ql], q, 0.125, out)
+    bad = torch.zeros(ql, 4, dtype=torch.bool)
+    bad[1, 2] = bad[ql - 1, 0] = True
+    assert bool(out[bad.cuda()].isnan().all())
+    want = q.clone()
+    want[bad.cuda()] = 0.0
+    out[bad.cuda()] = torch.from_numpy(O.attend(_np(want), K[0], V[0], 0.125, 4))[bad].half().cuda()
+    _check_rows(_np(out), _np(want), K[0], V[0], 0.125, 4, torch.float16, True)
+
+
+def test_prefill_strides_and_offsets():
+    """Chunks whose queries are slices of a fused projection or lie off 16 bytes, outputs with gaps."""
+    lay, seqs, qls = _lay(2, 64, 64), [200, 77], [130, 60]
+    cache, table, K, V = _filled(lay, seqs, 16, seed=8)
+    T = sum(qls)
+    qkv = torch.randn(T, 10, 64, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    big = torch.full((T * 10 * 64 + 1,), 9.0, device="cuda", dtype=torch.bfloat16)
+    wide = big[1:].view(T, 10, 64)
+    _prefill(lay, cache, table, seqs, qls, qkv[:, :6], 0.1, wide[:, 2:8])
+    shifted = torch.empty(T * 6 * 64 + 1, device="cuda", dtype=torch.bfloat16)
+    shifted[1:] = qkv[:, :6].reshape(-1)
+    out = torch.empty(T, 6, 64, device="cuda", dtype=torch.bfloat16)
+    _prefill(lay, cache, table, seqs, qls, shifted[1:].view(T, 6, 64), 0.1, out)
+    assert torch.equal(out, wide[:, 2:8])
+    assert bool((wide[:, :2] == 9).all()) and bool((wide[:, 8:] == 9).all())
+    for r, (a, n) in enumerate(((0, 130), (130, 60))):
+        _check_rows(_np(out[a:a + n]), _np(qkv[a:a + n, :6]), K[r], V[r], 0.1, 3, torch.bfloat16, True)
+
+
+def test_offsets_behind_32_bits():
+    """A cache beyond 2^32 bytes, and rows of k, v, q and out more than 2^31 elements apart."""
+    from vllm_ttkv import ops
+    lay, bs = _lay(2, 128, 128), 16
+    n_blocks = 2 ** 32 // (2 * lay.panel_bytes) + 50
+    cache = torch.empty(lay.cache_shape(n_blocks, bs), dtype=torch.uint8, device="cuda")
+    stride = 2 ** 30 + 64
+    flat = torch.empty(3 * stride, dtype=torch.float16, device="cuda")
+
+    def apart(n, heads, at):
+        return torch.as_strided(flat, (n, heads, 128), (stride, 128, 1), at)
+
+    gen = torch.Generator().manual_seed(0)
+    blocks = [n_blocks - 1, 3, n_blocks - 30, n_blocks - 7, n_blocks // 2, 0, n_blocks - 2]
+    n = 16 * len(blocks) - 5
+    table = torch.tensor([blocks], dtype=torch.int32, device="cuda")
+    t = torch.arange(n, device="cuda")
+    slots = table[0].long()[t // bs] * bs + t % bs
+    k, v = (torch.randn(n, 2, 128, generator=gen).half().cuda() for _ in range(2))
+    ops.reset_status()
+    ops.q4_write_paged(lay, cache, slots[:-3], k[:-3], v[:-3])
+    kf, vf = apart(3, 2, 0), apart(3, 2, 4096)
+    kf.copy_(k[-3:])
+    vf.copy_(v[-3:])
+    ops.q4_write_paged(lay, cache, slots[-3:], kf, vf)
+    ko, vo = apart(3, 2, 8192), apart(3, 2, 12288)
+    ops.q4_read_paged(lay, cache, slots[-3:], ko, vo)
+    K, V = (O.values(*O.quantise(_np(x), 128)) for x in (k, v))
+    assert torch.equal(ko.cpu(), torch.from_numpy(K[-3:]).half()) and torch.equal(vo.cpu(), torch.from_numpy(V[-3:]).half())
+    for heads, ql in ((4, 1), (4, 3), (32, 3)):          # streamed, and a chunk
+        q, out = apart(ql, heads, 16384), apart(ql, heads, 32768)
+        q.copy_(torch.randn(ql, heads, 128, generator=gen).half())
+        if ql == 1:
+            ops.q4_decode_paged(lay, cache, table, torch.tensor([n], dtype=torch.int32, device="cuda"), q, 0.08, out)
+        else:
+            _prefill(lay, cache, table, [n], [ql], q, 0.08, out)
+        ops.check_status()
+        _check_rows(_np(out), _np(q), K, V, 0.08, heads // 2, torch.float16, True)
+
+
+def test_many_heads_a_group_and_many_requests_of_a_chunk():
+    from vllm_ttkv import ops
+    lay = _lay(1, 64, 64)
+    cache, table, K, V = _filled(lay, [300, 70], 16, seed=6)
+    q = torch.randn(2, 71, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    ops.q4_decode_paged(lay, cache, table, torch.tensor([300, 70], dtype=torch.int32, device="cuda"), q, 0.1, out)
+    for r in range(2):
+        _check_rows(_np(out[r:r + 1]), _np(q[r:r + 1]), K[r], V[r], 0.1, 71, torch.float16, False)
+    rng = np.random.default_rng(1)
+    qls = [int(x) for x in rng.integers(0, 4, 400)]
+    qls[200] = 90
+    seqs = [n + int(x) if n else 0 for n, x in zip(qls, rng.integers(0, 60, 400))]
+    cache, table, K, V = _filled(lay, seqs, 16, seed=7)
+    q = torch.randn(sum(qls), 2, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    starts = _prefill(lay, cache, table, seqs, qls, q, 0.1, out)
+    ops.check_status()
+    for r, (a, n) in enumerate(zip(starts, qls)):
+        if n:
+            _check_rows(_np(out[a:a + n]), _np(q[a:a + n]), K[r], V[r], 0.1, 2, torch.float16, True)
+
+
+def test_prefill_in_two_graphs_at_once():
+    """Two captured chunk calls and an eager one, replayed at once on three streams: no shared scratch, and
+    each answer the same bits every time."""
+    from vllm_ttkv import ops
+    lay, seqs, qls = _lay(1, 128, 128), [2500, 700], [100, 64]
+    cache, table, K, V = _filled(lay, seqs, 16, seed=2)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    seq, qs, ql = i32(seqs), i32([0, 100]), i32(qls)
+    qq = [torch.randn(164, 4, 128, generator=torch.Generator().manual_seed(i)).half().cuda() for i in range(3)]
+    outs = [torch.empty_like(x) for x in qq]
+    want = [torch.empty_like(x) for x in qq]
+    ops.status_word()
+
+    def call(i, out):
+        ops.q4_prefill_paged(lay, cache, table, seq, qs, ql, qq[i], 0.1, out[i], 100, 2500)
+
+    for i in range(3):
+        call(i, want)
+        for r, (a, n) in enumerate(((0, 100), (100, 64))):
+            _check_rows(_np(want[i][a:a + n]), _np(qq[i][a:a + n]), K[r], V[r], 0.1, 4, torch.float16, True)
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(i, outs)
+        graphs.append(g)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(10):
+        for i in range(3):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay() if i < 2 else call(2, outs)
+    torch.cuda.synchronize()
+    ops.check_status()
+    for i in range(3):
+        assert torch.equal(outs[i], want[i])
+
+
 # ------------------------------------------------------------------ refusals before a launch
+def test_the_binding_refuses_other_types():
+    from vllm_ttkv import ops
+    lay = _lay(1, 64, 64)
+    cache = lay.new_cache(2, 16)
+    kv, sl = torch.zeros(3, 1, 64, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    i32 = torch.zeros(3, dtype=torch.int32, device="cuda")
+    bt, q = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), kv.half()
+    for call in (lambda: ops.q4_write_paged(lay, None, sl, kv, kv), lambda: ops.q4_write_paged(lay, cache, [0, 1, 2], kv, kv),
+                 lambda: ops.q4_write_paged(lay, cache, sl, kv.cpu().numpy(), kv), lambda: ops.q4_write_paged(lay, cache, sl, kv, 3),
+                 lambda: ops.q4_write_paged(lay, cache, sl, kv, kv, status=7),
+                 lambda: ops.q4_decode_paged(lay, cache, bt, i32, q, "a", q), lambda: ops.q4_decode_paged(lay, cache, bt, i32, q, None, q),
+                 lambda: ops.q4_prefill_paged(lay, cache, bt, i32, i32, i32, q, 1.0, q, 1.5, 1),
+                 lambda: ops.q4_prefill_paged(lay, cache, bt, i32, i32, i32, q, 1.0, q, 1, None),
+                 lambda: ops.plan_step(bt, i32, i32, i32, i32[:1], "16", sl), lambda: ops.release_blocks(bt, i32, None, i32[:1], 16)):
+        with pytest.raises((TypeError, ValueError, AttributeError)):
+            call()
+    for call in (lambda: ops.q4_prefill_paged(lay, cache, bt, i32, i32, i32, q, 1.0, q, 2 ** 40, 1),
+                 lambda: ops.q4_prefill_paged(lay, cache, bt, i32, i32, i32, q, 1.0, q, 2 ** 70, 1)):
+        with pytest.raises(ValueError):
+            call()
+    torch.cuda.synchronize()
+
+
 def test_ops_refuse_what_does_not_fit():
     from vllm_ttkv import ops
     lay = _lay(2, 64, 32)

@@ -14,7 +14,7 @@
 // word (the next nibble's come out as c 2^-20: q is stored with the factor, o divided by it); eight
 // values cost five instructions. p_t s_t is rounded to fp16, an operand of the matrix product, after
 // scaling by a power of two that keeps the largest near 2^14. It multiplies c - 7.5 (the second sum
-// takes the rounded weight's share of 7.5: sum p' of a unit comes from one more product, with ones), so
+// takes the rounded weight's share of 7.5: sum p' of a unit comes from one more product, with 15s), so
 // the rounding error is that of weights on centred values: 2^-12 of each term at most.
 #include <algorithm>
 
@@ -707,7 +707,10 @@ __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParam
     const Req rq = request(P, r, false);
     const int per_head = P.max_q * P.G;
     const int h = blockIdx.x / per_head, row = blockIdx.x - h * per_head;
-    if (rq.ql <= 0 || row >= rq.ql * P.G) return;
+    if (rq.ql <= 0 || row >= rq.ql * P.G) {
+        pdl_wait();                                              // this grid ends after the streaming kernel
+        return;
+    }
     const int lanes = D / 4, grp = tid / lanes, ngrp = kMergeThreads / lanes, ln = 4 * (tid - grp * lanes);
     const int U = units_of(rq);
     const int nrb = row_blocks(rq, P.G, rows_block), rb = row / rows_block, i = row - rb * rows_block;
