@@ -141,6 +141,23 @@ def test_store_strides(case):
     ops.check_status()
 
 
+@pytest.mark.parametrize("kt,vt", [("bf16", "fp32"), ("fp32", "fp16"), ("fp16", "bf16")])
+def test_store_of_two_types(kt, vt):
+    from vllm_ttkv import ops
+    lay, bs = _lay(2, 128, 32), 16
+    gen = torch.Generator().manual_seed(5)
+    k, v = torch.randn(40, 2, 128, generator=gen).to(DT[kt]).cuda(), torch.randn(40, 2, 128, generator=gen).to(DT[vt]).cuda()
+    slots = torch.arange(5, 45, device="cuda")
+    a, b = lay.new_cache(3, bs), lay.new_cache(3, bs)
+    ops.q4_write_paged(lay, a, slots, k, v)
+    ops.q4_write_paged(lay, b, slots, k.float(), v.float())
+    assert torch.equal(a, b)
+    ko, vo, kf, vf = torch.empty_like(k), torch.empty_like(v), torch.empty_like(k).float(), torch.empty_like(v).float()
+    ops.q4_read_paged(lay, a, slots, ko, vo)
+    ops.q4_read_paged(lay, a, slots, kf, vf)
+    assert torch.equal(ko, kf.to(DT[kt])) and torch.equal(vo, vf.to(DT[vt]))
+
+
 def test_store_skips_and_refuses_slots():
     from vllm_ttkv import ops
     lay, bs = _lay(1, 128, 64), 16

@@ -1,10 +1,14 @@
 // The 4-bit paged cache: quantise and scatter (ttkv_q4_write), gather and dequantise (ttkv_q4_read).
 //
-// Bound: memory. A token of one head moves 4 d bytes of 16-bit K and V and d + 8 d / group packed
-// bytes, each once. d / 8 consecutive lanes of a warp own a (token, head) row, eight values a lane
-// (one 16-byte load of each 16-bit row): the group's minimum and maximum are shuffles within the
-// group's lanes, and a lane's eight K codes are one 32-bit word of the panel, its V codes two 16-bit
-// ones (the V order pairs tokens, so a lone token's bytes lie apart).
+// A token of one head moves 4 d bytes of 16-bit K and V and d + 8 d / group packed bytes, each once.
+// Consecutive lanes of a warp own a row of a token and head (16 values a lane in the write, 8 of K and 8
+// of V in the read-back), so a group's minimum and maximum are shuffles within its lanes, and a lane's
+// codes are whole words of the panel (16-bit halves in V's order, which pairs tokens).
+//
+// 16384 tokens of 8 heads of 128 bf16 lanes, 86 MB: the write takes 29 us, bound by its instructions (20
+// a value, 80 percent of the issue slots), the read-back 17, against 13 of memory. In steps: 38 us with 8
+// values of K and of V a lane, whose group sums and shuffles are done twice as often, at 5 CTAs an SM;
+// 31 with 16 values of one of them at 6; 29 with a kernel a type and unaligned loads out of the way.
 #include "ttkv_async.cuh"
 #include "ttkv_q4.cuh"
 
@@ -13,7 +17,7 @@ namespace {
 
 using namespace q4;
 
-constexpr int kStoreThreads = 256;
+constexpr int kStoreThreads = 256, kWriteCtas = 6;
 
 struct StoreParams {
     uint8_t* cache;
@@ -28,16 +32,13 @@ struct StoreParams {
     int32_t* status;
 };
 
-// Scale and minimum of a group whose lanes hold x, and the codes of this lane's eight. G lanes per
-// group.
-//
 // The format rounds the scale once from (hi - lo) / 15 and a code once from (x - m) / s. fp32 settles
 // both except next to a border between two results: a scale within 3 units of the middle of the 13
 // bits that fp16 drops, a few in ten thousand, which is redone in fp64 out of the way; and a code's
-// quotient, off by 5e-6 at most, within 1e-5 of one half. Of 16-bit values one in a few thousand lies
-// exactly there, so this is settled in fp32, by the exact remainder x - m - c s: the difference's own
-// rounding error is known, and the remainder of a product of 15 bits is exact.
-// What bounds a long write is the number of instructions a value.
+// quotient near one half. x inv - m inv is off by 5e-6 and 15 2^-23 |m inv| at most (m inv is rounded);
+// within twice that of one half it is settled by the exact remainder x - m - c s: the difference's own
+// rounding error is known, and the remainder of a product of 15 bits is exact. Of 16-bit values one in
+// a few thousand lies exactly there.
 // Values beyond the limit need no clamp of their own: the ends of the group are clamped, and the
 // quotient as a fraction of 15 by its saturation. It is rounded by adding 1.5 2^23, which leaves the
 // integer in the low bits of the sum, where eight of them are packed by shifts and adds (the sum's
@@ -60,22 +61,78 @@ __device__ __forceinline__ uint32_t exact_code(float x, float m, float s, float 
     return uint32_t(fminf(fmaxf(c, 0.f), 15.f));
 }
 
+// Minima and maxima of three, NaN if any is.
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// a b + c of two pairs at once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+        " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+// The codes of eight values of a group with minimum m and scale s, inv = 1 / (15 s), mi = m inv.
+__device__ __forceinline__ uint32_t codes8(const float (&x)[8], float m, float s, float inv, float mi, float border) {
+    constexpr float MAGIC = 12582912.f;
+    const float2 fifteen = make_float2(15.f, 15.f), magic = make_float2(MAGIC, MAGIC), minus = make_float2(-1.f, -1.f);
+    uint32_t codes = 0;
+    float near = 0.f;
+    #pragma unroll
+    for (int j = 6; j >= 0; j -= 2) {
+        const float2 t = make_float2(__saturatef(fmaf(x[j], inv, -mi)), __saturatef(fmaf(x[j + 1], inv, -mi)));
+        const float2 u = fma2(t, fifteen, magic), r = fma2(t, fifteen, fma2(u, minus, magic));
+        asm("max.abs.f32 %0, %0, %1, %2;" : "+f"(near) : "f"(r.x), "f"(r.y));
+        codes = (codes * 16u + __float_as_uint(u.y)) * 16u + __float_as_uint(u.x);
+    }
+    // the high bits 0x4b400000 of the last three values packed; those of the others were shifted out
+    codes -= 0x4b400000u + (0x4b400000u << 4) + (0x4b400000u << 8);
+    if (near > border) {
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float t = __saturatef((x[j] - m) * inv), c = fmaf(t, 15.f, MAGIC) - MAGIC;
+            if (fabsf(fmaf(t, 15.f, -c)) > border)
+                codes = (codes & ~(15u << (4 * j))) | exact_code(x[j], m, s, c) << (4 * j);
+        }
+    }
+    return codes;
+}
+
+// Scale and minimum of a group whose G lanes hold x and y, and the codes of this lane's sixteen.
 template <int G>
-__device__ __forceinline__ uint32_t quantise_group(const float (&x)[8], uint32_t& meta) {
-    float lo = x[0], hi = x[0], bad = x[0] * 0.f;             // 0, or NaN where x is not finite
+__device__ __forceinline__ uint2 quantise_group(const float (&x)[8], const float (&y)[8], uint32_t& meta) {
+    float lo = min_nan(x[0], y[0]), hi = max_nan(x[0], y[0]);
     #pragma unroll
     for (int j = 1; j < 8; ++j) {
-        bad = fmaf(x[j], 0.f, bad);
-        lo = fminf(lo, x[j]);
-        hi = fmaxf(hi, x[j]);
+        lo = min3(lo, x[j], y[j]);
+        hi = max3(hi, x[j], y[j]);
     }
     #pragma unroll
     for (int o = 1; o < G; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    constexpr uint32_t MASK = (1u << G) - 1u;                 // (G is 16 at most)
-    const bool nan = __ballot_sync(0xffffffffu, bad != bad) & (MASK << (threadIdx.x & 31 & ~(G - 1)));
+    const bool nan = !(fmaxf(-lo, hi) < INFINITY && lo == lo);  // a NaN or an infinity in the group
     lo = fminf(fmaxf(lo, -kLimit), kLimit);
     hi = fminf(fmaxf(hi, -kLimit), kLimit);
 
@@ -88,26 +145,10 @@ __device__ __forceinline__ uint32_t quantise_group(const float (&x)[8], uint32_t
     const float s = __half2float(__ushort_as_half(uint16_t(sb)));
     float inv = 0.f;
     if (s > 0.f) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(15.f * s));
-    constexpr float MAGIC = 12582912.f;
-    uint32_t codes = 0;
-    float near = 0.f;
-    #pragma unroll
-    for (int j = 7; j >= 0; --j) {
-        const float t = __saturatef((x[j] - m) * inv), u = fmaf(t, 15.f, MAGIC);
-        near = fmaxf(near, fabsf(fmaf(t, 15.f, MAGIC - u)));
-        codes = codes * 16u + __float_as_uint(u);
-    }
-    // the high bits 0x4b400000 of the last three values packed; those of the others were shifted out
-    codes -= 0x4b400000u + (0x4b400000u << 4) + (0x4b400000u << 8);
-    if (near > 0.49999f) {
-        codes = 0;
-        #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            codes |= exact_code(x[j], m, s, fmaf(__saturatef((x[j] - m) * inv), 15.f, MAGIC) - MAGIC) << (4 * j);
-    }
-    if (nan) codes = 0;
+    const float mi = m * inv, border = fmaf(fabsf(mi), -1.8e-6f, 0.49999f);
+    const uint2 c = make_uint2(codes8(x, m, s, inv, mi, border), codes8(y, m, s, inv, mi, border));
     meta = nan ? 0x7e00u : sb | (uint32_t(__half_as_ushort(mh)) << 16);
-    return codes;
+    return nan ? make_uint2(0u, 0u) : c;
 }
 
 __device__ __forceinline__ bool slot_ok(const StoreParams& P, int64_t slot, bool first) {
@@ -124,36 +165,44 @@ __device__ __forceinline__ uint8_t* panel_of(const StoreParams& P, int64_t slot,
     return P.cache + ((blk * P.H + h) * (P.block_size / kPanelTokens) + off / kPanelTokens) * panel;
 }
 
-// A CTA's rows are consecutive tokens of head blockIdx.y, D / 8 threads each: two tokens of a pair lie in
-// one warp, whose stores then fill whole sectors. (Two rows a thread, with twice the loads in flight,
-// took 62 us against 48 for 16384 tokens: the registers cost more warps than that gives.)
-template <int D, int GRP>
-__global__ void __launch_bounds__(kStoreThreads) q4_write_kernel(const StoreParams P) {
-    constexpr int TPR = D / 8, G = GRP / 8, NG = D / GRP;
+// A CTA's rows are consecutive tokens of K (blockIdx.z + first = 0) or V (1) of head blockIdx.y, of type
+// DT, D / 16 threads each: two tokens of a pair lie in one warp, whose stores then fill whole sectors.
+template <int D, int GRP, int DT>
+__global__ void __launch_bounds__(kStoreThreads, kWriteCtas) q4_write_kernel(const StoreParams P, int first) {
+    constexpr int TPR = D / 16, G = GRP / 16, NG = D / GRP;
     const int i = threadIdx.x % TPR, h = blockIdx.y;
+    const bool is_v = blockIdx.z + first;
     const int64_t row = int64_t(blockIdx.x) * (kStoreThreads / TPR) + threadIdx.x / TPR;
     const int64_t tok = min(row, int64_t(P.n - 1));  // (rows behind the last token load it again and store nothing)
     pdl_wait();
     pdl_trigger();
-    float x[8], y[8];
     const int64_t slot = P.slots[tok];
-    load8(P.k, P.k_dtype, tok * P.k_stride + h * D + 8 * i, P.k_vec, x);
-    load8(P.v, P.v_dtype, tok * P.v_stride + h * D + 8 * i, P.v_vec, y);
-    uint32_t km, vm;
-    const uint32_t kc = quantise_group<G>(x, km), vc = quantise_group<G>(y, vm);
-    if (row >= P.n || !slot_ok(P, slot, i == 0 && h == 0)) return;
+    const void* src = is_v ? P.v : P.k;
+    const bool vec = is_v ? P.v_vec : P.k_vec;
+    const int64_t at = tok * (is_v ? P.v_stride : P.k_stride) + h * D + 16 * i;
+    float x[8], y[8];
+    load8(src, DT, at, vec, x);
+    load8(src, DT, at + 8, vec, y);
+    uint32_t meta;
+    const uint2 c = quantise_group<G>(x, y, meta);
+    if (row >= P.n || !slot_ok(P, slot, i == 0 && h == 0 && blockIdx.z == 0)) return;
     int o;
     uint8_t* pan = panel_of(P, slot, h, panel_bytes(D, GRP), o);
-    // lanes 8 i .. + 8 = 32 w + 8 a: word w of chunk a; = 32 j + 4 b with b = 2 (i % 4) + (0, 1)
-    const int w = i / 4, a = i % 4;
-    *reinterpret_cast<uint32_t*>(pan + o * (D / 2) + a * (D / 8) + 4 * w) = kc;
-    uint8_t* pv = pan + 8 * D + (o / 2) * D + (2 * a) * (D / 8) + 4 * w + 2 * (o & 1);
-    *reinterpret_cast<uint16_t*>(pv) = uint16_t(vc & 0xffffu);
-    *reinterpret_cast<uint16_t*>(pv + D / 8) = uint16_t(vc >> 16);
-    if (i % G == 0) {
-        *reinterpret_cast<uint32_t*>(pan + k_meta_offset(D) + (o * NG + i / G) * 4) = km;
-        *reinterpret_cast<uint32_t*>(pan + v_meta_offset(D, GRP) + (o * NG + i / G) * 4) = vm;
+    // lanes 16 i .. + 16 = 32 w + 8 a, a = 2 (i % 2) + (0, 1): word w of chunks a; = 32 j + 4 b, b = 4 (i % 2) + (0..3)
+    const int w = i / 2, a = i % 2 * 2;
+    if (is_v) {
+        uint8_t* pv = pan + 8 * D + (o / 2) * D + (2 * a) * (D / 8) + 4 * w + 2 * (o & 1);
+        *reinterpret_cast<uint16_t*>(pv) = uint16_t(c.x & 0xffffu);
+        *reinterpret_cast<uint16_t*>(pv + D / 8) = uint16_t(c.x >> 16);
+        *reinterpret_cast<uint16_t*>(pv + 2 * (D / 8)) = uint16_t(c.y & 0xffffu);
+        *reinterpret_cast<uint16_t*>(pv + 3 * (D / 8)) = uint16_t(c.y >> 16);
+    } else {
+        uint8_t* pk = pan + o * (D / 2) + a * (D / 8) + 4 * w;
+        *reinterpret_cast<uint32_t*>(pk) = c.x;
+        *reinterpret_cast<uint32_t*>(pk + D / 8) = c.y;
     }
+    if (i % G == 0)
+        *reinterpret_cast<uint32_t*>(pan + (is_v ? v_meta_offset(D, GRP) : k_meta_offset(D)) + (o * NG + i / G) * 4) = meta;
 }
 
 __device__ __forceinline__ void values8(uint32_t codes, uint32_t meta, float (&x)[8]) {
@@ -203,39 +252,57 @@ int check_store(const ttkv_q4_store_args_t* a) {
     return TTKV_OK;
 }
 
-template <bool WRITE>
-int launch_store(const ttkv_q4_store_args_t* a) {
-    if (int e = check_store(a)) return e;
-    if (a->n == 0) return TTKV_OK;
-    const ttkv_q4_cache_t* c = &a->cache;
-    const int32_t n = a->n;
-    int shift = -1;
-    for (int b = 0; b < 31; ++b)
-        if (c->block_size == (1 << b)) shift = b;
-    StoreParams P{c->base, c->n_blocks * c->block_size, c->H, c->block_size, shift, a->slots, n, c->flags & TTKV_CACHE_SKIP_PAD,
-                  a->k, a->v, a->k_dtype, a->v_dtype, rows_aligned(a->k, a->k_dtype, a->k_stride),
-                  rows_aligned(a->v, a->v_dtype, a->v_stride), a->k_stride, a->v_stride, a->status};
-    const int per = kStoreThreads / (c->d / 8), ctas = (n + per - 1) / per;
-    // may start while the kernel before it runs, and waits for it before its first access
+// A launch of `per_row` threads a token and head, that may start while the kernel before it runs and waits for it
+// before its first access.
+template <typename... KP, typename... A>
+cudaError_t launch_rows(void (*kernel)(KP...), const ttkv_q4_store_args_t* a, int per_row, int parts, const A&... args) {
+    const int per = kStoreThreads / per_row;
     cudaLaunchAttribute pdl[1];
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(ctas), unsigned(c->H));
+    cfg.gridDim = dim3(unsigned((a->n + per - 1) / per), unsigned(a->cache.H), unsigned(parts));
     cfg.blockDim = dim3(kStoreThreads);
     cfg.stream = static_cast<cudaStream_t>(a->stream);
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// K and V in one launch where their types agree.
+template <int D, int GRP>
+cudaError_t launch_write(const ttkv_q4_store_args_t* a, const StoreParams& P) {
+    const int parts = P.k_dtype == P.v_dtype ? 2 : 1;
+    for (int first = 0; first < 2; first += parts) {
+        const int dt = first ? P.v_dtype : P.k_dtype;
+        const cudaError_t e = launch_rows(dt == TTKV_BF16  ? q4_write_kernel<D, GRP, TTKV_BF16>
+                                          : dt == TTKV_F16 ? q4_write_kernel<D, GRP, TTKV_F16>
+                                                           : q4_write_kernel<D, GRP, TTKV_F32>,
+                                          a, D / 16, parts, P, first);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+int store(const ttkv_q4_store_args_t* a, bool write) {
+    if (int e = check_store(a)) return e;
+    if (a->n == 0) return TTKV_OK;
+    const ttkv_q4_cache_t* c = &a->cache;
+    int shift = -1;
+    for (int b = 0; b < 31; ++b)
+        if (c->block_size == (1 << b)) shift = b;
+    StoreParams P{c->base, c->n_blocks * c->block_size, c->H, c->block_size, shift, a->slots, a->n, c->flags & TTKV_CACHE_SKIP_PAD,
+                  a->k, a->v, a->k_dtype, a->v_dtype, rows_aligned(a->k, a->k_dtype, a->k_stride),
+                  rows_aligned(a->v, a->v_dtype, a->v_stride), a->k_stride, a->v_stride, a->status};
     cudaError_t e = cudaErrorInvalidValue;
 #define TTKV_Q4_STORE(D, GRP)                                                                      \
     if (c->d == D && c->group == GRP)                                                              \
-        e = cudaLaunchKernelEx(&cfg, WRITE ? q4_write_kernel<D, GRP>               \
-                                           : q4_read_kernel<D, GRP>, P);
+        e = write ? launch_write<D, GRP>(a, P) : launch_rows(q4_read_kernel<D, GRP>, a, D / 8, 1, P);
     TTKV_Q4_STORE(64, 32) TTKV_Q4_STORE(64, 64) TTKV_Q4_STORE(128, 32) TTKV_Q4_STORE(128, 64) TTKV_Q4_STORE(128, 128)
 #undef TTKV_Q4_STORE
     if (e != cudaSuccess) {
         cudaGetLastError();
-        return fail(TTKV_ERR_CUDA, "%s: %s", WRITE ? "q4_write_kernel" : "q4_read_kernel", cudaGetErrorString(e));
+        return fail(TTKV_ERR_CUDA, "%s: %s", write ? "q4_write_kernel" : "q4_read_kernel", cudaGetErrorString(e));
     }
     return TTKV_OK;
 }
@@ -249,6 +316,6 @@ extern "C" size_t ttkv_q4_panel_bytes(int32_t d, int32_t group) {
     return q4::geometry_ok(d, group) ? size_t(q4::panel_bytes(d, group)) : 0;
 }
 
-extern "C" int ttkv_q4_write(const ttkv_q4_store_args_t* args) { return launch_store<true>(args); }
+extern "C" int ttkv_q4_write(const ttkv_q4_store_args_t* args) { return store(args, true); }
 
-extern "C" int ttkv_q4_read(const ttkv_q4_store_args_t* args) { return launch_store<false>(args); }
+extern "C" int ttkv_q4_read(const ttkv_q4_store_args_t* args) { return store(args, false); }
