@@ -134,6 +134,12 @@ __device__ __forceinline__ __half2 codes2(uint32_t w) {
     return __hsub2(u2h((w & 0x000f000fu) | 0x64006400u), u2h(0x64006400u));
 }
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one;
+}
+
 // The panels of a stored tile, one each in lanes 0 to 7: index in the cache, or that there is none or
 // that its block id is outside the cache.
 constexpr int kNoPanel = -1, kBadPanel = -2;
@@ -619,26 +625,33 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsProducts));
-        if (w < 18 && lane == 0) {
+        if (__shfl_sync(0xffffffffu, w, 0) < 18) {
         // ============================================================== the products of row tile x
-        const int x = w - 16;
+        // the whole warp keeps step, one lane issues: what the instructions need is then uniform
+        const int x = __shfl_sync(0xffffffffu, w, 0) - 16;
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const bool one = elect_one();
         constexpr uint32_t ID_S = idesc_f16(TM, TH, false, false), ID_PV = idesc_f16(TM, D, false, false);
-        const uint64_t dq = sw128_desc(smem_u32(smem + S::off_q + x * S::Q), 16, 1024);
-        const uint64_t dk0 = sw128_desc(smem_u32(smem + S::off_k), 16, 1024), dv0 = sw128_desc(smem_u32(smem + S::off_v), 16, 1024);
+        const uint64_t DESC = sw128_desc(0, 16, 1024);
+        const uint32_t aq = smem_u32(smem + S::off_q + x * S::Q) >> 4, ak = smem_u32(smem + S::off_k) >> 4, av = smem_u32(smem + S::off_v) >> 4;
         uint32_t n_tile = 0, n_s = 0, n_pv = 0, n_q = 0;      // stored tiles; halves scored; halves summed
         // S of half `half` of the k-th tile of the CTA, into the buffer of its turn
         auto score = [&](uint32_t k, int half) {
             const int st = k & 1;
             if (half == 0) wait(&B.kfull[st], k >> 1);
             tc_after();
-            const uint64_t dk = dk0 + uint64_t((st * S::K + half * TH * 128) >> 4);
-            #pragma unroll
-            for (int e = 0; e < D / 16; ++e) {
-                const uint64_t step = uint64_t(((e >> 2) * S::KATOM + (e & 3) * 32) >> 4);
-                mma_f16(tmem + s_col(x, n_s & 1), dq + step, dk + step, ID_S, e > 0 ? 1u : 0u);
+            const uint32_t ah = ak + ((st * S::K + half * TH * 128) >> 4);
+            if (one) {
+                #pragma unroll
+                for (int e = 0; e < D / 16; ++e) {
+                    constexpr int A = S::KATOM;
+                    const uint32_t step = ((e >> 2) * A + (e & 3) * 32) >> 4;
+                    mma_f16(tm + s_col(x, n_s & 1), DESC + (aq + step), DESC + (ah + step), ID_S, e > 0 ? 1u : 0u);
+                }
+                mma_commit(&B.sfull[x][n_s & 1]);
+                if (half) mma_commit(&B.kempty[st]);
             }
-            mma_commit(&B.sfull[x][n_s & 1]);
-            if (half) mma_commit(&B.kempty[st]);
+            __syncwarp();
             ++n_s;
         };
         while (sg.u < sg.ue) {
@@ -647,9 +660,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 for (int i = 0; i < n; ++i, ++n_tile) {
                     const int st = n_tile & 1;
                     wait(&B.kfull[st], n_tile >> 1);
-                    mbar_arrive(&B.kempty[st]);
+                    if (one) mbar_arrive(&B.kempty[st]);
                     wait(&B.vfull[st], n_tile >> 1);
-                    mbar_arrive(&B.vempty[st]);
+                    if (one) mbar_arrive(&B.vempty[st]);
                 }
                 sg.skip(P, n);
                 continue;
@@ -667,13 +680,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 if (half == 0) wait(&B.vfull[st], k >> 1);
                 wait(&B.pfull[x][n_pv & 1], n_pv >> 1);
                 tc_after();
-                const uint64_t dv = dv0 + uint64_t((st * S::V + half * S::VATOM) >> 4);
-                #pragma unroll
-                for (int e = 0; e < TH / 16; ++e)
-                    mma_f16_ts(tmem + o_col(x), tmem + s_col(x, n_pv & 1) + 8 * e, dv + uint64_t((e * 32) >> 4), ID_PV,
-                               (i > 0 || e > 0) ? 1u : 0u);
-                mma_commit(&B.pvdone[x][n_pv & 1]);
-                if (half) mma_commit(&B.vempty[st]);
+                const uint32_t ah = av + ((st * S::V + half * S::VATOM) >> 4);
+                if (one) {
+                    #pragma unroll
+                    for (int e = 0; e < TH / 16; ++e)
+                        mma_f16_ts(tm + o_col(x), tm + s_col(x, n_pv & 1) + 8 * e, DESC + (ah + 2 * e), ID_PV,
+                                   (i > 0 || e > 0) ? 1u : 0u);
+                    mma_commit(&B.pvdone[x][n_pv & 1]);
+                    if (half) mma_commit(&B.vempty[st]);
+                }
+                __syncwarp();
                 ++n_pv;
             }
             n_tile += n;
