@@ -586,29 +586,39 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     }
                     // a NaN scale counts as nothing here: a weight of 0 must not spread it. The rows that see
                     // its token are told by flags
-                    bool nan = false;
+                    uint32_t s2[4], m2[4];                    // of the pairs of tokens
+                    auto pair_up = [&]() {
+                        #pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            s2[k] = __byte_perm(vm[2 * k], vm[2 * k + 1], 0x5410);
+                            m2[k] = __byte_perm(vm[2 * k], vm[2 * k + 1], 0x7632);
+                        }
+                    };
+                    pair_up();
+                    __half2 nan = u2h(0u);                    // 0, or NaN (scales are finite otherwise)
                     #pragma unroll
-                    for (int k = 0; k < 8; ++k) nan |= (vm[k] & 0x7fffu) > 0x7c00u;
-                    if (__any_sync(0xffffffffu, nan)) {
+                    for (int k = 0; k < 4; ++k) nan = __hfma2(u2h(s2[k]), u2h(0u), nan);
+                    if (__any_sync(0xffffffffu, (h2u(nan) & 0x7fff7fffu) != 0u)) {
                         const int f = n_tile & (kFlags - 1);
                         #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            if ((vm[k] & 0x7fffu) <= 0x7c00u) continue;
+                            if ((vm[k] & 0x7fffu) < 0x7c00u) continue;
                             const int tok = 8 * hp + k;
                             vm[k] = 0u;
                             atomicOr(reinterpret_cast<unsigned*>(&vbad[f][tok & ~3]), (1u << (j / WPG)) << (8 * (tok & 3)));
                             any_bad[f] = 1;
                         }
+                        pair_up();
                     }
                     uint32_t out[4][4];                       // [lane of the quad][pair of tokens]
                     #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const uint32_t ma = vm[2 * k], mb = vm[2 * k + 1], v = vw[k];
-                        const __half2 s2 = u2h(__byte_perm(ma, mb, 0x5410)), m2 = u2h(__byte_perm(ma, mb, 0x7632));
-                        out[0][k] = h2u(__hfma2(codes2<false>(v), s2, m2));
-                        out[1][k] = h2u(__hfma2(codes2<true>(v), s2, m2));
-                        out[2][k] = h2u(__hfma2(codes2<false>(v >> 8), s2, m2));
-                        out[3][k] = h2u(__hfma2(codes2<true>(v >> 8), s2, m2));
+                        const uint32_t v = vw[k];
+                        const __half2 sk = u2h(s2[k]), mk = u2h(m2[k]);
+                        out[0][k] = h2u(__hfma2(codes2<false>(v), sk, mk));
+                        out[1][k] = h2u(__hfma2(codes2<true>(v), sk, mk));
+                        out[2][k] = h2u(__hfma2(codes2<false>(v >> 8), sk, mk));
+                        out[3][k] = h2u(__hfma2(codes2<true>(v >> 8), sk, mk));
                     }
                     #pragma unroll
                     for (int q = 0; q < 4; ++q)               // lane 32 j + 4 b + q is row 32 j + 8 q + b, chunk hp
