@@ -380,6 +380,23 @@ def test_prefill_splits(H, HQ, ql, n):
     _check_rows(_np(out), _np(q), K[0], V[0], 0.08, HQ // H, torch.float16, True)
 
 
+@pytest.mark.parametrize("R,H,ql", [(40, 1, 4), (40, 1, 5), (40, 1, 8), (40, 1, 9), (3, 2, 12), (3, 2, 13), (17, 2, 12)])
+def test_prefill_streamed_or_not(R, H, ql):
+    """Row counts, batches and bounds on both sides of the choice between the two kernels."""
+    from vllm_ttkv import ops
+    lay = _lay(H, 64, 64)
+    rng = np.random.default_rng(ql)
+    seqs = [ql + int(x) for x in rng.integers(0, 300, R)]
+    cache, table, K, V = _filled(lay, seqs, 16, seed=R)
+    q = torch.randn(R * ql, 4 * H, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+    for bound in (max(seqs), 1535, 1536, 100000):
+        out = torch.empty_like(q)
+        starts = _prefill(lay, cache, table, seqs, [ql] * R, q, 0.125, out, max_seq=bound)
+        ops.check_status()
+        for r, a in enumerate(starts):
+            _check_rows(_np(out[a:a + ql]), _np(q[a:a + ql]), K[r], V[r], 0.125, 4, torch.float16, True)
+
+
 def test_prefill_a_nan_reaches_the_queries_that_see_it():
     from vllm_ttkv import ops
     lay = _lay(1, 64, 32)

@@ -777,7 +777,8 @@ __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParam
 
 // ------------------------------------------------------------------ host
 
-// Rows a streaming warp takes at once: 8 (query, head) rows a fragment, two fragments above that.
+// Rows a streaming warp takes at once: 8 (query, head) rows a fragment, two fragments above that. (16 rows
+// of 64 requests of 6000 tokens, d = 64 in groups of 32: 177 us with two, 224 with one; 32 rows 321 and 417.)
 int stream_nt(int64_t rows) { return rows > 8 ? 2 : 1; }
 
 // Workspace: two parts a CTA for the merge, a part a warp.
@@ -872,9 +873,22 @@ AttnParams attn_params(const ttkv_q4_attn_args_t* a) {
     return P;
 }
 
-// Chunks of at most this many (query, head) rows a KV head are streamed, the cache read once per 16 of
-// them; above it the chunk kernel's tiles are fuller.
-constexpr int kStreamRows = 32;
+// Whether chunks of `rows` (query, head) rows a KV head are streamed, the cache read and its codes fed to
+// the tensor cores once per 16 rows, or go to the chunk kernel, whose tiles of 256 rows each dequantise
+// the cache once. Streamed against chunked, d = 128 in groups of 128, 8 KV heads, us:
+//   requests x tokens   16 rows      24           32           48           64
+//   64 x 130            60 / 73      81 / 75      95 / 75      134 / 75
+//   16 x 500            34 / 36      42 / 36      46 / 34
+//   64 x 1500           110 / 189    167 / 196    185 / 188    261 / 196
+//   64 x 6000           226 / 503    376 / 525    400 / 499    568 / 517
+//   4 x 3000            30 / 48      38 / 50      40 / 48      46 / 50      58 / 48
+//   1 x 130             20 / 24      20 / 26      22 / 26      22 / 26      22 / 26
+//   1 x 16000           34 / 71      42 / 75      42 / 79      48 / 79      56 / 81
+// So up to 16 rows always, up to 32 over long rows, up to 48 where few (request, head) pairs would leave
+// most of the chunk kernel's tiles waiting.
+bool streams(int64_t rows, int64_t pairs, int max_seq) {
+    return rows <= 16 || (rows <= 32 && max_seq >= 1536) || (rows <= 48 && pairs <= 32);
+}
 
 }  // namespace
 }  // namespace ttkv
@@ -897,7 +911,8 @@ extern "C" int ttkv_q4_decode(const ttkv_q4_attn_args_t* args) {
 extern "C" size_t ttkv_q4_prefill_workspace_bytes(int32_t d, int32_t n_reqs, int32_t group_heads, int32_t max_q_len) {
     if (n_reqs < 0 || max_q_len < 0) return 0;
     const int64_t rows = int64_t(max_q_len) * group_heads;
-    return rows > kStreamRows ? chunk_workspace_bytes(d) : stream_ws(d, stream_nt(rows)).bytes;
+    const bool some = streams(rows, 0, INT32_MAX), all = streams(rows, INT64_MAX, 0);     // are streamed
+    return std::max(some ? stream_ws(d, stream_nt(rows)).bytes : 0, all ? 0 : chunk_workspace_bytes(d));
 }
 
 extern "C" int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args) {
@@ -911,7 +926,7 @@ extern "C" int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args) {
     P.q_start = args->q_start; P.q_len = args->q_len; P.n_rows = args->n_rows; P.max_q = args->max_q_len;
     P.max_seq = std::max(args->max_seq_len, 1);
     const cudaStream_t st = static_cast<cudaStream_t>(args->stream);
-    return int64_t(args->max_q_len) * P.G > kStreamRows
-        ? run_chunk(&args->cache, P, args->workspace, args->workspace_bytes, st)
-        : run_stream(&args->cache, P, args->workspace, args->workspace_bytes, st);
+    return streams(int64_t(args->max_q_len) * P.G, int64_t(args->n_reqs) * P.H, P.max_seq)
+        ? run_stream(&args->cache, P, args->workspace, args->workspace_bytes, st)
+        : run_chunk(&args->cache, P, args->workspace, args->workspace_bytes, st);
 }
