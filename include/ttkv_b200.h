@@ -418,7 +418,8 @@ int ttkv_q4_read(const ttkv_q4_store_args_t* args);
  * seq_len - q_len + j, which sees the stored tokens up to and with its own position. max_q_len and
  * max_seq_len bound the batch's q_len and seq_lens; a request above either is refused
  * (TTKV_STATUS_QUERY, TTKV_STATUS_SEQ_BOUND), as is one with q_len > seq_len or with query rows outside
- * [0, n_rows) (TTKV_STATUS_QUERY). Rows of no request are left as they were.
+ * [0, n_rows) (TTKV_STATUS_QUERY). Rows of no request are left as they were. With max_q_len or n_rows 0
+ * nothing is launched or checked on the device. `scale` is finite.
  *
  * Both: a request longer than its block-table row is refused (TTKV_STATUS_ROW_SHORT); a refused
  * request's rows are left as they were. Queries that see a block id outside the cache get NaN

@@ -454,6 +454,29 @@ def test_prefill_refusals_on_the_device():
         assert bool((out[ql:] == 5).all())
 
 
+def test_prefill_bounds_of_nothing():
+    """No tokens allowed: every request is refused. No queries allowed: nothing is done."""
+    from vllm_ttkv import ops
+    lay = _lay(1, 64, 64)
+    cache, table, K, V = _filled(lay, [1, 1], 16, seed=4)
+    q = torch.randn(2, 2, 64, device="cuda").half()
+    out = torch.full_like(q, 5.0)
+    ops.reset_status()
+    _prefill(lay, cache, table, [1, 1], [1, 1], q, 0.1, out, max_seq=0)
+    with pytest.raises(RuntimeError):
+        ops.check_status()
+    _prefill(lay, cache, table, [1, 1], [1, 1], q, 0.1, out, max_q=0)
+    ops.check_status()
+    assert bool((out == 5).all())
+    _prefill(lay, cache, table, [1, 1], [1, 1], q, 0.1, out, max_seq=1)
+    ops.check_status()
+    for r in range(2):
+        _check_rows(_np(out[r:r + 1]), _np(q[r:r + 1]), K[r], V[r], 0.1, 2, torch.float16, True)
+    for scale in (float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            _prefill(lay, cache, table, [1, 1], [1, 1], q, scale, out)
+
+
 def test_prefill_captured():
     from vllm_ttkv import ops
     lay = _lay(1, 128, 128)

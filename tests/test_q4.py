@@ -126,7 +126,8 @@ def test_attention_refusals():
             (dict(q_stride=-1), _lib.ERR_ARG), (dict(out_stride=-8), _lib.ERR_ARG), (dict(HQ=3), _lib.ERR_ARG),
             (dict(HQ=1), _lib.ERR_ARG), (dict(workspace=0), _lib.ERR_WORKSPACE), (dict(workspace=A + 4), _lib.ERR_ALIGN),
             (dict(q=A + 1), _lib.ERR_ALIGN), (dict(block_table=0), _lib.ERR_ARG), (dict(seq_lens=0), _lib.ERR_ARG),
-            (dict(n_reqs=-1), _lib.ERR_ARG), (dict(bt_cols=-1), _lib.ERR_ARG), (dict(n_reqs=70000), _lib.ERR_UNSUPPORTED))
+            (dict(n_reqs=-1), _lib.ERR_ARG), (dict(bt_cols=-1), _lib.ERR_ARG), (dict(n_reqs=70000), _lib.ERR_UNSUPPORTED),
+            (dict(scale=float("nan")), _lib.ERR_ARG), (dict(scale=-float("inf")), _lib.ERR_ARG))
     for fn, extra in ((L.ttkv_q4_decode, {}), (L.ttkv_q4_prefill, {}), (L.ttkv_q4_prefill, dict(max_q_len=64))):
         for kw, code in both:
             assert _attn(fn, **(extra | kw)) == code, kw

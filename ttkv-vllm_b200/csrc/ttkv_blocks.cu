@@ -148,13 +148,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanParam
         if (held < P.bt_cols) P.block_table[int64_t(r) * P.bt_stride + held] = -1;
     }
     // the blocks taken, into their rows
-    for (int e = at; e < used; e += step) {
+    for (unsigned i = at; i < unsigned(used); i += step) {
+        const int e = int(i);
         const int r = find(M.end, P.n_reqs, e), first = r ? M.end[r - 1] : 0;
         const int held = blocks_of(M.len[r] - (M.start[r + 1] - M.start[r]), P.block_size);
         P.block_table[int64_t(r) * P.bt_stride + held + (e - first)] = P.free_blocks[count - 1 - e];
     }
     // the tokens
-    for (int t = at; t < P.n_tokens; t += step) {
+    for (unsigned i = at; i < unsigned(P.n_tokens); i += step) {
+        const int t = int(i);
         const int r = find(M.start + 1, P.n_reqs, t);
         int64_t slot = -1;
         int pos = 0;
@@ -184,7 +186,8 @@ __global__ void __launch_bounds__(kPlanThreads) release_blocks_kernel(const Plan
     const int used = assign_ranges<true>(P, P.capacity - count, M, wsum, &taken);
     bool bad = false;
     #pragma unroll 4
-    for (int e = at; e < used; e += step) {
+    for (unsigned i = at; i < unsigned(used); i += step) {
+        const int e = int(i);
         const int r = find(M.end, P.n_reqs, e);
         const int32_t id = __ldg(P.block_table + int64_t(r) * P.bt_stride + (e - (r ? M.end[r - 1] : 0)));
         bad |= id < 0;

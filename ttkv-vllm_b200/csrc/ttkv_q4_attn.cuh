@@ -23,7 +23,7 @@ struct AttnParams {
     const int32_t* seq_lens;
     const int32_t* q_start;                 // null: one query per request
     const int32_t* q_len;
-    int32_t n_reqs, n_rows, max_q, max_seq;
+    int32_t n_reqs, n_rows, max_q, max_seq; // the last two bound q_len and seq_lens
     const void* q;
     int32_t dtype, q_vec, out_vec;
     int64_t q_stride;
@@ -52,7 +52,7 @@ __device__ __forceinline__ Req request(const AttnParams& P, int r, bool tell) {
     int code = 0;
     if (P.q_len && a.ql > 0 &&
         (a.ql > a.seq || a.ql > P.max_q || a.q0 < 0 || int64_t(a.q0) + a.ql > P.n_rows)) code = TTKV_STATUS_QUERY;
-    else if (P.max_seq > 0 && a.seq > P.max_seq && a.ql > 0) code = TTKV_STATUS_SEQ_BOUND;
+    else if (a.seq > P.max_seq && a.ql > 0) code = TTKV_STATUS_SEQ_BOUND;
     else if (a.seq > int64_t(P.bt_cols) * P.block_size && a.ql > 0) code = TTKV_STATUS_ROW_SHORT;
     if (code && tell) report(P.status, code);
     if (code || a.ql < 0) a.ql = 0;

@@ -21,6 +21,7 @@
 // takes the rounded weight's share of 7.5: sum p' of a unit comes from one more product, with 15s), so
 // the rounding error is that of weights on centred values: 2^-12 of each term at most.
 #include <algorithm>
+#include <cmath>
 
 #include "ttkv_q4_attn.cuh"
 
@@ -809,6 +810,7 @@ int check_attn(const ttkv_q4_attn_args_t* a) {
     if (a->HQ < a->cache.H || a->HQ % a->cache.H) return fail(TTKV_ERR_ARG, "HQ=%d is not a multiple of H=%d", a->HQ, a->cache.H);
     if (a->dtype != TTKV_F16 && a->dtype != TTKV_BF16)
         return fail(TTKV_ERR_UNSUPPORTED, "4-bit read: queries and outputs are fp16 or bf16");
+    if (!std::isfinite(a->scale)) return fail(TTKV_ERR_ARG, "4-bit read: a scale of %g", double(a->scale));
     if (a->q_stride < 0 || a->out_stride < 0) return fail(TTKV_ERR_ARG, "4-bit read: a negative stride");
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 1)
         return fail(TTKV_ERR_ALIGN, "4-bit read: q or out at an odd address");
@@ -909,6 +911,7 @@ extern "C" int ttkv_q4_decode(const ttkv_q4_attn_args_t* args) {
     AttnParams P = attn_params(args);
     P.n_rows = args->n_reqs;
     P.max_q = 1;
+    P.max_seq = INT32_MAX;
     return run_stream(&args->cache, P, args->workspace, args->workspace_bytes, static_cast<cudaStream_t>(args->stream));
 }
 
@@ -928,7 +931,7 @@ extern "C" int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args) {
         return fail(TTKV_ERR_UNSUPPORTED, "4-bit prefill: %d queries of %d heads", args->max_q_len, args->HQ);
     AttnParams P = attn_params(args);
     P.q_start = args->q_start; P.q_len = args->q_len; P.n_rows = args->n_rows; P.max_q = args->max_q_len;
-    P.max_seq = std::max(args->max_seq_len, 1);
+    P.max_seq = args->max_seq_len;
     const cudaStream_t st = static_cast<cudaStream_t>(args->stream);
     return streams(int64_t(args->max_q_len) * P.G, int64_t(args->n_reqs) * P.H, P.max_seq)
         ? run_stream(&args->cache, P, args->workspace, args->workspace_bytes, st)

@@ -12,6 +12,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <cmath>
+
 #include "ttkv_b200.h"
 
 namespace {
@@ -207,6 +209,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const double scale = PyFloat_AsDouble(a[5]);
         if (scale == -1.0 && PyErr_Occurred()) throw Refused{};
         s.scale = float(scale);
+        if (!std::isfinite(s.scale)) refuse(PyExc_ValueError, "scale is not a finite number");
         s.status = status_word(a[7], dev);
         if (prefill) {
             s.q_start = static_cast<const int32_t*>(vector(a[8], at::kInt, s.n_reqs, "q_start", dev));
