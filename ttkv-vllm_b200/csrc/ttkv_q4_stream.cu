@@ -4,7 +4,7 @@
 //   o = sum_t p_t V_t / sum_t p_t,   p_t = exp(scale q . K_t),   K_t = m_t + s_t c_t (V alike)
 //
 // q4_stream_kernel reads every stored byte once per block of 8 NT (query, head) rows. 64 requests of up to
-// 14402 tokens (8 KV heads of 128 lanes, 3 query heads each, groups of 128; 477 MB) take 125 us, 3.8 TB/s
+// 14402 tokens (8 KV heads of 128 lanes, 3 query heads each, groups of 128; 477 MB) take 110 us, 4.3 TB/s
 // or 58 percent of a measured copy, and 1074 instructions a unit of 64 tokens: two warps a scheduler
 // (their registers allow no more) issue in 47 percent of the cycles, half of them on the half-rate pipe
 // of the masks. 131071 tokens of 2 KV heads take 26 us, 8 requests of 4322 tokens 21, one of 257 9: there
@@ -35,10 +35,11 @@ constexpr int kUnit = 64;                   // tokens of a unit of work: one sof
 __device__ __forceinline__ int units_of(const Req& a) { return a.ql > 0 ? (a.seq + kUnit - 1) / kUnit : 0; }
 
 // ------------------------------------------------------------------ warp-level products
-// D += A (16 x 16, row) . B (16 x 8, column), fp16 operands and fp32 sums.
+// D += A (16 x 16, row) . B (16 x 8, column), fp16 operands and fp32 sums. (Not volatile, nor is the
+// transposition: in their written order they take 20 registers more.)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -46,7 +47,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 
@@ -441,15 +442,18 @@ struct WarpRows {
 // and what is still a part then goes to the workspace for q4_merge_kernel (at most the CTA's first and
 // its last).
 //
-// Every warp streams its own run through its own ring of three units in shared memory, filled by bulk
-// copies (a panel is one contiguous piece of memory), two units ahead of the one that is worked on, so
-// no warp waits for another and an SM keeps about 140 KB in flight, more than its share of bandwidth
-// times latency (44 GB/s x 1 us). 8 warps of an SM: with 10 or 12 their registers spill, and a batch of 64
-// requests of up to 14402 tokens took 142 and 136 us against 133.
+// Every warp streams its own run through its own ring of two or three units in shared memory, filled by
+// bulk copies (a panel is one contiguous piece of memory), ahead of the one that is worked on, so no warp
+// waits for another and an SM keeps about 100 to 140 KB in flight, more than its share of bandwidth times
+// latency (44 GB/s x 1 us). As many warps as their registers allow without spilling: 64 requests of 6000
+// tokens with 3 query heads a KV head take 122 us with 8 warps and 108 with 12 (d = 128, groups of 128),
+// 132 and 122 (groups of 64), 99 and 89 (d = 64, groups of 64), 110 and 99 (groups of 32); groups of 32 at
+// d = 128 spill with 10 (155 and 181), as do two fragments of rows with 12 (194 and 263).
 template <int D, int GRP, int NT>
 struct Stream {
-    static constexpr int PANEL = panel_bytes(D, GRP), UNIT = 4 * PANEL, RING = 12 * PANEL * 8 <= 216 * 1024 ? 3 : 2;
-    static constexpr int WARPS = 8;
+    static constexpr int PANEL = panel_bytes(D, GRP), UNIT = 4 * PANEL;
+    static constexpr int WARPS = NT == 1 && (D == 64 || GRP > 32) ? 12 : 8;
+    static constexpr int RING = 3 * UNIT * WARPS <= 216 * 1024 ? 3 : 2;
     static constexpr int THREADS = 32 * WARPS, ROWS = 8 * NT, SLOTS = 2 * WARPS;
     static constexpr int PART = ROWS * (D + 2);                                 // floats of a part: o, then (m, l)
     static constexpr int RING_BYTES = WARPS * RING * UNIT;
@@ -796,7 +800,7 @@ StreamWs stream_ws(int d, int nt) {
     const size_t rows = size_t(kMaxCtas) * 2 * 8 * nt;
     w.part_ml = rows * d * sizeof(float);
     w.first = w.part_ml + rows * 2 * sizeof(float);
-    w.bytes = w.first + size_t(kMaxCtas) * Stream<128, 128, 1>::WARPS * 8 * nt * (d + 2) * sizeof(float);
+    w.bytes = w.first + size_t(kMaxCtas) * (nt == 1 ? Stream<128, 128, 1>::WARPS : Stream<128, 128, 2>::WARPS) * 8 * nt * (d + 2) * sizeof(float);
     return w;
 }
 
