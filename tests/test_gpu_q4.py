@@ -397,6 +397,25 @@ def test_prefill_streamed_or_not(R, H, ql):
             _check_rows(_np(out[a:a + ql]), _np(q[a:a + ql]), K[r], V[r], 0.125, 4, torch.float16, True)
 
 
+@pytest.mark.parametrize("d,g", GEOMETRIES)
+def test_prefill_many_tiles(d, g):
+    """Some 40 stored tiles a CTA: every place of its ring of panels is filled again and again. The requests
+    share one sequence's blocks."""
+    from vllm_ttkv import ops
+    lay, R, ql, n, G = _lay(1, d, g), 64, 64, 6000, 8
+    cache, table, K, V = _filled(lay, [n], 16, seed=d + g)
+    q = torch.randn(R * ql, G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    starts = _prefill(lay, cache, table.expand(R, -1), [n - 3 * r for r in range(R)], [ql] * R, q, 0.05, out)
+    ops.check_status()
+    for r in (0, 23, 47, 63):
+        a, m = starts[r], n - 3 * r
+        _check_rows(_np(out[a:a + ql]), _np(q[a:a + ql]), K[0][:m], V[0][:m], 0.05, G, torch.float16, True)
+    again = torch.empty_like(q)
+    _prefill(lay, cache, table.expand(R, -1), [n - 3 * r for r in range(R)], [ql] * R, q, 0.05, again)
+    assert torch.equal(out, again)
+
+
 def test_prefill_a_nan_reaches_the_queries_that_see_it():
     from vllm_ttkv import ops
     lay = _lay(1, 64, 32)

@@ -63,7 +63,11 @@ __device__ __forceinline__ uint32_t o_col(int x) { return 256u + 128u * x; }
 template <int D, int GRP>
 struct ChunkSmem {
     static constexpr int Q = TM * D * 2, K = TN * D * 2, V = D * TN * 2;
-    static constexpr int PANEL = panel_bytes(D, GRP), RING = std::min(16, 28160 / PANEL);
+    // Panels of the ring: a multiple of four, so that a place always holds panels of the same warps of K and V.
+    // Each warp then sees every phase of its places; one that skipped some could take the phase before the
+    // last for the one that it waits for, and read a place that is still being filled
+    static constexpr int PANEL = panel_bytes(D, GRP), RING = std::min(16, 30720 / PANEL) / 4 * 4;
+    static_assert(RING >= 8 && RING % 4 == 0, "places of the ring");
     static constexpr int off_q = 0, off_k = 2 * Q, off_v = off_k + 2 * K, off_ring = off_v + 2 * V;
     static constexpr int BYTES = off_ring + RING * PANEL + 1024;
     static constexpr int KATOM = TN * 128, VATOM = D * 128;   // 64 dims of 128 tokens; 64 tokens of D lanes
@@ -197,7 +201,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ ChunkBars B;
     __shared__ uint32_t tmem_base;
-    __shared__ int pre[kChunkThreads + 1];
+    int* pre = reinterpret_cast<int*>(smem + S::off_ring);   // [kChunkThreads + 1], until the roles begin
     __shared__ long long wsum[kChunkThreads / 32];
     __shared__ __align__(16) uint8_t vbad[kFlags][TN];                    // groups whose V is NaN, a bit each
     __shared__ int any_bad[kFlags];
@@ -282,6 +286,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         sg.r = lo * per;
         sg.seek(P, ca - pre[lo]);
     }
+    fence_async_smem();                                       // `pre` gives way to the first panels
+    __syncthreads();
     if (tid == 0) {                                           // for the merge: no row block begun here and cut, so far
         P.rec[8 * blockIdx.x] = -1;
     }
@@ -744,6 +750,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                         }
                     }
                     id = next;
+                    __syncwarp();                             // in step: no lane a tile ahead of another's place
                 }
             }
             // every copy has landed: the operands' warps have waited for it, or the wait is made up for
