@@ -380,15 +380,16 @@ def test_prefill_splits(H, HQ, ql, n):
     _check_rows(_np(out), _np(q), K[0], V[0], 0.08, HQ // H, torch.float16, True)
 
 
-@pytest.mark.parametrize("R,H,ql", [(40, 1, 4), (40, 1, 5), (40, 1, 8), (40, 1, 9), (3, 2, 12), (3, 2, 13), (17, 2, 12)])
+@pytest.mark.parametrize("R,H,ql", [(40, 1, 4), (40, 1, 6), (40, 1, 7), (40, 1, 8), (40, 1, 9), (3, 2, 12), (3, 2, 16),
+                                    (3, 2, 17), (17, 2, 12)])
 def test_prefill_streamed_or_not(R, H, ql):
     """Row counts, batches and bounds on both sides of the choice between the two kernels."""
     from vllm_ttkv import ops
-    lay = _lay(H, 64, 64)
+    lay = _lay(H, 128, 64) if R == 3 else _lay(H, 64, 64)
     rng = np.random.default_rng(ql)
     seqs = [ql + int(x) for x in rng.integers(0, 300, R)]
     cache, table, K, V = _filled(lay, seqs, 16, seed=R)
-    q = torch.randn(R * ql, 4 * H, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+    q = torch.randn(R * ql, 4 * H, lay.d, generator=torch.Generator().manual_seed(3)).half().cuda()
     for bound in (max(seqs), 1535, 1536, 100000):
         out = torch.empty_like(q)
         starts = _prefill(lay, cache, table, seqs, [ql] * R, q, 0.125, out, max_seq=bound)

@@ -786,9 +786,19 @@ __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParam
 
 // ------------------------------------------------------------------ host
 
-// Rows a streaming warp takes at once: 8 (query, head) rows a fragment, two fragments above that. (16 rows
-// of 64 requests of 6000 tokens, d = 64 in groups of 32: 177 us with two, 224 with one; 32 rows 321 and 417.)
-int stream_nt(int64_t rows) { return rows > 8 ? 2 : 1; }
+// Fragments of 8 (query, head) rows that a streaming warp takes at once: two above 8 rows, but at d = 128 only
+// where that leaves none empty, and in groups of 32 there not at all, since two spill. 64 requests of 6000
+// tokens, 8 KV heads, us with two and with one:
+//   d, group   16 rows    24         32
+//   64, 32     172/195    299/281    313/365   (and ragged, 1 to 20 rows: 36/38)
+//   64, 64     154/174    262/252    281/328
+//   128, 128   197/213    332/305    352/397
+//   128, 64    225/242    389/348    414/453
+//   128, 32    324/307    590/444    610/584
+int stream_nt(int d, int group, int64_t rows) {
+    if (d == 64) return rows > 8 ? 2 : 1;
+    return group == 32 || (rows + 7) / 8 % 2 ? 1 : 2;
+}
 
 // Workspace: two parts a CTA for the merge, a part a warp.
 struct StreamWs {
@@ -848,7 +858,7 @@ int launch_stream(const AttnParams& P, cudaStream_t st) {
 }
 
 int run_stream(const ttkv_q4_cache_t* c, AttnParams P, void* ws, size_t ws_bytes, cudaStream_t st) {
-    const int nt = stream_nt(int64_t(P.max_q) * P.G);
+    const int nt = stream_nt(c->d, c->group, int64_t(P.max_q) * P.G);
     const StreamWs w = stream_ws(c->d, nt);
     if (!ws || ws_bytes < w.bytes)
         return fail(TTKV_ERR_WORKSPACE, "4-bit read: workspace of %zu bytes, %zu needed", ws ? ws_bytes : 0, w.bytes);
@@ -862,7 +872,8 @@ int run_stream(const ttkv_q4_cache_t* c, AttnParams P, void* ws, size_t ws_bytes
     P.first = reinterpret_cast<float*>(base + w.first);
 #define TTKV_Q4_STREAM(D, GRP)                                                                     \
     if (c->d == D && c->group == GRP) return nt == 2 ? launch_stream<D, GRP, 2>(P, st) : launch_stream<D, GRP, 1>(P, st);
-    TTKV_Q4_STREAM(64, 32) TTKV_Q4_STREAM(64, 64) TTKV_Q4_STREAM(128, 32) TTKV_Q4_STREAM(128, 64) TTKV_Q4_STREAM(128, 128)
+    TTKV_Q4_STREAM(64, 32) TTKV_Q4_STREAM(64, 64) TTKV_Q4_STREAM(128, 64) TTKV_Q4_STREAM(128, 128)
+    if (c->d == 128 && c->group == 32) return launch_stream<128, 32, 1>(P, st);
 #undef TTKV_Q4_STREAM
     return fail(TTKV_ERR_UNSUPPORTED, "4-bit read: geometry");
 }
@@ -887,17 +898,17 @@ AttnParams attn_params(const ttkv_q4_attn_args_t* a) {
 // the tensor cores once per 16 rows, or go to the chunk kernel, whose tiles of 256 rows each dequantise
 // the cache once. Streamed against chunked, d = 128 in groups of 128, 8 KV heads, us:
 //   requests x tokens   16 rows      24           32           48           64
-//   64 x 130            60 / 73      81 / 75      95 / 75      134 / 75
-//   16 x 500            34 / 36      42 / 36      46 / 34
-//   64 x 1500           110 / 189    167 / 196    185 / 188    261 / 196
-//   64 x 6000           226 / 503    376 / 525    400 / 499    568 / 517
-//   4 x 3000            30 / 48      38 / 50      40 / 48      46 / 50      58 / 48
-//   1 x 130             20 / 24      20 / 26      22 / 26      22 / 26      22 / 26
-//   1 x 16000           34 / 71      42 / 75      42 / 79      48 / 79      56 / 81
-// So up to 16 rows always, up to 32 over long rows, up to 48 where few (request, head) pairs would leave
-// most of the chunk kernel's tiles waiting.
+//   64 x 130            56 / 73      73 / 77      87 / 77      126 / 77     155 / 79
+//   16 x 500            32 / 36      36 / 36      42 / 34      52 / 36      65 / 34
+//   64 x 1500           93 / 196     132 / 202    161 / 191    228 / 200    292 / 198
+//   64 x 6000           192 / 525    302 / 548    349 / 519    503 / 540    658 / 542
+//   4 x 3000            28 / 48      30 / 52      36 / 50      40 / 52      50 / 50
+//   1 x 130             20 / 26      17 / 28      20 / 28      20 / 28      22 / 28
+//   1 x 16000           30 / 73      32 / 87      36 / 85      42 / 87      46 / 85
+// So up to 24 rows always, up to 32 over long rows, up to 64 where few (request, head) pairs leave most of
+// the chunk kernel's time to latency.
 bool streams(int64_t rows, int64_t pairs, int max_seq) {
-    return rows <= 16 || (rows <= 32 && max_seq >= 1536) || (rows <= 48 && pairs <= 32);
+    return rows <= 24 || (rows <= 32 && max_seq >= 1536) || (rows <= 64 && pairs <= 32);
 }
 
 }  // namespace
@@ -906,7 +917,7 @@ bool streams(int64_t rows, int64_t pairs, int max_seq) {
 using namespace ttkv;
 
 extern "C" size_t ttkv_q4_decode_workspace_bytes(int32_t d, int32_t n_reqs, int32_t group_heads) {
-    return n_reqs < 0 ? 0 : stream_ws(d, stream_nt(group_heads)).bytes;
+    return n_reqs < 0 ? 0 : stream_ws(d, group_heads > 8 ? 2 : 1).bytes;      // (two fragments need more than one)
 }
 
 extern "C" int ttkv_q4_decode(const ttkv_q4_attn_args_t* args) {
@@ -923,7 +934,7 @@ extern "C" size_t ttkv_q4_prefill_workspace_bytes(int32_t d, int32_t n_reqs, int
     if (n_reqs < 0 || max_q_len < 0) return 0;
     const int64_t rows = int64_t(max_q_len) * group_heads;
     const bool some = streams(rows, 0, INT32_MAX), all = streams(rows, INT64_MAX, 0);     // are streamed
-    return std::max(some ? stream_ws(d, stream_nt(rows)).bytes : 0, all ? 0 : chunk_workspace_bytes(d));
+    return std::max(some ? stream_ws(d, rows > 8 ? 2 : 1).bytes : 0, all ? 0 : chunk_workspace_bytes(d));
 }
 
 extern "C" int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args) {
