@@ -666,11 +666,13 @@ __global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kern
         }
     }
     __syncthreads();
-    for (int s0 = 0; s0 < SLOTS;) {
-        const int id = pid[s0];
-        int s1 = s0 + 1;
-        if (id < 0) { s0 = s1; continue; }
-        while (s1 < SLOTS && (pid[s1] < 0 || pid[s1] == id)) ++s1;
+    static_assert(SLOTS <= 32, "a slot a lane");
+    const int mine = lane < SLOTS ? pid[lane] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, mine);
+    for (uint32_t heads = __ballot_sync(0xffffffffu, mine >= 0 && (same & ((1u << lane) - 1u)) == 0u); heads; heads &= heads - 1u) {
+        const int s0 = __ffs(heads) - 1, id = __shfl_sync(0xffffffffu, mine, s0);
+        const uint32_t slots = __shfl_sync(0xffffffffu, same, s0);
+        const int s1 = 32 - __clz(slots);
         const Req rq = request(P, pr[s0], false);
         const int h = ph[s0], rb = prb[s0], live = min(ROWS, rq.ql * P.G - rb * ROWS);
         const bool whole = id >= ca && id + units_of(rq) <= cb;
@@ -679,12 +681,12 @@ __global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kern
             const int i = e / (D / 4), ln = 4 * (e - i * (D / 4));
             float M = -INFINITY;
             for (int k = s0; k < s1; ++k)
-                if (pid[k] >= 0) M = fmaxf(M, pm[k][i]);
+                if (slots >> k & 1u) M = fmaxf(M, pm[k][i]);
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
             float l = 0.f;
             #pragma unroll 4
             for (int k = s0; k < s1; ++k) {
-                if (pid[k] < 0) continue;
+                if (!(slots >> k & 1u)) continue;
                 const float wt = part_weight(pm[k][i], M);
                 const float4 x = *reinterpret_cast<const float4*>(part_of(k) + i * D + ln);
                 l = fmaf(wt, pl[k][i], l);
@@ -697,7 +699,6 @@ __global__ void __launch_bounds__(Stream<D, GRP, NT>::THREADS, 1) q4_stream_kern
                 if (ln == 0) *reinterpret_cast<float2*>(P.part_ml + (g0 + i) * 2) = make_float2(M, l);
             }
         }
-        s0 = s1;
     }
 }
 
