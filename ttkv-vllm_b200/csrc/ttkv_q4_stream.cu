@@ -5,8 +5,8 @@
 //
 // q4_stream_kernel reads every stored byte once per block of 8 NT (query, head) rows. 64 requests of up to
 // 14402 tokens (8 KV heads of 128 lanes, 3 query heads each, groups of 128; 477 MB) take 110 us, 4.3 TB/s
-// or 58 percent of a measured copy, and 1074 instructions a unit of 64 tokens: two warps a scheduler
-// (their registers allow no more) issue in 47 percent of the cycles, half of them on the half-rate pipe
+// or 66 percent of a measured copy, and 1110 instructions a unit of 64 tokens: three warps a scheduler
+// (their registers allow no more) issue in 57 percent of the cycles, half of them on the half-rate pipe
 // of the masks. 131071 tokens of 2 KV heads take 26 us, 8 requests of 4322 tokens 21, one of 257 9: there
 // launch, schedule and the first copies' latency come before the bytes. The codes c are never turned into values: they are exact operands of the tensor cores,
 // and scales and minima act on the products,
