@@ -66,7 +66,7 @@ struct ChunkSmem {
     // Panels of the ring: a multiple of four, so that a place always holds panels of the same warps of K and V.
     // Each warp then sees every phase of its places; one that skipped some could take the phase before the
     // last for the one that it waits for, and read a place that is still being filled
-    static constexpr int PANEL = panel_bytes(D, GRP), RING = std::min(16, 30720 / PANEL) / 4 * 4;
+    static constexpr int PANEL = panel_bytes(D, GRP), RING = std::min(16, 30 * 1024 / PANEL) / 4 * 4;
     static_assert(RING >= 8 && RING % 4 == 0, "places of the ring");
     static constexpr int off_q = 0, off_k = 2 * Q, off_v = off_k + 2 * K, off_ring = off_v + 2 * V;
     static constexpr int BYTES = off_ring + RING * PANEL + 1024;
