@@ -14,7 +14,6 @@ The cache: uint8 [blocks, H, block_size / 16, panel bytes]. A panel holds 16 tok
 K codes (8 d bytes), V codes (8 d bytes), then (scale, minimum) as two fp16 per token and group of
 lanes, for K and for V. A code c of a group stands for minimum + scale * c.
 """
-import functools
 import pathlib
 import sys
 
@@ -338,15 +337,13 @@ def _plain_plan(s):
 
 
 # ------------------------------------------------------------------ the framework's calls
-@functools.cache
 def _framework():
-    """The package, imported once as a program does."""
     root = str(pathlib.Path(__file__).resolve().parents[1] / "ttkv-vllm_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
     from vllm_ttkv import ops
     from vllm_ttkv.q4 import Q4Layout
-    return ops, functools.cache(Q4Layout)       # a program keeps its layers' layouts
+    return ops, Q4Layout
 
 
 def _own_run(s):
