@@ -462,8 +462,12 @@ int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args);
  *
  * ttkv_release_blocks: pushes the ceil(lens[r] / block_size) blocks of each request's row onto the
  * free list, in request order (lens[r] <= 0: none). capacity = the entries free_blocks has room for;
- * requests that do not fit are left out (TTKV_STATUS_POOL_FULL), every later one too. (query_start_loc,
- * slots, positions and n_tokens are not read.)
+ * requests that do not fit are left out (TTKV_STATUS_POOL_FULL), every later one too. A request with a
+ * negative id among its blocks returns none of them (TTKV_STATUS_BLOCK_RANGE), the others theirs: a
+ * request that ttkv_plan_step refused holds the blocks of its len - new, and is released with that
+ * length. Entries of free_blocks behind the new count are unspecified after such a refusal.
+ * (query_start_loc, slots, positions and n_tokens are not read.) A negative id on the list is given out
+ * by ttkv_plan_step like another, reported (TTKV_STATUS_BLOCK_RANGE), and its tokens get slots -1.
  *
  * n_reqs is at most TTKV_PLAN_MAX_REQS. */
 #define TTKV_PLAN_MAX_REQS 16384

@@ -92,3 +92,18 @@ def plan(table, seq, qsl, free, count, block_size, n_tokens):
             pos[t] = p
             slots[t] = int(table[r, p // block_size]) * block_size + p % block_size
     return table, slots, pos, len(free), refused
+
+
+def release(table, lens, free, count, block_size):
+    """The free list after the blocks of `lens` tokens of each row have been returned: (list, refused rows)."""
+    out, refused, full = list(free[:count]), [], False
+    for r, n in enumerate(lens):
+        ids = [int(x) for x in table[r, :max(0, -(-int(n) // block_size))]]
+        if -(-int(n) // block_size) > table.shape[1] or min(ids, default=0) < 0:
+            refused.append(r)
+        elif ids and (full or len(out) + len(ids) > len(free)):
+            full = True
+            refused.append(r)
+        else:
+            out += ids
+    return out, refused

@@ -167,3 +167,111 @@ def test_plan_captured():
         assert np.array_equal(table.cpu().numpy(), ref) and slots.tolist() == s.tolist()
         assert pos.tolist() == p.tolist() and int(count) == c
     ops.check_status()
+
+
+# ------------------------------------------------------------------ ids that are none
+def _release(table, lens, free, count, bs):
+    from vllm_ttkv import ops
+    f, c = _i32(free), _i32([count])
+    ops.release_blocks(_i32(table), _i32(lens), f, c, bs)
+    return f.cpu().tolist()[:int(c)]
+
+
+@pytest.mark.parametrize("n,hi", [(1, 40), (5, 400), (40, 5000), (700, 90), (5000, 40)])
+def test_release_refuses_a_row_that_holds_no_id(n, hi):
+    """A request with a negative id among its blocks returns none of them, the others all of theirs; one
+    behind its blocks does not matter."""
+    from vllm_ttkv import ops
+    rng = np.random.default_rng(n)
+    lens = rng.integers(1, hi + 1, n)
+    nb = -(-lens // 16)
+    cols = int(nb.max()) + 1
+    table = rng.permutation(n * cols).reshape(n, cols)
+    table[np.arange(n), nb] = -1
+    for r in rng.permutation(n)[:max(1, n // 9)]:
+        table[r, rng.integers(0, nb[r])] = -1 - int(rng.integers(0, 3))
+    free = np.concatenate([np.arange(9) + 10 ** 6, np.full(int(nb.sum()), -1)])
+    want, refused = O.release(table, lens, free, 9, 16)
+    assert refused
+    ops.reset_status()
+    got = _release(table, lens, free, 9, 16)
+    with pytest.raises(IndexError):
+        ops.check_status()
+    assert got == want and min(got) >= 0
+
+
+def test_release_of_bad_rows_and_little_room():
+    """The room of a refused request goes to those behind it; what does not fit even so is refused."""
+    from vllm_ttkv import ops
+    table = np.array([[1, -1, 3], [4, 5, 6], [7, 8, 9], [10, 11, 12], [-1, -1, -1]])
+    for room, want in ((6, [4, 5, 6, 7, 8, 9]), (5, [4, 5, 6]), (8, [4, 5, 6, 7, 8, 9]), (9, [4, 5, 6, 7, 8, 9, 10, 11, 12])):
+        free = np.full(room, -1)
+        assert O.release(table, [48, 48, 48, 48, 0], free, 0, 16)[0] == want
+        ops.reset_status()
+        assert _release(table, [48, 48, 48, 48, 0], free, 0, 16) == want
+        with pytest.raises((IndexError, RuntimeError)):
+            ops.check_status()
+    ops.reset_status()
+    assert _release(table[1:], [33, 0, 48, 0], np.full(6, -1), 0, 16) == [4, 5, 6, 10, 11, 12]
+    ops.check_status()
+
+
+def test_a_refused_request_is_released():
+    """A request that a step refused: released with the length it was planned with it is refused again, and
+    nothing of its row reaches the list; released with the length it had, it returns what it held."""
+    from vllm_ttkv import ops
+    table = _i32([[3, 4, -7, -7], [5, 0, 1, 2], [-7, -7, -7, -7]])
+    free, count = _i32([9, 8, -1, -1, -1, -1, -1]), _i32([2])
+    slots = torch.zeros(60, dtype=torch.int64, device="cuda")
+    ops.reset_status()
+    ops.plan_step(table, _i32([33, 47, 0]), _i32([0, 1, 41, 41]), free, count, 16, slots)     # 1 block, then 2 of 1
+    with pytest.raises(RuntimeError):
+        ops.check_status()
+    assert table.cpu().tolist()[:2] == [[3, 4, 8, -7], [5, -1, 1, 2]] and int(count) == 1
+    ops.release_blocks(table, _i32([0, 47, 0]), free, count, 16)
+    with pytest.raises(IndexError):
+        ops.check_status()
+    assert int(count) == 1 and int(free[0]) == 9
+    ops.release_blocks(table, _i32([33, 7, 0]), free, count, 16)
+    ops.check_status()
+    assert free.cpu().tolist()[:int(count)] == [9, 3, 4, 8, 5]
+    ops.plan_step(table, _i32([0, 0, 80]), _i32([0, 0, 0, 80]), free, count, 16, torch.zeros(80, dtype=torch.int64, device="cuda"))
+    with pytest.raises(RuntimeError):                    # (four columns)
+        ops.check_status()
+    ops.plan_step(table, _i32([0, 0, 60]), _i32([0, 0, 0, 60]), free, count, 16, slots)
+    ops.check_status()
+    assert table[2].tolist() == [5, 8, 4, 3] and int(count) == 1 and int(slots.min()) >= 0
+
+
+def test_plan_reports_an_id_that_is_none():
+    from vllm_ttkv import ops
+    table, slots = _i32([[-7, -7], [-7, -7]]), torch.zeros(40, dtype=torch.int64, device="cuda")
+    ops.reset_status()
+    ops.plan_step(table, _i32([20, 20]), _i32([0, 20, 40]), _i32([4, 3, -1, 2]), _i32([4]), 16, slots)
+    with pytest.raises(IndexError):
+        ops.check_status()
+    assert table.tolist() == [[2, -1], [3, 4]]
+    assert slots.tolist() == [32 + i for i in range(16)] + [-1] * 4 + [48 + i for i in range(16)] + [64 + i for i in range(4)]
+
+
+def test_release_captured():
+    """A captured release, replayed with a row that holds no id and without."""
+    from vllm_ttkv import ops
+    table, lens = _i32([[1, 2], [3, 4], [5, 6]]), _i32([0, 0, 0])
+    free, count, left = _i32(np.full(8, -1)), _i32([0]), _i32([-5])
+    ops.status_word()
+    ops.reset_status()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.release_blocks(table, lens, free, count, 16, free_count_out=left)
+    for ns, row, want in (([20, 1, 0], [3, 4], [1, 2, 3]), ([20, 1, 32], [-1, 4], [1, 2, 5, 6]), ([0, 32, 1], [3, 4], [3, 4, 5]),
+                          ([0, 32, 1], [3, -1], [5])):
+        lens.copy_(_i32(ns))
+        table[1].copy_(_i32(row))
+        g.replay()
+        assert free.tolist()[:int(left)] == want and int(count) == 0
+        if min(row) < 0:
+            with pytest.raises(IndexError):
+                ops.check_status()
+        else:
+            ops.check_status()

@@ -6,15 +6,18 @@
 // lies in slot table[r][p / bs] * bs + p % bs. All integers.
 //
 // Bound: launch and load latency (a step moves a few KB to a few hundred KB). So one launch, one
-// cluster of CTAs: every CTA repeats the prefix sum over all requests (a few
-// hundred loads) rather than waiting for another CTA's, keeps each request's lengths and its end in the
-// free list in shared memory, and then takes its share of the blocks that change hands and of the
-// tokens, each found by a binary search, so that a step has two rounds of loads whatever its mix of
-// lengths. One decode token for each of 8, 1024, 4096 and 16384 requests takes 8.3, 12.3, 20.5 and 64 us
-// from an idle GPU (8.6, 13.3, 32.8 and 111 with one CTA), 16384 tokens of 64 requests 12.3 (45 with
-// one). The cluster's barrier orders every CTA's read of the count before the write of the new one,
-// which may be the same word.
+// cluster of CTAs: every CTA repeats the prefix sum over all requests (a few hundred loads) rather than
+// waiting for another CTA's, keeps each request's lengths and its end in the free list in shared
+// memory, and then takes its share of the blocks that change hands and of the tokens, each found by a
+// binary search, so that a step has two rounds of loads whatever its mix of lengths. One decode token
+// for each of 8, 1024, 4096 and 16384 requests takes 8.3, 12.3, 20.5 and 64 us from an idle GPU (8.6,
+// 13.3, 32.8 and 111 with one CTA), 16384 tokens of 64 requests 12.3 (45 with one). A release writes
+// the ids as it reads them, behind the list's end, and starts over without a request's where one is
+// negative: looking at all of them first would be a third round of loads. The cluster's barrier orders
+// every CTA's read of the count before the write of the new one, which may be the same word.
 #include <cooperative_groups.h>
+
+#include <utility>
 
 #include "ttkv_async.cuh"
 #include "ttkv_common.cuh"
@@ -64,9 +67,14 @@ struct PlanSmem {
     int32_t* start;                                  // [n_reqs + 1]
 };
 
-// Fills len and end; returns the blocks taken or returned in all.
+// Release: the length of a request whose row holds a negative id.
+constexpr int32_t kBadRow = INT32_MIN;
+
+// Fills len and end; returns the blocks taken or returned in all, and whether the room was too little.
+// again (release): requests whose length is kBadRow are left out.
 template <bool RELEASE>
-__device__ int assign_ranges(const PlanParams& P, int avail, const PlanSmem& M, long long* wsum, int32_t* taken) {
+__device__ int assign_ranges(const PlanParams& P, int avail, const PlanSmem& M, long long* wsum, int32_t* taken, bool& lacking,
+                             bool again = false) {
     const int tid = threadIdx.x;
     const bool first = blockIdx.x == 0;
     long long carry = 0;
@@ -79,7 +87,8 @@ __device__ int assign_ranges(const PlanParams& P, int avail, const PlanSmem& M, 
         if (ok) {
             seq = P.lens[r];
             if (RELEASE) {
-                need = blocks_of(seq, P.block_size);
+                ok = !again || M.len[r] != kBadRow;
+                need = ok ? blocks_of(seq, P.block_size) : 0;
             } else {
                 const int a = P.query_start_loc[r], b = P.query_start_loc[r + 1];
                 M.start[r] = a;
@@ -99,10 +108,7 @@ __device__ int assign_ranges(const PlanParams& P, int avail, const PlanSmem& M, 
         }
         long long total;
         const long long end = carry + scan_inclusive(need, wsum, total);
-        if (ok && need > 0 && end > avail) {         // and so for every later request with a need
-            ok = false;
-            if (first) report(P.status, RELEASE ? TTKV_STATUS_POOL_FULL : TTKV_STATUS_POOL_EMPTY);
-        }
+        if (ok && need > 0 && end > avail) ok = false;      // and so for every later request with a need
         if (ok && need > 0) atomicMax(taken, int32_t(end));
         if (r < P.n_reqs) {
             M.len[r] = ok ? seq : ~max(seq, 0);
@@ -110,6 +116,7 @@ __device__ int assign_ranges(const PlanParams& P, int avail, const PlanSmem& M, 
         }
         carry += total;
     }
+    lacking = carry > avail;
     __syncthreads();
     // from the first refusal for want of room on, every end is the last one granted
     const int used = *taken;
@@ -139,7 +146,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanParam
     pdl_wait();
     pdl_trigger();
     const int count = min(max(*P.free_count, 0), P.capacity);
-    const int used = assign_ranges<false>(P, count, M, wsum, &taken);
+    bool lacking;
+    const int used = assign_ranges<false>(P, count, M, wsum, &taken, lacking);
+    if (lacking && at == 0) report(P.status, TTKV_STATUS_POOL_EMPTY);
 
     // a refused request's row: no block behind those that it holds
     for (int r = at; r < P.n_reqs; r += step) {
@@ -152,7 +161,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanParam
         const int e = int(i);
         const int r = find(M.end, P.n_reqs, e), first = r ? M.end[r - 1] : 0;
         const int held = blocks_of(M.len[r] - (M.start[r + 1] - M.start[r]), P.block_size);
-        P.block_table[int64_t(r) * P.bt_stride + held + (e - first)] = P.free_blocks[count - 1 - e];
+        const int32_t id = P.free_blocks[count - 1 - e];
+        if (id < 0) report(P.status, TTKV_STATUS_BLOCK_RANGE);
+        P.block_table[int64_t(r) * P.bt_stride + held + (e - first)] = id;
     }
     // the tokens
     for (unsigned i = at; i < unsigned(P.n_tokens); i += step) {
@@ -174,16 +185,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanParam
     if (at == 0) *P.free_count_out = count - used;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) release_blocks_kernel(const PlanParams P) {
-    extern __shared__ int32_t plan_smem[];
-    __shared__ long long wsum[32];
-    __shared__ int32_t taken;
-    const PlanSmem M{plan_smem, plan_smem + P.n_reqs, nullptr};
-    const int at = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
-    pdl_wait();
-    pdl_trigger();
-    const int count = min(max(*P.free_count, 0), P.capacity);
-    const int used = assign_ranges<true>(P, P.capacity - count, M, wsum, &taken);
+// The granted requests' ids onto the list's end, this thread's share of them; whether one is negative.
+__device__ bool push_ids(const PlanParams& P, const PlanSmem& M, int count, int used, int at, int step) {
     bool bad = false;
     #pragma unroll 4
     for (unsigned i = at; i < unsigned(used); i += step) {
@@ -193,9 +196,48 @@ __global__ void __launch_bounds__(kPlanThreads) release_blocks_kernel(const Plan
         bad |= id < 0;
         P.free_blocks[count + e] = id;
     }
-    if (bad) report(P.status, TTKV_STATUS_BLOCK_RANGE);
-    cg::this_cluster().sync();
-    if (at == 0) *P.free_count_out = count + used;
+    return bad;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) release_blocks_kernel(const PlanParams P) {
+    extern __shared__ int32_t plan_smem[];
+    __shared__ long long wsum[32];
+    __shared__ int32_t taken;
+    __shared__ int bad_row;                          // some CTA of the cluster met a negative id
+    const PlanSmem M{plan_smem, plan_smem + P.n_reqs, nullptr};
+    const int at = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
+    cg::cluster_group cluster = cg::this_cluster();
+    if (threadIdx.x == 0) bad_row = 0;
+    auto begun = cluster.barrier_arrive();
+    pdl_wait();
+    pdl_trigger();
+    const int count = min(max(*P.free_count, 0), P.capacity), avail = P.capacity - count;
+    bool lacking;
+    int used = assign_ranges<true>(P, avail, M, wsum, &taken, lacking);
+    cluster.barrier_wait(std::move(begun));          // every CTA's bad_row may be written
+    if (push_ids(P, M, count, used, at, step)) {
+        report(P.status, TTKV_STATUS_BLOCK_RANGE);
+        for (int c = 0; c < kPlanCtas; ++c) *cluster.map_shared_rank(&bad_row, c) = 1;
+    }
+    cluster.sync();
+    if (bad_row) {                                   // (the same in every CTA) once more without the rows that hold one
+        const int lane = threadIdx.x & 31;
+        for (int r = threadIdx.x >> 5; r < P.n_reqs; r += kPlanThreads / 32) {
+            const int nb = blocks_of(P.lens[r], P.block_size);
+            bool bad = false;
+            if (nb <= P.bt_cols)
+                for (int k = lane; k < nb; k += 32) bad |= P.block_table[int64_t(r) * P.bt_stride + k] < 0;
+            bad = __any_sync(0xffffffffu, bad);
+            if (lane == 0) M.len[r] = bad ? kBadRow : 0;
+        }
+        __syncthreads();
+        used = assign_ranges<true>(P, avail, M, wsum, &taken, lacking, true);
+        push_ids(P, M, count, used, at, step);
+    }
+    if (at == 0) {
+        if (lacking) report(P.status, TTKV_STATUS_POOL_FULL);
+        *P.free_count_out = count + used;
+    }
 }
 
 int check_plan(const ttkv_plan_args_t* p) {

@@ -482,7 +482,9 @@ def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, free_blocks: t
                    status: torch.Tensor | None = None) -> None:
     """Return the blocks of finished requests: the ceil(lens[r] / block_size) blocks of each row go onto
     the end of free_blocks[:free_count], in request order (lens[r] = 0: none). The table's rows are left
-    as they are. Each block may be returned once."""
+    as they are. Each block may be returned once. A request with a negative id among those blocks is
+    refused (`check_status`) and returns none of them: one that `plan_step` refused holds the blocks of
+    the length that it had before that step, and is released with it."""
     code = _lib.torch_binding().plan(block_table, lens, free_blocks, free_count,
                                      free_count if free_count_out is None else free_count_out, block_size,
                                      _status_of(block_table, status))
