@@ -1,0 +1,98 @@
+"""What the attention over the 4-bit cache keeps of its precision where values are hard: tokens that some
+rows of a block do not see, NaN beside numbers. The helpers, and the tolerances' terms, are those of
+`test_gpu_q4.py`."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import q4 as O
+from test_gpu_q4 import GEOMETRIES, _check_rows, _filled, _lay, _np, _prefill
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ drafted tokens that earlier rows do not see
+def _small_values(lay, n, last, bs=16):
+    """One request of n tokens, V of about 1e-3 but for `last` [k, H, d], the V of the last k tokens:
+    (cache, table, K, V stored)."""
+    from vllm_ttkv import ops
+    rng = np.random.default_rng(n)
+    nb = -(-n // bs)
+    cache = lay.new_cache(nb, bs)
+    table = torch.from_numpy(rng.permutation(nb)).int()[None].cuda()
+    t = torch.arange(n, device="cuda")
+    k = torch.from_numpy(rng.standard_normal((n, lay.H, lay.d))).float().cuda()
+    v = torch.from_numpy(rng.standard_normal((n, lay.H, lay.d)) * 1e-3).float().cuda()
+    v[n - len(last):] = last
+    ops.q4_write_paged(lay, cache, table[0].long()[t // bs] * bs + t % bs, k, v)
+    return cache, table, *(O.values(*O.quantise(_np(x), lay.group)) for x in (k, v))
+
+
+@pytest.mark.parametrize("d,g", GEOMETRIES)
+@pytest.mark.parametrize("G,ql,n", [(1, 5, 70), (2, 4, 64), (4, 6, 203), (3, 8, 1000)])
+@pytest.mark.parametrize("what", ["nan", "large", "infinite lane"])
+def test_a_later_token_costs_earlier_rows_nothing(d, g, G, ql, n, what):
+    """The last two tokens' V are NaN or 10^7 times the others': the rows before them, of the same block and the
+    same unit of tokens, are as exact as without them."""
+    lay = _lay(1, d, g)
+    last = torch.full((2, 1, d), float("nan") if what == "nan" else 3e4, device="cuda")
+    if what == "large":
+        last *= torch.linspace(0.5, 1, d, device="cuda")
+    if what == "infinite lane":
+        last = torch.full((2, 1, d), 1e-3, device="cuda")
+        last[..., 5] = float("inf")
+    cache, table, K, V = _small_values(lay, n, last)
+    q = torch.randn(ql, G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    _prefill(lay, cache, table, [n], [ql], q, d ** -0.5, out)
+    _check_rows(_np(out[:-2]), _np(q[:-2]), K[:n - 2], V[:n - 2], d ** -0.5, G, torch.float16, False)
+    if what == "large":
+        _check_rows(_np(out[-2:]), _np(q[-2:]), K, V, d ** -0.5, G, torch.float16, False)
+    else:                                                # the lanes of the groups that hold one, and no other
+        spoilt = torch.zeros(d, dtype=torch.bool)
+        spoilt[:d if what == "nan" else g] = True
+        assert bool(out[-2:, :, spoilt.cuda()].isnan().all())
+        if g < d and what != "nan":
+            rest = ~spoilt.numpy()
+            got, want = _np(out[-2:])[..., rest], O.attend(_np(q[-2:]), K, np.where(np.isnan(V), 0, V), d ** -0.5, G)[..., rest]
+            R = np.nanmax(np.abs(V))
+            assert np.all(np.abs(got - want) <= 2.0 ** -11 * np.abs(want) + 2 * 2.0 ** -12 * R)
+
+
+@pytest.mark.parametrize("d,g", [(64, 32), (128, 128)])
+def test_a_bad_block_of_the_last_rows_costs_the_others_nothing(d, g):
+    from vllm_ttkv import ops
+    lay, n, ql, G = _lay(1, d, g), 66, 6, 2
+    cache, table, K, V = _small_values(lay, n, torch.full((2, 1, d), 1e-3, device="cuda"))
+    table[0, -1] = cache.shape[0] + 3                    # tokens 64 and 65: the last two queries
+    q = torch.randn(ql, G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    ops.reset_status()
+    _prefill(lay, cache, table, [n], [ql], q, d ** -0.5, out)
+    with pytest.raises(IndexError):
+        ops.check_status()
+    assert bool(out[-2:].isnan().all())
+    _check_rows(_np(out[:-2]), _np(q[:-2]), K[:n - 2], V[:n - 2], d ** -0.5, G, torch.float16, False)
+
+
+@pytest.mark.parametrize("d,g", GEOMETRIES)
+def test_scales_that_rise_and_parts_that_meet(d, g):
+    """V scales that grow along the tokens, over parts of several CTAs, with rows that end in different units."""
+    lay, n, ql, G = _lay(2, d, g), 5003, 9, 2
+    from vllm_ttkv import ops
+    rng = np.random.default_rng(7)
+    nb = -(-n // 16)
+    cache = lay.new_cache(nb, 16)
+    table = torch.from_numpy(rng.permutation(nb)).int()[None].cuda()
+    t = torch.arange(n, device="cuda")
+    k = torch.from_numpy(rng.standard_normal((n, 2, d))).float().cuda()
+    v = torch.from_numpy(rng.standard_normal((n, 2, d)) * np.exp2(np.linspace(-14, 6, n))[:, None, None]).float().cuda()
+    v[n - 7::2] *= 500
+    ops.q4_write_paged(lay, cache, table[0].long()[t // 16] * 16 + t % 16, k, v)
+    K, V = (O.values(*O.quantise(_np(x), g)) for x in (k, v))
+    q = torch.randn(ql, 2 * G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    _prefill(lay, cache, table, [n], [ql], q, d ** -0.5, out)
+    for j in range(ql):                                  # row by row: R is what the row itself sees
+        m = n - ql + j + 1
+        _check_rows(_np(out[j:j + 1]), _np(q[j:j + 1]), K[:m], V[:m], d ** -0.5, G, torch.float16, False)

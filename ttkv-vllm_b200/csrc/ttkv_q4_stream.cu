@@ -67,6 +67,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // left to centre is 7.5 times the difference of even and odd weights.
 constexpr float kWeightsMost = 512.f;
 
+// Exponent field of a stored scale, 0 for a NaN's.
+__device__ __forceinline__ uint32_t scale_field(uint32_t meta) {
+    const uint32_t e = (meta >> 10) & 31u;
+    return e == 31u ? 0u : e;
+}
+
 template <int D, int GRP, int NT>
 struct WarpRows {
     static constexpr int NW = D / 32, NG = D / GRP, WPG = GRP / 32, ROWS = 8 * NT, PANEL = panel_bytes(D, GRP);
@@ -77,6 +83,7 @@ struct WarpRows {
     float o[2 * NW][NT][4];             // (p s 2^vn) . (c - 7.5), 2^-24 of it or (rows + 8 of a fragment) 2^-20
     float dsum[NT][2][NG];              // this lane's share of 2^vn p (m + 7.5 s)
     uint32_t vexp;                      // fp16 exponent field of the largest V scale so far; vn = 20 - vexp
+    uint32_t below;                     // a byte each row: how far its own largest lies under that (see step)
     bool fresh;                         // no unit yet
 
     __device__ __forceinline__ void start(const AttnParams& P, const Req& rq, int h, int rb, int lane) {
@@ -162,6 +169,7 @@ struct WarpRows {
         }
         min_lim = __reduce_min_sync(0xffffffffu, min_lim);
         vexp = 0;
+        below = 0;
         fresh = true;
     }
 
@@ -275,7 +283,8 @@ struct WarpRows {
         for (int nt = 0; nt < NT; ++nt)
             #pragma unroll
             for (int c = 0; c < 2; ++c) l[nt][c] = fmaf(l[nt][c], corr[nt][c], ls[nt][c]);
-        // the V scales of this lane's tokens (each token's lanes hold the same); the largest's exponent
+        // the V scales of this lane's tokens (each token's lanes hold the same); the largest's exponent. A NaN's
+        // (field 31) is none: its rows are NaN whatever the power, the other groups and rows need theirs
         uint32_t vm[4][2][NG], vmax = 0;
         #pragma unroll
         for (int p = 0; p < 4; ++p)
@@ -290,21 +299,66 @@ struct WarpRows {
                 for (int g = 0; g < NG; ++g) vmax = __vmaxu2(vmax, vm[p][i][g]);
             }
         vmax = __reduce_max_sync(0xffffffffu, (vmax >> 10) & 31u);
+        if (vmax == 31u) {
+            vmax = 0u;
+            #pragma unroll
+            for (int p = 0; p < 4; ++p)
+                #pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    #pragma unroll
+                    for (int g = 0; g < NG; ++g) vmax = max(vmax, scale_field(vm[p][i][g]));
+            vmax = __reduce_max_sync(0xffffffffu, vmax);
+        }
         const uint32_t ve = max(vexp, vmax);
         const float vfall = __uint_as_float((127u + vexp - ve) << 23);        // 2^(old - new)
         moved |= ve != vexp;
-        vexp = ve;
         const float vn = __uint_as_float((127u + 20u - ve) << 23);
+        if (tail) {
+            // a token's scale must not cost the rows that do not see it their bits: each row's weights go by
+            // the largest scale that it has seen, a power of two above the common one
+            moved = true;
+            uint32_t now = 0;
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                #pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t was = vexp - ((below >> (16 * nt + 8 * c)) & 31u);
+                    uint32_t e = was;
+                    #pragma unroll
+                    for (int p = 0; p < 4; ++p)
+                        #pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            #pragma unroll
+                            for (int g = 0; g < NG; ++g)
+                                if (t0 + 16 * p + b + 8 * i < lim[nt][c]) e = max(e, scale_field(vm[p][i][g]));
+                    #pragma unroll
+                    for (int k = 4; k < 32; k <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, k));
+                    now |= (ve - e) << (16 * nt + 8 * c);
+                    corr[nt][c] *= __uint_as_float((127u + was - e) << 23);
+                    const float up = __uint_as_float((127u + ve - e) << 23);
+                    #pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        s[p][nt][c] *= up;
+                        s[p][nt][2 + c] *= up;
+                    }
+                }
+            below = now;
+        } else if (moved) {
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                corr[nt][0] *= vfall;
+                corr[nt][1] *= vfall;
+            }
+        }
+        vexp = ve;
 
         if (moved) {                                              // (the same in every lane)
             #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    corr[nt][c] *= vfall;
+                for (int c = 0; c < 2; ++c)
                     #pragma unroll
                     for (int g = 0; g < NG; ++g) dsum[nt][c][g] *= corr[nt][c];
-                }
             #pragma unroll
             for (int i = 0; i < 2 * NW; ++i)
                 #pragma unroll
@@ -373,11 +427,12 @@ struct WarpRows {
 
     // Sums over the lanes that share columns; o becomes sum p V relative to m, l the whole sum.
     __device__ __forceinline__ void finish() {
-        const float back = __uint_as_float((127u + vexp - 20u) << 23);
+        float back[NT][2];
         #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
+                back[nt][c] = __uint_as_float((127u + vexp - ((below >> (16 * nt + 8 * c)) & 31u) - 20u) << 23);
                 #pragma unroll
                 for (int k = 4; k < 32; k <<= 1) {
                     l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], k);
@@ -391,7 +446,7 @@ struct WarpRows {
             for (int nt = 0; nt < NT; ++nt)
                 #pragma unroll
                 for (int k = 0; k < 4; ++k)                       // rows + 8 of a fragment came in as c 2^-20
-                    o[i][nt][k] = fmaf(o[i][nt][k], k < 2 ? 16777216.f : 1048576.f, dsum[nt][k & 1][i / 2 / WPG]) * back;
+                    o[i][nt][k] = fmaf(o[i][nt][k], k < 2 ? 16777216.f : 1048576.f, dsum[nt][k & 1][i / 2 / WPG]) * back[nt][k & 1];
     }
 
     __device__ __forceinline__ float4 four(int nt, int c, int k) const {      // output lanes 32 k + 4 b + (0..3)
