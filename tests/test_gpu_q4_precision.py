@@ -96,3 +96,42 @@ def test_scales_that_rise_and_parts_that_meet(d, g):
     for j in range(ql):                                  # row by row: R is what the row itself sees
         m = n - ql + j + 1
         _check_rows(_np(out[j:j + 1]), _np(q[j:j + 1]), K[:m], V[:m], d ** -0.5, G, torch.float16, False)
+
+
+# ------------------------------------------------------------------ NaN in chunks
+@pytest.mark.parametrize("d,g", [(64, 32), (128, 128)])
+def test_nan_by_row_tiles_in_turn(d, g):
+    """Row blocks of two row tiles and of one in turn, many in a CTA: a NaN of V in a block's last tokens reaches
+    the rows that see it, and the rows of no other block."""
+    from vllm_ttkv import ops
+    lay, R, G, n0 = _lay(1, d, g), 700, 4, 300
+    qls = [60 if r % 2 else 20 for r in range(R)]        # 240 and 80 rows
+    seqs = [n0 - 10 + r % 40 for r in range(R)]
+    # every request reads one of eight stored sequences; in the odd ones a token near the end is NaN
+    cache, table, K, V = _filled(lay, [n0 + 40] * 8, 16, seed=d)
+    at = [seqs[-1] - 12 - 3 * i for i in range(8)]
+    for i in range(1, 8, 2):
+        one = torch.zeros(1, 1, d, device="cuda")
+        bad = one.clone()
+        bad[..., 1] = float("nan")
+        ops.q4_write_paged(lay, cache, table[i, at[i] // 16].long()[None] * 16 + at[i] % 16, one, bad)
+        K[i][at[i]] = 0.0
+    own = [(r * 3) % 8 for r in range(R)]
+    q = torch.randn(sum(qls), G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    ops.reset_status()
+    starts = _prefill(lay, cache, table[torch.tensor(own, device="cuda")].contiguous(), seqs, qls, q, d ** -0.5, out, max_q=100)
+    ops.check_status()
+    nan = out.isnan().cpu().numpy()
+    for r in range(R):
+        i, a, ql, n = own[r], starts[r], qls[r], seqs[r]
+        sees = (n - ql + np.arange(ql)) >= at[i] if i % 2 else np.zeros(ql, bool)
+        assert np.array_equal(nan[a:a + ql, :, :g].all((1, 2)), sees) and np.array_equal(nan[a:a + ql, :, :g].any((1, 2)), sees), r
+        assert not nan[a:a + ql, :, g:].any(), r
+        if r % 50 < 3:
+            clean = V[i].copy()
+            clean[at[i]] = 0.0 if i % 2 else clean[at[i]]
+            got, ref = _np(out[a:a + ql]), _np(q[a:a + ql])
+            if sees.any():
+                got[sees, :, :g] = O.attend(ref, K[i][:n], clean[:n], d ** -0.5, G)[sees, :, :g]
+            _check_rows(got, ref, K[i][:n], clean[:n], d ** -0.5, G, torch.float16, True)

@@ -79,6 +79,7 @@ struct ChunkBars {
     // row tiles; of halves one for each buffer: a half is waited for before the one after the next is made,
     // so no phase is missed
     uint64_t qfull[2], sfull[2][2], pfull[2][2], pvdone[2][2];
+    uint64_t noted[2];                                        // a segment's flags of NaN have all been read
 };
 
 // A CTA's (or a role's) place in the work list.
@@ -216,6 +217,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             mbar_init(&B.vfull[i], 128);
             mbar_init(&B.vempty[i], 2);
             mbar_init(&B.qfull[i], 128);
+            mbar_init(&B.noted[i], 128);
             for (int y = 0; y < 2; ++y) {
                 mbar_init(&B.sfull[i][y], 1);
                 mbar_init(&B.pfull[i][y], 128);
@@ -452,6 +454,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             wait(&B.pvdone[x][(n_s - 1) & 1], (n_s - 1) >> 1);
             tc_after();
             note_bad(n - 1, n_tile - 1);
+            mbar_arrive(&B.noted[x]);
             const bool whole = begin == 0 && n == U;
             // 32 output lanes at a time, through the warp's rows of Q (read by the last product) so that
             // neighbouring lanes of the warp write neighbouring bytes
@@ -566,8 +569,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             for (int it = 0; it < n; ++it, ++n_tile) {
                 const int st = n_tile & 1;
                 wait_idle(&B.vempty[st], (n_tile >> 1) + 1);
-                // the flags of the tile four behind are read by every row that sees it (the first half of its
-                // successor does, and V of this tile follows that by more)
+                // the flags of the tile four behind have been read by every row that sees it: the products of the
+                // tile two behind have ended, which its weights come before, or, where a row tile has none,
+                // a wait for `noted`
                 {
                     const int f = (n_tile + 4) & (kFlags - 1);
                     vbad[f][tid - 384] = 0;
@@ -683,6 +687,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         while (sg.u < sg.ue) {
             const int n = sg.here();
             if (sg.rb * CROWS + x * TM >= sg.rq.ql * P.G) {   // no rows: the operands are passed on
+                if (n_q) wait(&B.noted[x], n_q - 1);          // V may write over the flags of this row tile's last
                 for (int i = 0; i < n; ++i, ++n_tile) {
                     const int st = n_tile & 1;
                     wait(&B.kfull[st], n_tile >> 1);
