@@ -135,3 +135,42 @@ def test_nan_by_row_tiles_in_turn(d, g):
             if sees.any():
                 got[sees, :, :g] = O.attend(ref, K[i][:n], clean[:n], d ** -0.5, G)[sees, :, :g]
             _check_rows(got, ref, K[i][:n], clean[:n], d ** -0.5, G, torch.float16, True)
+
+
+# ------------------------------------------------------------------ small weights beside a large one
+@pytest.mark.parametrize("d,g", [(64, 64), (128, 128)])
+@pytest.mark.parametrize("R,ql,n", [(1, 1, 16384), (160, 1, 4000), (1, 66, 50000), (160, 33, 16384)])
+@pytest.mark.parametrize("nats", [8, 13, 17, 18, 20])
+def test_a_token_that_takes_most(d, g, R, ql, n, nats):
+    """The first token's weight is e^nats times each other's, and its value is 0: the output is what the many small
+    weights carry. Keys, values and queries lie on grids that fp16 holds, so that nothing is rounded but
+    weights, sums and the output, in chunks as well. Tolerance: half a step of the output; 2^-11 of each
+    weight, which acts on the value or on half its group's range, and 2^-12 of the same for what is in fp32;
+    and 2^-30 of the largest weight in each, where fp16 has no bits left. Few requests (a row in parts, of
+    which one holds the first token) and many (rows whole)."""
+    from vllm_ttkv import ops
+    lay, G = _lay(1, d, g), 2
+    rng = np.random.default_rng(ql)
+    nb = -(-n // 16)
+    cache, table = lay.new_cache(nb, 16), torch.from_numpy(rng.permutation(nb)).int()[None].cuda()
+    k, v = (rng.integers(-7, 9, (n, 1, d)) / 8.0 for _ in range(2))
+    for x in (k, v):                                     # every group's codes go from 0 to 15
+        x[:, :, ::g], x[:, :, 1::g] = -7 / 8, 1.0
+    v[1:, :, 2:] = np.abs(v[1:, :, 2:])
+    v[0] = 0.0
+    k[0] = np.where(np.arange(d) % 2, 1.0, -7 / 8)
+    t = torch.arange(n, device="cuda")
+    kt, vt = (torch.from_numpy(x).float().cuda() for x in (k, v))
+    ops.q4_write_paged(lay, cache, table[0].long()[t // 16] * 16 + t % 16, kt, vt)
+    K, V = (O.values(*O.quantise(x, g)) for x in (k, v))
+    assert np.array_equal(K, k) and np.array_equal(V, v)
+    q = torch.from_numpy(np.where(np.arange(d) % 2, 1.0, -1.0) * np.ones((ql, G, 1))).half().cuda()
+    s = (K[:, 0] @ q[0, 0].double().cpu().numpy())       # the first is the largest of all
+    scale = nats / (s[0] - np.median(s[1:]))
+    out = torch.empty(R * ql, G, d, device="cuda", dtype=torch.float16)
+    _prefill(lay, cache, table.expand(R, -1), [n] * R, [ql] * R, q.repeat(R, 1, 1), scale, out)
+    want = O.attend(_np(q), K, V, scale, G)
+    W = np.maximum(np.abs(V), np.where(np.arange(n) > 0, 7.5 / 8, 0.0)[:, None, None])
+    tol = 2.0 ** -11 * np.abs(want) + (2.0 ** -11 + 2.0 ** -12) * O.attend(_np(q), K, W, scale, G) + n * 2.0 ** -30
+    err = np.abs(_np(out).reshape(R, ql, G, d) - want)
+    assert np.all(err <= tol), (float((err / tol).max()), float((err / np.abs(want).max()).max()))

@@ -7,8 +7,11 @@
 // turn) over stored tiles of 128 tokens. Each stored tile is turned into fp16 operands once for both:
 // K^ = m + s c and V^, rounded once to fp16 (half a step, 2^-12 of an element; the codes as exact
 // operands with their scales applied to S and P would cost the softmax twice its instructions, and
-// with groups below d a product each). Scores, sums and O are fp32; P is fp16, at most 2^15: the
-// running maximum moves only when weights outgrow that (then O in tensor memory is rescaled).
+// with groups below d a product each). Scores, sums and O are fp32. P is fp16, of which the weights are
+// held in the upper part: the largest of a segment's first half is 2^8 and none passes 2^15, so they keep
+// 11 bits down to 2^-22 of it and vanish only below 2^-33 (2^-25 with a largest of 1, where the many small
+// weights beside a token that takes most were lost: 2.5e-3 of the output at 16384 tokens, 18 nats below it).
+// The running maximum moves only when a half's weights outgrow that (then O in tensor memory is rescaled).
 //
 // Roles: two softmax warpgroups (a thread owns a row, i.e. a lane of tensor memory), a warpgroup that
 // dequantises K and one for V, two warps that issue the products, one per row tile, and a warp that
@@ -54,6 +57,9 @@ constexpr int kRegsLaunch = 96, kRegsSoftmax = 128, kRegsOperands = 80, kRegsPro
 static_assert(2 * kRegsSoftmax + 2 * kRegsOperands + kRegsProducts <= 5 * kRegsLaunch, "register shares");
 constexpr uint32_t kTmemCols = 512;          // S of row tile 0 and 1, O of each, at 128 columns
 constexpr float kWeightMost = 32768.f;       // of a half's weights in all: each is a finite fp16
+constexpr float kWeightBits = 8.f;           // the largest weight when the maximum has been looked for, as a power of two:
+                                             // 64 such weights stay below that, so a flat row does not look again
+static_assert(TH * 256 <= 32768, "a half of the largest weights");
 constexpr int kFlags = 8;                    // tiles whose NaN values are remembered
 
 // Row tiles' tensor memory: S of a half in buffer y (then P in its first 32 columns) and O.
@@ -370,7 +376,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             fence_async_smem();
             mbar_arrive(&B.qfull[x]);
 
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f;                     // m: what scores are taken against, 8 below a maximum
             uint32_t bad = 0;                                 // groups of V that are NaN in a token that this row sees
             auto note_bad = [&](int i, uint32_t k) {          // tile i of the segment, k-th of the CTA: V consumed
                 const uint32_t f = k & (kFlags - 1);
@@ -406,7 +412,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                         for (int c = 0; c < 2; ++c)
                             #pragma unroll
                             for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], s[c][k]);
-                        const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * qf;
+                        const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * qf - kWeightBits;
                         float corr = 1.f;
                         if (mt > m) {                         // (m is -inf at first)
                             corr = m == -INFINITY ? 0.f : ex2(m - mt);
