@@ -174,3 +174,32 @@ def test_a_token_that_takes_most(d, g, R, ql, n, nats):
     tol = 2.0 ** -11 * np.abs(want) + (2.0 ** -11 + 2.0 ** -12) * O.attend(_np(q), K, W, scale, G) + n * 2.0 ** -30
     err = np.abs(_np(out).reshape(R, ql, G, d) - want)
     assert np.all(err <= tol), (float((err / tol).max()), float((err / np.abs(want).max()).max()))
+
+
+# ------------------------------------------------------------------ queries of no number
+@pytest.mark.parametrize("d,g", GEOMETRIES)
+@pytest.mark.parametrize("ql,G", [(1, 2), (5, 3), (140, 2)])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("scale", [0.1, -0.1])
+def test_an_infinite_query_is_nan(d, g, ql, G, sign, scale):
+    """Keys of one sign in the lane that the query is infinite in, and groups whose least value has that sign or
+    not: all the scores are then +inf or all -inf, and the formula's answer is NaN."""
+    from vllm_ttkv import ops
+    lay, n = _lay(1, d, g), ql + 70
+    rng = np.random.default_rng(ql)
+    cache, table = lay.new_cache(-(-n // 16), 16), torch.arange(-(-n // 16), dtype=torch.int32, device="cuda")[None]
+    k, v = (torch.from_numpy(rng.uniform(0.5, 2, (n, 1, d))).float().cuda() for _ in range(2))
+    ops.q4_write_paged(lay, cache, torch.arange(n, device="cuda"), k, v)
+    K, V = (O.values(*O.quantise(_np(x), g)) for x in (k, v))
+    q = torch.randn(ql, G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    q[ql // 2, 1, 7] = sign * float("inf")
+    out = torch.empty_like(q)
+    if ql == 1:
+        ops.q4_decode_paged(lay, cache, table, torch.tensor([n], dtype=torch.int32, device="cuda"), q, scale, out)
+    else:
+        _prefill(lay, cache, table, [n], [ql], q, scale, out)
+    assert bool(out[ql // 2, 1].isnan().all())
+    got, ref = _np(out), _np(q)
+    ref[ql // 2, 1] = 0.0
+    got[ql // 2, 1] = O.attend(ref, K, V, scale, G)[ql // 2, 1]
+    _check_rows(got, ref, K, V, scale, G, torch.float16, True)

@@ -368,9 +368,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     *place(i) = make_uint4(half2_bits(v[0] * up, v[4] * up), half2_bits(v[1] * up, v[5] * up),
                                            half2_bits(v[2] * up, v[6] * up), half2_bits(v[3] * up, v[7] * up));
                     const int e_row = __shfl_sync(0xffffffffu, e, (lane % RPI) * LPR);
+                    const float big_row = __shfl_sync(0xffffffffu, big, (lane % RPI) * LPR);
                     if (lane / RPI == i)                      // this lane's own row
-                        // (not 0, which would make NaN of a masked score of -inf)
-                        qf = fmaxf(fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e_row, 1)) << 23), 1e-38f);
+                        // (not 0, which would make NaN of a masked score of -inf. A row with an infinity is NaN, also
+                        // where its scores all come out as -inf, whose weights would be 0)
+                        qf = big_row == INFINITY ? __int_as_float(0x7fc00000)
+                                                 : fmaxf(fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e_row, 1)) << 23), 1e-38f);
                 }
             }
             fence_async_smem();

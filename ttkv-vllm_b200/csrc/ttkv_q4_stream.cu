@@ -142,7 +142,9 @@ struct WarpRows {
                 qf[nt][2 * w + 1][0] = half2_bits(x[w][2], x[w][6]);
                 qf[nt][2 * w + 1][1] = half2_bits(x[w][3] * 0.0625f, x[w][7] * 0.0625f);
             }
-            const float fac = P.scale * kLog2e * __uint_as_float(uint32_t(max(127 - e, 1)) << 23);
+            // a row with an infinity is NaN, also where its scores all come out as -inf (whose weights would be 0)
+            const float fac = big == INFINITY ? __int_as_float(0x7fc00000)
+                                              : P.scale * kLog2e * __uint_as_float(uint32_t(max(127 - e, 1)) << 23);
             const int seen = live ? rq.seq - rq.ql + j + 1 : 0;
             if (live) min_lim = min(min_lim, seen);
             #pragma unroll
