@@ -40,10 +40,13 @@ struct StoreParams {
 // within twice that of one half it is settled by the exact remainder x - m - c s: the difference's own
 // rounding error is known, and the remainder of a product of 15 bits is exact. Of 16-bit values one in
 // a few thousand lies exactly there.
-// Values beyond the limit need no clamp of their own: the ends of the group are clamped, and the
-// quotient as a fraction of 15 by its saturation. It is rounded by adding 1.5 2^23, which leaves the
-// integer in the low bits of the sum, where eight of them are packed by shifts and adds (the sum's
-// high bits, the same in every value, are taken off at the end).
+// Of values beyond the limit the ends of the group are clamped, and the quotient as a fraction of 15 by
+// its saturation. 16-bit values need no more: next to the limit they are fp16 numbers, so the minimum is
+// exact and the limit's own code 15. In fp32 the minimum may be rounded up, as far as the limit, which
+// then has a lower code: there the values are clamped too, where the group has such a one.
+// A quotient is rounded by adding 1.5 2^23, which leaves the integer in the low bits of the sum, where
+// eight of them are packed by shifts and adds (the sum's high bits, the same in every value, are taken
+// off at the end).
 __device__ __noinline__ uint32_t exact_scale(float lo, float hi) {
     // round to odd in fp32 first: its 13 extra bits then decide the fp16 rounding exactly
     const double e = __ddiv_rn(double(hi) - double(lo), 15.0);
@@ -120,8 +123,8 @@ __device__ __forceinline__ uint32_t codes8(const float (&x)[8], float m, float s
 }
 
 // Scale and minimum of a group whose G lanes hold x and y, and the codes of this lane's sixteen.
-template <int G>
-__device__ __forceinline__ uint2 quantise_group(const float (&x)[8], const float (&y)[8], uint32_t& meta) {
+template <int G, int DT>
+__device__ __forceinline__ uint2 quantise_group(float (&x)[8], float (&y)[8], uint32_t& meta) {
     float lo = min_nan(x[0], y[0]), hi = max_nan(x[0], y[0]);
     #pragma unroll
     for (int j = 1; j < 8; ++j) {
@@ -134,6 +137,13 @@ __device__ __forceinline__ uint2 quantise_group(const float (&x)[8], const float
         hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     const bool nan = !(fmaxf(-lo, hi) < INFINITY && lo == lo);  // a NaN or an infinity in the group
+    if (DT == TTKV_F32 && hi > kLimit) {
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[j] = fminf(x[j], kLimit);
+            y[j] = fminf(y[j], kLimit);
+        }
+    }
     lo = fminf(fmaxf(lo, -kLimit), kLimit);
     hi = fminf(fmaxf(hi, -kLimit), kLimit);
 
@@ -185,7 +195,7 @@ __global__ void __launch_bounds__(kStoreThreads, kWriteCtas) q4_write_kernel(con
     load8(src, DT, at, vec, x);
     load8(src, DT, at + 8, vec, y);
     uint32_t meta;
-    const uint2 c = quantise_group<G>(x, y, meta);
+    const uint2 c = quantise_group<G, DT>(x, y, meta);
     if (row >= P.n || !slot_ok(P, slot, i == 0 && h == 0 && blockIdx.z == 0)) return;
     int o;
     uint8_t* pan = panel_of(P, slot, h, panel_bytes(D, GRP), o);
