@@ -203,3 +203,21 @@ def test_an_infinite_query_is_nan(d, g, ql, G, sign, scale):
     ref[ql // 2, 1] = 0.0
     got[ql // 2, 1] = O.attend(ref, K, V, scale, G)[ql // 2, 1]
     _check_rows(got, ref, K, V, scale, G, torch.float16, True)
+
+
+def test_an_infinite_query_of_a_long_row_is_nan():
+    """As above, the row in parts of many CTAs, some of them behind what the row sees."""
+    lay, n, ql = _lay(1, 64, 64), 3000, 200
+    from vllm_ttkv import ops
+    rng = np.random.default_rng(1)
+    cache, table = lay.new_cache(-(-n // 16), 16), torch.arange(-(-n // 16), dtype=torch.int32, device="cuda")[None]
+    k, v = (torch.from_numpy(rng.uniform(0.5, 2, (n, 1, 64))).float().cuda() for _ in range(2))
+    ops.q4_write_paged(lay, cache, torch.arange(n, device="cuda"), k, v)
+    q = torch.randn(ql, 2, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+    q[11, 0, 7] = q[150, 1, 40] = -float("inf")
+    out = torch.empty_like(q)
+    _prefill(lay, cache, table, [n], [ql], q, 0.1, out)
+    want = torch.zeros(ql, 2, dtype=torch.bool)
+    want[11, 0] = want[150, 1] = True
+    nan = out.isnan().cpu()
+    assert torch.equal(nan.all(-1), want) and torch.equal(nan.any(-1), want)

@@ -368,12 +368,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     *place(i) = make_uint4(half2_bits(v[0] * up, v[4] * up), half2_bits(v[1] * up, v[5] * up),
                                            half2_bits(v[2] * up, v[6] * up), half2_bits(v[3] * up, v[7] * up));
                     const int e_row = __shfl_sync(0xffffffffu, e, (lane % RPI) * LPR);
-                    const float big_row = __shfl_sync(0xffffffffu, big, (lane % RPI) * LPR);
                     if (lane / RPI == i)                      // this lane's own row
-                        // (not 0, which would make NaN of a masked score of -inf. A row with an infinity is NaN, also
-                        // where its scores all come out as -inf, whose weights would be 0)
-                        qf = big_row == INFINITY ? __int_as_float(0x7fc00000)
-                                                 : fmaxf(fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e_row, 1)) << 23), 1e-38f);
+                        // (not 0, which would make NaN of a masked score of -inf)
+                        qf = fmaxf(fabsf(P.scale) * kLog2e * __uint_as_float(uint32_t(max(127 - e_row, 1)) << 23), 1e-38f);
                 }
             }
             fence_async_smem();
@@ -468,7 +465,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             // 32 output lanes at a time, through the warp's rows of Q (read by the last product) so that
             // neighbouring lanes of the warp write neighbouring bytes
             const int64_t pr = (int64_t(blockIdx.x) * 2 + (ca >= u0 ? 0 : 1)) * CROWS + x * TM + t;
-            const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+            // (a row that has queries sees a token; its weights add up to 0 only where its scores are all -inf, of a
+            // query with an infinity: 0 times 1 / 0 is the NaN that it should be)
+            const float inv = whole ? 1.f / l : 1.f;
             const int64_t dst = !live ? -1 : whole ? int64_t(rq.q0 + j) * P.out_stride + int64_t(h * P.G + g) * D : pr * D;
             uint4* stage = reinterpret_cast<uint4*>(qb + (w & 3) * 4096);
             #pragma unroll 1
@@ -828,7 +827,8 @@ __global__ void __launch_bounds__(kMergeRows / kMergeEach * (D / 4)) q4_chunk_me
     }
     #pragma unroll
     for (int k = 0; k < kMergeEach; ++k)
-        if (i0 + k * STEP < n_rows) store_out(P, rq, h, rb * CROWS + i0 + k * STEP, D, ln, o[k], l[k]);
+        if (i0 + k * STEP < n_rows)                           // (sums of 0 are NaN, as above)
+            store_out(P, rq, h, rb * CROWS + i0 + k * STEP, D, ln, o[k], l[k] == 0.f ? __int_as_float(0x7fc00000) : l[k]);
 }
 
 template <int D, int GRP>
