@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     }
                     if (i & 1) {
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&B.rempty[slot]);
+                        if (lane == 0 && !dead) mbar_arrive(&B.rempty[slot]);
                     }
                 }
                 fence_async_smem();
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                             make_uint4(out[q][0], out[q][1], out[q][2], out[q][3]);
                     if (D == 64 || (i & 1)) {
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&B.rempty[slot]);
+                        if (lane == 0 && !dead) mbar_arrive(&B.rempty[slot]);
                     }
                 }
                 fence_async_smem();
@@ -673,13 +673,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         const uint64_t DESC = sw128_desc(0, 16, 1024);
         const uint32_t aq = smem_u32(smem + S::off_q + x * S::Q) >> 4, ak = smem_u32(smem + S::off_k) >> 4, av = smem_u32(smem + S::off_v) >> 4;
         uint32_t n_tile = 0, n_s = 0, n_pv = 0, n_q = 0;      // stored tiles; halves scored; halves summed
+        uint32_t s_end = 0, pv_end = 0;                       // one behind the last that was issued
         // S of half `half` of the k-th tile of the CTA, into the buffer of its turn
         auto score = [&](uint32_t k, int half) {
             const int st = k & 1;
             if (half == 0) wait(&B.kfull[st], k >> 1);
             tc_after();
             const uint32_t ah = ak + ((st * S::K + half * TH * 128) >> 4);
-            if (one) {
+            if (one && !dead) {
                 #pragma unroll
                 for (int e = 0; e < D / 16; ++e) {
                     constexpr int A = S::KATOM;
@@ -688,6 +689,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 }
                 mma_commit(&B.sfull[x][n_s & 1]);
                 if (half) mma_commit(&B.kempty[st]);
+                s_end = n_s + 1;
             }
             __syncwarp();
             ++n_s;
@@ -720,13 +722,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 wait(&B.pfull[x][n_pv & 1], n_pv >> 1);
                 tc_after();
                 const uint32_t ah = av + ((st * S::V + half * S::VATOM) >> 4);
-                if (one) {
+                if (one && !dead) {
                     #pragma unroll
                     for (int e = 0; e < TH / 16; ++e)
                         mma_f16_ts(tm + o_col(x), tm + s_col(x, n_pv & 1) + 8 * e, DESC + (ah + 2 * e), ID_PV,
                                    (i > 0 || e > 0) ? 1u : 0u);
                     mma_commit(&B.pvdone[x][n_pv & 1]);
                     if (half) mma_commit(&B.vempty[st]);
+                    pv_end = n_pv + 1;
                 }
                 __syncwarp();
                 ++n_pv;
@@ -735,39 +738,47 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             sg.skip(P, n);
         }
         // every product has ended before the tensor memory is freed (their operands are read, too)
-        if (n_pv) mbar_wait(&B.pvdone[x][(n_pv - 1) & 1], ((n_pv - 1) >> 1) & 1u);
+        if (s_end) mbar_wait(&B.sfull[x][(s_end - 1) & 1], ((s_end - 1) >> 1) & 1u);
+        if (pv_end) mbar_wait(&B.pvdone[x][(pv_end - 1) & 1], ((pv_end - 1) >> 1) & 1u);
         } else if (w == 18) {
             // ========================================================== the stored panels, one each of lanes 0 to 7
-            uint32_t g = lane;                                // panels of the CTA
+            uint32_t g = lane, fills = 0;                     // panels of the CTA; how often place `lane` has been filled
             while (sg.u < sg.ue) {
                 const int n = sg.here(), first = sg.ui, seq = sg.rq.seq, h = sg.h, r = sg.r;
                 sg.skip(P, n);
                 int id = panels_of(P, r, h, first, seq, lane);
                 for (int it = 0; it < n; ++it, g += 8) {
+                    bool filled = false;
                     const int next = it + 1 < n ? panels_of(P, r, h, first + it + 1, seq, lane) : kNoPanel;
                     if (lane < 8) {
                         const uint32_t slot = g % RING;
                         wait_idle(&B.rempty[slot], g / RING + 1);
                         unsigned char* pan = smem + S::off_ring + slot * PANEL;
-                        if (id >= 0) {
-                            mbar_expect_tx(&B.rfull[slot], PANEL);
-                            bulk_g2s(pan, P.cache + int64_t(id) * PANEL, PANEL, &B.rfull[slot]);
-                        } else {
-                            if (id == kBadPanel) {            // NaN keys: so are the rows that see them
-                                report(P.status, TTKV_STATUS_BLOCK_RANGE);
-                                for (int k = 0; k < 2 * 16 * NG; ++k)
-                                    reinterpret_cast<uint32_t*>(pan + k_meta_offset(D))[k] = k < 16 * NG ? 0x7e00u : 0u;
-                                fence_async_smem();
+                        if (!dead) {                          // (a place that never came free is left as it is)
+                            filled = true;
+                            if (id >= 0) {
+                                mbar_expect_tx(&B.rfull[slot], PANEL);
+                                bulk_g2s(pan, P.cache + int64_t(id) * PANEL, PANEL, &B.rfull[slot]);
+                            } else {
+                                if (id == kBadPanel) {        // NaN keys: so are the rows that see them
+                                    report(P.status, TTKV_STATUS_BLOCK_RANGE);
+                                    for (int k = 0; k < 2 * 16 * NG; ++k)
+                                        reinterpret_cast<uint32_t*>(pan + k_meta_offset(D))[k] = k < 16 * NG ? 0x7e00u : 0u;
+                                    fence_async_smem();
+                                }
+                                mbar_arrive(&B.rfull[slot]);  // (behind the last token nothing is read but codes)
                             }
-                            mbar_arrive(&B.rfull[slot]);      // (behind the last token nothing is read but codes)
                         }
                     }
                     id = next;
-                    __syncwarp();                             // in step: no lane a tile ahead of another's place
+                    // (in step: no lane a tile ahead of another's place) place `lane` is the k-th of these eight
+                    const uint32_t k = (lane + RING - (g - lane) % RING) % RING, all = __ballot_sync(0xffffffffu, filled);
+                    fills += lane < RING && k < 8 && (all >> k & 1u);
                 }
             }
-            // every copy has landed: the operands' warps have waited for it, or the wait is made up for
-            if (lane < 8 && g >= 8 + uint32_t(lane)) mbar_wait(&B.rfull[(g - 8) % RING], ((g - 8) / RING) & 1u);
+            // every copy has landed: the operands' warps have waited for it, or where a wait ran out that is
+            // made up for. (One whose wait ran out gives no place back, so only a place's last copy can be out)
+            if (fills) mbar_wait(&B.rfull[lane], (fills - 1) & 1u);
         }
     }
     __syncwarp();
