@@ -421,8 +421,8 @@ int ttkv_q4_read(const ttkv_q4_store_args_t* args);
  * [0, n_rows) (TTKV_STATUS_QUERY). Rows of no request are left as they were. With max_q_len or n_rows 0
  * nothing is launched or checked on the device. `scale` is finite.
  *
- * Both: a request longer than its block-table row is refused (TTKV_STATUS_ROW_SHORT); a refused
- * request's rows are left as they were. Queries that see a block id outside the cache get NaN
+ * Both: a request longer than its block-table row is refused (TTKV_STATUS_ROW_SHORT), as is one of more
+ * than 2^31 - 256 tokens (TTKV_STATUS_SEQ_BOUND); a refused request's rows are left as they were. Queries that see a block id outside the cache get NaN
  * (TTKV_STATUS_BLOCK_RANGE). `workspace` is 16-byte aligned and used by one call at a time. */
 typedef struct ttkv_q4_attn_args {
     ttkv_q4_cache_t cache;

@@ -221,3 +221,31 @@ def test_an_infinite_query_of_a_long_row_is_nan():
     want[11, 0] = want[150, 1] = True
     nan = out.isnan().cpu()
     assert torch.equal(nan.all(-1), want) and torch.equal(nan.any(-1), want)
+
+
+def test_lengths_next_to_32_bits_are_refused():
+    """A row of 2048 blocks of 2^20 tokens: longer requests than a 32-bit position behind their last tile allows are
+    refused on the device, the others served."""
+    from vllm_ttkv import ops
+    lay, bs = _lay(1, 64, 64), 2 ** 20
+    cache = lay.new_cache(1, bs)
+    table = torch.zeros(3, 2048, dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(40, 1, 64, generator=torch.Generator().manual_seed(i)).cuda() for i in range(2))
+    ops.q4_write_paged(lay, cache, torch.arange(40, device="cuda"), k, v)
+    K, V = (O.values(*O.quantise(_np(x), 64)) for x in (k, v))
+    for n in (2 ** 31 - 255, 2 ** 31 - 60, 2 ** 31 - 1):
+        for ql, G in ((1, 2), (2, 4), (100, 4)):
+            q = torch.randn(3 * ql, G, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+            out = torch.full_like(q, 5.0)
+            seqs = [40, n, 40]
+            ops.reset_status()
+            if ql == 1:
+                ops.q4_decode_paged(lay, cache, table, torch.tensor(seqs, dtype=torch.int32, device="cuda"), q, 0.1, out)
+            else:
+                _prefill(lay, cache, table, seqs, [min(ql, 40), ql, min(ql, 40)], q, 0.1, out, max_q=ql)
+            with pytest.raises(RuntimeError, match="seq_len"):
+                ops.check_status()
+            m = min(ql, 40)
+            assert bool((out[m:m + ql] == 5).all())
+            for a in (0, m + ql):
+                _check_rows(_np(out[a:a + m]), _np(q[a:a + m]), K, V, 0.1, G, torch.float16, True)

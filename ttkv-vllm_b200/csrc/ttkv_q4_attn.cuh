@@ -12,6 +12,7 @@ namespace q4 {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxCtas = 148;               // one CTA per SM of a B200; workspaces are sized for it
+constexpr int kMaxSeq = 0x7fffff00;         // a tile behind the last token still has a 32-bit position
 
 struct AttnParams {
     const uint8_t* cache;

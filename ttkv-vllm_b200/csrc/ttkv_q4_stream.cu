@@ -983,7 +983,7 @@ extern "C" int ttkv_q4_decode(const ttkv_q4_attn_args_t* args) {
     AttnParams P = attn_params(args);
     P.n_rows = args->n_reqs;
     P.max_q = 1;
-    P.max_seq = INT32_MAX;
+    P.max_seq = kMaxSeq;
     return run_stream(&args->cache, P, args->workspace, args->workspace_bytes, static_cast<cudaStream_t>(args->stream));
 }
 
@@ -1003,7 +1003,7 @@ extern "C" int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args) {
         return fail(TTKV_ERR_UNSUPPORTED, "4-bit prefill: %d queries of %d heads", args->max_q_len, args->HQ);
     AttnParams P = attn_params(args);
     P.q_start = args->q_start; P.q_len = args->q_len; P.n_rows = args->n_rows; P.max_q = args->max_q_len;
-    P.max_seq = args->max_seq_len;
+    P.max_seq = std::min(args->max_seq_len, kMaxSeq);
     const cudaStream_t st = static_cast<cudaStream_t>(args->stream);
     return streams(int64_t(args->max_q_len) * P.G, int64_t(args->n_reqs) * P.H, P.max_seq)
         ? run_stream(&args->cache, P, args->workspace, args->workspace_bytes, st)
