@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from oracle import q4 as O
-from test_gpu_q4 import GEOMETRIES, _check_rows, _filled, _lay, _np, _prefill
+from q4_bounds import bound, worst
+from test_gpu_q4 import DT, GEOMETRIES, _check_rows, _filled, _lay, _np, _prefill
 
 pytestmark = pytest.mark.gpu
 
@@ -249,3 +250,65 @@ def test_lengths_next_to_32_bits_are_refused():
             assert bool((out[m:m + ql] == 5).all())
             for a in (0, m + ql):
                 _check_rows(_np(out[a:a + m]), _np(q[a:a + m]), K, V, 0.1, G, torch.float16, True)
+
+
+# ------------------------------------------------------------------ chunks, tile by tile
+def _check_tight(out, q, K, V, scale, G, lay, chunk):
+    w = worst(_np(out), *bound(_np(q), K, V, scale, G, torch.finfo(out.dtype).eps / 2, lay.group, chunk))
+    assert w <= 1, w
+
+
+@pytest.mark.parametrize("d,g", GEOMETRIES)
+@pytest.mark.parametrize("H,HQ,dtype,bs", [(1, 1, "fp16", 16), (2, 6, "bf16", 16), (1, 13, "fp16", 64), (2, 16, "fp16", 32)])
+@pytest.mark.parametrize("qls", [(100, 127, 128, 129), (300, 0, 33, 65), (1, 257, 2, 90)])
+def test_chunks(d, g, H, HQ, dtype, bs, qls):
+    """Every query is as exact as its operands allow: a stored tile that is lost or stale, or a limit that is off
+    by a token, would show (`test_q4_bounds.py`)."""
+    lay = _lay(H, d, g)
+    seqs = [n + extra if n else 0 for n, extra in zip(qls, (0, 130, 5, 333))]
+    cache, table, K, V = _filled(lay, seqs, bs, seed=HQ + d)
+    q = torch.randn(sum(qls), HQ, d, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
+    out = torch.full_like(q, 5.0)
+    starts = _prefill(lay, cache, table, seqs, qls, q, d ** -0.5, out)
+    for r, (a, n) in enumerate(zip(starts, qls)):
+        if n:
+            _check_tight(out[a:a + n], q[a:a + n], K[r], V[r], d ** -0.5, HQ // H, lay, True)
+
+
+@pytest.mark.parametrize("d,g", GEOMETRIES)
+@pytest.mark.parametrize("scale", [0.05, 0.2])
+def test_chunks_of_many_tiles(d, g, scale):
+    """Some 40 stored tiles a CTA, many times round the ring of panels and the operands' stages."""
+    lay, R, ql, n, G = _lay(1, d, g), 64, 64, 6000, 8
+    cache, table, K, V = _filled(lay, [n], 16, seed=d + g)
+    q = torch.randn(R * ql, G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    starts = _prefill(lay, cache, table.expand(R, -1), [n - 3 * r for r in range(R)], [ql] * R, q, scale, out)
+    for r in (0, 11, 23, 38, 47, 63):
+        a, m = starts[r], n - 3 * r
+        _check_tight(out[a:a + ql], q[a:a + ql], K[0][:m], V[0][:m], scale, G, lay, True)
+
+
+@pytest.mark.parametrize("H,HQ,ql,n", [(1, 2, 200, 5000), (2, 8, 40, 3001), (1, 16, 9, 9000), (1, 5, 700, 2100)])
+def test_chunks_in_parts(H, HQ, ql, n):
+    lay = _lay(H, 128, 128)
+    cache, table, K, V = _filled(lay, [n], 16, seed=ql)
+    q = torch.randn(ql, HQ, 128, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    _prefill(lay, cache, table, [n], [ql], q, 0.08, out)
+    _check_tight(out, q, K[0], V[0], 0.08, HQ // H, lay, True)
+
+
+@pytest.mark.parametrize("d,g", GEOMETRIES)
+@pytest.mark.parametrize("R,H,G,ql,n", [(5, 2, 3, 1, 1031), (40, 1, 4, 4, 300), (7, 2, 4, 6, 2000), (3, 1, 8, 3, 700), (1, 1, 5, 4, 9000)])
+def test_few_rows(d, g, R, H, G, ql, n):
+    """At most 24 rows of a KV head: streamed, with keys and values as they are stored."""
+    lay = _lay(H, d, g)
+    seqs = [ql + int(x) for x in np.random.default_rng(R).integers(0, n, R)]
+    seqs[0] = n
+    cache, table, K, V = _filled(lay, seqs, 16, seed=R)
+    q = torch.randn(R * ql, G * H, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    starts = _prefill(lay, cache, table, seqs, [ql] * R, q, d ** -0.5, out)
+    for r, a in enumerate(starts):
+        _check_tight(out[a:a + ql], q[a:a + ql], K[r], V[r], d ** -0.5, G, lay, False)
