@@ -312,3 +312,19 @@ def test_few_rows(d, g, R, H, G, ql, n):
     starts = _prefill(lay, cache, table, seqs, [ql] * R, q, d ** -0.5, out)
     for r, a in enumerate(starts):
         _check_tight(out[a:a + ql], q[a:a + ql], K[r], V[r], d ** -0.5, G, lay, False)
+
+
+@pytest.mark.parametrize("d,g", [(128, 32), (128, 128)])
+@pytest.mark.parametrize("ql,G", [(7, 4), (8, 4), (3, 11)])
+def test_rows_next_to_the_choice_of_kernel(d, g, ql, G):
+    """25 to 33 rows of a KV head over long rows, which go to one kernel or the other by the groups."""
+    lay, R = _lay(1, d, g), 40
+    seqs = [1400 + 7 * r for r in range(R)]
+    cache, table, K, V = _filled(lay, [max(seqs)], 16, seed=R)
+    q = torch.randn(R * ql, G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    out = torch.empty_like(q)
+    starts = _prefill(lay, cache, table.expand(R, -1), seqs, [ql] * R, q, d ** -0.5, out)
+    for r in range(0, R, 9):
+        a, m = starts[r], seqs[r]
+        streamed = g > 32 and ql * G <= 32
+        _check_tight(out[a:a + ql], q[a:a + ql], K[0][:m], V[0][:m], d ** -0.5, G, lay, not streamed)

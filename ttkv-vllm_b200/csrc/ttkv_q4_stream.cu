@@ -952,20 +952,26 @@ AttnParams attn_params(const ttkv_q4_attn_args_t* a) {
 }
 
 // Whether chunks of `rows` (query, head) rows a KV head are streamed, the cache read and its codes fed to
-// the tensor cores once per 16 rows, or go to the chunk kernel, whose tiles of 256 rows each dequantise
-// the cache once. Streamed against chunked, d = 128 in groups of 128, 8 KV heads, us:
+// the tensor cores once per 16 rows (8 in groups of 32 at d = 128, `narrow`), or go to the chunk kernel,
+// whose tiles of 256 rows each dequantise the cache once. Streamed against chunked, d = 128 in groups of 128,
+// 8 KV heads, us:
 //   requests x tokens   16 rows      24           32           48           64
-//   64 x 130            56 / 73      73 / 77      87 / 77      126 / 77     155 / 79
-//   16 x 500            32 / 36      36 / 36      42 / 34      52 / 36      65 / 34
-//   64 x 1500           93 / 196     132 / 202    161 / 191    228 / 200    292 / 198
-//   64 x 6000           192 / 525    302 / 548    349 / 519    503 / 540    658 / 542
-//   4 x 3000            28 / 48      30 / 52      36 / 50      40 / 52      50 / 50
-//   1 x 130             20 / 26      17 / 28      20 / 28      20 / 28      22 / 28
-//   1 x 16000           30 / 73      32 / 87      36 / 85      42 / 87      46 / 85
-// So up to 24 rows always, up to 32 over long rows, up to 64 where few (request, head) pairs leave most of
-// the chunk kernel's time to latency.
-bool streams(int64_t rows, int64_t pairs, int max_seq) {
-    return rows <= 24 || (rows <= 32 && max_seq >= 1536) || (rows <= 64 && pairs <= 32);
+//   64 x 130            56 / 73      73 / 77      91 / 77      128 / 77     159 / 79
+//   16 x 500            32 / 36      36 / 36      42 / 34      52 / 36      67 / 36
+//   64 x 1500           96 / 206     136 / 216    169 / 200    241 / 208    310 / 204
+//   64 x 6000           202 / 550    316 / 579    370 / 531    531 / 552    693 / 548
+//   4 x 3000            28 / 50      30 / 54      34 / 50      40 / 54      50 / 50
+//   1 x 130             19 / 26      17 / 28      19 / 28      22 / 28      22 / 28
+//   1 x 16000           30 / 77      32 / 87      38 / 85      42 / 89      46 / 87
+// and in groups of 32:
+//   64 x 1500           128 / 206    177 / 216    232 / 202    331 / 210    447 / 204
+//   64 x 6000           318 / 544    466 / 566    607 / 533    896 / 556    1183 / 560
+//   4 x 3000            30 / 50      34 / 54      44 / 50      52 / 54      62 / 52
+// (d = 64 as the first, with 325 / 423 and 286 / 421 at 64 x 6000 and 32 rows). So up to 24 rows always, up to
+// 32 over long rows unless narrow, up to 64 where few (request, head) pairs leave most of the chunk kernel's time
+// to latency. Many short requests of 17 to 24 rows are the worst of it (64 x 130: up to 18 percent).
+bool streams(int64_t rows, int64_t pairs, int max_seq, bool narrow) {
+    return rows <= 24 || (rows <= 32 && max_seq >= 1536 && !narrow) || (rows <= 64 && pairs <= 32);
 }
 
 }  // namespace
@@ -990,7 +996,7 @@ extern "C" int ttkv_q4_decode(const ttkv_q4_attn_args_t* args) {
 extern "C" size_t ttkv_q4_prefill_workspace_bytes(int32_t d, int32_t n_reqs, int32_t group_heads, int32_t max_q_len) {
     if (n_reqs < 0 || max_q_len < 0) return 0;
     const int64_t rows = int64_t(max_q_len) * group_heads;
-    const bool some = streams(rows, 0, INT32_MAX), all = streams(rows, INT64_MAX, 0);     // are streamed
+    const bool some = streams(rows, 0, INT32_MAX, false), all = streams(rows, INT64_MAX, 0, true);    // are streamed
     return std::max(some ? stream_ws(d, rows > 8 ? 2 : 1).bytes : 0, all ? 0 : chunk_workspace_bytes(d));
 }
 
@@ -1005,7 +1011,8 @@ extern "C" int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args) {
     P.q_start = args->q_start; P.q_len = args->q_len; P.n_rows = args->n_rows; P.max_q = args->max_q_len;
     P.max_seq = std::min(args->max_seq_len, kMaxSeq);
     const cudaStream_t st = static_cast<cudaStream_t>(args->stream);
-    return streams(int64_t(args->max_q_len) * P.G, int64_t(args->n_reqs) * P.H, P.max_seq)
+    const bool narrow = args->cache.d == 128 && args->cache.group == 32;
+    return streams(int64_t(args->max_q_len) * P.G, int64_t(args->n_reqs) * P.H, P.max_seq, narrow)
         ? run_stream(&args->cache, P, args->workspace, args->workspace_bytes, st)
         : run_chunk(&args->cache, P, args->workspace, args->workspace_bytes, st);
 }
