@@ -457,8 +457,10 @@ int ttkv_q4_prefill(const ttkv_q4_attn_args_t* args);
  * written, -1 and 0 for tokens of no request. *free_count_out = blocks left (may be free_count).
  * Requests are served in order until the list runs out: that one and every later one that needs a
  * block get none (TTKV_STATUS_POOL_EMPTY). A refused request (that, a row too short:
- * TTKV_STATUS_ROW_SHORT, new > len or tokens outside n_tokens: TTKV_STATUS_QUERY) gets slots -1, and
- * where its row has room the entry behind its held blocks becomes -1, so a read of it is refused too.
+ * TTKV_STATUS_ROW_SHORT, new > len or tokens outside n_tokens: TTKV_STATUS_QUERY) gets slots -1, and the
+ * entries of its row behind its held blocks become -1, as many as its len needs (one at least, where the
+ * row has room; the first alone where new > len), so that a read of it is refused too, and a later step
+ * that counts it as served finds no other request's blocks there.
  *
  * ttkv_release_blocks: pushes the ceil(lens[r] / block_size) blocks of each request's row onto the
  * free list, in request order (lens[r] <= 0: none). capacity = the entries free_blocks has room for;

@@ -82,8 +82,8 @@ def plan(table, seq, qsl, free, count, block_size, n_tokens):
             bad = dry = True
         if bad:
             refused.append(r)
-            if held < table.shape[1]:
-                table[r, held] = -1
+            end = 1 if new > n else max(want, held + 1)
+            table[r, held:end] = -1
             continue
         for i in range(held, want):
             table[r, i] = free.pop()

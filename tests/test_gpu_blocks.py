@@ -227,7 +227,7 @@ def test_a_refused_request_is_released():
     ops.plan_step(table, _i32([33, 47, 0]), _i32([0, 1, 41, 41]), free, count, 16, slots)     # 1 block, then 2 of 1
     with pytest.raises(RuntimeError):
         ops.check_status()
-    assert table.cpu().tolist()[:2] == [[3, 4, 8, -7], [5, -1, 1, 2]] and int(count) == 1
+    assert table.cpu().tolist()[:2] == [[3, 4, 8, -7], [5, -1, -1, 2]] and int(count) == 1
     ops.release_blocks(table, _i32([0, 47, 0]), free, count, 16)
     with pytest.raises(IndexError):
         ops.check_status()
@@ -275,3 +275,42 @@ def test_release_captured():
                 ops.check_status()
         else:
             ops.check_status()
+
+
+def test_a_step_after_a_refusal_meets_no_other_blocks():
+    """A request that was refused and whose next steps count its tokens as stored: its row holds ids that another
+    request left there, and no token of it gets a slot in them."""
+    from vllm_ttkv import ops
+    bs, left = 16, [7, 6, 5, 4, 3, 2]                    # another request's blocks by now
+    for first, new in ((20, 60), (1, 90), (16, 17)):
+        table = _i32([[9] + left[1:]])
+        if first > bs:
+            table[0, 1] = 8
+        free, count, slots = _i32([1, 0]), _i32([1]), torch.zeros(96, dtype=torch.int64, device="cuda")
+        ops.reset_status()
+        ops.plan_step(table, _i32([first + new]), _i32([0, new]), free, count, bs, slots)
+        with pytest.raises(RuntimeError):
+            ops.check_status()
+        assert bool((slots == -1).all()) and int(count) == 1
+        n = first + new
+        while n < 96:
+            n += 1
+            ops.plan_step(table, _i32([n]), _i32([0, 1]), free, count, bs, slots[:1])
+            if int(slots[0]) >= 0:                       # a block of its own, taken for this token or one before
+                assert int(slots[0]) // bs == 1
+        ops.reset_status()
+
+
+def test_refused_rows_against_the_oracle():
+    from vllm_ttkv import ops
+    rng = np.random.default_rng(5)
+    for _ in range(20):
+        table, seq, qsl, free, count = _batch(rng, 60, 40, 300, 16, 20, -int(rng.integers(1, 60)))
+        table = table[:, :int(rng.integers(15, 21))]
+        T = int(qsl[-1]) - int(rng.integers(0, 3)) * 7
+        want = O.plan(table, seq, qsl, free, count, 16, T)
+        ops.reset_status()
+        got = _run(table, seq, qsl, free, count, 16, T)
+        with pytest.raises(RuntimeError):
+            ops.check_status()
+        assert all(np.array_equal(a, b) for a, b in zip(got[:3], want[:3])) and got[3] == want[3]

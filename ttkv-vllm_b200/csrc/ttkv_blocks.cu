@@ -150,11 +150,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanParam
     const int used = assign_ranges<false>(P, count, M, wsum, &taken, lacking);
     if (lacking && at == 0) report(P.status, TTKV_STATUS_POOL_EMPTY);
 
-    // a refused request's row: no block behind those that it holds
+    // a refused request's row: no block behind those that it holds, as far as it would have reached, so that
+    // a later step that takes them for its own does not meet what another request left there
     for (int r = at; r < P.n_reqs; r += step) {
         if (M.len[r] >= 0) continue;
-        const int held = blocks_of(~M.len[r] - max(M.start[r + 1] - M.start[r], 0), P.block_size);
-        if (held < P.bt_cols) P.block_table[int64_t(r) * P.bt_stride + held] = -1;
+        const int seq = ~M.len[r], fresh = max(M.start[r + 1] - M.start[r], 0), held = blocks_of(seq - fresh, P.block_size);
+        const int end = fresh > seq ? 1 : min(max(blocks_of(seq, P.block_size), held + 1), P.bt_cols);
+        for (int i = held; i < min(end, P.bt_cols); ++i) P.block_table[int64_t(r) * P.bt_stride + i] = -1;
     }
     // the blocks taken, into their rows
     for (unsigned i = at; i < unsigned(used); i += step) {

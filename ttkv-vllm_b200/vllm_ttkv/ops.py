@@ -469,7 +469,7 @@ def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc
     -1 and 0 behind the last request's (the padding of a captured size, which `q4_write_paged` and
     `write_paged` skip with skip_pad). The blocks left go to `free_count_out` (default: free_count).
     A request that is refused (the list is empty, its row is short, its lengths disagree) has slots -1
-    and, behind the blocks it holds, a block id -1, which the reads refuse; see `check_status`."""
+    and, in place of the blocks it lacks, block ids -1, which the reads refuse; see `check_status`."""
     code = _lib.torch_binding().plan(block_table, seq_lens, free_blocks, free_count,
                                      free_count if free_count_out is None else free_count_out, block_size,
                                      _status_of(block_table, status), query_start_loc, slot_mapping, positions)
