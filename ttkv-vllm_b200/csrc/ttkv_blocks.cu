@@ -194,7 +194,7 @@ __device__ bool push_ids(const PlanParams& P, const PlanSmem& M, int count, int 
     for (unsigned i = at; i < unsigned(used); i += step) {
         const int e = int(i);
         const int r = find(M.end, P.n_reqs, e);
-        const int32_t id = __ldg(P.block_table + int64_t(r) * P.bt_stride + (e - (r ? M.end[r - 1] : 0)));
+        const int32_t id = P.block_table[int64_t(r) * P.bt_stride + (e - (r ? M.end[r - 1] : 0))];
         bad |= id < 0;
         P.free_blocks[count + e] = id;
     }

@@ -36,15 +36,17 @@ inline int check_cache(const ttkv_q4_cache_t* c) {
 static __device__ __noinline__ uint4 load_bytes16(const uint16_t* p) {
     uint32_t w[4];
     #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = uint32_t(__ldg(p + 2 * j)) | (uint32_t(__ldg(p + 2 * j + 1)) << 16);
+    for (int j = 0; j < 4; ++j) w[j] = uint32_t(p[2 * j]) | (uint32_t(p[2 * j + 1]) << 16);
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// (Ordinary loads, here as in the other kernels that start while the one before them runs: what that one
+// writes is not constant for this kernel's whole life, which the read-only path supposes.)
 // Eight consecutive elements from element index i of p (fp32, fp16 or bf16). vec: p + i is 16-byte aligned.
 __device__ __forceinline__ void load8(const void* p, int dtype, int64_t i, bool vec, float (&x)[8]) {
     auto load = [&](int64_t byte) {
         const uint8_t* b = static_cast<const uint8_t*>(p) + byte;
-        return vec ? __ldg(reinterpret_cast<const uint4*>(b)) : load_bytes16(reinterpret_cast<const uint16_t*>(b));
+        return vec ? *reinterpret_cast<const uint4*>(b) : load_bytes16(reinterpret_cast<const uint16_t*>(b));
     };
     if (dtype == TTKV_F32) {
         const uint4 a = load(4 * i), b = load(4 * i + 16);

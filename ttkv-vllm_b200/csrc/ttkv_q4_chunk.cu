@@ -169,7 +169,7 @@ __device__ __forceinline__ int panels_of(const AttnParams& P, int r, int h, int 
     const int t = tile * TN + 16 * lane;
     if (lane >= 8 || t >= seq) return kNoPanel;
     const int bi = t / P.block_size;
-    const int blk = __ldg(P.block_table + int64_t(r) * P.bt_stride + bi);
+    const int blk = P.block_table[int64_t(r) * P.bt_stride + bi];
     if (blk < 0 || blk >= P.n_blocks) return kBadPanel;
     // (an index of panels: the memory of a GPU holds fewer than 2^31)
     return int((int64_t(blk) * P.H + h) * (P.block_size / kPanelTokens)) + (t - bi * P.block_size) / kPanelTokens;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     #pragma unroll
                     for (int i = 0; i < LPR; ++i) {
                         const int64_t from = __shfl_sync(0xffffffffu, src, i * RPI + lane / LPR);
-                        raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) + max(from, int64_t(0)) + 8 * c));
+                        raw[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) + max(from, int64_t(0)) + 8 * c);
                     }
                     #pragma unroll
                     for (int i = 0; i < LPR; ++i) *place(i) = raw[i];

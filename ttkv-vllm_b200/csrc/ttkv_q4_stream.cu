@@ -101,7 +101,7 @@ struct WarpRows {
             uint4 raw[NW];
             if (P.q_vec) {
                 #pragma unroll
-                for (int w = 0; w < NW; ++w) raw[w] = __ldg(reinterpret_cast<const uint4*>(src + 32 * w));
+                for (int w = 0; w < NW; ++w) raw[w] = *reinterpret_cast<const uint4*>(src + 32 * w);
             } else {
                 #pragma unroll
                 for (int w = 0; w < NW; ++w) {
