@@ -328,3 +328,51 @@ def test_rows_next_to_the_choice_of_kernel(d, g, ql, G):
         a, m = starts[r], seqs[r]
         streamed = g > 32 and ql * G <= 32
         _check_tight(out[a:a + ql], q[a:a + ql], K[0][:m], V[0][:m], d ** -0.5, G, lay, not streamed)
+
+
+# ------------------------------------------------------------------ calls one behind the other
+def test_a_chain_of_calls_without_a_pause():
+    """Plan, write, read back, attend and release, each of which may start while the one before it runs: the same
+    bits as with the device waited for after every call."""
+    from vllm_ttkv import ops
+    lay, bs, R, HQ, T = _lay(2, 64, 32), 16, 24, 8, 24 * 40
+    rng = np.random.default_rng(3)
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+    steps, lens = [], np.zeros(R, np.int64)
+    for step in range(30):
+        done = (rng.uniform(size=R) < 0.15) & (lens > 0)
+        gone = np.where(done, lens, 0)
+        lens = np.where(done, 0, lens)
+        new = np.where(lens == 0, rng.integers(1, 41, R), 1 if step % 3 else rng.integers(1, 9, R))
+        lens = lens + new
+        kv = [torch.from_numpy(rng.standard_normal((T, 2, 64))).half().cuda() for _ in range(2)]
+        steps.append((i32(gone), i32(lens), i32(np.concatenate([[0], np.cumsum(new)])), i32(np.cumsum(new) - new), i32(new),
+                      *kv, torch.from_numpy(rng.standard_normal((T, HQ, 64))).half().cuda(), int(new.max()), int(lens.max())))
+
+    def run(pause):
+        cache = lay.new_cache(400, bs)
+        table = torch.full((R, 30), -1, dtype=torch.int32, device="cuda")
+        free, count = torch.arange(400, dtype=torch.int32, device="cuda"), i32([400])
+        slots, pos = (torch.zeros(T, dtype=torch.int64, device="cuda") for _ in range(2))
+        outs = []
+        torch.cuda.synchronize()
+        for gone, ln, qsl, qs, ql, k, v, q, max_q, max_n in steps:
+            out, dec, ko, vo = (torch.zeros_like(x) for x in (q, q[:R], k, v))
+            for call in (lambda: ops.release_blocks(table, gone, free, count, bs),
+                         lambda: ops.plan_step(table, ln, qsl, free, count, bs, slots, positions=pos),
+                         lambda: ops.q4_write_paged(lay, cache, slots, k, v, skip_pad=True),
+                         lambda: ops.q4_read_paged(lay, cache, slots, ko, vo, skip_pad=True),
+                         lambda: ops.q4_write_paged(lay, cache, slots, ko, vo, skip_pad=True),
+                         lambda: ops.q4_prefill_paged(lay, cache, table, ln, qs, ql, q, 0.125, out, max_q, max_n),
+                         lambda: ops.q4_decode_paged(lay, cache, table, ln, out[:R], 0.125, dec)):
+                call()
+                if pause:
+                    torch.cuda.synchronize()
+            outs += [out, dec, ko, vo, slots.clone(), table.clone(), free[:10].clone()]
+        ops.check_status()
+        return outs
+
+    ops.reset_status()
+    want = run(True)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(run(False), want))
