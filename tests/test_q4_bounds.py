@@ -2,6 +2,7 @@
 lies outside, one with the kernel's roundings inside. Mistakes and roundings are made in the oracle."""
 import numpy as np
 import pytest
+import torch
 
 from oracle import q4 as O
 from q4_bounds import bound, rounded, worst
@@ -33,13 +34,20 @@ def _case(d, g, n, nq, dtype):
 SHAPES = [(64, 32, 1000, 150, 0.125), (128, 128, 5000, 40, 0.08), (128, 64, 6000, 64, 0.05), (64, 64, 300, 130, 0.125)]
 
 
+def _type(x, dtype):
+    """A result in its type, as 64 bits."""
+    return torch.from_numpy(x).to({"bf16": torch.bfloat16, "fp16": torch.float16}[dtype]).double().numpy()
+
+
 @pytest.mark.parametrize("d,g,n,nq,scale", SHAPES)
-def test_the_kernels_roundings_lie_within(d, g, n, nq, scale):
-    q, K, V, eps = _case(d, g, n, nq, "fp16")
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_the_kernels_roundings_lie_within(d, g, n, nq, scale, dtype):
+    q, K, V, eps = _case(d, g, n, nq, dtype)
     want, tol = bound(q, K, V, scale, 2, eps, g, True)
-    got = _attend(q, rounded(K), rounded(V), scale, 2, weights=lambda p: rounded(p * 256) / 256).astype(np.float16)
+    k = rounded(K) + (rounded(K - rounded(K)) if dtype == "fp16" else 0)
+    got = _type(_attend(q, k, rounded(V), scale, 2, weights=lambda p: rounded(p * 256) / 256), dtype)
     assert worst(got, want, tol) <= 1
-    got = _attend(q, K, V, scale, 2).astype(np.float16)
+    got = _type(_attend(q, K, V, scale, 2), dtype)
     assert worst(got, *bound(q, K, V, scale, 2, eps, g, False)) <= 1
 
 
@@ -48,17 +56,15 @@ def test_the_kernels_roundings_lie_within(d, g, n, nq, scale):
 def test_mistakes_lie_outside(d, g, n, nq, scale, mistake):
     q, K, V, eps = _case(d, g, n, nq, "fp16")
     want, tol = bound(q, K, V, scale, 2, eps, g, True)
-    K, V, late = rounded(K), rounded(V), 0
+    V, late = rounded(V), 0
     if mistake == "tile lost":
         V = np.delete(V, np.s_[64:192], 0)
         K = np.delete(K, np.s_[64:192], 0)
     elif mistake == "stale values":
-        V = V.copy()
         V[128:256] = V[0:128]
     elif mistake == "a panel's values zero":
-        V = V.copy()
         V[n // 2 // 16 * 16:][:16] = 0
     else:
         late = 1 if mistake == "own token hidden" else -1
-    got = _attend(q, K, V, scale, 2, late).astype(np.float16)
+    got = _type(_attend(q, K, V, scale, 2, late), "fp16")
     assert worst(got, want, tol) > 1

@@ -5,12 +5,18 @@
 // A chunk has many (query, head) rows per stored token, so products bound it, not memory: a CTA takes
 // 256 rows of one KV head (two tiles of 128, the M of an MMA, whose products and softmaxes run in
 // turn) over stored tiles of 128 tokens. Each stored tile is turned into fp16 operands once for both:
-// K^ = m + s c and V^, rounded once to fp16 (half a step, 2^-12 of an element; the codes as exact
-// operands with their scales applied to S and P would cost the softmax twice its instructions, and
-// with groups below d a product each). Scores, sums and O are fp32. P is fp16, of which the weights are
+// K^ = m + s c and V^, rounded once to fp16 (the codes as exact operands with their scales applied to S
+// and P would cost the softmax twice its instructions, and with groups below d a product each). V^ is off
+// by 2^-11 of an element at most, as is each weight, which is what fp16 outputs are off by themselves.
+// Rounded keys put 2^-11 of sum |q_i K_i| on a score at most, which grows with the keys and not with their
+// spread: 4e-4 to 1e-3 of the output with a few large channels, 2e-3 where channels have offsets of three
+// times their spread, against the 1.7e-3 that bf16 outputs are off by themselves and the 2.1e-4 of fp16.
+// So for fp16 queries (FINE) a key is the sum of two fp16, its rounding and what that leaves, with a product
+// each: 3.2e-4 in all; the chunks below take 286 and 802 us for 253 and 695. (V as a sum of two as well
+// gives 2.7e-4 and takes 353 and 1001.) Scores, sums and O are fp32. P is fp16, of which the weights are
 // held in the upper part: the largest of a segment's first half is 2^8 and none passes 2^15, so they keep
-// 11 bits down to 2^-22 of it and vanish only below 2^-33 (2^-25 with a largest of 1, where the many small
-// weights beside a token that takes most were lost: 2.5e-3 of the output at 16384 tokens, 18 nats below it).
+// 11 bits down to 2^-22 of it and vanish only below 2^-33 (2^-25 with a largest of 1, which lost half of what
+// 16383 tokens weigh together, each 18 nats below the first).
 // The running maximum moves only when a half's weights outgrow that (then O in tensor memory is rescaled).
 //
 // Roles: two softmax warpgroups (a thread owns a row, i.e. a lane of tensor memory), a warpgroup that
@@ -66,8 +72,9 @@ constexpr int kFlags = 8;                    // tiles whose NaN values are remem
 __device__ __forceinline__ uint32_t s_col(int x, uint32_t y) { return 128u * x + 64u * y; }
 __device__ __forceinline__ uint32_t o_col(int x) { return 256u + 128u * x; }
 
-template <int D, int GRP>
+template <int D, int GRP, bool FINE>
 struct ChunkSmem {
+    // A stage of K: a tile, or a half of one with what its rounding left behind it
     static constexpr int Q = TM * D * 2, K = TN * D * 2, V = D * TN * 2;
     // Panels of the ring: a multiple of four, so that a place always holds panels of the same warps of K and V.
     // Each warp then sees every phase of its places; one that skipped some could take the phase before the
@@ -76,7 +83,8 @@ struct ChunkSmem {
     static_assert(RING >= 8 && RING % 4 == 0, "places of the ring");
     static constexpr int off_q = 0, off_k = 2 * Q, off_v = off_k + 2 * K, off_ring = off_v + 2 * V;
     static constexpr int BYTES = off_ring + RING * PANEL + 1024;
-    static constexpr int KATOM = TN * 128, VATOM = D * 128;   // 64 dims of 128 tokens; 64 tokens of D lanes
+    // 64 dims of 128 rows; of a stage's tokens; 64 tokens of D lanes
+    static constexpr int QATOM = TM * 128, KATOM = (FINE ? TH : TN) * 128, VATOM = D * 128;
 };
 
 struct ChunkBars {
@@ -155,6 +163,16 @@ __device__ __forceinline__ __half2 codes2(uint32_t w) {
     return __hsub2(u2h((w & 0x000f000fu) | 0x64006400u), u2h(0x64006400u));
 }
 
+// minimum + scale * code of two codes, exact to fp32, as the sum of an fp16 and of the fp16 of what that leaves.
+__device__ __forceinline__ void split2(__half2 codes, float2 sm, uint32_t& hi, uint32_t& lo) {
+    const float2 c = __half22float2(codes);
+    const float2 x = make_float2(fmaf(c.x, sm.x, sm.y), fmaf(c.y, sm.x, sm.y));
+    const __half2 h = __floats2half2_rn(x.x, x.y);
+    const float2 r = __half22float2(h);
+    hi = h2u(h);
+    lo = half2_bits(x.x - r.x, x.y - r.y);
+}
+
 __device__ __forceinline__ bool elect_one() {
     uint32_t one;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
@@ -200,9 +218,9 @@ __device__ __forceinline__ void store_chunk_unaligned(uint16_t* p, uint4 v) {
     }
 }
 
-template <int D, int GRP>
+template <int D, int GRP, bool FINE>
 __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnParams P) {
-    using S = ChunkSmem<D, GRP>;
+    using S = ChunkSmem<D, GRP, FINE>;
     constexpr int NG = D / GRP, NW = D / 32, WPG = GRP / 32, PANEL = S::PANEL, RING = S::RING;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -323,7 +341,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 const int c = lane % LPR;
                 const int64_t src = live ? int64_t(rq.q0 + j) * P.q_stride + int64_t(h * P.G + g) * D : -1;
                 auto place = [&](int i) -> uint4* {           // the chunk of row i RPI + lane / LPR of the warp
-                    return reinterpret_cast<uint4*>(qb + (c >> 3) * S::KATOM + kmajor_off(t - lane + i * RPI + lane / LPR, c & 7));
+                    return reinterpret_cast<uint4*>(qb + (c >> 3) * S::QATOM + kmajor_off(t - lane + i * RPI + lane / LPR, c & 7));
                 };
                 // as it is, all loads in flight at once; then each chunk in place
                 if (P.q_vec) {
@@ -532,14 +550,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
             const int n = sg.here(), first = sg.ui, seq = sg.rq.seq;
             sg.skip(P, n);
             for (int it = 0; it < n; ++it, ++n_tile) {
-                const int st = n_tile & 1;
-                wait_idle(&B.kempty[st], (n_tile >> 1) + 1);
-                unsigned char* kb = smem + S::off_k + st * S::K;
+                if (!FINE) wait_idle(&B.kempty[n_tile & 1], (n_tile >> 1) + 1);
                 #pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
-                    const int p = wk + 4 * (i >> 1), o = 8 * (i & 1) + b, row = 16 * p + o;
+                    const int p = wk + 4 * (i >> 1), o = 8 * (i & 1) + b, row = 16 * p + o, st = FINE ? i >> 1 : n_tile & 1;
                     const uint32_t g = 8 * n_tile + p, slot = g % RING;
                     const unsigned char* pan = smem + S::off_ring + slot * PANEL;
+                    unsigned char* kb = smem + S::off_k + st * S::K;
+                    if (FINE && (i & 1) == 0) wait_idle(&B.kempty[st], n_tile + 1);
                     if ((i & 1) == 0) wait(&B.rfull[slot], g / RING);
                     uint32_t kw[NW], km[NG];
                     load_words(pan + o * (D / 2) + a * (D / 8), kw);
@@ -548,19 +566,33 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                     #pragma unroll
                     for (int k = 0; k < NW; ++k) {
                         const uint32_t meta = none ? 0u : km[k / WPG], v = kw[k];
-                        const __half2 s2 = u2h(__byte_perm(meta, 0, 0x1010)), m2 = u2h(__byte_perm(meta, 0, 0x3232));
                         const int c = 4 * k + a;
-                        *reinterpret_cast<uint4*>(kb + (c >> 3) * S::KATOM + kmajor_off(row, c & 7)) =
-                            make_uint4(h2u(__hfma2(codes2<false>(v), s2, m2)), h2u(__hfma2(codes2<true>(v), s2, m2)),
-                                       h2u(__hfma2(codes2<false>(v >> 8), s2, m2)), h2u(__hfma2(codes2<true>(v >> 8), s2, m2)));
+                        unsigned char* at = kb + (c >> 3) * S::KATOM + kmajor_off(FINE ? row & (TH - 1) : row, c & 7);
+                        if (FINE) {
+                            const float2 sm = __half22float2(u2h(meta));
+                            uint4 hi, lo;
+                            split2(codes2<false>(v), sm, hi.x, lo.x);
+                            split2(codes2<true>(v), sm, hi.y, lo.y);
+                            split2(codes2<false>(v >> 8), sm, hi.z, lo.z);
+                            split2(codes2<true>(v >> 8), sm, hi.w, lo.w);
+                            *reinterpret_cast<uint4*>(at) = hi;
+                            *reinterpret_cast<uint4*>(at + S::K / 2) = lo;
+                        } else {
+                            const __half2 s2 = u2h(__byte_perm(meta, 0, 0x1010)), m2 = u2h(__byte_perm(meta, 0, 0x3232));
+                            *reinterpret_cast<uint4*>(at) =
+                                make_uint4(h2u(__hfma2(codes2<false>(v), s2, m2)), h2u(__hfma2(codes2<true>(v), s2, m2)),
+                                           h2u(__hfma2(codes2<false>(v >> 8), s2, m2)), h2u(__hfma2(codes2<true>(v >> 8), s2, m2)));
+                        }
                     }
                     if (i & 1) {
                         __syncwarp();
                         if (lane == 0 && !dead) mbar_arrive(&B.rempty[slot]);
                     }
+                    if (i == 3 || (FINE && i == 1)) {
+                        fence_async_smem();
+                        mbar_arrive(&B.kfull[st]);
+                    }
                 }
-                fence_async_smem();
-                mbar_arrive(&B.kfull[st]);
             }
         }
     } else if (w < 16) {
@@ -676,19 +708,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
         uint32_t s_end = 0, pv_end = 0;                       // one behind the last that was issued
         // S of half `half` of the k-th tile of the CTA, into the buffer of its turn
         auto score = [&](uint32_t k, int half) {
-            const int st = k & 1;
-            if (half == 0) wait(&B.kfull[st], k >> 1);
+            const int st = FINE ? half : k & 1;
+            if (FINE || half == 0) wait(&B.kfull[st], FINE ? k : k >> 1);
             tc_after();
-            const uint32_t ah = ak + ((st * S::K + half * TH * 128) >> 4);
+            const uint32_t ah = ak + ((st * S::K + (FINE ? 0 : half * TH * 128)) >> 4);
             if (one && !dead) {
                 #pragma unroll
-                for (int e = 0; e < D / 16; ++e) {
-                    constexpr int A = S::KATOM;
-                    const uint32_t step = ((e >> 2) * A + (e & 3) * 32) >> 4;
-                    mma_f16(tm + s_col(x, n_s & 1), DESC + (aq + step), DESC + (ah + step), ID_S, e > 0 ? 1u : 0u);
+                for (int e = 0; e < (FINE ? 2 : 1) * (D / 16); ++e) {
+                    const int f = e % (D / 16);               // (then what K's rounding left, FINE)
+                    const uint32_t sq = ((f >> 2) * S::QATOM + (f & 3) * 32) >> 4;
+                    const uint32_t sk = ((f >> 2) * S::KATOM + (f & 3) * 32 + (e / (D / 16)) * (S::K / 2)) >> 4;
+                    mma_f16(tm + s_col(x, n_s & 1), DESC + (aq + sq), DESC + (ah + sk), ID_S, e > 0 ? 1u : 0u);
                 }
                 mma_commit(&B.sfull[x][n_s & 1]);
-                if (half) mma_commit(&B.kempty[st]);
+                if (FINE || half) mma_commit(&B.kempty[st]);
                 s_end = n_s + 1;
             }
             __syncwarp();
@@ -700,8 +733,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) q4_chunk_kernel(const AttnPa
                 if (n_q) wait(&B.noted[x], n_q - 1);          // V may write over the flags of this row tile's last
                 for (int i = 0; i < n; ++i, ++n_tile) {
                     const int st = n_tile & 1;
-                    wait(&B.kfull[st], n_tile >> 1);
-                    if (one) mbar_arrive(&B.kempty[st]);
+                    for (int half = 0; half < (FINE ? 2 : 1); ++half) {
+                        const int ks = FINE ? half : st;
+                        wait(&B.kfull[ks], FINE ? n_tile : n_tile >> 1);
+                        if (one) mbar_arrive(&B.kempty[ks]);
+                    }
                     wait(&B.vfull[st], n_tile >> 1);
                     if (one) mbar_arrive(&B.vempty[st]);
                 }
@@ -842,9 +878,9 @@ __global__ void __launch_bounds__(kMergeRows / kMergeEach * (D / 4)) q4_chunk_me
             store_out(P, rq, h, rb * CROWS + i0 + k * STEP, D, ln, o[k], l[k] == 0.f ? __int_as_float(0x7fc00000) : l[k]);
 }
 
-template <int D, int GRP>
+template <int D, int GRP, bool FINE>
 int launch_chunk(const AttnParams& P, cudaStream_t st) {
-    auto k = q4_chunk_kernel<D, GRP>;
+    auto k = q4_chunk_kernel<D, GRP, FINE>;
     if (int e = raise_smem_limit(reinterpret_cast<const void*>(k), "q4_chunk_kernel")) return e;
     cudaFuncAttributes fa{};
     if (cudaFuncGetAttributes(&fa, k) != cudaSuccess || fa.numRegs != kRegsLaunch) {
@@ -857,7 +893,7 @@ int launch_chunk(const AttnParams& P, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(P.n_ctas));
     cfg.blockDim = dim3(kChunkThreads);
-    cfg.dynamicSmemBytes = ChunkSmem<D, GRP>::BYTES;
+    cfg.dynamicSmemBytes = ChunkSmem<D, GRP, FINE>::BYTES;
     cfg.stream = st;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
@@ -890,7 +926,9 @@ int run_chunk(const ttkv_q4_cache_t* c, AttnParams P, void* ws, size_t ws_bytes,
     P.rec = static_cast<int32_t*>(ws);
     P.part_ml = reinterpret_cast<float*>(P.rec + 8 * kMaxCtas);
     P.part_o = P.part_ml + size_t(kMaxCtas) * 2 * CROWS * 2;
-#define TTKV_Q4_CHUNK(D, GRP) if (c->d == D && c->group == GRP) return launch_chunk<D, GRP>(P, st);
+#define TTKV_Q4_CHUNK(D, GRP)                                                                      \
+    if (c->d == D && c->group == GRP)                                                              \
+        return P.dtype == TTKV_F16 ? launch_chunk<D, GRP, true>(P, st) : launch_chunk<D, GRP, false>(P, st);
     TTKV_Q4_CHUNK(64, 32) TTKV_Q4_CHUNK(64, 64) TTKV_Q4_CHUNK(128, 32) TTKV_Q4_CHUNK(128, 64) TTKV_Q4_CHUNK(128, 128)
 #undef TTKV_Q4_CHUNK
     return fail(TTKV_ERR_UNSUPPORTED, "4-bit read: geometry");
