@@ -101,7 +101,8 @@ def test_scales_that_rise_and_parts_that_meet(d, g):
 
 # ------------------------------------------------------------------ NaN in chunks
 @pytest.mark.parametrize("d,g", [(64, 32), (128, 128)])
-def test_nan_by_row_tiles_in_turn(d, g):
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_nan_by_row_tiles_in_turn(d, g, dtype):
     """Row blocks of two row tiles and of one in turn, many in a CTA: a NaN of V in a block's last tokens reaches
     the rows that see it, and the rows of no other block."""
     from vllm_ttkv import ops
@@ -118,7 +119,7 @@ def test_nan_by_row_tiles_in_turn(d, g):
         ops.q4_write_paged(lay, cache, table[i, at[i] // 16].long()[None] * 16 + at[i] % 16, one, bad)
         K[i][at[i]] = 0.0
     own = [(r * 3) % 8 for r in range(R)]
-    q = torch.randn(sum(qls), G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    q = torch.randn(sum(qls), G, d, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
     out = torch.empty_like(q)
     ops.reset_status()
     starts = _prefill(lay, cache, table[torch.tensor(own, device="cuda")].contiguous(), seqs, qls, q, d ** -0.5, out, max_q=100)
@@ -135,14 +136,15 @@ def test_nan_by_row_tiles_in_turn(d, g):
             got, ref = _np(out[a:a + ql]), _np(q[a:a + ql])
             if sees.any():
                 got[sees, :, :g] = O.attend(ref, K[i][:n], clean[:n], d ** -0.5, G)[sees, :, :g]
-            _check_rows(got, ref, K[i][:n], clean[:n], d ** -0.5, G, torch.float16, True)
+            _check_rows(got, ref, K[i][:n], clean[:n], d ** -0.5, G, DT[dtype], True)
 
 
 # ------------------------------------------------------------------ small weights beside a large one
 @pytest.mark.parametrize("d,g", [(64, 64), (128, 128)])
 @pytest.mark.parametrize("R,ql,n", [(1, 1, 16384), (160, 1, 4000), (1, 66, 50000), (160, 33, 16384)])
 @pytest.mark.parametrize("nats", [8, 13, 17, 18, 20])
-def test_a_token_that_takes_most(d, g, R, ql, n, nats):
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_a_token_that_takes_most(d, g, R, ql, n, nats, dtype):
     """The first token's weight is e^nats times each other's, and its value is 0: the output is what the many small
     weights carry. Keys, values and queries lie on grids that fp16 holds, so that nothing is rounded but
     weights, sums and the output, in chunks as well. Tolerance: half a step of the output; 2^-11 of each
@@ -165,14 +167,14 @@ def test_a_token_that_takes_most(d, g, R, ql, n, nats):
     ops.q4_write_paged(lay, cache, table[0].long()[t // 16] * 16 + t % 16, kt, vt)
     K, V = (O.values(*O.quantise(x, g)) for x in (k, v))
     assert np.array_equal(K, k) and np.array_equal(V, v)
-    q = torch.from_numpy(np.where(np.arange(d) % 2, 1.0, -1.0) * np.ones((ql, G, 1))).half().cuda()
+    q = torch.from_numpy(np.where(np.arange(d) % 2, 1.0, -1.0) * np.ones((ql, G, 1))).to(DT[dtype]).cuda()
     s = (K[:, 0] @ q[0, 0].double().cpu().numpy())       # the first is the largest of all
     scale = nats / (s[0] - np.median(s[1:]))
-    out = torch.empty(R * ql, G, d, device="cuda", dtype=torch.float16)
+    out = torch.empty(R * ql, G, d, device="cuda", dtype=DT[dtype])
     _prefill(lay, cache, table.expand(R, -1), [n] * R, [ql] * R, q.repeat(R, 1, 1), scale, out)
     want = O.attend(_np(q), K, V, scale, G)
     W = np.maximum(np.abs(V), np.where(np.arange(n) > 0, 7.5 / 8, 0.0)[:, None, None])
-    tol = 2.0 ** -11 * np.abs(want) + (2.0 ** -11 + 2.0 ** -12) * O.attend(_np(q), K, W, scale, G) + n * 2.0 ** -30
+    tol = torch.finfo(DT[dtype]).eps / 2 * np.abs(want) + (2.0 ** -11 + 2.0 ** -12) * O.attend(_np(q), K, W, scale, G) + n * 2.0 ** -30
     err = np.abs(_np(out).reshape(R, ql, G, d) - want)
     assert np.all(err <= tol), (float((err / tol).max()), float((err / np.abs(want).max()).max()))
 
@@ -206,7 +208,8 @@ def test_an_infinite_query_is_nan(d, g, ql, G, sign, scale):
     _check_rows(got, ref, K, V, scale, G, torch.float16, True)
 
 
-def test_an_infinite_query_of_a_long_row_is_nan():
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_an_infinite_query_of_a_long_row_is_nan(dtype):
     """As above, the row in parts of many CTAs, some of them behind what the row sees."""
     lay, n, ql = _lay(1, 64, 64), 3000, 200
     from vllm_ttkv import ops
@@ -214,7 +217,7 @@ def test_an_infinite_query_of_a_long_row_is_nan():
     cache, table = lay.new_cache(-(-n // 16), 16), torch.arange(-(-n // 16), dtype=torch.int32, device="cuda")[None]
     k, v = (torch.from_numpy(rng.uniform(0.5, 2, (n, 1, 64))).float().cuda() for _ in range(2))
     ops.q4_write_paged(lay, cache, torch.arange(n, device="cuda"), k, v)
-    q = torch.randn(ql, 2, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+    q = torch.randn(ql, 2, 64, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
     q[11, 0, 7] = q[150, 1, 40] = -float("inf")
     out = torch.empty_like(q)
     _prefill(lay, cache, table, [n], [ql], q, 0.1, out)
@@ -276,12 +279,12 @@ def test_chunks(d, g, H, HQ, dtype, bs, qls):
 
 
 @pytest.mark.parametrize("d,g", GEOMETRIES)
-@pytest.mark.parametrize("scale", [0.05, 0.2])
-def test_chunks_of_many_tiles(d, g, scale):
+@pytest.mark.parametrize("scale,dtype", [(0.05, "fp16"), (0.2, "fp16"), (0.05, "bf16")])
+def test_chunks_of_many_tiles(d, g, scale, dtype):
     """Some 40 stored tiles a CTA, many times round the ring of panels and the operands' stages."""
     lay, R, ql, n, G = _lay(1, d, g), 64, 64, 6000, 8
     cache, table, K, V = _filled(lay, [n], 16, seed=d + g)
-    q = torch.randn(R * ql, G, d, generator=torch.Generator().manual_seed(3)).half().cuda()
+    q = torch.randn(R * ql, G, d, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
     out = torch.empty_like(q)
     starts = _prefill(lay, cache, table.expand(R, -1), [n - 3 * r for r in range(R)], [ql] * R, q, scale, out)
     for r in (0, 11, 23, 38, 47, 63):
@@ -290,10 +293,11 @@ def test_chunks_of_many_tiles(d, g, scale):
 
 
 @pytest.mark.parametrize("H,HQ,ql,n", [(1, 2, 200, 5000), (2, 8, 40, 3001), (1, 16, 9, 9000), (1, 5, 700, 2100)])
-def test_chunks_in_parts(H, HQ, ql, n):
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_chunks_in_parts(H, HQ, ql, n, dtype):
     lay = _lay(H, 128, 128)
     cache, table, K, V = _filled(lay, [n], 16, seed=ql)
-    q = torch.randn(ql, HQ, 128, generator=torch.Generator().manual_seed(3)).half().cuda()
+    q = torch.randn(ql, HQ, 128, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
     out = torch.empty_like(q)
     _prefill(lay, cache, table, [n], [ql], q, 0.08, out)
     _check_tight(out, q, K[0], V[0], 0.08, HQ // H, lay, True)
