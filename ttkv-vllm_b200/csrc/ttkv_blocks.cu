@@ -10,7 +10,7 @@
 // waiting for another CTA's, keeps each request's lengths and its end in the free list in shared
 // memory, and then takes its share of the blocks that change hands and of the tokens, each found by a
 // binary search, so that a step has two rounds of loads whatever its mix of lengths. One decode token
-// for each of 8, 1024, 4096 and 16384 requests takes 8.3, 12.3, 20.5 and 64 us from an idle GPU (8.6,
+// for each of 8, 1024, 4096 and 16384 requests takes 8.3, 12.3, 22.5 and 64 us from an idle GPU (8.6,
 // 13.3, 32.8 and 111 with one CTA), 16384 tokens of 64 requests 12.3 (45 with one). A release writes
 // the ids as it reads them, behind the list's end, and starts over without a request's where one is
 // negative: looking at all of them first would be a third round of loads. The cluster's barrier orders

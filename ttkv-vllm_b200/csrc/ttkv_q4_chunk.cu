@@ -9,11 +9,11 @@
 // and P would cost the softmax twice its instructions, and with groups below d a product each). V^ is off
 // by 2^-11 of an element at most, as is each weight, which is what fp16 outputs are off by themselves.
 // Rounded keys put 2^-11 of sum |q_i K_i| on a score at most, which grows with the keys and not with their
-// spread: 4e-4 to 1e-3 of the output with a few large channels, 2e-3 where channels have offsets of three
-// times their spread, against the 1.7e-3 that bf16 outputs are off by themselves and the 2.1e-4 of fp16.
-// So for fp16 queries (FINE) a key is the sum of two fp16, its rounding and what that leaves, with a product
-// each: 3.2e-4 in all; the chunks below take 286 and 802 us for 253 and 695. (V as a sum of two as well
-// gives 2.7e-4 and takes 353 and 1001.) Scores, sums and O are fp32. P is fp16, of which the weights are
+// spread: 5e-4 to 1e-3 of the output with a few large channels, up to 1.8e-3 where channels have offsets of
+// three times their spread, against the 1.7e-3 that bf16 outputs are off by themselves and the 2.1e-4 of
+// fp16. So for fp16 queries (FINE) a key is the sum of two fp16, its rounding and what that leaves, with a
+// product each: 3.3e-4 in all, and 282 and 854 us for the 251 and 734 of the chunks below. (V as a sum of two
+// as well gives 2.7e-4 and takes 20 to 25 percent more.) Scores, sums and O are fp32. P is fp16, of which the weights are
 // held in the upper part: the largest of a segment's first half is 2^8 and none passes 2^15, so they keep
 // 11 bits down to 2^-22 of it and vanish only below 2^-33 (2^-25 with a largest of 1, which lost half of what
 // 16383 tokens weigh together, each 18 nats below the first).
@@ -30,15 +30,15 @@
 // kept short (rolled where the data lies in shared memory): together they have to stay in the SM's
 // instruction cache, and unrolled they streamed 19 KB of code per tile through it.
 //
-// 256 queries of 24 heads over 7379 tokens of each of 8 requests take 241 us without the merge, 757
-// TFLOP/s; 1024 to 2048 queries of 32 heads over 8192 to 16384 tokens of two requests 700, 870 TFLOP/s,
-// half of a library matrix product's rate. A stored tile takes about 4500 cycles, in 2050 of which the
+// 256 queries of 24 heads over 7379 tokens of each of 8 requests take 251 us without the merge, 727
+// TFLOP/s; 1024 to 2048 queries of 32 heads over 8192 to 16384 tokens of two requests 734, 827 TFLOP/s,
+// half of a library matrix product's rate (bf16, under the profiler; 230 and 680 in a program). A stored tile takes about 4500 cycles, in 2050 of which the
 // tensor cores compute; the exponentials take 2050 of their pipe, the operands 2700 of shared memory's
 // (A of the scores is read again with each 64 tokens), and each role is busy for 3500 to 4000, slowed by
 // the others' instructions. Without any one role's arithmetic it is 4 to 6 percent faster, without all 10.
-// Scores a half ahead in a buffer of their own, with the maximum sought in every half, took 710 us for
-// 690; rings of their own for K and V changed nothing; product warps of one running lane took 722, as
-// what their instructions need was then moved lane by lane.
+// Scores a half ahead in a buffer of their own, with the maximum sought in every half, took 3 percent more
+// time; rings of their own for K and V changed nothing; product warps of one running lane took 5 percent
+// more, as what their instructions need was then moved lane by lane.
 //
 // The work list is (request, KV head, row block, stored tile up to the block's causal limit), shared
 // out evenly to one CTA per SM as in the streaming kernel; the parts that a share's borders cut go

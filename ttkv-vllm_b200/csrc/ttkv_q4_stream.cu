@@ -19,7 +19,7 @@
 // values cost five instructions. p_t s_t is rounded to fp16, an operand of the matrix product, after
 // scaling by a power of two that keeps the largest near 2^14. It multiplies c - 7.5 (the second sum
 // takes the rounded weight's share of 7.5: sum p' of a unit comes from one more product, with 15s), so
-// the rounding error is that of weights on centred values: 2^-12 of each term at most.
+// the rounding error is that of weights on centred values: 2^-11 of each term at most.
 #include <algorithm>
 #include <cmath>
 
@@ -488,8 +488,8 @@ struct WarpRows {
 };
 
 // ------------------------------------------------------------------ the streaming kernel
-// The work is the list of (request, KV head, row block, 64-token unit), shared out evenly: CTA c of
-// n owns [c T / n, (c + 1) T / n), each of its warps an equal part of that. A warp's run crosses from
+// The work is the list of (request, KV head, row block, 64-token unit), shared out in order: of T units CTA c of
+// n owns [c S, (c + 1) S), S = ceil(T / n), each of its warps an equal part of that. A warp's run crosses from
 // one (request, head, row block) to the next; what a run holds of one is a segment. Starting and ending
 // a segment costs about as much as a unit (its queries, its sums), so each one counts as a unit more.
 // A segment that is whole writes its output; the others meet in shared memory at the end of the CTA,
@@ -847,11 +847,11 @@ __global__ void __launch_bounds__(kMergeThreads) q4_merge_kernel(const AttnParam
 // where that leaves none empty, and in groups of 32 there not at all, since two spill. 64 requests of 6000
 // tokens, 8 KV heads, us with two and with one:
 //   d, group   16 rows    24         32
-//   64, 32     172/195    299/281    313/365   (and ragged, 1 to 20 rows: 36/38)
-//   64, 64     154/174    262/252    281/328
-//   128, 128   197/213    332/305    352/397
-//   128, 64    225/242    389/348    414/453
-//   128, 32    324/307    590/444    610/584
+//   64, 32     176/197    305/283    322/369   (and ragged, 1 to 20 rows: 36/38)
+//   64, 64     158/176    270/254    283/330
+//   128, 128   203/219    348/315    369/410
+//   128, 64    229/244    399/352    422/459
+//   128, 32    350/317    637/463    649/606
 int stream_nt(int d, int group, int64_t rows) {
     if (d == 64) return rows > 8 ? 2 : 1;
     return group == 32 || (rows + 7) / 8 % 2 ? 1 : 2;
@@ -954,7 +954,7 @@ AttnParams attn_params(const ttkv_q4_attn_args_t* a) {
 // Whether chunks of `rows` (query, head) rows a KV head are streamed, the cache read and its codes fed to
 // the tensor cores once per 16 rows (8 in groups of 32 at d = 128, `narrow`), or go to the chunk kernel,
 // whose tiles of 256 rows each dequantise the cache once. Streamed against chunked, d = 128 in groups of 128,
-// 8 KV heads, us:
+// 8 KV heads, bf16 (chunks of fp16 queries take 11 to 16 percent more), us:
 //   requests x tokens   16 rows      24           32           48           64
 //   64 x 130            56 / 73      73 / 77      91 / 77      128 / 77     159 / 79
 //   16 x 500            32 / 36      36 / 36      42 / 34      52 / 36      67 / 36

@@ -1,5 +1,6 @@
-// tcgen05 and tensor-memory helpers shared by the sm_100a kernels: descriptors, the MMA and its commit,
-// allocation, and loads and stores of a thread's tensor-memory lane.
+// tcgen05 and tensor-memory helpers of the chunk kernel of the 4-bit cache (ttkv_q4_chunk.cu): descriptors, the
+// MMA and its commit, allocation, and loads and stores of a thread's tensor-memory lane. The TT-KV decode and
+// continuation have theirs in ttkv_decode_tc.cuh.
 #pragma once
 
 #include <cuda_runtime.h>
