@@ -211,6 +211,14 @@ def test_release_of_bad_rows_and_little_room():
         assert _release(table, [48, 48, 48, 48, 0], free, 0, 16) == want
         with pytest.raises((IndexError, RuntimeError)):
             ops.check_status()
+    # one that would not fit and holds none: those behind it do
+    free = np.full(5, -1)
+    want = O.release(table[:3], [48, 32, 48], free, 3, 16)[0]
+    assert want == [-1, -1, -1, 4, 5]
+    ops.reset_status()
+    assert _release(table[:3], [48, 32, 48], free, 3, 16) == want
+    with pytest.raises((IndexError, RuntimeError)):
+        ops.check_status()
     ops.reset_status()
     assert _release(table[1:], [33, 0, 48, 0], np.full(6, -1), 0, 16) == [4, 5, 6, 10, 11, 12]
     ops.check_status()

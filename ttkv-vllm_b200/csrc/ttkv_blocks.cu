@@ -13,7 +13,7 @@
 // for each of 8, 1024, 4096 and 16384 requests takes 8.3, 12.3, 22.5 and 64 us from an idle GPU (8.6,
 // 13.3, 32.8 and 111 with one CTA), 16384 tokens of 64 requests 12.3 (45 with one). A release writes
 // the ids as it reads them, behind the list's end, and starts over without a request's where one is
-// negative: looking at all of them first would be a third round of loads. The cluster's barrier orders
+// negative or the room was too little: looking at all of them first would be a third round of loads. The cluster's barrier orders
 // every CTA's read of the count before the write of the new one, which may be the same word.
 #include <cooperative_groups.h>
 
@@ -217,12 +217,10 @@ __global__ void __launch_bounds__(kPlanThreads) release_blocks_kernel(const Plan
     bool lacking;
     int used = assign_ranges<true>(P, avail, M, wsum, &taken, lacking);
     cluster.barrier_wait(std::move(begun));          // every CTA's bad_row may be written
-    if (push_ids(P, M, count, used, at, step)) {
-        report(P.status, TTKV_STATUS_BLOCK_RANGE);
+    if (push_ids(P, M, count, used, at, step))
         for (int c = 0; c < kPlanCtas; ++c) *cluster.map_shared_rank(&bad_row, c) = 1;
-    }
     cluster.sync();
-    if (bad_row) {                                   // (the same in every CTA) once more without the rows that hold one
+    if (bad_row || lacking) {                        // (the same in every CTA) once more without the rows that hold one
         const int lane = threadIdx.x & 31;
         for (int r = threadIdx.x >> 5; r < P.n_reqs; r += kPlanThreads / 32) {
             const int nb = blocks_of(P.lens[r], P.block_size);
@@ -231,6 +229,7 @@ __global__ void __launch_bounds__(kPlanThreads) release_blocks_kernel(const Plan
                 for (int k = lane; k < nb; k += 32) bad |= P.block_table[int64_t(r) * P.bt_stride + k] < 0;
             bad = __any_sync(0xffffffffu, bad);
             if (lane == 0) M.len[r] = bad ? kBadRow : 0;
+            if (bad && lane == 0 && blockIdx.x == 0) report(P.status, TTKV_STATUS_BLOCK_RANGE);
         }
         __syncthreads();
         used = assign_ranges<true>(P, avail, M, wsum, &taken, lacking, true);
